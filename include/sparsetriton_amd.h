@@ -814,6 +814,59 @@ int st_bn_backward(const void* Y, const void* out, const void* dout, int64_t n, 
                    const float* invstd, const int32_t* counts, float* workspace, int64_t workspace_floats, void* dY,
                    void* dres, float* dweight, float* dbias, st_stream_t stream);
 
+/* ------------------------------------------------------------ layer norm
+ *
+ * Layer norm over the C channels of each of n rows, with the residual add of a
+ * pre-norm block in the same pass (the reference applies torch's layer norm to
+ * the features, nn/modules/norm.py; these entry points have no counterpart):
+ *   h = X + residual (rounded to `dtype`, stored to H); without a residual (and H) h = X
+ *   Y = (h - mean) * rstd * weight + bias,  rstd = 1 / sqrt(mean_c (h - mean)^2 + eps)
+ * X, residual, H, Y: (n, C) contiguous of `dtype` (ST_F32, ST_F16, ST_BF16);
+ * weight, bias: (C) of weight_dtype (`dtype` or ST_F32), NULL = 1 and 0;
+ * mean, rstd: fp32 (n), both or neither (the backward reads them).  Rows at
+ * 16-byte addresses take 16-byte accesses, others element accesses.
+ * st_ln_backward: H is the forward's h (X without a residual), dY the gradient
+ * at Y, dH (NULL = none) the one at h; dX (NULL = not wanted) the gradient of
+ * X and of the residual alike, dweight, dbias (of weight_dtype, NULL = not
+ * wanted) added over the rows in a fixed order.  workspace: at least
+ * st_ln_backward_workspace floats at a 16-byte address, needed with dweight or dbias.
+ */
+int st_ln_forward(const void* X, const void* residual, int64_t n, int C, int dtype, const void* weight,
+                  const void* bias, int weight_dtype, float eps, void* H, void* Y, float* mean, float* rstd,
+                  st_stream_t stream);
+int st_ln_backward_workspace(int64_t n, int C, int dtype, int64_t* floats);
+int st_ln_backward(const void* H, const void* dY, const void* dH, int64_t n, int C, int dtype, const void* weight,
+                   int weight_dtype, const float* mean, const float* rstd, float* workspace, int64_t workspace_floats,
+                   void* dX, void* dweight, void* dbias, st_stream_t stream);
+
+/* ------------------------------------------------------------ rotary positions
+ *
+ * Turns the channel pairs of q (n, heads, dim) and k (n, kv_heads, dim) by the
+ * row's position (no counterpart in the reference): pair p by
+ * positions[row][axis[p]] * turns[p] whole turns (inverse: by the negative,
+ * which is the gradient), channels from 2 * pairs on copied.  Pairs are
+ * (p, p + pairs), interleaved (2p, 2p + 1).  Row and head strides are in
+ * elements, channels adjacent; the outputs are contiguous.  positions: rows
+ * of pos_dtype (st_coord_dtype, or ST_POS_F32) pos_row elements apart; turns:
+ * fp64, axis: int32, both (pairs) on the device.  q or k may be NULL.
+ */
+#define ST_POS_F32 3
+typedef struct st_rotary_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_row, q_head, k_row, k_head;
+  const void* positions;
+  int64_t pos_row;
+  const double* turns;
+  const int32_t* axis;
+  int64_t n;
+  int32_t heads, kv_heads, dim, pairs;
+  int32_t dtype, pos_dtype, interleaved, inverse;
+} st_rotary_args;
+int st_rotary(const st_rotary_args* args, st_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@ ERR_UNSUPPORTED = -3
 ERRORS = {-1: "invalid argument", -2: "HIP runtime error", -3: "unsupported dtype or size"}
 
 COORD_DTYPES = {torch.int16: 0, torch.int32: 1, torch.int64: 2}
+POSITION_DTYPES = {**COORD_DTYPES, torch.float32: 3}
 FEAT_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 STATUS_WORDS = 4
@@ -59,6 +60,17 @@ class Lookup(ctypes.Structure):
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = (
+        [(n, _P) for n in ("q", "k", "q_out", "k_out")]
+        + [(n, _L) for n in ("q_row", "q_head", "k_row", "k_head")]
+        + [("positions", _P), ("pos_row", _L), ("turns", _P), ("axis", _P), ("n", _L)]
+        + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "pairs", "dtype", "pos_dtype", "interleaved",
+                                         "inverse")]
+    )
+
 
 # name -> argtypes (all functions return int unless listed in _RESTYPES)
 _SIGNATURES = {
@@ -124,6 +136,10 @@ _SIGNATURES = {
     "st_bn_forward": [_P, _L, _I, _I, _P, _I, _I, _P, _P, _P, _I, _I, ctypes.c_float, ctypes.c_float, _P, _P, _P,
                       _P, _P, _P, _L, _P, _P],
     "st_bn_backward": [_P, _P, _P, _L, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P, _L, _P, _P, _P, _P, _P],
+    "st_ln_forward": [_P, _P, _L, _I, _I, _P, _P, _I, ctypes.c_float, _P, _P, _P, _P, _P],
+    "st_ln_backward_workspace": [_L, _I, _I, ctypes.POINTER(_L)],
+    "st_ln_backward": [_P, _P, _P, _L, _I, _I, _P, _I, _P, _P, _P, _L, _P, _P, _P, _P],
+    "st_rotary": [ctypes.POINTER(RotaryArgs), _P],
     "st_hashfly_wgrad": [_P, _L, _P, _P, _I, _L, _P, ctypes.POINTER(Lookup), _P, _P, _L, _I, _I, _I, _P, _L, _P,
                          _I, _P],
 }

@@ -1,0 +1,204 @@
+// Rotary positions with several axes: each head's channels are paired, pair p
+// belongs to one axis of the row's position and turns by
+//   angle = pos[axis(p)] * f(p):   (a, b) -> (a cos - b sin, a sin + b cos),
+// channels past the pairs go through unchanged.  The gradient is the turn by
+// -angle.  Pairs are (p, p + P) or, interleaved, (2p, 2p + 1).
+//
+// Bound by memory (each element in and out once), as long as the angles' sines
+// are not paid for each head: a workgroup takes `rows` rows, computes their
+// rows x P cosines and sines once into LDS, and every head of both tensors
+// reads them there.  No table of positions is needed, so any coordinate works.
+// The angle is reduced in turns in 64-bit arithmetic (frequency / 2 pi as a
+// double, minus the nearest whole turn): an fp32 product pos * f of a few
+// hundred radians is already off by 1e-5.
+#include "common.h"
+
+namespace st {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotTable = 2048;  // cosine / sine pairs in LDS (16 KB)
+constexpr int kRotItems = 2048;  // vectors of a workgroup's rows, about
+
+template <typename T>
+struct RotArgs {
+  const T* in[2];
+  T* out[2];
+  int64_t in_row[2], in_head[2];
+  int heads[2];
+  const void* pos;
+  int64_t pos_row;
+  const double* turns;
+  const int32_t* axis;
+  int64_t n;
+  int D, P, rows;
+  int chunks;                       // vectors of a head: pair vectors, then the unchanged channels'
+  int per_row;                      // vectors of a row, both tensors
+  uint64_t per_row_inv, chunks_inv; // ceil(2^32 / ...): i / d = i * inv >> 32 for i * d < 2^32
+};
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) RotVec {
+  T e[V];
+};
+
+__device__ __forceinline__ double rot_pos(const int16_t* p, int a) { return p[a]; }
+__device__ __forceinline__ double rot_pos(const int32_t* p, int a) { return p[a]; }
+__device__ __forceinline__ double rot_pos(const int64_t* p, int a) { return (double)p[a]; }
+__device__ __forceinline__ double rot_pos(const float* p, int a) { return p[a]; }
+
+template <typename T, typename PT, int V, bool INTERLEAVED, bool INVERSE>
+__global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs<T> g) {
+  using Vec = RotVec<T, V>;
+  __shared__ float2 table[kRotTable];
+  const int64_t row0 = (int64_t)blockIdx.x * g.rows;
+  const int rows = g.n - row0 < g.rows ? (int)(g.n - row0) : g.rows;
+  for (int i = threadIdx.x; i < rows * g.P; i += kRotThreads) {
+    const int r = i / g.P, p = i - r * g.P;
+    const PT* pos = (const PT*)g.pos + (row0 + r) * g.pos_row;
+    const double t = rot_pos(pos, g.axis[p]) * g.turns[p];
+    float s, c;
+    sincospif(2.f * (float)(t - rint(t)), &s, &c);
+    table[i] = make_float2(c, INVERSE ? -s : s);
+  }
+  __syncthreads();
+  const int pair_chunks = INTERLEAVED ? 2 * g.P / V : g.P / V;
+  for (int i = threadIdx.x; i < rows * g.per_row; i += kRotThreads) {
+    const int r = (int)((uint64_t)i * g.per_row_inv >> 32);
+    const int in_row = i - r * g.per_row;
+    int h = (int)((uint64_t)in_row * g.chunks_inv >> 32);
+    const int ch = in_row - h * g.chunks;
+    const int which = h >= g.heads[0];
+    h -= which ? g.heads[0] : 0;
+    const T* in = g.in[which] + (row0 + r) * g.in_row[which] + h * g.in_head[which];
+    T* out = g.out[which] + ((row0 + r) * g.heads[which] + h) * g.D;
+    const float2* t = table + r * g.P;
+    if (ch >= pair_chunks) {
+      const int d = 2 * g.P + (ch - pair_chunks) * V;
+      *reinterpret_cast<Vec*>(out + d) = *reinterpret_cast<const Vec*>(in + d);
+    } else if constexpr (INTERLEAVED && V > 1) {
+      const Vec x = *reinterpret_cast<const Vec*>(in + ch * V);
+      Vec y;
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const float2 cs = t[ch * (V / 2) + e / 2];
+        const float a = (float)x.e[e], b = (float)x.e[e + 1];
+        y.e[e] = (T)(a * cs.x - b * cs.y);
+        y.e[e + 1] = (T)(a * cs.y + b * cs.x);
+      }
+      *reinterpret_cast<Vec*>(out + ch * V) = y;
+    } else if constexpr (INTERLEAVED) {  // one channel, its partner read beside it
+      const float2 cs = t[ch >> 1];
+      const float x = (float)in[ch], other = (float)in[ch ^ 1];
+      out[ch] = (T)((ch & 1) ? other * cs.y + x * cs.x : x * cs.x - other * cs.y);
+    } else {
+      const int p = ch * V;
+      const Vec xa = *reinterpret_cast<const Vec*>(in + p), xb = *reinterpret_cast<const Vec*>(in + g.P + p);
+      Vec ya, yb;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float2 cs = t[p + e];
+        const float a = (float)xa.e[e], b = (float)xb.e[e];
+        ya.e[e] = (T)(a * cs.x - b * cs.y);
+        yb.e[e] = (T)(a * cs.y + b * cs.x);
+      }
+      *reinterpret_cast<Vec*>(out + p) = ya;
+      *reinterpret_cast<Vec*>(out + g.P + p) = yb;
+    }
+  }
+}
+
+// Whether vectors of V channels cut every head evenly and lie at their own size's alignment.
+template <typename T, int V>
+static bool rot_vec_ok(const RotArgs<T>& g, bool interleaved) {
+  if (g.D % V || (interleaved ? 2 * g.P : g.P) % V || (2 * g.P) % V) return false;
+  for (int w = 0; w < 2; ++w) {
+    if (!g.heads[w]) continue;
+    if (g.in_row[w] % V || g.in_head[w] % V) return false;
+    if (((uintptr_t)g.in[w] | (uintptr_t)g.out[w]) % (V * sizeof(T))) return false;
+  }
+  return true;
+}
+
+template <typename T, typename PT, int V>
+static int rot_launch(RotArgs<T> g, bool interleaved, bool inverse, hipStream_t s) {
+  const int pairs = interleaved ? 2 * g.P / V : g.P / V;
+  g.chunks = pairs + (g.D - 2 * g.P) / V;
+  const int64_t per_row = (int64_t)(g.heads[0] + g.heads[1]) * g.chunks;
+  if (per_row >= (1 << 15)) return ST_ERR_UNSUPPORTED;
+  g.per_row = (int)per_row;
+  // rows of a workgroup: what LDS and a few vectors a thread hold, fewer while there are not 1024 workgroups
+  int64_t rows = g.P ? kRotTable / g.P : kRotItems;
+  if (kRotItems / per_row < rows) rows = kRotItems / per_row;
+  if (g.n / 1024 < rows) rows = g.n / 1024;
+  g.rows = rows > 0 ? (int)rows : 1;
+  g.per_row_inv = ((1ull << 32) + g.per_row - 1) / g.per_row;
+  g.chunks_inv = ((1ull << 32) + g.chunks - 1) / g.chunks;
+  const int64_t blocks = (g.n + g.rows - 1) / g.rows;
+  if (blocks >= (1ll << 31)) return ST_ERR_ARG;
+  const dim3 grid((unsigned)blocks);
+  if (interleaved && inverse)
+    rotary_kernel<T, PT, V, true, true><<<grid, kRotThreads, 0, s>>>(g);
+  else if (interleaved)
+    rotary_kernel<T, PT, V, true, false><<<grid, kRotThreads, 0, s>>>(g);
+  else if (inverse)
+    rotary_kernel<T, PT, V, false, true><<<grid, kRotThreads, 0, s>>>(g);
+  else
+    rotary_kernel<T, PT, V, false, false><<<grid, kRotThreads, 0, s>>>(g);
+  ST_CHECK_LAUNCH();
+  return ST_OK;
+}
+
+template <typename T, typename PT>
+static int rot_vectors(const RotArgs<T>& g, bool interleaved, bool inverse, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  if (rot_vec_ok<T, V>(g, interleaved)) return rot_launch<T, PT, V>(g, interleaved, inverse, s);
+  if (rot_vec_ok<T, V / 2>(g, interleaved)) return rot_launch<T, PT, V / 2>(g, interleaved, inverse, s);
+  return rot_launch<T, PT, 1>(g, interleaved, inverse, s);
+}
+
+template <typename T>
+static int rot_positions(const st_rotary_args* a, int pos_dtype, hipStream_t s) {
+  RotArgs<T> g{};
+  g.in[0] = (const T*)a->q, g.in[1] = (const T*)a->k;
+  g.out[0] = (T*)a->q_out, g.out[1] = (T*)a->k_out;
+  g.in_row[0] = a->q_row, g.in_row[1] = a->k_row;
+  g.in_head[0] = a->q_head, g.in_head[1] = a->k_head;
+  g.heads[0] = a->q ? a->heads : 0, g.heads[1] = a->k ? a->kv_heads : 0;
+  g.pos = a->positions, g.pos_row = a->pos_row;
+  g.turns = a->turns, g.axis = a->axis;
+  g.n = a->n, g.D = a->dim, g.P = a->pairs;
+  const bool il = a->interleaved != 0, inv = a->inverse != 0;
+  switch (pos_dtype) {
+    case ST_COORD_I16:
+      return rot_vectors<T, int16_t>(g, il, inv, s);
+    case ST_COORD_I32:
+      return rot_vectors<T, int32_t>(g, il, inv, s);
+    case ST_COORD_I64:
+      return rot_vectors<T, int64_t>(g, il, inv, s);
+    case ST_POS_F32:
+      return rot_vectors<T, float>(g, il, inv, s);
+    default:
+      return ST_ERR_UNSUPPORTED;
+  }
+}
+
+}  // namespace st
+
+extern "C" int st_rotary(const st_rotary_args* a, st_stream_t stream) {
+  if (!a || a->n < 0 || a->dim <= 0 || a->pairs < 0 || 2 * a->pairs > a->dim || a->pairs > st::kRotTable) return ST_ERR_ARG;
+  if ((!a->q && !a->k) || (a->q && (!a->q_out || a->heads <= 0)) || (a->k && (!a->k_out || a->kv_heads <= 0)))
+    return a->n == 0 ? ST_OK : ST_ERR_ARG;
+  if (a->n == 0) return ST_OK;
+  if (a->pairs && (!a->positions || !a->turns || !a->axis)) return ST_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  switch (a->dtype) {
+    case ST_F32:
+      return st::rot_positions<float>(a, a->pos_dtype, s);
+    case ST_F16:
+      return st::rot_positions<_Float16>(a, a->pos_dtype, s);
+    case ST_BF16:
+      return st::rot_positions<__bf16>(a, a->pos_dtype, s);
+    default:
+      return ST_ERR_UNSUPPORTED;
+  }
+}

@@ -15,18 +15,22 @@ Both run as HIP kernels (``st_bn_forward`` / ``st_bn_backward``): two
 deterministic statistics passes and one output pass forward, one statistics
 pass and one gradient pass backward, each autograd-differentiable in the
 features, the residual and the affine parameters.
+
+``sparse_layer_norm`` normalises each row over its channels, with the residual
+add of a pre-norm transformer block in the same pass (``st_ln_forward`` /
+``st_ln_backward``).
 """
 
 import ctypes
 import functools
-from typing import Optional
+from typing import Optional, Tuple, Union
 
 import torch
 
 from sparsetriton_amd import _lib
 from sparsetriton_amd.tensor import SparseTensor
 
-__all__ = ["sparse_batch_norm", "sparse_batch_norm_act"]
+__all__ = ["sparse_batch_norm", "sparse_batch_norm_act", "sparse_layer_norm"]
 
 
 def _f32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -158,3 +162,119 @@ def sparse_batch_norm(
 ) -> SparseTensor:
     """Per-sample batch normalisation (reference ``norm.py:20-112``)."""
     return sparse_batch_norm_act(tensor, weight, bias, running_mean, running_var, training, eps, momentum)
+
+
+@functools.lru_cache(maxsize=256)
+def _ln_workspace_floats(n: int, C: int, code: int) -> int:
+    floats = ctypes.c_int64()
+    _lib.call("st_ln_backward_workspace", n, C, code, ctypes.byref(floats))
+    return floats.value
+
+
+def _ln_params(x, weight, bias):
+    """weight and bias as the kernels take them: one dtype for both, the features' or fp32."""
+    w, b = weight, bias
+    dt = (w if w is not None else b).dtype if (w is not None or b is not None) else torch.float32
+    if dt not in (x.dtype, torch.float32) or (w is not None and b is not None and b.dtype != dt):
+        dt = torch.float32
+    w = w.detach().to(dt).contiguous() if w is not None else None
+    b = b.detach().to(dt).contiguous() if b is not None else None
+    return w, b, _lib.FEAT_DTYPES[dt]
+
+
+def _ln_forward(x, weight, bias, residual, eps, stats):
+    C = x.shape[-1]
+    x = x.contiguous()
+    n = x.numel() // C
+    res = residual.contiguous() if residual is not None else None
+    w, b, wcode = _ln_params(x, weight, bias)
+    y = torch.empty_like(x)
+    h = torch.empty_like(x) if res is not None else None
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0)
+    _lib.call("st_ln_forward", _lib.ptr(x), _lib.ptr(res), n, C, _lib.FEAT_DTYPES[x.dtype], _lib.ptr(w), _lib.ptr(b),
+              wcode, eps, _lib.ptr(h), _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd), _lib.stream_of(x.device))
+    return y, h, x, w, wcode, mean, rstd
+
+
+class _LayerNorm(torch.autograd.Function):
+    """(y,) or, with a residual, (y, h): y = norm(h), h = x + residual."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, eps):
+        y, h, xc, w, wcode, mean, rstd = _ln_forward(x, weight, bias, residual, eps, True)
+        ctx.save_for_backward(xc if h is None else h, w, mean, rstd)
+        ctx.meta = (wcode, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, w, mean, rstd = ctx.saved_tensors
+        wcode, wdt, bdt = ctx.meta
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        C = h.shape[-1]
+        n = h.numel() // C
+        if dy is None:  # nothing arrives at y: the stream's gradient goes through
+            def zero(dt):
+                return torch.zeros((C,), dtype=dt, device=h.device)
+            return dh, zero(wdt) if need_w else None, zero(bdt) if need_b else None, dh if need_r else None, None
+        dy = dy.contiguous()
+        dh = dh.contiguous() if dh is not None else None
+        dx = torch.empty_like(h) if (need_x or need_r) else None
+        wtype = torch.float32 if wcode == _lib.FEAT_DTYPES[torch.float32] else h.dtype
+        dw = torch.empty((C,), dtype=wtype, device=h.device) if need_w else None
+        db = torch.empty((C,), dtype=wtype, device=h.device) if need_b else None
+        ws, floats = None, 0
+        if need_w or need_b:
+            floats = _ln_workspace_floats(n, C, _lib.FEAT_DTYPES[h.dtype])
+            ws = torch.empty((floats,), dtype=torch.float32, device=h.device)
+        _lib.call("st_ln_backward", _lib.ptr(h), _lib.ptr(dy), _lib.ptr(dh), n, C, _lib.FEAT_DTYPES[h.dtype],
+                  _lib.ptr(w), wcode, _lib.ptr(mean), _lib.ptr(rstd), _lib.ptr(ws), floats, _lib.ptr(dx),
+                  _lib.ptr(dw), _lib.ptr(db), _lib.stream_of(h.device))
+        if dw is not None and dw.dtype != wdt:
+            dw = dw.to(wdt)
+        if db is not None and db.dtype != bdt:
+            db = db.to(bdt)
+        return dx if need_x else None, dw, db, dx if need_r else None, None
+
+
+def sparse_layer_norm(
+    input: Union[SparseTensor, torch.Tensor],
+    weight: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    eps: float = 1e-5,
+    residual: Optional[Union[SparseTensor, torch.Tensor]] = None,
+) -> Union[SparseTensor, torch.Tensor, Tuple]:
+    """Layer norm of each row over its channels: ``norm(x) * weight + bias``.
+
+    With ``residual`` (same shape and dtype), the pre-norm block's add runs in the same pass and
+    the result is ``(norm(h), h)`` with ``h = x + residual``, the stream that goes on.  ``input``
+    (and ``residual``) are a ``SparseTensor`` or a tensor (..., C) of float32, float16 or bfloat16;
+    the results are of the same kind.  Statistics and products are fp32; the gradients of
+    ``weight`` and ``bias`` are added in a fixed order.
+    """
+    x = input.F if isinstance(input, SparseTensor) else input
+    res = residual.F if isinstance(residual, SparseTensor) else residual
+    _lib.require_device(x, "layer norm input")
+    _lib.feat_code(x.dtype)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"layer norm needs at least one channel (got shape {tuple(x.shape)})")
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (t.shape != x.shape[-1:] or t.device != x.device):
+            raise ValueError(f"layer norm {what} must be ({x.shape[-1]},) on {x.device} "
+                             f"(got {tuple(t.shape)} on {t.device})")
+        if t is not None:
+            _lib.feat_code(t.dtype)
+    if res is not None and (res.shape != x.shape or res.dtype != x.dtype or res.device != x.device):
+        raise ValueError("the residual must match the input's shape, dtype and device")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, res)):
+        out = _LayerNorm.apply(x, weight, bias, res, float(eps))
+        y, h = out if res is not None else (out, None)
+    else:
+        y, h = _ln_forward(x, weight, bias, res, float(eps), False)[:2]
+    if isinstance(input, SparseTensor):
+        y, h = input.replace(y), (input.replace(h) if h is not None else None)
+    return y if h is None else (y, h)
