@@ -867,6 +867,67 @@ typedef struct st_rotary_args {
 } st_rotary_args;
 int st_rotary(const st_rotary_args* args, st_stream_t stream);
 
+/* ------------------------------------------------------------ attention
+ *
+ * Attention over segments of packed rows (no counterpart in the reference):
+ * in each segment, with c = scale,
+ *   O = softmax(c Q K^T) V over the keys that a row may see, zeros if there are none
+ * and its gradients, the probabilities recomputed from lse.  q, o, dout, dq:
+ * (rows, heads, dim); k, v, dk, dv: (rows, kv_heads, dim); query head h reads
+ * key head h / (heads / kv_heads), whose gradients are summed over its query
+ * heads.  q, k, v and dout lie at the given row and head strides (elements; 16-byte
+ * multiples), o, dq, dk, dv are contiguous.  dim: a multiple of 8, at most
+ * ST_ATTN_MAX_DIM.  dtype: ST_F32, ST_F16, ST_BF16.  scale > 0.
+ * key_mask (key rows; NULL = all): 0 leaves a key out, whatever its row of K and
+ * V holds; its gradients are zero.  causal: the segment's query i of nq sees keys
+ * up to i + nk - nq.
+ *
+ * The caller lays the work out (int32, device memory).  Packed row r of a
+ * segment is its query r / g at head r % g of the key head's group, g = heads /
+ * kv_heads.  q_items: ST_ATTN_ITEM_WORDS each, {first query row, queries, first
+ * key row, keys, first packed row of the tile (of ST_ATTN_TILE), first key, end
+ * of the keys to go over, part}: every tile with a row, once with part -1 and all
+ * keys that any of its rows sees, or in parts, in ascending slots of its own;
+ * then q_joins: ST_ATTN_JOIN_WORDS each, {the first five words, first slot,
+ * parts, 0} for every tile in parts.  k_items, k_joins likewise with tiles of
+ * keys and ranges of packed rows (every row that sees a key of the tile).
+ * parts: fp32 workspace, 16-byte address, st_attn_workspace floats for the
+ * slots used.  lse (rows, heads) fp32, base-2 logarithm, INFINITY for a row
+ * without keys: written when not NULL, needed by the backward; delta (rows,
+ * heads) fp32: scratch of the backward.  n_k_items = 0 leaves dK and dV out.
+ * All sums are in a fixed order.
+ */
+#define ST_ATTN_TILE 128
+#define ST_ATTN_KEYS 64
+#define ST_ATTN_MAX_DIM 128
+#define ST_ATTN_ITEM_WORDS 8
+#define ST_ATTN_JOIN_WORDS 8
+typedef struct st_attn_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* delta;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, dout_row, dout_head;
+  const uint8_t* key_mask;
+  const int32_t* q_items;
+  const int32_t* q_joins;
+  const int32_t* k_items;
+  const int32_t* k_joins;
+  int64_t n_q_items, n_q_joins, n_k_items, n_k_joins;
+  float* parts;
+  int32_t heads, kv_heads, dim, dtype, causal;
+  float scale;
+} st_attn_args;
+int st_attn_workspace(int kv_heads, int dim, int64_t q_parts, int64_t k_parts, int64_t* floats);
+int st_attn_forward(const st_attn_args* args, st_stream_t stream);
+int st_attn_backward(const st_attn_args* args, st_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,6 +33,7 @@ GATHER_B_KN = 2
 COLUMN_SUM_NOALLOC_MAX_C = 2048
 MAX_KVOL = 512
 TILE_ROWS = 128
+ATTN_TILE, ATTN_KEYS, ATTN_MAX_DIM, ATTN_WORDS = 128, 64, 128, 8
 
 
 class OutGeom(ctypes.Structure):
@@ -69,6 +70,19 @@ class RotaryArgs(ctypes.Structure):
         + [("positions", _P), ("pos_row", _L), ("turns", _P), ("axis", _P), ("n", _L)]
         + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "pairs", "dtype", "pos_dtype", "interleaved",
                                          "inverse")]
+    )
+
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = (
+        [(n, _P) for n in ("q", "k", "v", "o", "lse", "dout", "dq", "dk", "dv", "delta")]
+        + [(n, _L) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "dout_row", "dout_head")]
+        + [(n, _P) for n in ("key_mask", "q_items", "q_joins", "k_items", "k_joins")]
+        + [(n, _L) for n in ("n_q_items", "n_q_joins", "n_k_items", "n_k_joins")]
+        + [("parts", _P)]
+        + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "dtype", "causal")]
+        + [("scale", ctypes.c_float)]
     )
 
 
@@ -139,6 +153,9 @@ _SIGNATURES = {
     "st_ln_forward": [_P, _P, _L, _I, _I, _P, _P, _I, ctypes.c_float, _P, _P, _P, _P, _P],
     "st_ln_backward_workspace": [_L, _I, _I, ctypes.POINTER(_L)],
     "st_ln_backward": [_P, _P, _P, _L, _I, _I, _P, _I, _P, _P, _P, _L, _P, _P, _P, _P],
+    "st_attn_workspace": [_I, _I, _L, _L, ctypes.POINTER(_L)],
+    "st_attn_forward": [ctypes.POINTER(AttnArgs), _P],
+    "st_attn_backward": [ctypes.POINTER(AttnArgs), _P],
     "st_rotary": [ctypes.POINTER(RotaryArgs), _P],
     "st_hashfly_wgrad": [_P, _L, _P, _P, _I, _L, _P, ctypes.POINTER(Lookup), _P, _P, _L, _I, _I, _I, _P, _L, _P,
                          _I, _P],

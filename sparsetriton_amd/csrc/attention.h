@@ -1,0 +1,838 @@
+// Attention over segments of packed rows: kernels (see attention.hip for the
+// host side).  For a segment with queries Q, keys K, values V and the scale c:
+//   S = c Q K^T,   P = softmax over the keys that the row may see,   O = P V
+// and, from dO and the saved L = log sum exp S,
+//   P = exp(S - L),  delta = rowsum(dO o O),  dP = dO V^T,  dS = P o (dP - delta),
+//   dQ = c dS K,   dK = c dS^T Q,   dV = P^T dO.
+// A row that sees no key has O = 0 and no gradient.
+//
+// Query heads that share a key head are rows of one matrix: "packed row" r of a
+// segment is query r / R, head hk R + r % R for R = heads / kv_heads.  One
+// pass over a key head's K and V serves its whole group, dK and dV are summed
+// over the group where they are made, and a single query row still fills R
+// rows of the matrix product.
+//
+// Every product is a 32 x 32 MFMA tile, laid out so that no operand goes back
+// through memory: the products whose result the next product reduces over are
+// computed transposed (S^T = K Q^T: lane = query, registers = keys), so that a
+// lane's registers are already its B operand of the next one (O^T += V^T P^T).  The
+// reduction index of an MFMA may be permuted if both operands agree: register
+// r of half h of the wave is key 8 (r / 4) + 4 h + r % 4, and the other operand
+// (V^T, K^T, Q^T, dO^T) is read from LDS in that order -- by transpose reads
+// (ds_read_b64_tr_b16) for 16-bit types.  Row sums and maxima of P are sums over a
+// lane's own registers and one exchange between the halves.
+//
+// fp32 tensors use the fp32 MFMA (32 x 32 x 2), eight of them in the place of a
+// 32 x 32 x 16, in the same layout: nothing is rounded below 32 bits.  16-bit
+// types round P and dS to the type for the second product (their sums, the
+// softmax statistics and all accumulators are fp32).
+#pragma once
+
+#include "common.h"
+#include "mfma.h"
+#include "wave_sum.h"
+
+namespace st {
+
+typedef float v8f __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+
+constexpr int kAttnThreads = 256;
+constexpr int kAttnTile = ST_ATTN_TILE;  // rows (or keys) of a workgroup: 32 for each of four waves
+
+struct AttnItem {  // ST_ATTN_ITEM_WORDS int32, written by the host
+  int q0, nq;      // the segment's first query row and their number
+  int k0, nk;      // its first key row and their number
+  int row0;        // first packed row (first key) of this tile in the segment
+  int lo, hi;      // keys (packed rows) to go over
+  int part;        // slot of the partial result, -1: the result itself
+};
+struct AttnJoin {  // ST_ATTN_JOIN_WORDS int32
+  int q0, nq, k0, nk, row0;
+  int part, parts;  // first slot and number of the partial results
+  int unused;
+};
+
+struct AttnArgs {
+  const void *q, *k, *v, *o, *dout;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta, *parts;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
+  const uint8_t* key_mask;
+  const AttnItem* items;
+  const AttnJoin* joins;
+  int n_items, n_joins;
+  int heads, kv_heads, group, D, causal;
+  float scale, scale_log2;  // c and c / ln 2
+};
+
+// ------------------------------------------------------------------ MFMA
+
+template <typename T>
+struct AttnFrag;  // eight reduction elements of a lane
+template <>
+struct AttnFrag<__bf16> {
+  using type = v8bf;
+};
+template <>
+struct AttnFrag<_Float16> {
+  using type = v8h;
+};
+template <>
+struct AttnFrag<float> {
+  using type = v8f;
+};
+
+__device__ __forceinline__ v16f mma32(const v8bf& a, const v8bf& b, const v16f& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mma32(const v8h& a, const v8h& b, const v16f& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mma32(const v8f& a, const v8f& b, v16f c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+template <typename T>
+__device__ __forceinline__ typename AttnFrag<T>::type to_frag(const v8f& x) {
+  if constexpr (sizeof(T) == 4)
+    return x;
+  else
+    return __builtin_convertvector(x, typename AttnFrag<T>::type);
+}
+__device__ __forceinline__ v8f regs8(const v16f& c, int j) {  // registers 8j .. 8j + 7 (j a constant)
+  return j == 0 ? __builtin_shufflevector(c, c, 0, 1, 2, 3, 4, 5, 6, 7)
+                : __builtin_shufflevector(c, c, 8, 9, 10, 11, 12, 13, 14, 15);
+}
+// Row (key) of register r in half `half`
+__device__ __forceinline__ int reg_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+// ------------------------------------------------------------------ LDS tiles
+
+// A tile of rows of DP elements, 16-byte chunks permuted within a row by an
+// XOR with a few bits of the row, so that both kinds of reads meet 16
+// different 16-byte bank groups: 16 consecutive rows at one chunk (row
+// fragments), and four consecutive rows at four aligned chunks (transpose
+// reads).  Which bits depends on how many rows share 256 bytes.
+template <typename T, int DP>
+struct AttnTile {
+  static constexpr int EPC = 16 / sizeof(T);  // elements of a chunk
+  static constexpr int CPR = DP / EPC;        // chunks of a row
+  using Frag = typename AttnFrag<T>::type;
+
+  static __device__ __forceinline__ int swz(int row) {
+    if constexpr (CPR == 4 || CPR == 12)
+      return (row >> 2) & 3;
+    else if constexpr (CPR == 8 || CPR == 24)
+      return ((row >> 1) & 1) * 4 + ((row >> 2) & 3);
+    else
+      return (row & 3) * 4 + ((row >> 2) & 3);
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * DP + (chunk ^ swz(row)) * EPC; }
+
+  // Elements col .. col + 7 (col a multiple of 8) of a row.
+  static __device__ __forceinline__ Frag rows(const T* tile, int row, int col) {
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const Frag*>(tile + at(row, col / EPC));
+    } else {
+      const v4f a = *reinterpret_cast<const v4f*>(tile + at(row, col / EPC));
+      const v4f b = *reinterpret_cast<const v4f*>(tile + at(row, col / EPC + 1));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  // Column d0 + lane % 32 of rows row0 + {4 half .. 4 half + 3, 8 + 4 half .. 8 + 4 half + 3}
+  // (row0 a multiple of 16, d0 of 32).  16-bit: two transpose reads; in a group of
+  // 16 lanes, lane l addresses row l / 4 at columns 4 (l % 4) and receives
+  // column l of the four rows.
+  static __device__ __forceinline__ Frag cols(const T* tile, int row0, int d0) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      typedef short v4s __attribute__((ext_vector_type(4)));
+      typedef short v8s __attribute__((ext_vector_type(8)));
+      using lds_v4s = __attribute__((address_space(3))) v4s;
+      const int row = row0 + 4 * half + ((lane >> 2) & 3);
+      const int chunk = d0 / 8 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), in = (lane & 1) * 4;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(tile + at(row, chunk) + in));
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(tile + at(row + 8, chunk) + in));
+      const v8s both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(Frag, both);
+    } else {
+      const int d = d0 + (lane & 31);
+      Frag f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int row = row0 + 4 * half + (e & 3) + 8 * (e >> 2);
+        f[e] = tile[at(row, d / 4) + d % 4];
+      }
+      return f;
+    }
+  }
+};
+
+// acc += A B where some of the 16 reduction indexes must not reach some columns:
+// bit i of `allowed` says whether index i (16-bit layout order: row0 + i of
+// AttnTile::cols) may reach this lane's column.  B is already zero there, but
+// zero times an infinity or a NaN in A is a NaN: on a tile that the causal order
+// cuts, a later row that is not finite would reach earlier ones.  Such
+// elements (none, as a rule: one check) are added on their own, index by index.
+template <typename T>
+__device__ __forceinline__ v16f mma32_guarded(typename AttnFrag<T>::type a, const typename AttnFrag<T>::type& b,
+                                              v16f acc, unsigned allowed) {
+  using Frag = typename AttnFrag<T>::type;
+  Frag bad = a;
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool finite = fabsf((float)a[e]) < INFINITY;
+    any |= !finite;
+    bad[e] = finite ? (T)0.f : a[e];
+    a[e] = finite ? a[e] : (T)0.f;
+  }
+  acc = mma32(a, b, acc);
+  if (!__any(any)) return acc;
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    for (int h = 0; h < 2; ++h) {
+      Frag one;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) one[k] = k == e && half == h ? bad[k] : (T)0.f;
+      const v16f next = mma32(one, b, acc);
+      const bool take = allowed >> (8 * (e >> 2) + 4 * h + (e & 3)) & 1;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) acc[k] = take ? next[k] : acc[k];
+    }
+  }
+  return acc;
+}
+
+// Rows of a tile on their way from memory to LDS: each thread carries N chunks.
+template <typename T, int DP, int ROWS>
+struct AttnStage {
+  using Tile = AttnTile<T, DP>;
+  static constexpr int N = ROWS * Tile::CPR / kAttnThreads;
+  static_assert(ROWS * Tile::CPR % kAttnThreads == 0, "whole chunks a thread");
+  v4u reg[N];
+
+  static __device__ __forceinline__ int row(int i) { return (threadIdx.x + i * kAttnThreads) / Tile::CPR; }
+  static __device__ __forceinline__ int chunk(int i) { return (threadIdx.x + i * kAttnThreads) % Tile::CPR; }
+  // `offset(row)`: byte offset of a row from `base`, or kOobOffset for a row of zeros
+  template <typename F>
+  __device__ __forceinline__ void load(const T* base, int D, F offset) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base, kOobOffset);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = chunk(i) * Tile::EPC, off = offset(row(i));
+      reg[i] = load16<v4u>(r, (c < D && off != kOobOffset) ? off + c * (int)sizeof(T) : kOobOffset);
+    }
+  }
+  __device__ __forceinline__ void store(T* tile) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<v4u*>(tile + Tile::at(row(i), chunk(i))) = reg[i];
+  }
+};
+
+// Eight elements of a row in global memory (16-byte aligned), zeros past D or for a dead row.
+template <typename T>
+__device__ __forceinline__ typename AttnFrag<T>::type load_row8(const T* row, int col, int D, bool live) {
+  typename AttnFrag<T>::type f;
+  if (live && col < D) return *reinterpret_cast<const typename AttnFrag<T>::type*>(row + col);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = (T)0.f;
+  return f;
+}
+
+// Stores a lane's row from accumulators that hold it transposed (registers =
+// channels): 16-bit halves exchange quads so that each lane stores whole chunks.
+template <typename T, int DB>
+__device__ __forceinline__ void store_row(T* row, const v16f (&acc)[DB], float scale, int D, bool live) {
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int b = 0; b < DB; ++b) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = b * 32 + 8 * j + 4 * half;
+        const v4f x = {acc[b][4 * j] * scale, acc[b][4 * j + 1] * scale, acc[b][4 * j + 2] * scale,
+                       acc[b][4 * j + 3] * scale};
+        if (live && d < D) *reinterpret_cast<v4f*>(row + d) = x;
+      }
+    } else {
+      typedef T v2t __attribute__((ext_vector_type(2)));
+      auto pack = [&](int r) {
+        const v2f x = {acc[b][r] * scale, acc[b][r + 1] * scale};
+        return __builtin_bit_cast(unsigned, __builtin_convertvector(x, v2t));
+      };
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const auto x = __builtin_amdgcn_permlane32_swap(pack(4 * j), pack(4 * j + 4), false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(pack(4 * j + 2), pack(4 * j + 6), false, false);
+        const int d = b * 32 + 8 * (j + half);
+        const v4u w = {x[0], y[0], x[1], y[1]};
+        if (live && d < D) *reinterpret_cast<v4u*>(row + d) = w;
+      }
+    }
+  }
+}
+// The same as fp32 partial sums at a row of DP floats.
+template <int DB>
+__device__ __forceinline__ void store_part(float* row, const v16f (&acc)[DB]) {
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<v4f*>(row + b * 32 + 8 * j + 4 * half) =
+          (v4f){acc[b][4 * j], acc[b][4 * j + 1], acc[b][4 * j + 2], acc[b][4 * j + 3]};
+}
+
+// Work item of a workgroup.  The hardware deals workgroups to the 8 XCDs
+// round-robin; runs of 16 consecutive items (tiles of one segment and key
+// head, which read the same rows) go to one XCD and its L2.
+__device__ __forceinline__ int attn_work(int n) {
+  const int id = blockIdx.x, base = id & ~127;
+  return base + 128 > n ? id : base + (id & 7) * 16 + ((id & 127) >> 3);
+}
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ------------------------------------------------------------------ forward
+
+constexpr int kAttnKeys = ST_ATTN_KEYS;  // keys of a step
+
+template <typename T, int DP>
+constexpr int attn_fwd_lds() {
+  return 2 * 2 * kAttnKeys * DP * (int)sizeof(T);
+}
+
+// A running maximum is raised only when a row's maximum passes it by more
+// than this (in powers of two): below, exp2(S - m) <= 2^8 loses nothing in
+// floating point, and the accumulators need no rescaling.
+constexpr float kAttnSlack = 8.f;
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kAttnThreads) void attn_forward_kernel(AttnArgs a) {
+  using Tile = AttnTile<T, DP>;
+  using Frag = typename Tile::Frag;
+  using Stage = AttnStage<T, DP, kAttnKeys>;
+  constexpr int KS = DP / 16, DB = DP / 32, NB = kAttnKeys / 32;
+  constexpr int TILE = kAttnKeys * DP;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* tiles = reinterpret_cast<T*>(lds);
+
+  const int w = attn_work(gridDim.x), hk = w / a.n_items;
+  const AttnItem it = a.items[w - hk * a.n_items];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int rows = it.nq * a.group, r = it.row0 + wave * 32 + (lane & 31);
+  const bool active = it.row0 + wave * 32 < rows, live = r < rows;
+  const int qi = r / a.group, head = hk * a.group + (r - qi * a.group);
+
+  Frag qf[KS];
+  {
+    const T* row = (const T*)a.q + (it.q0 + (int64_t)qi) * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = load_row8<T>(row, 16 * s + 8 * half, a.D, live);
+  }
+  const int see = a.causal ? qi + it.nk - it.nq : 0x7FFFFFFF;  // last key that this lane's row sees
+
+  Stage ks, vs;
+  uint8_t chunk_kept[Stage::N], key_kept = 1;
+  const uint8_t* mask = a.key_mask ? a.key_mask + it.k0 : nullptr;
+  auto fetch = [&](int kt) {
+    const int left = it.hi - kt;
+    const int64_t row = it.k0 + (int64_t)kt;
+    const int krow = (int)(a.k_row * sizeof(T)), vrow = (int)(a.v_row * sizeof(T));
+    if (mask) {
+#pragma unroll
+      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[kt + Stage::row(i)] : 0;
+      key_kept = lane < left ? mask[kt + lane] : 0;
+    }
+    ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, a.D, [&](int x) { return x < left ? x * krow : kOobOffset; });
+    vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, a.D, [&](int x) { return x < left ? x * vrow : kOobOffset; });
+  };
+
+  v16f o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b) o[b] = (v16f)(0.f);
+  float m = -INFINITY, l = 0.f;
+  if (it.lo < it.hi) fetch(it.lo);
+  for (int kt = it.lo, buf = 0; kt < it.hi; kt += kAttnKeys, buf ^= 1) {
+    T* kl = tiles + buf * 2 * TILE;
+    T* vl = kl + TILE;
+    uint64_t seen = ~0ull;  // keys of this step that exist and are not masked
+    if (it.hi - kt < kAttnKeys) seen >>= kAttnKeys - (it.hi - kt);
+    if (mask) {
+      seen &= __ballot(key_kept);
+#pragma unroll
+      for (int i = 0; i < Stage::N; ++i)  // (whatever a masked row holds, not finite included, stays out of the products)
+        if (!chunk_kept[i]) ks.reg[i] = vs.reg[i] = (v4u)(0u);
+    }
+    ks.store(kl);
+    vs.store(vl);
+    __syncthreads();
+    if (kt + kAttnKeys < it.hi) fetch(kt + kAttnKeys);
+    if (!active || !__any(live && kt <= see)) continue;
+
+    v16f s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      s[b] = (v16f)(0.f);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) s[b] = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s[b]);
+    }
+    const bool cut = __any(see - kt < kAttnKeys - 1);  // by the causal order
+    const int last = see - kt;
+    const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
+    if (cut || seen != ~0ull) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[b][e] = (bits >> reg_row(e, 0)) & 1 ? s[b][e] : -INFINITY;
+      }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[b][e]);
+    top = fmaxf(top, other_half(top)) * a.scale_log2;
+    const bool raise = top > m + kAttnSlack;
+    if (__any(raise)) {  // (each row by its own maximum alone: its bits do not depend on the rows beside it)
+      const float shrink = raise ? fast_exp2(m - top) : 1.f;
+      m = raise ? top : m;
+      l *= shrink;
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[b][e] *= shrink;
+    }
+    const float base = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[b][e] = fast_exp2(fmaf(s[b][e], a.scale_log2, base));
+        l += s[b][e];
+      }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const Frag p = to_frag<T>(regs8(s[b], j));
+        if (!cut) {
+#pragma unroll
+          for (int d = 0; d < DB; ++d) o[d] = mma32(Tile::cols(vl, b * 32 + 16 * j, d * 32), p, o[d]);
+        } else {
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+            o[d] = mma32_guarded<T>(Tile::cols(vl, b * 32 + 16 * j, d * 32), p, o[d], (unsigned)(keep >> (32 * b + 16 * j)));
+        }
+      }
+  }
+
+  l += other_half(l);
+  if (it.part >= 0) {
+    // a row of DP sums, then its maximum (in powers of two) and sum
+    float* row = a.parts + (((int64_t)it.part * a.kv_heads + hk) * kAttnTile + wave * 32 + (lane & 31)) * (DP + 4);
+    store_part<DB>(row, o);
+    if (half == 0) {
+      row[DP] = m;
+      row[DP + 1] = l;
+    }
+    return;
+  }
+  if (!active) return;
+  const int64_t q = it.q0 + (int64_t)qi;
+  store_row<T, DB>((T*)a.out + (q * a.heads + head) * a.D, o, l > 0.f ? 1.f / l : l, a.D, live);
+  if (a.lse && live && half == 0) a.lse[q * a.heads + head] = l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l;
+}
+
+// Partial results of split rows into the result: weights 2^(m_i - max), a thread for each four channels of a row.
+template <typename T, int DP>
+__global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArgs a) {
+  const AttnJoin jn = a.joins[blockIdx.x / a.kv_heads];
+  const int hk = blockIdx.x % a.kv_heads;
+  const int rows = min(kAttnTile, jn.nq * a.group - jn.row0);
+  const int64_t step = (int64_t)a.kv_heads * kAttnTile * (DP + 4);
+  for (int i = threadIdx.x; i < rows * (DP / 4); i += kAttnThreads) {
+    const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+    const float* p = a.parts + (((int64_t)jn.part * a.kv_heads + hk) * kAttnTile + row) * (DP + 4);
+    float m = -INFINITY;
+    for (int k = 0; k < jn.parts; ++k) m = fmaxf(m, p[k * step + DP]);
+    v4f sum = (v4f)(0.f);
+    float l = 0.f;
+    for (int k = 0; k < jn.parts; ++k) {
+      const float mk = p[k * step + DP], lk = p[k * step + DP + 1];
+      const float w = mk == -INFINITY ? (lk == 0.f ? 0.f : 1.f) : fast_exp2(mk - m);
+      l += w * lk;
+      sum += w * *reinterpret_cast<const v4f*>(p + k * step + d);
+    }
+    const int r = jn.row0 + row, qi = r / a.group, head = hk * a.group + (r - qi * a.group);
+    const int64_t at = (jn.q0 + (int64_t)qi) * a.heads + head;
+    const float inv = l > 0.f ? 1.f / l : l;
+    if (d < a.D) {
+      typedef T v4t __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<v4t*>((T*)a.out + at * a.D + d) = __builtin_convertvector(sum * inv, v4t);
+    }
+    if (a.lse && d == 0) a.lse[at] = l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l;
+  }
+}
+
+// ------------------------------------------------------------------ backward: queries
+
+// dQ of a tile of rows, and delta = rowsum(dO o O) for the keys' pass after it.
+template <typename T, int DP>
+__global__ __launch_bounds__(kAttnThreads) void attn_dq_kernel(AttnArgs a) {
+  using Tile = AttnTile<T, DP>;
+  using Frag = typename Tile::Frag;
+  using Stage = AttnStage<T, DP, kAttnKeys>;
+  constexpr int KS = DP / 16, DB = DP / 32, NB = kAttnKeys / 32;
+  constexpr int TILE = kAttnKeys * DP;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* tiles = reinterpret_cast<T*>(lds);
+
+  const int w = attn_work(gridDim.x), hk = w / a.n_items;
+  const AttnItem it = a.items[w - hk * a.n_items];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int rows = it.nq * a.group, r = it.row0 + wave * 32 + (lane & 31);
+  const bool active = it.row0 + wave * 32 < rows, live = r < rows;
+  const int qi = r / a.group, head = hk * a.group + (r - qi * a.group);
+  const int64_t q = it.q0 + (int64_t)qi, at = q * a.heads + head;
+
+  Frag qf[KS], gf[KS];
+  float lse = INFINITY, delta = 0.f;
+  {
+    const T* qrow = (const T*)a.q + q * a.q_row + head * a.q_head;
+    const T* grow = (const T*)a.dout + q * a.do_row + head * a.do_head;
+    const T* orow = (const T*)a.o + at * a.D;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qf[s] = load_row8<T>(qrow, 16 * s + 8 * half, a.D, live);
+      gf[s] = load_row8<T>(grow, 16 * s + 8 * half, a.D, live);
+      const Frag of = load_row8<T>(orow, 16 * s + 8 * half, a.D, live);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)of[e], delta);
+    }
+    delta += other_half(delta);
+    if (live) {
+      lse = a.lse[at];
+      if (half == 0) a.delta[at] = delta;
+    }
+  }
+  const int see = a.causal ? qi + it.nk - it.nq : 0x7FFFFFFF;
+
+  Stage ks, vs;
+  uint8_t chunk_kept[Stage::N], key_kept = 1;
+  const uint8_t* mask = a.key_mask ? a.key_mask + it.k0 : nullptr;
+  auto fetch = [&](int kt) {
+    const int left = it.hi - kt;
+    const int64_t row = it.k0 + (int64_t)kt;
+    const int krow = (int)(a.k_row * sizeof(T)), vrow = (int)(a.v_row * sizeof(T));
+    if (mask) {
+#pragma unroll
+      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[kt + Stage::row(i)] : 0;
+      key_kept = lane < left ? mask[kt + lane] : 0;
+    }
+    ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, a.D, [&](int x) { return x < left ? x * krow : kOobOffset; });
+    vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, a.D, [&](int x) { return x < left ? x * vrow : kOobOffset; });
+  };
+
+  v16f dq[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b) dq[b] = (v16f)(0.f);
+  if (it.lo < it.hi) fetch(it.lo);
+  for (int kt = it.lo, buf = 0; kt < it.hi; kt += kAttnKeys, buf ^= 1) {
+    T* kl = tiles + buf * 2 * TILE;
+    T* vl = kl + TILE;
+    uint64_t seen = ~0ull;
+    if (it.hi - kt < kAttnKeys) seen >>= kAttnKeys - (it.hi - kt);
+    if (mask) {
+      seen &= __ballot(key_kept);
+#pragma unroll
+      for (int i = 0; i < Stage::N; ++i)
+        if (!chunk_kept[i]) ks.reg[i] = vs.reg[i] = (v4u)(0u);
+    }
+    ks.store(kl);
+    vs.store(vl);
+    __syncthreads();
+    if (kt + kAttnKeys < it.hi) fetch(kt + kAttnKeys);
+    if (!active || !__any(live && kt <= see)) continue;
+    const bool cut = __any(see - kt < kAttnKeys - 1);
+    const int last = see - kt;
+    const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      v16f s = (v16f)(0.f), dp = (v16f)(0.f);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        s = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s);
+        dp = mma32(Tile::rows(vl, b * 32 + (lane & 31), 16 * i + 8 * half), gf[i], dp);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], a.scale_log2, -lse)) * (dp[e] - delta);
+      if (cut || seen != ~0ull) {
+        const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = (bits >> reg_row(e, 0)) & 1 ? s[e] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const Frag ds = to_frag<T>(regs8(s, j));
+        if (!cut) {
+#pragma unroll
+          for (int d = 0; d < DB; ++d) dq[d] = mma32(Tile::cols(kl, b * 32 + 16 * j, d * 32), ds, dq[d]);
+        } else {
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+            dq[d] = mma32_guarded<T>(Tile::cols(kl, b * 32 + 16 * j, d * 32), ds, dq[d], (unsigned)(keep >> (32 * b + 16 * j)));
+        }
+      }
+    }
+  }
+
+  if (it.part >= 0) {
+    store_part<DB>(
+        a.parts + (((int64_t)it.part * a.kv_heads + hk) * kAttnTile + wave * 32 + (lane & 31)) * DP, dq);
+    return;
+  }
+  if (!active) return;
+  store_row<T, DB>((T*)a.dq + at * a.D, dq, a.scale, a.D, live);
+}
+
+// ------------------------------------------------------------------ backward: keys
+
+template <typename T, int DP>
+constexpr int attn_q_rows() {  // packed rows of a step
+  return DP * (int)sizeof(T) <= 192 ? 64 : 32;
+}
+template <typename T, int DP>
+constexpr int attn_dkv_lds() {
+  return 2 * (2 * attn_q_rows<T, DP>() * DP * (int)sizeof(T) + 2 * attn_q_rows<T, DP>() * 4);
+}
+
+// dK and dV of a tile of keys: the waves hold 32 keys each (K, V and both sums in
+// registers) while the packed rows' Q, dO, L and delta go by through LDS.
+template <typename T, int DP>
+__global__ __launch_bounds__(kAttnThreads) void attn_dkv_kernel(AttnArgs a) {
+  using Tile = AttnTile<T, DP>;
+  using Frag = typename Tile::Frag;
+  constexpr int BQ = attn_q_rows<T, DP>();
+  using Stage = AttnStage<T, DP, BQ>;
+  constexpr int KS = DP / 16, DB = DP / 32, NB = BQ / 32;
+  constexpr int TILE = BQ * DP;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* tiles = reinterpret_cast<T*>(lds);
+  float* stats = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers of BQ L, BQ delta
+
+  const int w = attn_work(gridDim.x), hk = w / a.n_items;
+  const AttnItem it = a.items[w - hk * a.n_items];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int kw = it.row0 + wave * 32, key = kw + (lane & 31);  // in the segment
+  const bool active = kw < it.nk, live = key < it.nk;
+  const int64_t krow = it.k0 + (int64_t)key;
+  const bool kept = live && (!a.key_mask || a.key_mask[krow]);
+
+  Frag kf[KS], vf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    kf[s] = load_row8<T>((const T*)a.k + krow * a.k_row + hk * a.k_head, 16 * s + 8 * half, a.D, kept);
+    vf[s] = load_row8<T>((const T*)a.v + krow * a.v_row + hk * a.v_head, 16 * s + 8 * half, a.D, kept);
+  }
+  // first packed row that sees this lane's key, and the first that sees any of the wave's
+  const int from = a.causal ? (key - (it.nk - it.nq)) * a.group : 0;
+  const int wave_from = a.causal ? (kw - (it.nk - it.nq)) * a.group : 0;
+
+  Stage qs, gs;
+  float stat = 0.f;
+  const int qrow = (int)(a.q_row * sizeof(T)), qhead = (int)(a.q_head * sizeof(T));
+  const int grow = (int)(a.do_row * sizeof(T)), ghead = (int)(a.do_head * sizeof(T));
+  const unsigned inv = (unsigned)(((1ull << 32) + a.group - 1) / a.group);  // x / group = x * inv >> 32 (group > 1)
+  auto fetch = [&](int rt) {
+    const int left = it.hi - rt, q0 = rt / a.group, h0 = rt - q0 * a.group;
+    const int64_t q = it.q0 + (int64_t)q0;
+    auto split = [&](int x, int& dq, int& dh) {
+      dq = a.group > 1 ? (int)__umulhi((unsigned)(h0 + x), inv) : x;
+      dh = h0 + x - dq * a.group;
+    };
+    auto offset = [&](int x, int row, int head) {
+      int dq, dh;
+      split(x, dq, dh);
+      return x < left ? dq * row + dh * head : kOobOffset;
+    };
+    qs.load((const T*)a.q + q * a.q_row + (int64_t)hk * a.group * a.q_head, a.D, [&](int x) { return offset(x, qrow, qhead); });
+    gs.load((const T*)a.dout + q * a.do_row + (int64_t)hk * a.group * a.do_head, a.D,
+            [&](int x) { return offset(x, grow, ghead); });
+    if (threadIdx.x < 2 * BQ) {
+      const int x = threadIdx.x & (BQ - 1);
+      int dq, dh;
+      split(x, dq, dh);
+      const int64_t at = (q + dq) * a.heads + hk * a.group + dh;
+      // (a row past the end: L = inf makes its P zero)
+      stat = threadIdx.x < BQ ? (x < left ? a.lse[at] : INFINITY) : (x < left ? a.delta[at] : 0.f);
+    }
+  };
+
+  v16f dk[DB], dv[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b) dk[b] = dv[b] = (v16f)(0.f);
+  if (it.lo < it.hi) fetch(it.lo);
+  for (int rt = it.lo, buf = 0; rt < it.hi; rt += BQ, buf ^= 1) {
+    T* ql = tiles + buf * 2 * TILE;
+    T* gl = ql + TILE;
+    float* st = stats + buf * 2 * BQ;
+    qs.store(ql);
+    gs.store(gl);
+    if (threadIdx.x < 2 * BQ) st[threadIdx.x] = stat;
+    __syncthreads();
+    if (rt + BQ < it.hi) fetch(rt + BQ);
+    if (!active || rt + BQ <= wave_from) continue;
+    const bool cut = a.causal && __any(from > rt);
+    auto allowed = [&](int row) {  // of 16 rows from `row` on, those that see this lane's key
+      const int n = from - row;
+      return n <= 0 ? 0xFFFFu : n >= 16 ? 0u : 0xFFFFu << n;
+    };
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      v16f s = (v16f)(0.f), dp = (v16f)(0.f);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        s = mma32(Tile::rows(ql, b * 32 + (lane & 31), 16 * i + 8 * half), kf[i], s);
+        dp = mma32(Tile::rows(gl, b * 32 + (lane & 31), 16 * i + 8 * half), vf[i], dp);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const v4f L = *reinterpret_cast<const v4f*>(st + b * 32 + 8 * j + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * j + e] = fast_exp2(fmaf(s[4 * j + e], a.scale_log2, -L[e]));
+      }
+      if (cut) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = rt + b * 32 + reg_row(e, half) >= from ? s[e] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const Frag p = to_frag<T>(regs8(s, j));
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+          dv[d] = cut ? mma32_guarded<T>(Tile::cols(gl, b * 32 + 16 * j, d * 32), p, dv[d], allowed(rt + b * 32 + 16 * j))
+                      : mma32(Tile::cols(gl, b * 32 + 16 * j, d * 32), p, dv[d]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const v4f dl = *reinterpret_cast<const v4f*>(st + BQ + b * 32 + 8 * j + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * j + e] *= dp[4 * j + e] - dl[e];
+      }
+      if (cut) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = rt + b * 32 + reg_row(e, half) >= from ? s[e] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const Frag ds = to_frag<T>(regs8(s, j));
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+          dk[d] = cut ? mma32_guarded<T>(Tile::cols(ql, b * 32 + 16 * j, d * 32), ds, dk[d], allowed(rt + b * 32 + 16 * j))
+                      : mma32(Tile::cols(ql, b * 32 + 16 * j, d * 32), ds, dk[d]);
+      }
+    }
+  }
+
+  if (!kept) {  // a masked key gets no gradient
+#pragma unroll
+    for (int b = 0; b < DB; ++b) dk[b] = dv[b] = (v16f)(0.f);
+  }
+  if (it.part >= 0) {
+    float* row = a.parts + ((((int64_t)it.part * a.kv_heads + hk) * 2) * kAttnTile + wave * 32 + (lane & 31)) * DP;
+    store_part<DB>(row, dk);
+    store_part<DB>(row + kAttnTile * DP, dv);
+    return;
+  }
+  if (!active) return;
+  const int64_t at = (krow * a.kv_heads + hk) * a.D;
+  store_row<T, DB>((T*)a.dk + at, dk, a.scale, a.D, live);
+  store_row<T, DB>((T*)a.dv + at, dv, 1.f, a.D, live);
+}
+
+// Sums of the partial gradients of split tiles, slots in order: dQ (KEYS = false), or dK and dV.
+template <typename T, int DP, bool KEYS>
+__global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a) {
+  typedef T v4t __attribute__((ext_vector_type(4)));
+  const AttnJoin jn = a.joins[blockIdx.x / a.kv_heads];
+  const int hk = blockIdx.x % a.kv_heads;
+  const int rows = min(kAttnTile, (KEYS ? jn.nk : jn.nq * a.group) - jn.row0);
+  constexpr int W = KEYS ? 2 : 1;
+  const int64_t step = (int64_t)a.kv_heads * W * kAttnTile * DP;
+  for (int i = threadIdx.x; i < W * rows * (DP / 4); i += kAttnThreads) {
+    const int which = i / (rows * (DP / 4)), in = i - which * rows * (DP / 4);
+    const int row = in / (DP / 4), d = in % (DP / 4) * 4;
+    const float* p = a.parts + ((((int64_t)jn.part * a.kv_heads + hk) * W + which) * kAttnTile + row) * DP + d;
+    v4f sum = (v4f)(0.f);
+    for (int k = 0; k < jn.parts; ++k) sum += *reinterpret_cast<const v4f*>(p + k * step);
+    if (d >= a.D) continue;
+    const int r = jn.row0 + row;
+    if constexpr (KEYS) {
+      const int64_t at = ((jn.k0 + (int64_t)r) * a.kv_heads + hk) * a.D + d;
+      *reinterpret_cast<v4t*>((T*)(which ? a.dv : a.dk) + at) =
+          __builtin_convertvector(which ? sum : sum * a.scale, v4t);
+    } else {
+      const int qi = r / a.group, head = hk * a.group + (r - qi * a.group);
+      *reinterpret_cast<v4t*>((T*)a.dq + ((jn.q0 + (int64_t)qi) * a.heads + head) * a.D + d) =
+          __builtin_convertvector(sum * a.scale, v4t);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ launches
+
+template <typename K>
+static int attn_launch(K kernel, int64_t blocks, int lds, const AttnArgs& a, hipStream_t s) {
+  if (blocks == 0) return ST_OK;
+  kernel<<<dim3((unsigned)blocks), kAttnThreads, lds, s>>>(a);
+  ST_CHECK_LAUNCH();
+  return ST_OK;
+}
+
+template <typename T, int DP>
+static int attn_forward_dp(const AttnArgs& a, hipStream_t s) {
+  const int rc = attn_launch(attn_forward_kernel<T, DP>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(), a, s);
+  if (rc != ST_OK) return rc;
+  return attn_launch(attn_forward_join_kernel<T, DP>, (int64_t)a.n_joins * a.kv_heads, 0, a, s);
+}
+template <typename T, int DP>
+static int attn_dq_dp(const AttnArgs& a, hipStream_t s) {
+  const int rc = attn_launch(attn_dq_kernel<T, DP>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(), a, s);
+  if (rc != ST_OK) return rc;
+  return attn_launch(attn_sum_parts_kernel<T, DP, false>, (int64_t)a.n_joins * a.kv_heads, 0, a, s);
+}
+template <typename T, int DP>
+static int attn_dkv_dp(const AttnArgs& a, hipStream_t s) {
+  const int rc = attn_launch(attn_dkv_kernel<T, DP>, (int64_t)a.n_items * a.kv_heads, attn_dkv_lds<T, DP>(), a, s);
+  if (rc != ST_OK) return rc;
+  return attn_launch(attn_sum_parts_kernel<T, DP, true>, (int64_t)a.n_joins * a.kv_heads, 0, a, s);
+}
+
+enum AttnPass { kAttnForward, kAttnDq, kAttnDkv };
+template <typename T>
+static int attn_run(AttnPass pass, const AttnArgs& a, hipStream_t s) {
+#define ST_ATTN_DP(dp)                                        \
+  if (a.D <= dp) {                                            \
+    if (pass == kAttnForward) return attn_forward_dp<T, dp>(a, s); \
+    if (pass == kAttnDq) return attn_dq_dp<T, dp>(a, s);      \
+    return attn_dkv_dp<T, dp>(a, s);                          \
+  }
+  ST_ATTN_DP(32)
+  ST_ATTN_DP(64)
+  ST_ATTN_DP(96)
+  ST_ATTN_DP(128)
+#undef ST_ATTN_DP
+  return ST_ERR_UNSUPPORTED;
+}
+int attn_run_bf16(AttnPass pass, const AttnArgs& a, hipStream_t s);
+int attn_run_f16(AttnPass pass, const AttnArgs& a, hipStream_t s);
+int attn_run_f32(AttnPass pass, const AttnArgs& a, hipStream_t s);
+
+}  // namespace st

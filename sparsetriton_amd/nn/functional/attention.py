@@ -1,0 +1,294 @@
+"""Attention between the rows of a segment: a sample, a window, a patch of a serialised scene (HIP
+kernels ``st_attn_forward`` / ``st_attn_backward``; no counterpart in the reference).
+
+The rows of all segments lie one after another, as features do; ``AttentionSegments`` holds their
+lengths and the tile lists that the kernels walk.
+"""
+
+import ctypes
+import math
+from typing import Optional, Sequence, Union
+
+import numpy as np
+import torch
+
+from sparsetriton_amd import _lib
+from sparsetriton_amd.tensor import SparseTensor
+
+__all__ = ["AttentionSegments", "sparse_attention"]
+
+# Workgroups below which a tile's keys (rows) are split over several, and what the split aims at:
+# two and four for each of 256 CUs.  A part takes four steps at least.
+_SPLIT_BELOW, _SPLIT_TO, _PART_STEPS = 512, 1024, 4
+
+
+def _lengths(lengths, what: str) -> np.ndarray:
+    if isinstance(lengths, torch.Tensor):
+        if lengths.dtype.is_floating_point or lengths.dtype == torch.bool:
+            raise TypeError(f"{what} must be integers (got {lengths.dtype})")
+        lengths = lengths.detach().cpu().numpy()
+    out = np.asarray(lengths)
+    if out.ndim != 1 or (out.size and out.dtype.kind not in "iu"):
+        raise ValueError(f"{what} must be a list of row counts")
+    out = out.astype(np.int64)
+    if (out < 0).any() or out.sum() >= 2 ** 31:
+        raise ValueError(f"{what} must not be negative, and at most 2^31 - 1 rows in all")
+    return out
+
+
+class _Tiles:
+    """Work items and joins of one pass, on the device: rows (4, 8) int32 as st_attn_args lays them out."""
+
+    def __init__(self, q0, nq, k0, nk, row0, lo, hi, kv_heads, device):
+        step = _lib.ATTN_KEYS
+        steps = -(-(hi - lo) // step)
+        n = steps.size
+        parts = np.ones(n, dtype=np.int64)
+        chunk = steps.copy()
+        if n and n * kv_heads < _SPLIT_BELOW:
+            most = max(_PART_STEPS, -(-int(steps.sum()) * kv_heads // _SPLIT_TO))
+            parts = np.maximum(1, -(-steps // most))
+            chunk = -(-steps // parts)
+            parts = np.maximum(1, -(-steps // np.maximum(chunk, 1)))
+        tile = np.repeat(np.arange(n), parts)
+        nth = np.arange(tile.size) - np.repeat(np.cumsum(parts) - parts, parts)
+        first = lo[tile] + nth * chunk[tile] * step
+        end = np.minimum(hi[tile], first + chunk[tile] * step)
+        split = parts > 1
+        slot0 = np.cumsum(np.where(split, parts, 0)) - np.where(split, parts, 0)
+        part = np.where(split[tile], slot0[tile] + nth, -1)
+        items = np.stack([q0[tile], nq[tile], k0[tile], nk[tile], row0[tile], first, end, part], 1)
+        # longest first: the last workgroups to start are short ones
+        items = items[np.argsort(first - end, kind="stable")]
+        at = np.flatnonzero(split)
+        joins = np.stack([q0[at], nq[at], k0[at], nk[at], row0[at], slot0[at], parts[at], np.zeros_like(at)], 1)
+        self.n_items, self.n_joins, self.slots = items.shape[0], joins.shape[0], int(parts[split].sum())
+        self.words = torch.from_numpy(np.concatenate([items, joins]).astype(np.int32)).to(device)
+        self.items = self.words.data_ptr()
+        self.joins = self.items + self.n_items * _lib.ATTN_WORDS * 4 if self.n_joins else None
+        self._stream = None
+
+    def use(self) -> None:
+        """The words' memory is not handed out again before this stream is through with them."""
+        if self.n_items and self.words.is_cuda:
+            s = _lib.stream_of(self.words.device)
+            if s != self._stream:
+                self.words.record_stream(torch.cuda.current_stream(self.words.device))
+                self._stream = s
+
+
+class AttentionSegments:
+    """Lengths of the row segments that attend among themselves, and the kernels' tile lists.
+
+    ``q_lengths``: rows of each segment, in the order in which the rows lie; ``k_lengths`` the key
+    rows where they are not the same (cross attention).  Both are sequences or integer tensors (a
+    device tensor is read back).  Either may be zero: a row without keys has a zero output.  Made
+    once for a set of rows and shared by the layers over them; the tile lists for a number of heads
+    and an order are built at the first call with them (so a call whose lists are not there yet
+    cannot be captured in a graph).
+    """
+
+    def __init__(self, q_lengths: Union[Sequence[int], torch.Tensor],
+                 k_lengths: Optional[Union[Sequence[int], torch.Tensor]] = None,
+                 device: Union[str, torch.device] = "cuda") -> None:
+        self._nq = _lengths(q_lengths, "q_lengths")
+        self._nk = self._nq if k_lengths is None else _lengths(k_lengths, "k_lengths")
+        if self._nq.size != self._nk.size:
+            raise ValueError(f"{self._nq.size} segments of queries, {self._nk.size} of keys")
+        self._q0, self._k0 = (np.cumsum(n) - n for n in (self._nq, self._nk))
+        self.count, self.q_rows, self.k_rows = self._nq.size, int(self._nq.sum()), int(self._nk.sum())
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None and torch.cuda.is_available():
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self._plans = {}
+
+    @classmethod
+    def from_tensor(cls, tensor: SparseTensor, patch: Optional[int] = None) -> "AttentionSegments":
+        """The samples of ``tensor`` (whose rows must lie sample by sample, in ascending order), or
+        with ``patch`` each sample's rows in their order cut in patches of ``patch`` rows, the last
+        one of a sample shorter."""
+        if patch is not None and int(patch) <= 0:
+            raise ValueError(f"patch must be positive (got {patch})")
+        b = tensor.C[:, 0].long()
+        counts = torch.bincount(b, minlength=max(int(tensor.batch_size or 0), 1))
+        if b.numel() and bool((b[1:] < b[:-1]).any()):
+            raise ValueError("the rows must lie sample by sample, in ascending batch order")
+        counts = counts.cpu().numpy()
+        if patch is not None:
+            full, rest = counts // int(patch), counts % int(patch)
+            counts = np.concatenate([np.asarray([int(patch)] * f + [r] * int(r > 0), dtype=np.int64)
+                                     for f, r in zip(full, rest)])
+        return cls(counts, device=tensor.F.device)
+
+    def _tiles(self, per_segment):
+        """(segment, first row) of each tile of ST_ATTN_TILE rows."""
+        n = -(-per_segment // _lib.ATTN_TILE)
+        seg = np.repeat(np.arange(n.size), n)
+        return seg, (np.arange(seg.size) - np.repeat(np.cumsum(n) - n, n)) * _lib.ATTN_TILE
+
+    def _plan(self, which: str, group: int, kv_heads: int, causal: bool) -> _Tiles:
+        key = (which, group, kv_heads, causal)
+        plan = self._plans.get(key)
+        if plan is None:
+            nq, nk = self._nq, self._nk
+            if int(nq.max(initial=0)) * group >= 2 ** 31 - _lib.ATTN_TILE:
+                raise ValueError(f"a segment has at most {(2 ** 31 - _lib.ATTN_TILE) // group} query rows at {group} heads a key head")
+            if which == "q":  # tiles of packed rows over keys lo .. hi
+                seg, row0 = self._tiles(nq * group)
+                lo, hi = np.zeros_like(row0), nk[seg]
+                if causal:
+                    last = np.minimum(row0 + _lib.ATTN_TILE, nq[seg] * group) - 1
+                    hi = np.clip(last // group + nk[seg] - nq[seg] + 1, 0, nk[seg])
+            else:  # tiles of keys over packed rows lo .. hi
+                seg, row0 = self._tiles(nk)
+                lo, hi = np.zeros_like(row0), nq[seg] * group
+                if causal:
+                    lo = np.minimum(np.maximum(0, row0 - (nk[seg] - nq[seg])) * group, hi)
+            plan = _Tiles(self._q0[seg], nq[seg], self._k0[seg], nk[seg], row0, lo, hi, kv_heads, self.device)
+            self._plans[key] = plan
+        plan.use()
+        return plan
+
+
+def _parts(kv_heads, dim, q_slots, k_slots, device):
+    if not q_slots and not k_slots:
+        return None
+    floats = ctypes.c_int64()
+    _lib.call("st_attn_workspace", kv_heads, dim, q_slots, k_slots, ctypes.byref(floats))
+    return torch.empty((floats.value,), dtype=torch.float32, device=device)
+
+
+def _rows(t: torch.Tensor, group: int) -> torch.Tensor:
+    """t, or a contiguous copy where the kernels' 16-byte accesses or 32-bit tile offsets do not reach its rows."""
+    e = t.element_size()
+    row, head, channel = t.stride()
+    if (channel == 1 and not (row * e | head * e | t.data_ptr()) & 15 and row < 2 ** 29 and head < 2 ** 29
+            and (row * (_lib.ATTN_KEYS + 1) + head * (group + 1) + t.shape[2]) * e < 2 ** 31 - 64):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _args(q, k, v, key_mask, o, lse, causal, scale) -> _lib.AttnArgs:
+    a = _lib.AttnArgs()
+    a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
+    a.q_row, a.q_head, _ = q.stride()
+    a.k_row, a.k_head, _ = k.stride()
+    a.v_row, a.v_head, _ = v.stride()
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    if key_mask is not None:
+        a.key_mask = key_mask.data_ptr()
+    a.heads, a.kv_heads, a.dim = q.shape[1], k.shape[1], q.shape[2]
+    a.dtype, a.causal, a.scale = _lib.FEAT_DTYPES[q.dtype], causal, scale
+    return a
+
+
+def _forward(q, k, v, segments, key_mask, causal, scale, stats):
+    n, heads, dim = q.shape
+    kv_heads = k.shape[1]
+    group = heads // kv_heads
+    q, k, v = _rows(q, group), _rows(k, group), _rows(v, group)
+    o = torch.empty((n, heads, dim), dtype=q.dtype, device=q.device)
+    lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if stats else None
+    plan = segments._plan("q", group, kv_heads, causal)
+    a = _args(q, k, v, key_mask, o, lse, causal, scale)
+    a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
+    parts = _parts(kv_heads, dim, plan.slots, 0, q.device)
+    if parts is not None:
+        a.parts = parts.data_ptr()
+    _lib.call("st_attn_forward", ctypes.byref(a), _lib.stream_of(q.device))
+    return o, lse, q, k, v
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, segments, key_mask, causal, scale):
+        o, lse, q, k, v = _forward(q, k, v, segments, key_mask, causal, scale, True)
+        ctx.save_for_backward(q, k, v, o, lse, key_mask)
+        ctx.meta = (segments, causal, scale)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, o, lse, key_mask = ctx.saved_tensors
+        segments, causal, scale = ctx.meta
+        heads, dim = q.shape[1:]
+        kv_heads = k.shape[1]
+        group = heads // kv_heads
+        dout = _rows(dout, group)
+        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+        dq, delta = new(q), torch.empty_like(lse)
+        plan = segments._plan("q", group, kv_heads, causal)
+        a = _args(q, k, v, key_mask, o, lse, causal, scale)
+        a.dout, a.dq, a.delta = dout.data_ptr(), dq.data_ptr(), delta.data_ptr()
+        a.dout_row, a.dout_head, _ = dout.stride()
+        a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
+        dk = dv = None
+        slots = 0
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dk, dv = new(k), new(v)
+            keys = segments._plan("k", group, kv_heads, causal)
+            a.dk, a.dv = dk.data_ptr(), dv.data_ptr()
+            a.k_items, a.k_joins, a.n_k_items, a.n_k_joins = keys.items, keys.joins, keys.n_items, keys.n_joins
+            slots = keys.slots
+        parts = _parts(kv_heads, dim, plan.slots, slots, q.device)
+        if parts is not None:
+            a.parts = parts.data_ptr()
+        _lib.call("st_attn_backward", ctypes.byref(a), _lib.stream_of(q.device))
+        need = ctx.needs_input_grad
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
+
+
+def sparse_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    segments: AttentionSegments,
+    scale: Optional[float] = None,
+    causal: bool = False,
+    key_mask: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``softmax(scale * q k^T) v`` in each segment, (rows, heads, D) contiguous in ``q``'s dtype.
+
+    ``q`` (``segments.q_rows``, heads, D); ``k``, ``v`` (``segments.k_rows``, kv_heads, D) of the
+    same dtype (float32, float16, bfloat16); ``heads`` a multiple of ``kv_heads``, whose key head
+    ``h // (heads / kv_heads)`` query head ``h`` reads; D a multiple of 8, at most 128.  Rows and
+    heads may lie at any stride (slices of one projection, say); where channels are apart or rows not
+    at 16-byte addresses a copy is made.  ``scale`` is positive, ``D ** -0.5`` by default.
+
+    ``causal``: query ``i`` of ``nq`` sees keys up to ``i + nk - nq`` of its segment.  ``key_mask``
+    (``segments.k_rows``) bool: False leaves a key out, whatever its rows hold.  A row that sees no
+    key gets zeros, and its gradients are zero.  Scores, softmax and sums are fp32 (fp32 inputs: the
+    products too); results do not depend on timing.
+    """
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        _lib.require_device(t, f"attention {what}")
+        _lib.feat_code(t.dtype)
+        if t.dim() != 3 or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{what} must be (rows, heads, D) of q's dtype and device (got {tuple(t.shape)} {t.dtype} "
+                             f"on {t.device})")
+    heads, dim = q.shape[1:]
+    if q.shape[0] != segments.q_rows or k.shape[0] != segments.k_rows:
+        raise ValueError(f"the segments have {segments.q_rows} query and {segments.k_rows} key rows, q and k have "
+                         f"{q.shape[0]} and {k.shape[0]}")
+    if k.shape != v.shape or k.shape[2] != dim or k.shape[1] == 0 or heads == 0 or heads % k.shape[1]:
+        raise ValueError(f"heads do not fit: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if dim == 0 or dim % 8 or dim > _lib.ATTN_MAX_DIM:
+        raise ValueError(f"the head size must be a multiple of 8 up to {_lib.ATTN_MAX_DIM} (got {dim})")
+    if segments.device != q.device:
+        raise ValueError(f"the segments are on {segments.device}, q on {q.device}")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite (got {scale})")
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool:
+            raise TypeError(f"key_mask must be bool (got {key_mask.dtype})")
+        if key_mask.shape != k.shape[:1] or key_mask.device != q.device:
+            raise ValueError(f"key_mask must be ({k.shape[0]},) on {q.device} (got {tuple(key_mask.shape)} on "
+                             f"{key_mask.device})")
+        key_mask = key_mask.contiguous()
+    causal = bool(causal)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(q, k, v, segments, key_mask, causal, scale)
+    return _forward(q, k, v, segments, key_mask, causal, scale, False)[0]

@@ -1,0 +1,461 @@
+"""sparse_attention (st_attn_forward / st_attn_backward) against the formulas in float64.
+
+Bounds, per element, from the roundings on the way (u: half a unit of the type, 2^-8, 2^-11 or 0 for
+fp32 products; w = 512 * 2^-24 for what fp32 does to a score of |q||k| c ~ 11 summed over 128
+channels, its exponential and the row's sum):
+  P    (u + w) P                                  (rounded for the second product)
+  O    (u + w) sum P |v|  + u |O|                 (float16 also loses 2^-25 of P below 2^-14)
+  dP - delta   w sum |dO||v|  + sum |dO| (error of O)
+  dS   (2 u + w) |dS| + P (error of dP - delta)
+  dQ, dK, dV   the error of dS or P through the product, plus u of the result.
+"""
+
+import pytest
+import torch
+
+from sparsetriton_amd import SparseTensor, _lib
+from sparsetriton_amd.nn.functional import AttentionSegments, sparse_attention
+
+UNIT = {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+W = 512 * 2.0 ** -24
+
+
+def _reference(q, k, v, do, ql, kl, scale, causal, mask):
+    """{name: (value, bound)} in float64; gradients of the key heads summed over their query heads."""
+    u, tiny = UNIT[q.dtype], 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    last = max(u, 2.0 ** -24)
+    group = q.shape[1] // k.shape[1]
+    q, k, v, do = (t.detach().double() for t in (q, k, v, do))
+    if mask is not None:
+        k, v = (t.masked_fill(~mask[:, None, None], 0.0) for t in (k, v))
+    val = {n: torch.zeros_like(t) for n, t in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+    err = {n: torch.zeros_like(t) for n, t in val.items()}
+    q0 = k0 = 0
+    for nq, nk in zip(ql, kl):
+        Q, K = slice(q0, q0 + nq), slice(k0, k0 + nk)
+        see = torch.ones((nq, nk), dtype=torch.bool, device=q.device)
+        if causal:
+            see = see.tril(nk - nq)
+        if mask is not None:
+            see = see & mask[K]
+        for h in range(q.shape[1] if nq and nk else 0):
+            a, b, c, g = q[Q, h], k[K, h // group], v[K, h // group], do[Q, h]
+            s = (a @ b.T * scale).masked_fill(~see, float("-inf"))
+            top = s.amax(1, keepdim=True).clamp_min(-1e300)
+            p = torch.exp(s - top)
+            total = p.sum(1, keepdim=True)
+            p = p / total.masked_fill(total == 0, 1.0)
+            o = p @ c
+            ep = (u + W) * p + tiny * see
+            eo = ep @ c.abs() + last * o.abs()
+            delta = (g * o).sum(1, keepdim=True)
+            ds = p * (g @ c.T - delta)
+            edp = W * (g.abs() @ c.abs().T) + (g.abs() * eo).sum(1, keepdim=True)
+            eds = (2 * u + W) * ds.abs() + p * edp + tiny * see
+            val["o"][Q, h], err["o"][Q, h] = o, eo
+            val["dq"][Q, h] = ds @ b * scale
+            err["dq"][Q, h] = eds @ b.abs() * scale
+            val["dk"][K, h // group] += ds.T @ a * scale
+            err["dk"][K, h // group] += eds.T @ a.abs() * scale
+            val["dv"][K, h // group] += p.T @ g
+            err["dv"][K, h // group] += ep.T @ g.abs()
+        q0, k0 = q0 + nq, k0 + nk
+    return {n: (t, err[n] + last * t.abs() + 1e-12) for n, t in val.items()}
+
+
+def _make(ql, kl, heads, kv_heads, dim, dtype, device, seed, masked=0.0):
+    g = torch.Generator().manual_seed(seed)
+    rand = lambda n, h: torch.randn((n, h, dim), generator=g).to(device, dtype)  # noqa: E731
+    q, do = rand(sum(ql), heads), rand(sum(ql), heads)
+    k, v = rand(sum(kl), kv_heads), rand(sum(kl), kv_heads)
+    mask = (torch.rand((sum(kl),), generator=g) >= masked).to(device) if masked else None
+    return q, k, v, do, mask
+
+
+def _check(q, k, v, do, ql, kl, causal=False, mask=None, scale=None):
+    segs = AttentionSegments(ql, kl, device=q.device)
+    with torch.no_grad():
+        plain = sparse_attention(q, k, v, segs, scale=scale, causal=causal, key_mask=mask)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = sparse_attention(q, k, v, segs, scale=scale, causal=causal, key_mask=mask)
+    assert torch.equal(o, plain) and o.is_contiguous()
+    got = dict(zip(("o", "dq", "dk", "dv"), (o.detach(),) + torch.autograd.grad(o, leaves, do)))
+    ref = _reference(q, k, v, do, ql, kl, q.shape[2] ** -0.5 if scale is None else scale, causal, mask)
+    for n, (want, bound) in ref.items():
+        assert got[n].shape == want.shape and got[n].dtype == q.dtype
+        over = (got[n].double() - want).abs() - bound
+        assert not torch.isnan(got[n]).any(), n
+        assert over.numel() == 0 or over.max().item() <= 0, (n, over.max().item(), want.abs().max().item())
+    return got
+
+
+LENGTHS = [
+    ([1], [1]), ([1, 1, 1], [1, 1, 1]), ([5], [64]), ([33, 1, 127, 2], [33, 1, 127, 2]), ([128, 129], [65, 64]),
+    ([0, 7, 0, 3], [4, 0, 0, 9]), ([300], [300]), ([1, 3], [700, 1]), ([200, 10], [3, 150]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ql,kl", LENGTHS)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(torch.bfloat16, 4, 4, 64), (torch.float16, 6, 2, 40),
+                                                     (torch.float32, 3, 1, 32), (torch.bfloat16, 8, 1, 128)])
+def test_lengths(device, ql, kl, causal, dtype, heads, kv_heads, dim):
+    q, k, v, do, _ = _make(ql, kl, heads, kv_heads, dim, dtype, device, sum(ql) + dim)
+    _check(q, k, v, do, ql, kl, causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [8, 16, 24, 32, 48, 64, 72, 80, 96, 104, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_head_sizes(device, dim, dtype, causal):
+    ql = [70, 3, 190]
+    q, k, v, do, mask = _make(ql, ql, 4, 2, dim, dtype, device, dim, masked=0.3)
+    _check(q, k, v, do, ql, ql, causal, mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (5, 5), (7, 1), (12, 4), (6, 3), (40, 2)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_shared_key_heads(device, heads, kv_heads, causal):
+    ql, kl = [45, 1, 130], [61, 77, 130]
+    q, k, v, do, mask = _make(ql, kl, heads, kv_heads, 32, torch.bfloat16, device, heads, masked=0.2)
+    _check(q, k, v, do, ql, kl, causal, mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ql,kl,heads,kv_heads,dim,causal", [
+    ([1], [5000], 4, 1, 64, False), ([1, 1, 2], [1, 4097, 300], 8, 2, 128, True), ([3], [9001], 1, 1, 32, False),
+    ([2500], [40], 2, 1, 32, False), ([1000], [1000], 1, 1, 64, True), ([1500, 20], [1, 2000], 2, 2, 48, False)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_work_split_over_the_long_side(device, ql, kl, heads, kv_heads, dim, causal, dtype):
+    q, k, v, do, mask = _make(ql, kl, heads, kv_heads, dim, dtype, device, 3 * dim, masked=0.1)
+    segs = AttentionSegments(ql, kl, device=device)
+    plans = [segs._plan(w, heads // kv_heads, kv_heads, causal) for w in "qk"]
+    assert any(p.n_joins for p in plans)
+    _check(q, k, v, do, ql, kl, causal, mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float32, 32)])
+@pytest.mark.parametrize("times", [3, 8])
+def test_many_tiles(device, causal, dtype, dim, times):
+    """Three times: partly split.  Eight times: enough workgroups (over 512 in both passes) that nothing is."""
+    ql = [700, 1, 333, 900, 64, 128, 2] * times
+    q, k, v, do, mask = _make(ql, ql, 8, 4, dim, dtype, device, 17, masked=0.05)
+    segs = AttentionSegments(ql, device=device)
+    assert times == 3 or not any(segs._plan(w, 2, 4, causal).n_joins for w in "qk")
+    _check(q, k, v, do, ql, ql, causal, mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1.0, 1e-3, 30.0])
+def test_scales(device, scale):
+    ql = [150, 20]
+    q, k, v, do, _ = _make(ql, ql, 2, 2, 32, torch.float32, device, 4)
+    if scale > 1:  # sharp rows: the scores' rounding grows with them
+        q, k = q * 0.1, k * 0.1
+    _check(q, k, v, do, ql, ql, False, None, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift", [-60.0, 60.0])
+def test_scores_far_from_zero(device, shift):
+    """One direction that all queries and keys share moves every score by the same amount, growing along the keys."""
+    ql = [40, 500]
+    q, k, v, do, _ = _make(ql, ql, 2, 1, 32, torch.float32, device, 5)
+    q[:, :, 0] = 1.0
+    k[:, :, 0] = shift * torch.linspace(0, 1, sum(ql), device=device)[:, None]
+    _check(q, k, v, do, ql, ql, False, None, 1.0 / 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("causal", [False, True])
+def test_rows_without_keys(device, dtype, causal):
+    """A segment whose keys are all masked, one without keys, and (causal) queries before the first key."""
+    ql, kl = [70, 5, 90, 100], [70, 0, 30, 200]
+    q, k, v, do, _ = _make(ql, kl, 4, 2, 64, dtype, device, 6)
+    mask = torch.ones(sum(kl), dtype=torch.bool, device=device)
+    mask[:70] = False
+    mask[100:140] = False
+    got = _check(q, k, v, do, ql, kl, causal, mask)
+    assert not got["o"][:75].any() and not got["dq"][:75].any() and not got["dk"][:70].any() and not got["dv"][:70].any()
+    if causal:
+        assert not got["o"][75:135].any() and not got["dq"][75:135].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_what_masked_keys_hold_does_not_matter(device, bad, dtype):
+    ql = [90, 40, 130]
+    q, k, v, do, mask = _make(ql, ql, 4, 2, 64, dtype, device, 7, masked=0.4)
+    clean = _check(q.clone(), k.clone(), v.clone(), do, ql, ql, False, mask)
+    k[~mask], v[~mask] = bad, bad
+    got = _check(q, k, v, do, ql, ql, False, mask)
+    assert all(torch.equal(got[n], clean[n]) for n in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 32)])
+@pytest.mark.parametrize("at", [37, 100, 128])
+def test_later_rows_do_not_reach_earlier_ones(device, bad, dtype, dim, at):
+    """Causal: a row that is not finite changes nothing for the rows before it, in its own tile too."""
+    ql = [200]
+    q, k, v, do, _ = _make(ql, ql, 4, 2, dim, dtype, device, 8)
+    clean = _check(q.clone(), k.clone(), v.clone(), do, ql, ql, True)
+    # values and keys: rows before `at` keep output and query gradient
+    for t in (v, k):
+        t2 = t.clone()
+        t2[at, :, 3] = bad
+        args = [t2 if t is x else x for x in (q, k, v)]
+        leaves = [x.detach().clone().requires_grad_(True) for x in args]
+        o = sparse_attention(*leaves, AttentionSegments(ql, device=device), causal=True)
+        dq, dk, dv = torch.autograd.grad(o, leaves, do)
+        assert torch.equal(o[:at], clean["o"][:at]) and torch.equal(dq[:at], clean["dq"][:at])
+        assert not torch.isfinite(o[at:]).all()
+    # a query and its gradient: keys after it keep theirs
+    for which in ("q", "do"):
+        q2, do2 = q.clone(), do.clone()
+        (q2 if which == "q" else do2)[at, :, 3] = bad
+        leaves = [x.detach().clone().requires_grad_(True) for x in (q2, k, v)]
+        o = sparse_attention(*leaves, AttentionSegments(ql, device=device), causal=True)
+        dq, dk, dv = torch.autograd.grad(o, leaves, do2)
+        assert torch.equal(dk[at + 1:], clean["dk"][at + 1:]) and torch.equal(dv[at + 1:], clean["dv"][at + 1:])
+        assert not torch.isfinite(dv[:at + 1]).all() or which == "q"
+
+
+@pytest.mark.gpu
+def test_a_row_that_is_not_finite_stays_in_its_segment(device):
+    ql = [60, 70, 200]
+    q, k, v, do, _ = _make(ql, ql, 2, 2, 32, torch.bfloat16, device, 9)
+    clean = _check(q.clone(), k.clone(), v.clone(), do, ql, ql)
+    k[70, 1, 0], v[80, 0, 5] = float("nan"), float("inf")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = sparse_attention(q, k, v, AttentionSegments(ql, device=device))
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    for rest in (slice(0, 60), slice(130, 330)):
+        assert torch.equal(o[rest], clean["o"][rest]) and torch.equal(dk[rest], clean["dk"][rest])
+    assert torch.isnan(o[60:130, 1]).all() and not torch.isfinite(o[60:130, 0, 5]).any()
+
+
+@pytest.mark.gpu
+def test_strides(device):
+    """Slices of one projection, heads first, rows off a 16-byte address, channels apart, one key head for all."""
+    n, g = 300, torch.Generator().manual_seed(10)
+    segs = AttentionSegments([100, 200], device=device)
+    qkv = torch.randn((n, 3, 4, 32), generator=g).to(device, torch.bfloat16)
+    q, k, v = qkv.unbind(1)
+    ref = sparse_attention(q.contiguous(), k.contiguous(), v.contiguous(), segs)
+    assert torch.equal(sparse_attention(q, k, v, segs), ref)
+    heads_first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    assert torch.equal(sparse_attention(*heads_first, segs), ref)
+    off = [torch.empty((n * 128 + 1,), dtype=torch.bfloat16, device=device)[1:].view(n, 4, 32).copy_(t) for t in (q, k, v)]
+    assert torch.equal(sparse_attention(*off, segs), ref)
+    apart = [torch.empty((n, 4, 32, 2), dtype=torch.bfloat16, device=device)[..., 1].copy_(t) for t in (q, k, v)]
+    assert torch.equal(sparse_attention(*apart, segs), ref)
+    one = k[:, :1].expand(n, 4, 32)
+    assert torch.equal(sparse_attention(q, one, v, segs), sparse_attention(q, one.contiguous(), v, segs))
+    # gradients of the slices come back into the projection; a gradient that is one value everywhere
+    qkv.requires_grad_(True)
+    sparse_attention(*qkv.unbind(1), segs).sum().backward()
+    leaves = [t.detach().contiguous().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(sparse_attention(*leaves, segs), leaves, torch.ones_like(ref))
+    assert all(torch.equal(qkv.grad[:, i], d) for i, d in enumerate(grads))
+    # a broadcast key: its gradient is the sum over the heads that it was given to
+    k1 = k[:, :1].detach().clone().requires_grad_(True)
+    do = torch.randn(ref.shape, generator=g).to(device, torch.bfloat16)
+    (d1,) = torch.autograd.grad(sparse_attention(leaves[0], k1.expand(n, 4, 32), leaves[2], segs), [k1], do)
+    k4 = k1.detach().expand(n, 4, 32).contiguous().requires_grad_(True)
+    (d4,) = torch.autograd.grad(sparse_attention(leaves[0], k4, leaves[2], segs), [k4], do)
+    assert torch.equal(d1, d4.sum(1, keepdim=True))
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(device):
+    """Keys spread over more than 2^32 bytes of one segment: rows 16 KB apart."""
+    n, dim = 400_000, 64
+    cache = torch.empty((n, 128, dim), dtype=torch.bfloat16, device=device)
+    g = torch.Generator(device=device).manual_seed(11)
+    k, v = cache[:, 3:4], cache[:, 77:78]
+    k.copy_(torch.randn((n, 1, dim), generator=g, device=device))
+    v.copy_(torch.randn((n, 1, dim), generator=g, device=device))
+    k[-1], v[-1] = 3.0, 50.0  # the far end counts
+    q = torch.full((2, 4, dim), 1.0, device=device, dtype=torch.bfloat16)
+    segs = AttentionSegments([2], [n], device=device)
+    got = sparse_attention(q, k, v, segs)
+    ref = sparse_attention(q, k.contiguous(), v.contiguous(), segs)
+    assert torch.equal(got, ref)
+    s = (q[0, 0].double() @ k[:, 0].double().T) * dim ** -0.5
+    want = torch.softmax(s, 0) @ v[:, 0].double()
+    assert (got[0, 0].double() - want).abs().max().item() <= 2 * 2.0 ** -8 * want.abs().max().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_gradients_against_differences(device, causal):
+    """Along random directions in fp32: central differences with e = 2^-6 (curvature e^2, rounding 2^-22 / e)."""
+    ql, kl = [20, 9], [20, 30]
+    q, k, v, do, mask = _make(ql, kl, 4, 2, 16, torch.float32, device, 12, masked=0.2)
+    segs = AttentionSegments(ql, kl, device=device)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    f = lambda ts: (sparse_attention(*ts, segs, causal=causal, key_mask=mask).double() * do.double()).sum()  # noqa: E731
+    grads = torch.autograd.grad(f(leaves), leaves)
+    e = 2.0 ** -6
+    for i in range(3):
+        d = torch.randn_like(leaves[i])
+        with torch.no_grad():
+            up, down = (f([t + s * e * d if j == i else t for j, t in enumerate(leaves)]) for s in (1, -1))
+        slope, got = (up - down) / (2 * e), (grads[i].double() * d.double()).sum()
+        assert (slope - got).abs() <= 1e-2 * (grads[i].double() * d.double()).norm(), (i, slope.item(), got.item())
+
+
+@pytest.mark.gpu
+def test_the_same_bits_on_every_run_and_stream(device):
+    ql = [1000, 37, 600]
+    q, k, v, do, mask = _make(ql, ql, 8, 2, 64, torch.bfloat16, device, 13, masked=0.1)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    segs = AttentionSegments(ql, device=device)
+
+    def once():
+        o = sparse_attention(q, k, v, segs, key_mask=mask)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, do)
+
+    first = once()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = once()
+    torch.cuda.current_stream().wait_stream(side)
+    for other in (second, once()):
+        assert all(torch.equal(a, b) for a, b in zip(first, other))
+
+
+@pytest.mark.gpu
+def test_one_gradient_alone(device):
+    ql = [80, 50]
+    q, k, v, do, _ = _make(ql, ql, 4, 2, 32, torch.bfloat16, device, 14)
+    segs = AttentionSegments(ql, device=device)
+    full = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(sparse_attention(*full, segs), full, do)
+    for i in range(3):
+        some = [t.clone().requires_grad_(j == i) for j, t in enumerate((q, k, v))]
+        (got,) = torch.autograd.grad(sparse_attention(*some, segs), [some[i]], do)
+        assert torch.equal(got, want[i])
+
+
+@pytest.mark.gpu
+def test_graph_capture_and_replay(device):
+    ql, kl = [1, 1], [3000, 500]
+    q, k, v, _, _ = _make(ql, kl, 8, 2, 64, torch.bfloat16, device, 15)
+    segs = AttentionSegments(ql, kl, device=device)
+    sparse_attention(q, k, v, segs)  # the tile lists are built by an eager call
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = sparse_attention(q, k, v, segs)
+    for i in range(3):
+        q.copy_(torch.randn(q.shape, device=device))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, sparse_attention(q, k, v, segs))
+
+
+@pytest.mark.gpu
+def test_segments_of_a_tensor(device):
+    b = torch.tensor([0] * 7 + [2] * 5 + [3] * 4)
+    coords = torch.stack([b, torch.arange(16), torch.arange(16), torch.arange(16)], 1).to(device)
+    x = SparseTensor(torch.zeros((16, 8), device=device), coords, spatial_shape=(16, 16, 16), batch_size=5)
+    assert AttentionSegments.from_tensor(x)._nq.tolist() == [7, 0, 5, 4, 0]
+    assert AttentionSegments.from_tensor(x, patch=4)._nq.tolist() == [4, 3, 4, 1, 4]
+    with pytest.raises(ValueError, match="sample"):
+        AttentionSegments.from_tensor(SparseTensor(x.F, coords.flip(0), spatial_shape=(16, 16, 16), batch_size=5))
+    with pytest.raises(ValueError, match="patch"):
+        AttentionSegments.from_tensor(x, patch=0)
+
+
+def test_tile_lists_cover_every_pair_once():
+    """Host arithmetic of the lists: each (row, key) that may be seen lies in exactly one item, and parts join in order."""
+    for ql, kl, group, kv, causal in [([300, 1, 0, 50], [700, 3, 5, 0], 3, 1, False), ([1], [5000], 1, 1, False),
+                                      ([400, 90], [400, 20], 2, 2, True), ([5], [1000], 7, 1, True)]:
+        s = AttentionSegments(ql, kl, device="cpu")
+        for which in "qk":
+            plan = s._plan(which, group, kv, causal)
+            items = plan.words[:plan.n_items].tolist()
+            joins = plan.words[plan.n_items:].tolist()
+            assert len(joins) == plan.n_joins
+            slots = sorted(i[7] for i in items if i[7] >= 0)
+            assert slots == list(range(plan.slots)) and sum(j[6] for j in joins) == plan.slots
+            q0 = k0 = 0
+            for nq, nk in zip(ql, kl):
+                mine = [i for i in items if i[:4] == [q0, nq, k0, nk]]
+                rows, length = (nq * group, nk) if which == "q" else (nk, nq * group)
+                for row0 in range(0, rows, 128):
+                    tile = sorted((i for i in mine if i[4] == row0), key=lambda i: i[5])
+                    seen = [j for i in tile for j in range(i[5], i[6])]
+                    assert len(seen) == len(set(seen)) and tile
+                    if which == "q":
+                        last = (min(rows, row0 + 128) - 1) // group + nk - nq if causal else nk - 1
+                        assert seen == list(range(0, min(nk, max(0, last + 1))))
+                    else:
+                        first = max(0, row0 - (nk - nq)) * group if causal else 0
+                        assert seen == list(range(min(first, length), length))
+                    if len(tile) > 1:
+                        (join,) = [j for j in joins if j[:5] == tile[0][:5]]
+                        assert [i[7] for i in tile] == list(range(join[5], join[5] + join[6]))
+                    else:
+                        assert tile[0][7] == -1
+                q0, k0 = q0 + nq, k0 + nk
+
+
+def test_refusals_before_any_launch():
+    for bad, err in (([1, -1], ValueError), ([[1]], ValueError), ([1.5], ValueError), ([2 ** 31], ValueError),
+                     (torch.tensor([1.0]), TypeError)):
+        with pytest.raises(err):
+            AttentionSegments(bad, device="cpu")
+    with pytest.raises(ValueError, match="segments of queries"):
+        AttentionSegments([1, 2], [3], device="cpu")
+    with pytest.raises(RuntimeError, match="GPU"):
+        sparse_attention(*[torch.zeros((3, 1, 8))] * 3, AttentionSegments([3], device="cpu"))
+    lib = _lib.lib()
+    a = _lib.AttnArgs()
+    assert lib.st_attn_forward(None, None) == -1 and lib.st_attn_forward(a, None) == -1
+    a.heads, a.kv_heads, a.dim, a.scale, a.dtype = 4, 2, 64, 0.125, 2
+    assert lib.st_attn_forward(a, None) == 0 and lib.st_attn_backward(a, None) == 0  # nothing to do
+    for field, value, rc in (("kv_heads", 3, -1), ("dim", 20, -3), ("dim", 136, -3), ("dtype", 3, -3), ("scale", 0.0, -1),
+                             ("scale", float("nan"), -1), ("n_q_items", -1, -1), ("n_q_items", 1, -1)):
+        old = getattr(a, field)
+        setattr(a, field, value)
+        assert lib.st_attn_forward(a, None) == rc, field
+        setattr(a, field, old)
+
+
+@pytest.mark.gpu
+def test_refusals(device):
+    segs = AttentionSegments([4, 2], device=device)
+    q = torch.zeros((6, 4, 16), device=device)
+    for args in ((q[:5], q, q), (q, q[:5], q[:5]), (q, q[:, :3], q[:, :3]), (q, q, q[:, :2]), (q[0], q, q),
+                 (q, q.half(), q.half()), (q, q[:, :0], q[:, :0])):
+        with pytest.raises(ValueError):
+            sparse_attention(*args, segs)
+    for dim in (4, 20, 136):
+        with pytest.raises(ValueError, match="head size"):
+            t = torch.zeros((6, 2, dim), device=device)
+            sparse_attention(t, t, t, segs)
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            sparse_attention(q, q, q, segs, scale=scale)
+    with pytest.raises(TypeError, match="bool"):
+        sparse_attention(q, q, q, segs, key_mask=torch.ones(6, device=device))
+    with pytest.raises(ValueError, match="key_mask"):
+        sparse_attention(q, q, q, segs, key_mask=torch.ones(5, device=device, dtype=torch.bool))
+    with pytest.raises(ValueError, match="segments are on"):
+        sparse_attention(q, q, q, AttentionSegments([4, 2], device="cpu"))
+    with pytest.raises(TypeError):
+        sparse_attention(q.double(), q.double(), q.double(), segs)
+    with pytest.raises(RuntimeError, match="GPU"):
+        sparse_attention(q.cpu(), q, q, segs)
