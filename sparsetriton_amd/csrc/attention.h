@@ -171,42 +171,61 @@ struct AttnTile {
   }
 };
 
-// acc += A B where some of the 16 reduction indexes must not reach some columns:
-// bit i of `allowed` says whether index i (16-bit layout order: row0 + i of
-// AttnTile::cols) may reach this lane's column.  B is already zero there, but
-// zero times an infinity or a NaN in A is a NaN: on a tile that the causal order
-// cuts, a later row that is not finite would reach earlier ones.  Such
-// elements (none, as a rule: one check) are added on their own, index by index.
-template <typename T>
-__device__ __forceinline__ v16f mma32_guarded(typename AttnFrag<T>::type a, const typename AttnFrag<T>::type& b,
-                                              v16f acc, unsigned allowed) {
-  using Frag = typename AttnFrag<T>::type;
-  Frag bad = a;
-  bool any = false;
+// A product over the rows of a tile that the causal order cuts: the other
+// operand is zero where a column must not see a row, but zero times an infinity
+// or a NaN is a NaN, so a later row that is not finite would reach earlier ones.
+// Such a tile (one check of it, by each wave that the order cuts it for) is
+// copied without those elements, the product taken over the copy, and what they
+// do to the columns that see them added at the end.
+template <typename T, int ROWS, int DP>
+__device__ __forceinline__ bool attn_not_finite(const T* tile) {
+  using Tile = AttnTile<T, DP>;
+  bool bad = false;
+#pragma unroll 4
+  for (int c = threadIdx.x & 63; c < ROWS * Tile::CPR; c += 64)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool finite = fabsf((float)a[e]) < INFINITY;
-    any |= !finite;
-    bad[e] = finite ? (T)0.f : a[e];
-    a[e] = finite ? a[e] : (T)0.f;
+    for (int e = 0; e < Tile::EPC; ++e) bad |= !(fabsf((float)tile[c * Tile::EPC + e]) < INFINITY);
+  return __any(bad);
+}
+// (Each wave that needs the copy writes all of it, the same values.)
+template <typename T, int ROWS, int DP>
+__device__ __forceinline__ void attn_copy_finite(const T* tile, T* copy) {
+  using Tile = AttnTile<T, DP>;
+#pragma unroll 1
+  for (int c = (threadIdx.x & 63) * Tile::EPC; c < ROWS * DP; c += 64 * Tile::EPC)
+#pragma unroll
+    for (int e = 0; e < Tile::EPC; ++e) copy[c + e] = fabsf((float)tile[c + e]) < INFINITY ? tile[c + e] : (T)0.f;
+}
+// What the left out elements do to a lane's sums (transposed: registers =
+// channels), a bit for each: infinities of either sign, both for a NaN.  In
+// loops that stay rolled: they take neither time nor registers from the products.
+struct AttnNotFinite {
+  uint64_t pos = 0, neg = 0;
+  template <typename T, int ROWS, int DP>
+  __device__ __forceinline__ void add(const T* tile, int first, int last) {  // rows first .. last
+    using Tile = AttnTile<T, DP>;
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll 1
+    for (int row = 0; row < ROWS; ++row)
+#pragma unroll 1
+      for (int r = 0; r < DP / 2; ++r) {
+        const int d = (r >> 4) * 32 + reg_row(r & 15, half);
+        const float x = (float)tile[Tile::at(row, d / Tile::EPC) + d % Tile::EPC];
+        const bool seen = row >= first && row <= last && !(fabsf(x) < INFINITY);
+        pos |= (uint64_t)(seen && x != -INFINITY) << r;
+        neg |= (uint64_t)(seen && x != INFINITY) << r;
+      }
   }
-  acc = mma32(a, b, acc);
-  if (!__any(any)) return acc;
-  const int half = (threadIdx.x >> 5) & 1;
+  template <int DB>
+  __device__ __forceinline__ void apply(v16f (&acc)[DB]) const {
+    if (!__any(pos | neg)) return;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    for (int h = 0; h < 2; ++h) {
-      Frag one;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) one[k] = k == e && half == h ? bad[k] : (T)0.f;
-      const v16f next = mma32(one, b, acc);
-      const bool take = allowed >> (8 * (e >> 2) + 4 * h + (e & 3)) & 1;
-#pragma unroll
-      for (int k = 0; k < 16; ++k) acc[k] = take ? next[k] : acc[k];
+    for (int r = 0; r < DB * 16; ++r) {
+      if (pos >> r & 1) acc[r / 16][r % 16] += INFINITY;
+      if (neg >> r & 1) acc[r / 16][r % 16] -= INFINITY;
     }
   }
-  return acc;
-}
+};
 
 // Rows of a tile on their way from memory to LDS: each thread carries N chunks.
 template <typename T, int DP, int ROWS>
@@ -298,13 +317,19 @@ __device__ __forceinline__ int attn_work(int n) {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Waves of a SIMD that the registers leave room for (a limit for the compiler).
+template <typename T, int DP>
+constexpr int attn_waves() {
+  return DP * sizeof(T) <= 256 ? 2 : 1;
+}
+
 // ------------------------------------------------------------------ forward
 
 constexpr int kAttnKeys = ST_ATTN_KEYS;  // keys of a step
 
 template <typename T, int DP>
-constexpr int attn_fwd_lds() {
-  return 2 * 2 * kAttnKeys * DP * (int)sizeof(T);
+constexpr int attn_fwd_lds(bool causal) {  // two buffers of K and V, a copy of one of them
+  return (causal ? 5 : 4) * kAttnKeys * DP * (int)sizeof(T);
 }
 
 // A running maximum is raised only when a row's maximum passes it by more
@@ -312,8 +337,8 @@ constexpr int attn_fwd_lds() {
 // floating point, and the accumulators need no rescaling.
 constexpr float kAttnSlack = 8.f;
 
-template <typename T, int DP>
-__global__ __launch_bounds__(kAttnThreads) void attn_forward_kernel(AttnArgs a) {
+template <typename T, int DP, bool CAUSAL>
+__global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forward_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
   using Stage = AttnStage<T, DP, kAttnKeys>;
@@ -335,7 +360,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_kernel(AttnArgs a) 
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = load_row8<T>(row, 16 * s + 8 * half, a.D, live);
   }
-  const int see = a.causal ? qi + it.nk - it.nq : 0x7FFFFFFF;  // last key that this lane's row sees
+  const int see = CAUSAL ? qi + it.nk - it.nq : 0x7FFFFFFF;  // last key that this lane's row sees
 
   Stage ks, vs;
   uint8_t chunk_kept[Stage::N], key_kept = 1;
@@ -357,6 +382,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_kernel(AttnArgs a) 
 #pragma unroll
   for (int b = 0; b < DB; ++b) o[b] = (v16f)(0.f);
   float m = -INFINITY, l = 0.f;
+  AttnNotFinite left_out;
   if (it.lo < it.hi) fetch(it.lo);
   for (int kt = it.lo, buf = 0; kt < it.hi; kt += kAttnKeys, buf ^= 1) {
     T* kl = tiles + buf * 2 * TILE;
@@ -373,7 +399,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_kernel(AttnArgs a) 
     vs.store(vl);
     __syncthreads();
     if (kt + kAttnKeys < it.hi) fetch(kt + kAttnKeys);
-    if (!active || !__any(live && kt <= see)) continue;
+    if (!active || (CAUSAL && !__any(live && kt <= see))) continue;
 
     v16f s[NB];
 #pragma unroll
@@ -382,7 +408,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_kernel(AttnArgs a) 
 #pragma unroll
       for (int i = 0; i < KS; ++i) s[b] = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s[b]);
     }
-    const bool cut = __any(see - kt < kAttnKeys - 1);  // by the causal order
+    const bool cut = CAUSAL && __any(see - kt < kAttnKeys - 1);  // by the causal order
     const int last = see - kt;
     const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
     if (cut || seen != ~0ull) {
@@ -417,22 +443,23 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_kernel(AttnArgs a) 
         s[b][e] = fast_exp2(fmaf(s[b][e], a.scale_log2, base));
         l += s[b][e];
       }
+    const T* vp = vl;
+    if (cut && attn_not_finite<T, kAttnKeys, DP>(vl)) {
+      attn_copy_finite<T, kAttnKeys, DP>(vl, tiles + 4 * TILE);
+      vp = tiles + 4 * TILE;
+      left_out.add<T, kAttnKeys, DP>(vl, 0, last);
+    }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const Frag p = to_frag<T>(regs8(s[b], j));
-        if (!cut) {
 #pragma unroll
-          for (int d = 0; d < DB; ++d) o[d] = mma32(Tile::cols(vl, b * 32 + 16 * j, d * 32), p, o[d]);
-        } else {
-#pragma unroll
-          for (int d = 0; d < DB; ++d)
-            o[d] = mma32_guarded<T>(Tile::cols(vl, b * 32 + 16 * j, d * 32), p, o[d], (unsigned)(keep >> (32 * b + 16 * j)));
-        }
+        for (int d = 0; d < DB; ++d) o[d] = mma32(Tile::cols(vp, b * 32 + 16 * j, d * 32), p, o[d]);
       }
   }
 
+  if (CAUSAL) left_out.apply(o);
   l += other_half(l);
   if (it.part >= 0) {
     // a row of DP sums, then its maximum (in powers of two) and sum
@@ -484,8 +511,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArg
 // ------------------------------------------------------------------ backward: queries
 
 // dQ of a tile of rows, and delta = rowsum(dO o O) for the keys' pass after it.
-template <typename T, int DP>
-__global__ __launch_bounds__(kAttnThreads) void attn_dq_kernel(AttnArgs a) {
+template <typename T, int DP, bool CAUSAL>
+__global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
   using Stage = AttnStage<T, DP, kAttnKeys>;
@@ -522,7 +549,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dq_kernel(AttnArgs a) {
       if (half == 0) a.delta[at] = delta;
     }
   }
-  const int see = a.causal ? qi + it.nk - it.nq : 0x7FFFFFFF;
+  const int see = CAUSAL ? qi + it.nk - it.nq : 0x7FFFFFFF;
 
   Stage ks, vs;
   uint8_t chunk_kept[Stage::N], key_kept = 1;
@@ -559,11 +586,16 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dq_kernel(AttnArgs a) {
     vs.store(vl);
     __syncthreads();
     if (kt + kAttnKeys < it.hi) fetch(kt + kAttnKeys);
-    if (!active || !__any(live && kt <= see)) continue;
-    const bool cut = __any(see - kt < kAttnKeys - 1);
+    if (!active || (CAUSAL && !__any(live && kt <= see))) continue;
+    const bool cut = CAUSAL && __any(see - kt < kAttnKeys - 1);
     const int last = see - kt;
     const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
-#pragma unroll
+    const T* kp = kl;  // (a row that sees a key that is not finite has a dS that is not)
+    if (cut && attn_not_finite<T, kAttnKeys, DP>(kl)) {
+      attn_copy_finite<T, kAttnKeys, DP>(kl, tiles + 4 * TILE);
+      kp = tiles + 4 * TILE;
+    }
+#pragma unroll 1
     for (int b = 0; b < NB; ++b) {
       v16f s = (v16f)(0.f), dp = (v16f)(0.f);
 #pragma unroll
@@ -581,14 +613,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dq_kernel(AttnArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const Frag ds = to_frag<T>(regs8(s, j));
-        if (!cut) {
 #pragma unroll
-          for (int d = 0; d < DB; ++d) dq[d] = mma32(Tile::cols(kl, b * 32 + 16 * j, d * 32), ds, dq[d]);
-        } else {
-#pragma unroll
-          for (int d = 0; d < DB; ++d)
-            dq[d] = mma32_guarded<T>(Tile::cols(kl, b * 32 + 16 * j, d * 32), ds, dq[d], (unsigned)(keep >> (32 * b + 16 * j)));
-        }
+        for (int d = 0; d < DB; ++d) dq[d] = mma32(Tile::cols(kp, b * 32 + 16 * j, d * 32), ds, dq[d]);
       }
     }
   }
@@ -609,14 +635,14 @@ constexpr int attn_q_rows() {  // packed rows of a step
   return DP * (int)sizeof(T) <= 192 ? 64 : 32;
 }
 template <typename T, int DP>
-constexpr int attn_dkv_lds() {
-  return 2 * (2 * attn_q_rows<T, DP>() * DP * (int)sizeof(T) + 2 * attn_q_rows<T, DP>() * 4);
+constexpr int attn_dkv_lds(bool causal) {
+  return attn_q_rows<T, DP>() * ((causal ? 6 : 4) * DP * (int)sizeof(T) + 4 * 4);
 }
 
 // dK and dV of a tile of keys: the waves hold 32 keys each (K, V and both sums in
 // registers) while the packed rows' Q, dO, L and delta go by through LDS.
-template <typename T, int DP>
-__global__ __launch_bounds__(kAttnThreads) void attn_dkv_kernel(AttnArgs a) {
+template <typename T, int DP, bool CAUSAL>
+__global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP * 3 / 2>())) void attn_dkv_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
   constexpr int BQ = attn_q_rows<T, DP>();
@@ -626,6 +652,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dkv_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
   float* stats = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers of BQ L, BQ delta
+  T* copies = reinterpret_cast<T*>(stats + 4 * BQ);           // CAUSAL: of a Q and a dO tile
 
   const int w = attn_work(gridDim.x), hk = w / a.n_items;
   const AttnItem it = a.items[w - hk * a.n_items];
@@ -642,8 +669,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dkv_kernel(AttnArgs a) {
     vf[s] = load_row8<T>((const T*)a.v + krow * a.v_row + hk * a.v_head, 16 * s + 8 * half, a.D, kept);
   }
   // first packed row that sees this lane's key, and the first that sees any of the wave's
-  const int from = a.causal ? (key - (it.nk - it.nq)) * a.group : 0;
-  const int wave_from = a.causal ? (kw - (it.nk - it.nq)) * a.group : 0;
+  const int from = CAUSAL ? (key - (it.nk - it.nq)) * a.group : 0;
+  const int wave_from = CAUSAL ? (kw - (it.nk - it.nq)) * a.group : 0;
 
   Stage qs, gs;
   float stat = 0.f;
@@ -678,6 +705,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dkv_kernel(AttnArgs a) {
   v16f dk[DB], dv[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) dk[b] = dv[b] = (v16f)(0.f);
+  AttnNotFinite left_out;
   if (it.lo < it.hi) fetch(it.lo);
   for (int rt = it.lo, buf = 0; rt < it.hi; rt += BQ, buf ^= 1) {
     T* ql = tiles + buf * 2 * TILE;
@@ -689,12 +717,15 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dkv_kernel(AttnArgs a) {
     __syncthreads();
     if (rt + BQ < it.hi) fetch(rt + BQ);
     if (!active || rt + BQ <= wave_from) continue;
-    const bool cut = a.causal && __any(from > rt);
-    auto allowed = [&](int row) {  // of 16 rows from `row` on, those that see this lane's key
-      const int n = from - row;
-      return n <= 0 ? 0xFFFFu : n >= 16 ? 0u : 0xFFFFu << n;
-    };
-#pragma unroll
+    const bool cut = CAUSAL && __any(from > rt);
+    const T *qp = ql, *gp = gl;  // (a row whose Q or dO is not finite has a delta, and so a dS, that is not)
+    if (cut && (attn_not_finite<T, BQ, DP>(ql) || attn_not_finite<T, BQ, DP>(gl))) {
+      attn_copy_finite<T, BQ, DP>(ql, copies);
+      attn_copy_finite<T, BQ, DP>(gl, copies + TILE);
+      qp = copies, gp = copies + TILE;
+      left_out.add<T, BQ, DP>(gl, from - rt, BQ);
+    }
+#pragma unroll 1
     for (int b = 0; b < NB; ++b) {
       v16f s = (v16f)(0.f), dp = (v16f)(0.f);
 #pragma unroll
@@ -716,9 +747,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dkv_kernel(AttnArgs a) {
       for (int j = 0; j < 2; ++j) {
         const Frag p = to_frag<T>(regs8(s, j));
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-          dv[d] = cut ? mma32_guarded<T>(Tile::cols(gl, b * 32 + 16 * j, d * 32), p, dv[d], allowed(rt + b * 32 + 16 * j))
-                      : mma32(Tile::cols(gl, b * 32 + 16 * j, d * 32), p, dv[d]);
+        for (int d = 0; d < DB; ++d) dv[d] = mma32(Tile::cols(gp, b * 32 + 16 * j, d * 32), p, dv[d]);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -734,13 +763,12 @@ __global__ __launch_bounds__(kAttnThreads) void attn_dkv_kernel(AttnArgs a) {
       for (int j = 0; j < 2; ++j) {
         const Frag ds = to_frag<T>(regs8(s, j));
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-          dk[d] = cut ? mma32_guarded<T>(Tile::cols(ql, b * 32 + 16 * j, d * 32), ds, dk[d], allowed(rt + b * 32 + 16 * j))
-                      : mma32(Tile::cols(ql, b * 32 + 16 * j, d * 32), ds, dk[d]);
+        for (int d = 0; d < DB; ++d) dk[d] = mma32(Tile::cols(qp, b * 32 + 16 * j, d * 32), ds, dk[d]);
       }
     }
   }
 
+  if (CAUSAL) left_out.apply(dv);
   if (!kept) {  // a masked key gets no gradient
 #pragma unroll
     for (int b = 0; b < DB; ++b) dk[b] = dv[b] = (v16f)(0.f);
@@ -798,19 +826,19 @@ static int attn_launch(K kernel, int64_t blocks, int lds, const AttnArgs& a, hip
 
 template <typename T, int DP>
 static int attn_forward_dp(const AttnArgs& a, hipStream_t s) {
-  const int rc = attn_launch(attn_forward_kernel<T, DP>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(), a, s);
+  const int rc = attn_launch(a.causal ? attn_forward_kernel<T, DP, true> : attn_forward_kernel<T, DP, false>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(a.causal), a, s);
   if (rc != ST_OK) return rc;
   return attn_launch(attn_forward_join_kernel<T, DP>, (int64_t)a.n_joins * a.kv_heads, 0, a, s);
 }
 template <typename T, int DP>
 static int attn_dq_dp(const AttnArgs& a, hipStream_t s) {
-  const int rc = attn_launch(attn_dq_kernel<T, DP>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(), a, s);
+  const int rc = attn_launch(a.causal ? attn_dq_kernel<T, DP, true> : attn_dq_kernel<T, DP, false>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(a.causal), a, s);
   if (rc != ST_OK) return rc;
   return attn_launch(attn_sum_parts_kernel<T, DP, false>, (int64_t)a.n_joins * a.kv_heads, 0, a, s);
 }
 template <typename T, int DP>
 static int attn_dkv_dp(const AttnArgs& a, hipStream_t s) {
-  const int rc = attn_launch(attn_dkv_kernel<T, DP>, (int64_t)a.n_items * a.kv_heads, attn_dkv_lds<T, DP>(), a, s);
+  const int rc = attn_launch(a.causal ? attn_dkv_kernel<T, DP, true> : attn_dkv_kernel<T, DP, false>, (int64_t)a.n_items * a.kv_heads, attn_dkv_lds<T, DP>(a.causal), a, s);
   if (rc != ST_OK) return rc;
   return attn_launch(attn_sum_parts_kernel<T, DP, true>, (int64_t)a.n_joins * a.kv_heads, 0, a, s);
 }
