@@ -477,34 +477,57 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
   if (a.lse && live && half == 0) a.lse[q * a.heads + head] = l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l;
 }
 
-// Partial results of split rows into the result: weights 2^(m_i - max), a thread for each four channels of a row.
+// Partial results of split rows into the result, the sums of each weighted
+// with 2^(its maximum - the largest): a thread for each four channels of a row
+// and each of kLanes shares of the parts, joined through LDS in order.  A row
+// has up to some hundred parts (few rows over many keys): serial over the parts
+// it took 33 us for 12 scenes' single queries, shared 8.
+constexpr int kAttnJoinRows = 32;  // workgroups of a tile's join
+
 template <typename T, int DP>
 __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArgs a) {
+  constexpr int QUADS = DP / 4, LANES = kAttnThreads / QUADS;
+  __shared__ v4f sums[LANES][QUADS];
+  __shared__ float tops[LANES], totals[LANES];
   const AttnJoin jn = a.joins[blockIdx.x / a.kv_heads];
   const int hk = blockIdx.x % a.kv_heads;
   const int rows = min(kAttnTile, jn.nq * a.group - jn.row0);
   const int64_t step = (int64_t)a.kv_heads * kAttnTile * (DP + 4);
-  for (int i = threadIdx.x; i < rows * (DP / 4); i += kAttnThreads) {
-    const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+  const int quad = threadIdx.x % QUADS, lane = threadIdx.x / QUADS;
+  // (m = up, both -inf for parts without keys among them, is weight 1: their sums are zero)
+  auto weight = [](float m, float up) { return m == up ? 1.f : fast_exp2(m - up); };
+  for (int row = blockIdx.y; row < rows; row += kAttnJoinRows) {
     const float* p = a.parts + (((int64_t)jn.part * a.kv_heads + hk) * kAttnTile + row) * (DP + 4);
-    float m = -INFINITY;
-    for (int k = 0; k < jn.parts; ++k) m = fmaxf(m, p[k * step + DP]);
     v4f sum = (v4f)(0.f);
-    float l = 0.f;
-    for (int k = 0; k < jn.parts; ++k) {
+    float m = -INFINITY, l = 0.f;
+    for (int k = lane; k < jn.parts && lane < LANES; k += LANES) {
       const float mk = p[k * step + DP], lk = p[k * step + DP + 1];
-      const float w = mk == -INFINITY ? (lk == 0.f ? 0.f : 1.f) : fast_exp2(mk - m);
-      l += w * lk;
-      sum += w * *reinterpret_cast<const v4f*>(p + k * step + d);
+      const v4f x = *reinterpret_cast<const v4f*>(p + k * step + quad * 4);
+      const float up = fmaxf(m, mk), w = weight(m, up), wk = weight(mk, up);
+      m = up;
+      l = w * l + wk * lk;
+      sum = w * sum + wk * x;
+    }
+    __syncthreads();
+    if (lane < LANES) {
+      sums[lane][quad] = sum;
+      if (quad == 0) tops[lane] = m, totals[lane] = l;
+    }
+    __syncthreads();
+    if (lane > 0) continue;
+    for (int k = 1; k < LANES && k < jn.parts; ++k) {
+      const float up = fmaxf(m, tops[k]), w = weight(m, up), wk = weight(tops[k], up);
+      m = up;
+      l = w * l + wk * totals[k];
+      sum = w * sum + wk * sums[k][quad];
     }
     const int r = jn.row0 + row, qi = r / a.group, head = hk * a.group + (r - qi * a.group);
     const int64_t at = (jn.q0 + (int64_t)qi) * a.heads + head;
-    const float inv = l > 0.f ? 1.f / l : l;
-    if (d < a.D) {
+    if (quad * 4 < a.D) {
       typedef T v4t __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<v4t*>((T*)a.out + at * a.D + d) = __builtin_convertvector(sum * inv, v4t);
+      *reinterpret_cast<v4t*>((T*)a.out + at * a.D + quad * 4) = __builtin_convertvector(sum * (l > 0.f ? 1.f / l : l), v4t);
     }
-    if (a.lse && d == 0) a.lse[at] = l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l;
+    if (a.lse && quad == 0) a.lse[at] = l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l;
   }
 }
 
@@ -785,30 +808,42 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP * 3 / 2>())) void a
   store_row<T, DB>((T*)a.dv + at, dv, 1.f, a.D, live);
 }
 
-// Sums of the partial gradients of split tiles, slots in order: dQ (KEYS = false), or dK and dV.
+// Sums of the partial gradients of split tiles, in a fixed order (shares of
+// the parts as above): dQ (KEYS = false), or dK and dV.
 template <typename T, int DP, bool KEYS>
 __global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a) {
   typedef T v4t __attribute__((ext_vector_type(4)));
+  constexpr int QUADS = DP / 4, LANES = kAttnThreads / QUADS, W = KEYS ? 2 : 1;
+  __shared__ v4f sums[LANES][QUADS];
   const AttnJoin jn = a.joins[blockIdx.x / a.kv_heads];
   const int hk = blockIdx.x % a.kv_heads;
   const int rows = min(kAttnTile, (KEYS ? jn.nk : jn.nq * a.group) - jn.row0);
-  constexpr int W = KEYS ? 2 : 1;
   const int64_t step = (int64_t)a.kv_heads * W * kAttnTile * DP;
-  for (int i = threadIdx.x; i < W * rows * (DP / 4); i += kAttnThreads) {
-    const int which = i / (rows * (DP / 4)), in = i - which * rows * (DP / 4);
-    const int row = in / (DP / 4), d = in % (DP / 4) * 4;
-    const float* p = a.parts + ((((int64_t)jn.part * a.kv_heads + hk) * W + which) * kAttnTile + row) * DP + d;
+  const int quad = threadIdx.x % QUADS, lane = threadIdx.x / QUADS;
+  // up to LANES parts: a whole row each for the lanes; more: the lanes share a row's
+  const bool share = jn.parts > LANES;
+  for (int i = blockIdx.y * (share ? 1 : LANES); i < W * rows; i += kAttnJoinRows * (share ? 1 : LANES)) {
+    const int in = share ? i : i + lane;
+    const int which = in >= rows, row = in - which * rows;
+    const float* p = a.parts + ((((int64_t)jn.part * a.kv_heads + hk) * W + which) * kAttnTile + row) * DP + quad * 4;
     v4f sum = (v4f)(0.f);
-    for (int k = 0; k < jn.parts; ++k) sum += *reinterpret_cast<const v4f*>(p + k * step);
-    if (d >= a.D) continue;
+    if (lane < LANES && in < W * rows)
+      for (int k = share ? lane : 0; k < jn.parts; k += share ? LANES : 1) sum += *reinterpret_cast<const v4f*>(p + k * step);
+    if (share) {
+      __syncthreads();
+      if (lane < LANES) sums[lane][quad] = sum;
+      __syncthreads();
+      for (int k = 1; k < LANES && lane == 0; ++k) sum += sums[k][quad];
+    }
+    if (lane >= (share ? 1 : LANES) || in >= W * rows || quad * 4 >= a.D) continue;
     const int r = jn.row0 + row;
     if constexpr (KEYS) {
-      const int64_t at = ((jn.k0 + (int64_t)r) * a.kv_heads + hk) * a.D + d;
+      const int64_t at = ((jn.k0 + (int64_t)r) * a.kv_heads + hk) * a.D + quad * 4;
       *reinterpret_cast<v4t*>((T*)(which ? a.dv : a.dk) + at) =
           __builtin_convertvector(which ? sum : sum * a.scale, v4t);
     } else {
       const int qi = r / a.group, head = hk * a.group + (r - qi * a.group);
-      *reinterpret_cast<v4t*>((T*)a.dq + ((jn.q0 + (int64_t)qi) * a.heads + head) * a.D + d) =
+      *reinterpret_cast<v4t*>((T*)a.dq + ((jn.q0 + (int64_t)qi) * a.heads + head) * a.D + quad * 4) =
           __builtin_convertvector(sum * a.scale, v4t);
     }
   }
@@ -817,9 +852,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a
 // ------------------------------------------------------------------ launches
 
 template <typename K>
-static int attn_launch(K kernel, int64_t blocks, int lds, const AttnArgs& a, hipStream_t s) {
+static int attn_launch(K kernel, int64_t blocks, int lds, const AttnArgs& a, hipStream_t s, int rows = 1) {
   if (blocks == 0) return ST_OK;
-  kernel<<<dim3((unsigned)blocks), kAttnThreads, lds, s>>>(a);
+  kernel<<<dim3((unsigned)blocks, rows), kAttnThreads, lds, s>>>(a);
   ST_CHECK_LAUNCH();
   return ST_OK;
 }
@@ -828,19 +863,19 @@ template <typename T, int DP>
 static int attn_forward_dp(const AttnArgs& a, hipStream_t s) {
   const int rc = attn_launch(a.causal ? attn_forward_kernel<T, DP, true> : attn_forward_kernel<T, DP, false>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(a.causal), a, s);
   if (rc != ST_OK) return rc;
-  return attn_launch(attn_forward_join_kernel<T, DP>, (int64_t)a.n_joins * a.kv_heads, 0, a, s);
+  return attn_launch(attn_forward_join_kernel<T, DP>, (int64_t)a.n_joins * a.kv_heads, 0, a, s, kAttnJoinRows);
 }
 template <typename T, int DP>
 static int attn_dq_dp(const AttnArgs& a, hipStream_t s) {
   const int rc = attn_launch(a.causal ? attn_dq_kernel<T, DP, true> : attn_dq_kernel<T, DP, false>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(a.causal), a, s);
   if (rc != ST_OK) return rc;
-  return attn_launch(attn_sum_parts_kernel<T, DP, false>, (int64_t)a.n_joins * a.kv_heads, 0, a, s);
+  return attn_launch(attn_sum_parts_kernel<T, DP, false>, (int64_t)a.n_joins * a.kv_heads, 0, a, s, kAttnJoinRows);
 }
 template <typename T, int DP>
 static int attn_dkv_dp(const AttnArgs& a, hipStream_t s) {
   const int rc = attn_launch(a.causal ? attn_dkv_kernel<T, DP, true> : attn_dkv_kernel<T, DP, false>, (int64_t)a.n_items * a.kv_heads, attn_dkv_lds<T, DP>(a.causal), a, s);
   if (rc != ST_OK) return rc;
-  return attn_launch(attn_sum_parts_kernel<T, DP, true>, (int64_t)a.n_joins * a.kv_heads, 0, a, s);
+  return attn_launch(attn_sum_parts_kernel<T, DP, true>, (int64_t)a.n_joins * a.kv_heads, 0, a, s, kAttnJoinRows);
 }
 
 enum AttnPass { kAttnForward, kAttnDq, kAttnDkv };
