@@ -237,15 +237,20 @@ struct AttnStage {
 
   static __device__ __forceinline__ int row(int i) { return (threadIdx.x + i * kAttnThreads) / Tile::CPR; }
   static __device__ __forceinline__ int chunk(int i) { return (threadIdx.x + i * kAttnThreads) % Tile::CPR; }
-  // `offset(row)`: byte offset of a row from `base`, or kOobOffset for a row of zeros
+  int off[N];  // byte offsets of this thread's chunks from the tile's first row
   template <typename F>
-  __device__ __forceinline__ void load(const T* base, int D, F offset) {
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(base, kOobOffset);
+  __device__ __forceinline__ void place(int D, F offset) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = chunk(i) * Tile::EPC, off = offset(row(i));
-      reg[i] = load16<v4u>(r, (c < D && off != kOobOffset) ? off + c * (int)sizeof(T) : kOobOffset);
+      const int c = chunk(i) * Tile::EPC;
+      off[i] = c < D ? offset(row(i)) + c * (int)sizeof(T) : kOobOffset;
     }
+  }
+  // `left` rows from `base` on, zeros after them
+  __device__ __forceinline__ void load(const T* base, int left) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base, kOobOffset);
+#pragma unroll
+    for (int i = 0; i < N; ++i) reg[i] = load16<v4u>(r, row(i) < left ? off[i] : kOobOffset);
   }
   __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
@@ -317,6 +322,21 @@ __device__ __forceinline__ int attn_work(int n) {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// For the scheduler: of N fragment reads, each followed by its MFMAs, kAhead
+// go out before the first product and one behind each product.  (Left to itself
+// it reads, waits ~130 cycles and multiplies, fragment by fragment.)
+template <typename T, int N, bool COLS = false>
+__device__ __forceinline__ void attn_reads_ahead() {
+  constexpr int kAhead = 4, READS = (COLS ? 2 : 1) * (sizeof(T) == 2 ? 1 : COLS ? 4 : 2);
+  constexpr int PRODUCTS = sizeof(T) == 2 ? 1 : 8;
+  __builtin_amdgcn_sched_group_barrier(0x100, (N < kAhead ? N : kAhead) * READS, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+    if (i + kAhead < N) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+}
+
 // Waves of a SIMD that the registers leave room for (a limit for the compiler).
 template <typename T, int DP>
 constexpr int attn_waves() {
@@ -363,19 +383,20 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
   const int see = CAUSAL ? qi + it.nk - it.nq : 0x7FFFFFFF;  // last key that this lane's row sees
 
   Stage ks, vs;
+  ks.place(a.D, [&](int x) { return x * (int)(a.k_row * sizeof(T)); });
+  vs.place(a.D, [&](int x) { return x * (int)(a.v_row * sizeof(T)); });
   uint8_t chunk_kept[Stage::N], key_kept = 1;
   const uint8_t* mask = a.key_mask ? a.key_mask + it.k0 : nullptr;
   auto fetch = [&](int kt) {
     const int left = it.hi - kt;
     const int64_t row = it.k0 + (int64_t)kt;
-    const int krow = (int)(a.k_row * sizeof(T)), vrow = (int)(a.v_row * sizeof(T));
     if (mask) {
 #pragma unroll
       for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[kt + Stage::row(i)] : 0;
       key_kept = lane < left ? mask[kt + lane] : 0;
     }
-    ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, a.D, [&](int x) { return x < left ? x * krow : kOobOffset; });
-    vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, a.D, [&](int x) { return x < left ? x * vrow : kOobOffset; });
+    ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, left);
+    vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, left);
   };
 
   v16f o[DB];
@@ -403,11 +424,12 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
 
     v16f s[NB];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      s[b] = (v16f)(0.f);
+    for (int b = 0; b < NB; ++b) s[b] = (v16f)(0.f);
 #pragma unroll
-      for (int i = 0; i < KS; ++i) s[b] = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s[b]);
-    }
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) s[b] = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s[b]);
+    attn_reads_ahead<T, NB * KS>();
     const bool cut = CAUSAL && __any(see - kt < kAttnKeys - 1);  // by the causal order
     const int last = see - kt;
     const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
@@ -436,13 +458,15 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
         for (int e = 0; e < 16; ++e) o[b][e] *= shrink;
     }
     const float base = m == -INFINITY ? 0.f : -m;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[b][e] = fast_exp2(fmaf(s[b][e], a.scale_log2, base));
-        l += s[b][e];
+        sum[e & 3] += s[b][e];
       }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     const T* vp = vl;
     if (cut && attn_not_finite<T, kAttnKeys, DP>(vl)) {
       attn_copy_finite<T, kAttnKeys, DP>(vl, tiles + 4 * TILE);
@@ -457,6 +481,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = mma32(Tile::cols(vp, b * 32 + 16 * j, d * 32), p, o[d]);
       }
+    attn_reads_ahead<T, NB * 2 * DB, true>();
   }
 
   if (CAUSAL) left_out.apply(o);
@@ -575,19 +600,20 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_k
   const int see = CAUSAL ? qi + it.nk - it.nq : 0x7FFFFFFF;
 
   Stage ks, vs;
+  ks.place(a.D, [&](int x) { return x * (int)(a.k_row * sizeof(T)); });
+  vs.place(a.D, [&](int x) { return x * (int)(a.v_row * sizeof(T)); });
   uint8_t chunk_kept[Stage::N], key_kept = 1;
   const uint8_t* mask = a.key_mask ? a.key_mask + it.k0 : nullptr;
   auto fetch = [&](int kt) {
     const int left = it.hi - kt;
     const int64_t row = it.k0 + (int64_t)kt;
-    const int krow = (int)(a.k_row * sizeof(T)), vrow = (int)(a.v_row * sizeof(T));
     if (mask) {
 #pragma unroll
       for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[kt + Stage::row(i)] : 0;
       key_kept = lane < left ? mask[kt + lane] : 0;
     }
-    ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, a.D, [&](int x) { return x < left ? x * krow : kOobOffset; });
-    vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, a.D, [&](int x) { return x < left ? x * vrow : kOobOffset; });
+    ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, left);
+    vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, left);
   };
 
   v16f dq[DB];
@@ -626,6 +652,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_k
         s = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s);
         dp = mma32(Tile::rows(vl, b * 32 + (lane & 31), 16 * i + 8 * half), gf[i], dp);
       }
+      attn_reads_ahead<T, 2 * KS>();
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], a.scale_log2, -lse)) * (dp[e] - delta);
       if (cut || seen != ~0ull) {
@@ -639,6 +666,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_k
 #pragma unroll
         for (int d = 0; d < DB; ++d) dq[d] = mma32(Tile::cols(kp, b * 32 + 16 * j, d * 32), ds, dq[d]);
       }
+      attn_reads_ahead<T, 2 * DB, true>();
     }
   }
 
@@ -697,28 +725,26 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP * 3 / 2>())) void a
 
   Stage qs, gs;
   float stat = 0.f;
-  const int qrow = (int)(a.q_row * sizeof(T)), qhead = (int)(a.q_head * sizeof(T));
-  const int grow = (int)(a.do_row * sizeof(T)), ghead = (int)(a.do_head * sizeof(T));
   const unsigned inv = (unsigned)(((1ull << 32) + a.group - 1) / a.group);  // x / group = x * inv >> 32 (group > 1)
+  auto place = [&](int h0) {  // packed rows from head h0 of a query on
+    auto offset = [&](int x, int64_t row, int64_t head) {
+      const int dq = a.group > 1 ? (int)__umulhi((unsigned)(h0 + x), inv) : x, dh = h0 + x - dq * a.group;
+      return dq * (int)(row * sizeof(T)) + dh * (int)(head * sizeof(T));
+    };
+    qs.place(a.D, [&](int x) { return offset(x, a.q_row, a.q_head); });
+    gs.place(a.D, [&](int x) { return offset(x, a.do_row, a.do_head); });
+  };
+  const bool same_heads = BQ % a.group == 0;  // every step begins at the same head
+  place(it.lo % a.group);
   auto fetch = [&](int rt) {
     const int left = it.hi - rt, q0 = rt / a.group, h0 = rt - q0 * a.group;
     const int64_t q = it.q0 + (int64_t)q0;
-    auto split = [&](int x, int& dq, int& dh) {
-      dq = a.group > 1 ? (int)__umulhi((unsigned)(h0 + x), inv) : x;
-      dh = h0 + x - dq * a.group;
-    };
-    auto offset = [&](int x, int row, int head) {
-      int dq, dh;
-      split(x, dq, dh);
-      return x < left ? dq * row + dh * head : kOobOffset;
-    };
-    qs.load((const T*)a.q + q * a.q_row + (int64_t)hk * a.group * a.q_head, a.D, [&](int x) { return offset(x, qrow, qhead); });
-    gs.load((const T*)a.dout + q * a.do_row + (int64_t)hk * a.group * a.do_head, a.D,
-            [&](int x) { return offset(x, grow, ghead); });
+    if (!same_heads) place(h0);
+    qs.load((const T*)a.q + q * a.q_row + (int64_t)hk * a.group * a.q_head, left);
+    gs.load((const T*)a.dout + q * a.do_row + (int64_t)hk * a.group * a.do_head, left);
     if (threadIdx.x < 2 * BQ) {
       const int x = threadIdx.x & (BQ - 1);
-      int dq, dh;
-      split(x, dq, dh);
+      const int dq = a.group > 1 ? (int)__umulhi((unsigned)(h0 + x), inv) : x, dh = h0 + x - dq * a.group;
       const int64_t at = (q + dq) * a.heads + hk * a.group + dh;
       // (a row past the end: L = inf makes its P zero)
       stat = threadIdx.x < BQ ? (x < left ? a.lse[at] : INFINITY) : (x < left ? a.delta[at] : 0.f);
@@ -756,6 +782,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP * 3 / 2>())) void a
         s = mma32(Tile::rows(ql, b * 32 + (lane & 31), 16 * i + 8 * half), kf[i], s);
         dp = mma32(Tile::rows(gl, b * 32 + (lane & 31), 16 * i + 8 * half), vf[i], dp);
       }
+      attn_reads_ahead<T, 2 * KS>();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const v4f L = *reinterpret_cast<const v4f*>(st + b * 32 + 8 * j + 4 * half);
@@ -772,6 +799,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP * 3 / 2>())) void a
 #pragma unroll
         for (int d = 0; d < DB; ++d) dv[d] = mma32(Tile::cols(gp, b * 32 + 16 * j, d * 32), p, dv[d]);
       }
+      attn_reads_ahead<T, 2 * DB, true>();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const v4f dl = *reinterpret_cast<const v4f*>(st + BQ + b * 32 + 8 * j + 4 * half);
@@ -788,6 +816,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP * 3 / 2>())) void a
 #pragma unroll
         for (int d = 0; d < DB; ++d) dk[d] = mma32(Tile::cols(qp, b * 32 + 16 * j, d * 32), ds, dk[d]);
       }
+      attn_reads_ahead<T, 2 * DB, true>();
     }
   }
 
