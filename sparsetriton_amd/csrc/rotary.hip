@@ -17,9 +17,11 @@ namespace st {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotTable = 2048;  // cosine / sine pairs in LDS (16 KB)
-// (256 / 512 / 1,024 / 2,048 vectors: 470,532 rows x 16 x 32 bf16 174 / 181 / 186 / 192 us, 60,001 rows x
-// 12 x 48 fp32 interleaved 94 / 63 / 68 / 75: too few leave threads idle, too many an uneven last round)
-constexpr int kRotItems = 512;   // vectors of a workgroup's rows, about: two a thread
+// Vectors of a workgroup's rows, about, and of a thread's batch.  470,532 rows x 16 x 32 bf16 and 60,001
+// rows x 12 x 48 fp32 interleaved: 178 and 45 us; batches of one 184 and 47; 1,024 vectors 189 and 44
+// (bf16: an uneven last round of workgroups); one vector at a time, loads behind stores: 181 and 72.
+constexpr int kRotItems = 512;
+constexpr int kRotBatch = 2;
 
 template <typename T>
 struct RotArgs {
@@ -39,8 +41,8 @@ struct RotArgs {
 };
 
 template <typename T, int V>
-struct alignas(sizeof(T) * V) RotVec {
-  T e[V];
+struct RotVec {
+  typedef T type __attribute__((ext_vector_type(V)));
 };
 
 __device__ __forceinline__ double rot_pos(const int16_t* p, int a) { return p[a]; }
@@ -50,10 +52,76 @@ __device__ __forceinline__ double rot_pos(const float* p, int a) { return p[a]; 
 
 template <typename T, typename PT, int V, bool INTERLEAVED, bool INVERSE>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs<T> g) {
-  using Vec = RotVec<T, V>;
+  using Vec = typename RotVec<T, V>::type;
   __shared__ float2 table[kRotTable];
   const int64_t row0 = (int64_t)blockIdx.x * g.rows;
   const int rows = g.n - row0 < g.rows ? (int)(g.n - row0) : g.rows;
+  const int pair_chunks = INTERLEAVED ? 2 * g.P / V : g.P / V;
+  const int items = rows * g.per_row;
+  // A thread's next two vectors: their loads all go out before the first store
+  // (the compiler keeps a load behind an earlier store), those of the first two
+  // before the table is made.
+  Vec xa[kRotBatch], xb[kRotBatch];  // a pair's channels, where they are not in one vector
+  T* out[kRotBatch];
+  int chunk[kRotBatch], at[kRotBatch];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kRotBatch; ++u) {
+      const int i = i0 + u * kRotThreads;
+      if (i < items) {
+        const int r = (int)((uint64_t)i * g.per_row_inv >> 32);
+        const int in_row = i - r * g.per_row;
+        int h = (int)((uint64_t)in_row * g.chunks_inv >> 32);
+        const int ch = in_row - h * g.chunks;
+        const int which = h >= g.heads[0];
+        h -= which ? g.heads[0] : 0;
+        const int d = ch < pair_chunks ? ch * V : 2 * g.P + (ch - pair_chunks) * V;
+        const T* in = g.in[which] + (row0 + r) * g.in_row[which] + h * g.in_head[which] + d;
+        out[u] = g.out[which] + ((row0 + r) * g.heads[which] + h) * g.D + d;
+        chunk[u] = ch;
+        at[u] = r * g.P;
+        xa[u] = *reinterpret_cast<const Vec*>(in);
+        if (!INTERLEAVED && ch < pair_chunks) xb[u] = *reinterpret_cast<const Vec*>(in + g.P);
+        if (INTERLEAVED && V == 1 && ch < pair_chunks) xb[u] = *reinterpret_cast<const Vec*>(ch & 1 ? in - 1 : in + 1);
+      }
+    }
+  };
+  auto turn = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kRotBatch; ++u) {
+      if (i0 + u * kRotThreads < items) {
+        const int ch = chunk[u];
+        const float2* t = table + at[u];
+        if (ch < pair_chunks) {
+          if constexpr (INTERLEAVED && V > 1) {
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+              const float2 cs = t[ch * (V / 2) + e / 2];
+              const float a = (float)xa[u][e], b = (float)xa[u][e + 1];
+              xa[u][e] = (T)(a * cs.x - b * cs.y);
+              xa[u][e + 1] = (T)(a * cs.y + b * cs.x);
+            }
+          } else if constexpr (INTERLEAVED) {
+            const float2 cs = t[ch >> 1];
+            const float a = (float)xa[u][0], b = (float)xb[u][0];
+            xa[u][0] = (T)((ch & 1) ? b * cs.y + a * cs.x : a * cs.x - b * cs.y);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float2 cs = t[ch * V + e];
+              const float a = (float)xa[u][e], b = (float)xb[u][e];
+              xa[u][e] = (T)(a * cs.x - b * cs.y);
+              xb[u][e] = (T)(a * cs.y + b * cs.x);
+            }
+            *reinterpret_cast<Vec*>(out[u] + g.P) = xb[u];
+          }
+        }
+        *reinterpret_cast<Vec*>(out[u]) = xa[u];
+      }
+    }
+  };
+
+  load(threadIdx.x);
   for (int i = threadIdx.x; i < rows * g.P; i += kRotThreads) {
     const int r = i / g.P, p = i - r * g.P;
     const PT* pos = (const PT*)g.pos + (row0 + r) * g.pos_row;
@@ -63,49 +131,10 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs<T> g) {
     table[i] = make_float2(c, INVERSE ? -s : s);
   }
   __syncthreads();
-  const int pair_chunks = INTERLEAVED ? 2 * g.P / V : g.P / V;
-  for (int i = threadIdx.x; i < rows * g.per_row; i += kRotThreads) {
-    const int r = (int)((uint64_t)i * g.per_row_inv >> 32);
-    const int in_row = i - r * g.per_row;
-    int h = (int)((uint64_t)in_row * g.chunks_inv >> 32);
-    const int ch = in_row - h * g.chunks;
-    const int which = h >= g.heads[0];
-    h -= which ? g.heads[0] : 0;
-    const T* in = g.in[which] + (row0 + r) * g.in_row[which] + h * g.in_head[which];
-    T* out = g.out[which] + ((row0 + r) * g.heads[which] + h) * g.D;
-    const float2* t = table + r * g.P;
-    if (ch >= pair_chunks) {
-      const int d = 2 * g.P + (ch - pair_chunks) * V;
-      *reinterpret_cast<Vec*>(out + d) = *reinterpret_cast<const Vec*>(in + d);
-    } else if constexpr (INTERLEAVED && V > 1) {
-      const Vec x = *reinterpret_cast<const Vec*>(in + ch * V);
-      Vec y;
-#pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float2 cs = t[ch * (V / 2) + e / 2];
-        const float a = (float)x.e[e], b = (float)x.e[e + 1];
-        y.e[e] = (T)(a * cs.x - b * cs.y);
-        y.e[e + 1] = (T)(a * cs.y + b * cs.x);
-      }
-      *reinterpret_cast<Vec*>(out + ch * V) = y;
-    } else if constexpr (INTERLEAVED) {  // one channel, its partner read beside it
-      const float2 cs = t[ch >> 1];
-      const float x = (float)in[ch], other = (float)in[ch ^ 1];
-      out[ch] = (T)((ch & 1) ? other * cs.y + x * cs.x : x * cs.x - other * cs.y);
-    } else {
-      const int p = ch * V;
-      const Vec xa = *reinterpret_cast<const Vec*>(in + p), xb = *reinterpret_cast<const Vec*>(in + g.P + p);
-      Vec ya, yb;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float2 cs = t[p + e];
-        const float a = (float)xa.e[e], b = (float)xb.e[e];
-        ya.e[e] = (T)(a * cs.x - b * cs.y);
-        yb.e[e] = (T)(a * cs.y + b * cs.x);
-      }
-      *reinterpret_cast<Vec*>(out + p) = ya;
-      *reinterpret_cast<Vec*>(out + g.P + p) = yb;
-    }
+  turn(threadIdx.x);
+  for (int i0 = threadIdx.x + kRotBatch * kRotThreads; i0 < items; i0 += kRotBatch * kRotThreads) {
+    load(i0);
+    turn(i0);
   }
 }
 
