@@ -898,7 +898,8 @@ int st_rotary(const st_rotary_args* args, st_stream_t stream);
  * All sums are in a fixed order.
  */
 #define ST_ATTN_TILE 128
-#define ST_ATTN_KEYS 64
+#define ST_ATTN_SMALL_TILE 32
+#define ST_ATTN_SMALL_TILE_BYTES 128 /* of a head's row: wider ones take ST_ATTN_TILE only */
 #define ST_ATTN_MAX_DIM 128
 #define ST_ATTN_ITEM_WORDS 8
 #define ST_ATTN_JOIN_WORDS 8
@@ -922,6 +923,7 @@ typedef struct st_attn_args {
   int64_t n_q_items, n_q_joins, n_k_items, n_k_joins;
   float* parts;
   int32_t heads, kv_heads, dim, dtype, causal;
+  int32_t q_tile, k_tile; /* ST_ATTN_TILE, or ST_ATTN_SMALL_TILE for segments of few rows (keys) */
   float scale;
 } st_attn_args;
 int st_attn_workspace(int kv_heads, int dim, int64_t q_parts, int64_t k_parts, int64_t* floats);

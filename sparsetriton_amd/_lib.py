@@ -33,7 +33,7 @@ GATHER_B_KN = 2
 COLUMN_SUM_NOALLOC_MAX_C = 2048
 MAX_KVOL = 512
 TILE_ROWS = 128
-ATTN_TILE, ATTN_KEYS, ATTN_MAX_DIM, ATTN_WORDS = 128, 64, 128, 8
+ATTN_TILE, ATTN_SMALL_TILE, ATTN_SMALL_TILE_BYTES, ATTN_MAX_DIM, ATTN_WORDS = 128, 32, 128, 128, 8
 
 
 class OutGeom(ctypes.Structure):
@@ -81,7 +81,7 @@ class AttnArgs(ctypes.Structure):
         + [(n, _P) for n in ("key_mask", "q_items", "q_joins", "k_items", "k_joins")]
         + [(n, _L) for n in ("n_q_items", "n_q_joins", "n_k_items", "n_k_joins")]
         + [("parts", _P)]
-        + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "dtype", "causal")]
+        + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "dtype", "causal", "q_tile", "k_tile")]
         + [("scale", ctypes.c_float)]
     )
 

@@ -38,8 +38,11 @@ typedef float v8f __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 
-constexpr int kAttnThreads = 256;
-constexpr int kAttnTile = ST_ATTN_TILE;  // rows (or keys) of a workgroup: 32 for each of four waves
+// Rows (or keys) of a workgroup: 32 for each of its waves, four of them or one.
+// Four share the tiles in LDS; one alone is for segments that would leave most of
+// the four without rows (a workgroup's latency, not its work, is the cost there).
+constexpr int kAttnTile = ST_ATTN_TILE;
+constexpr int kAttnThreads = 256;  // of the joins
 
 struct AttnItem {  // ST_ATTN_ITEM_WORDS int32, written by the host
   int q0, nq;      // the segment's first query row and their number
@@ -64,6 +67,7 @@ struct AttnArgs {
   const AttnJoin* joins;
   int n_items, n_joins;
   int heads, kv_heads, group, D, causal;
+  int tile;  // rows of the items' tiles: ST_ATTN_TILE or ST_ATTN_SMALL_TILE
   float scale, scale_log2;  // c and c / ln 2
 };
 
@@ -228,15 +232,15 @@ struct AttnNotFinite {
 };
 
 // Rows of a tile on their way from memory to LDS: each thread carries N chunks.
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, int WAVES>
 struct AttnStage {
   using Tile = AttnTile<T, DP>;
-  static constexpr int N = ROWS * Tile::CPR / kAttnThreads;
-  static_assert(ROWS * Tile::CPR % kAttnThreads == 0, "whole chunks a thread");
+  static constexpr int THREADS = 64 * WAVES, N = ROWS * Tile::CPR / THREADS;
+  static_assert(ROWS * Tile::CPR % THREADS == 0, "whole chunks a thread");
   v4u reg[N];
 
-  static __device__ __forceinline__ int row(int i) { return (threadIdx.x + i * kAttnThreads) / Tile::CPR; }
-  static __device__ __forceinline__ int chunk(int i) { return (threadIdx.x + i * kAttnThreads) % Tile::CPR; }
+  static __device__ __forceinline__ int row(int i) { return (threadIdx.x + i * THREADS) / Tile::CPR; }
+  static __device__ __forceinline__ int chunk(int i) { return (threadIdx.x + i * THREADS) % Tile::CPR; }
   int off[N];  // byte offsets of this thread's chunks from the tile's first row
   template <typename F>
   __device__ __forceinline__ void place(int D, F offset) {
@@ -302,8 +306,9 @@ __device__ __forceinline__ void store_row(T* row, const v16f (&acc)[DB], float s
 }
 // The same as fp32 partial sums at a row of DP floats.
 template <int DB>
-__device__ __forceinline__ void store_part(float* row, const v16f (&acc)[DB]) {
+__device__ __forceinline__ void store_part(float* row, const v16f (&acc)[DB], bool live) {
   const int half = (threadIdx.x >> 5) & 1;
+  if (!live) return;
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
@@ -345,11 +350,15 @@ constexpr int attn_waves() {
 
 // ------------------------------------------------------------------ forward
 
-constexpr int kAttnKeys = ST_ATTN_KEYS;  // keys of a step
+// Keys of a step: 64, or 32 for a wave alone (its lanes carry the whole step on its way to LDS).
+template <int WAVES>
+constexpr int attn_keys() {
+  return WAVES == 1 ? 32 : 64;
+}
 
-template <typename T, int DP>
+template <typename T, int DP, int WAVES>
 constexpr int attn_fwd_lds(bool causal) {  // two buffers of K and V, a copy of one of them
-  return (causal ? 5 : 4) * kAttnKeys * DP * (int)sizeof(T);
+  return (causal ? 5 : 4) * attn_keys<WAVES>() * DP * (int)sizeof(T);
 }
 
 // A running maximum is raised only when a row's maximum passes it by more
@@ -357,13 +366,14 @@ constexpr int attn_fwd_lds(bool causal) {  // two buffers of K and V, a copy of 
 // floating point, and the accumulators need no rescaling.
 constexpr float kAttnSlack = 8.f;
 
-template <typename T, int DP, bool CAUSAL>
-__global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forward_kernel(AttnArgs a) {
+template <typename T, int DP, bool CAUSAL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forward_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
-  using Stage = AttnStage<T, DP, kAttnKeys>;
-  constexpr int KS = DP / 16, DB = DP / 32, NB = kAttnKeys / 32;
-  constexpr int TILE = kAttnKeys * DP;
+  constexpr int BK = attn_keys<WAVES>();
+  using Stage = AttnStage<T, DP, BK, WAVES>;
+  constexpr int KS = DP / 16, DB = DP / 32, NB = BK / 32;
+  constexpr int TILE = BK * DP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
 
@@ -405,11 +415,12 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
   float m = -INFINITY, l = 0.f;
   AttnNotFinite left_out;
   if (it.lo < it.hi) fetch(it.lo);
-  for (int kt = it.lo, buf = 0; kt < it.hi; kt += kAttnKeys, buf ^= 1) {
+  for (int kt = it.lo, buf = 0; kt < it.hi; kt += BK, buf ^= 1) {
     T* kl = tiles + buf * 2 * TILE;
     T* vl = kl + TILE;
-    uint64_t seen = ~0ull;  // keys of this step that exist and are not masked
-    if (it.hi - kt < kAttnKeys) seen >>= kAttnKeys - (it.hi - kt);
+    constexpr uint64_t ALL = ~0ull >> (64 - BK);
+    uint64_t seen = ALL;  // keys of this step that exist and are not masked
+    if (it.hi - kt < BK) seen >>= BK - (it.hi - kt);
     if (mask) {
       seen &= __ballot(key_kept);
 #pragma unroll
@@ -419,7 +430,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
     ks.store(kl);
     vs.store(vl);
     __syncthreads();
-    if (kt + kAttnKeys < it.hi) fetch(kt + kAttnKeys);
+    if (kt + BK < it.hi) fetch(kt + BK);
     if (!active || (CAUSAL && !__any(live && kt <= see))) continue;
 
     v16f s[NB];
@@ -430,10 +441,10 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
 #pragma unroll
       for (int b = 0; b < NB; ++b) s[b] = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s[b]);
     attn_reads_ahead<T, NB * KS>();
-    const bool cut = CAUSAL && __any(see - kt < kAttnKeys - 1);  // by the causal order
+    const bool cut = CAUSAL && __any(see - kt < BK - 1);  // by the causal order
     const int last = see - kt;
     const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
-    if (cut || seen != ~0ull) {
+    if (cut || seen != ALL) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
@@ -468,10 +479,10 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
       }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     const T* vp = vl;
-    if (cut && attn_not_finite<T, kAttnKeys, DP>(vl)) {
-      attn_copy_finite<T, kAttnKeys, DP>(vl, tiles + 4 * TILE);
+    if (cut && attn_not_finite<T, BK, DP>(vl)) {
+      attn_copy_finite<T, BK, DP>(vl, tiles + 4 * TILE);
       vp = tiles + 4 * TILE;
-      left_out.add<T, kAttnKeys, DP>(vl, 0, last);
+      left_out.add<T, BK, DP>(vl, 0, last);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -489,8 +500,8 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
   if (it.part >= 0) {
     // a row of DP sums, then its maximum (in powers of two) and sum
     float* row = a.parts + (((int64_t)it.part * a.kv_heads + hk) * kAttnTile + wave * 32 + (lane & 31)) * (DP + 4);
-    store_part<DB>(row, o);
-    if (half == 0) {
+    store_part<DB>(row, o, live);
+    if (live && half == 0) {
       row[DP] = m;
       row[DP + 1] = l;
     }
@@ -503,11 +514,13 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_forw
 }
 
 // Partial results of split rows into the result, the sums of each weighted
-// with 2^(its maximum - the largest): a thread for each four channels of a row
-// and each of kLanes shares of the parts, joined through LDS in order.  A row
-// has up to some hundred parts (few rows over many keys): serial over the parts
-// it took 33 us for 12 scenes' single queries, shared 8.
-constexpr int kAttnJoinRows = 32;  // workgroups of a tile's join
+// with 2^(its maximum - the largest): a thread for each four channels.  A row
+// has up to some hundred parts (few rows over many keys): more than kAttnFewParts
+// are shared between the lanes and joined through LDS in order, fewer are a
+// lane's own, and the lanes take rows.  (12 single queries of ~100 parts: 33 us
+// unshared, 7 shared; 300 queries x 8 heads of up to 29 parts: 47 and 9 us.)
+constexpr int kAttnJoinBlocks = 48;  // workgroups of a tile's join
+constexpr int kAttnFewParts = 16;
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArgs a) {
@@ -516,36 +529,52 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArg
   __shared__ float tops[LANES], totals[LANES];
   const AttnJoin jn = a.joins[blockIdx.x / a.kv_heads];
   const int hk = blockIdx.x % a.kv_heads;
-  const int rows = min(kAttnTile, jn.nq * a.group - jn.row0);
+  const int rows = min(a.tile, jn.nq * a.group - jn.row0);
   const int64_t step = (int64_t)a.kv_heads * kAttnTile * (DP + 4);
   const int quad = threadIdx.x % QUADS, lane = threadIdx.x / QUADS;
+  const bool share = jn.parts > kAttnFewParts;
+  const int stride = share ? 1 : LANES;  // rows of a workgroup at once
   // (m = up, both -inf for parts without keys among them, is weight 1: their sums are zero)
   auto weight = [](float m, float up) { return m == up ? 1.f : fast_exp2(m - up); };
-  for (int row = blockIdx.y; row < rows; row += kAttnJoinRows) {
+  for (int row0 = blockIdx.y * stride; row0 < rows; row0 += kAttnJoinBlocks * stride) {
+    const int row = share ? row0 : row0 + lane;
     const float* p = a.parts + (((int64_t)jn.part * a.kv_heads + hk) * kAttnTile + row) * (DP + 4);
     v4f sum = (v4f)(0.f);
     float m = -INFINITY, l = 0.f;
-    for (int k = lane; k < jn.parts && lane < LANES; k += LANES) {
-      const float mk = p[k * step + DP], lk = p[k * step + DP + 1];
-      const v4f x = *reinterpret_cast<const v4f*>(p + k * step + quad * 4);
-      const float up = fmaxf(m, mk), w = weight(m, up), wk = weight(mk, up);
+    if (lane < LANES && row < rows)
+      for (int k = share ? lane : 0; k < jn.parts; k += share ? LANES : 1) {
+        const float mk = p[k * step + DP], lk = p[k * step + DP + 1];
+        const v4f x = *reinterpret_cast<const v4f*>(p + k * step + quad * 4);
+        const float up = fmaxf(m, mk), w = weight(m, up), wk = weight(mk, up);
+        m = up;
+        l = w * l + wk * lk;
+        sum = w * sum + wk * x;
+      }
+    if (share) {
+      __syncthreads();
+      if (lane < LANES && quad == 0) tops[lane] = m;
+      __syncthreads();
+      float up = tops[0];
+#pragma unroll
+      for (int k = 1; k < LANES; ++k) up = fmaxf(up, tops[k]);
+      const float w = weight(m, up);
+      if (lane < LANES) {
+        sums[lane][quad] = w * sum;
+        if (quad == 0) totals[lane] = w * l;
+      }
+      __syncthreads();
       m = up;
-      l = w * l + wk * lk;
-      sum = w * sum + wk * x;
+      if (lane == 0) {
+        l = totals[0];
+        sum = sums[0][quad];
+#pragma unroll
+        for (int k = 1; k < LANES; ++k) {
+          l += totals[k];
+          sum += sums[k][quad];
+        }
+      }
     }
-    __syncthreads();
-    if (lane < LANES) {
-      sums[lane][quad] = sum;
-      if (quad == 0) tops[lane] = m, totals[lane] = l;
-    }
-    __syncthreads();
-    if (lane > 0) continue;
-    for (int k = 1; k < LANES && k < jn.parts; ++k) {
-      const float up = fmaxf(m, tops[k]), w = weight(m, up), wk = weight(tops[k], up);
-      m = up;
-      l = w * l + wk * totals[k];
-      sum = w * sum + wk * sums[k][quad];
-    }
+    if (lane >= stride || row >= rows) continue;
     const int r = jn.row0 + row, qi = r / a.group, head = hk * a.group + (r - qi * a.group);
     const int64_t at = (jn.q0 + (int64_t)qi) * a.heads + head;
     if (quad * 4 < a.D) {
@@ -559,13 +588,14 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArg
 // ------------------------------------------------------------------ backward: queries
 
 // dQ of a tile of rows, and delta = rowsum(dO o O) for the keys' pass after it.
-template <typename T, int DP, bool CAUSAL>
-__global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_kernel(AttnArgs a) {
+template <typename T, int DP, bool CAUSAL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
-  using Stage = AttnStage<T, DP, kAttnKeys>;
-  constexpr int KS = DP / 16, DB = DP / 32, NB = kAttnKeys / 32;
-  constexpr int TILE = kAttnKeys * DP;
+  constexpr int BK = attn_keys<WAVES>();
+  using Stage = AttnStage<T, DP, BK, WAVES>;
+  constexpr int KS = DP / 16, DB = DP / 32, NB = BK / 32;
+  constexpr int TILE = BK * DP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
 
@@ -620,11 +650,12 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_k
 #pragma unroll
   for (int b = 0; b < DB; ++b) dq[b] = (v16f)(0.f);
   if (it.lo < it.hi) fetch(it.lo);
-  for (int kt = it.lo, buf = 0; kt < it.hi; kt += kAttnKeys, buf ^= 1) {
+  for (int kt = it.lo, buf = 0; kt < it.hi; kt += BK, buf ^= 1) {
     T* kl = tiles + buf * 2 * TILE;
     T* vl = kl + TILE;
-    uint64_t seen = ~0ull;
-    if (it.hi - kt < kAttnKeys) seen >>= kAttnKeys - (it.hi - kt);
+    constexpr uint64_t ALL = ~0ull >> (64 - BK);
+    uint64_t seen = ALL;
+    if (it.hi - kt < BK) seen >>= BK - (it.hi - kt);
     if (mask) {
       seen &= __ballot(key_kept);
 #pragma unroll
@@ -634,14 +665,14 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_k
     ks.store(kl);
     vs.store(vl);
     __syncthreads();
-    if (kt + kAttnKeys < it.hi) fetch(kt + kAttnKeys);
+    if (kt + BK < it.hi) fetch(kt + BK);
     if (!active || (CAUSAL && !__any(live && kt <= see))) continue;
-    const bool cut = CAUSAL && __any(see - kt < kAttnKeys - 1);
+    const bool cut = CAUSAL && __any(see - kt < BK - 1);
     const int last = see - kt;
     const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
     const T* kp = kl;  // (a row that sees a key that is not finite has a dS that is not)
-    if (cut && attn_not_finite<T, kAttnKeys, DP>(kl)) {
-      attn_copy_finite<T, kAttnKeys, DP>(kl, tiles + 4 * TILE);
+    if (cut && attn_not_finite<T, BK, DP>(kl)) {
+      attn_copy_finite<T, BK, DP>(kl, tiles + 4 * TILE);
       kp = tiles + 4 * TILE;
     }
 #pragma unroll 1
@@ -655,7 +686,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_k
       attn_reads_ahead<T, 2 * KS>();
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], a.scale_log2, -lse)) * (dp[e] - delta);
-      if (cut || seen != ~0ull) {
+      if (cut || seen != ALL) {
         const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = (bits >> reg_row(e, 0)) & 1 ? s[e] : 0.f;
@@ -672,7 +703,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_k
 
   if (it.part >= 0) {
     store_part<DB>(
-        a.parts + (((int64_t)it.part * a.kv_heads + hk) * kAttnTile + wave * 32 + (lane & 31)) * DP, dq);
+        a.parts + (((int64_t)it.part * a.kv_heads + hk) * kAttnTile + wave * 32 + (lane & 31)) * DP, dq, live);
     return;
   }
   if (!active) return;
@@ -681,23 +712,24 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP>())) void attn_dq_k
 
 // ------------------------------------------------------------------ backward: keys
 
-template <typename T, int DP>
+template <typename T, int DP, int WAVES>
 constexpr int attn_q_rows() {  // packed rows of a step
+  if (WAVES == 1) return 32;
   return DP * (int)sizeof(T) <= 192 ? 64 : 32;
 }
-template <typename T, int DP>
+template <typename T, int DP, int WAVES>
 constexpr int attn_dkv_lds(bool causal) {
-  return attn_q_rows<T, DP>() * ((causal ? 6 : 4) * DP * (int)sizeof(T) + 4 * 4);
+  return attn_q_rows<T, DP, WAVES>() * ((causal ? 6 : 4) * DP * (int)sizeof(T) + 4 * 4);
 }
 
 // dK and dV of a tile of keys: the waves hold 32 keys each (K, V and both sums in
 // registers) while the packed rows' Q, dO, L and delta go by through LDS.
-template <typename T, int DP, bool CAUSAL>
-__global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP * 3 / 2>())) void attn_dkv_kernel(AttnArgs a) {
+template <typename T, int DP, bool CAUSAL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void attn_dkv_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
-  constexpr int BQ = attn_q_rows<T, DP>();
-  using Stage = AttnStage<T, DP, BQ>;
+  constexpr int BQ = attn_q_rows<T, DP, WAVES>();
+  using Stage = AttnStage<T, DP, BQ, WAVES>;
   constexpr int KS = DP / 16, DB = DP / 32, NB = BQ / 32;
   constexpr int TILE = BQ * DP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -827,8 +859,8 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<T, DP * 3 / 2>())) void a
   }
   if (it.part >= 0) {
     float* row = a.parts + ((((int64_t)it.part * a.kv_heads + hk) * 2) * kAttnTile + wave * 32 + (lane & 31)) * DP;
-    store_part<DB>(row, dk);
-    store_part<DB>(row + kAttnTile * DP, dv);
+    store_part<DB>(row, dk, live);
+    store_part<DB>(row + kAttnTile * DP, dv, live);
     return;
   }
   if (!active) return;
@@ -846,12 +878,11 @@ __global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a
   __shared__ v4f sums[LANES][QUADS];
   const AttnJoin jn = a.joins[blockIdx.x / a.kv_heads];
   const int hk = blockIdx.x % a.kv_heads;
-  const int rows = min(kAttnTile, (KEYS ? jn.nk : jn.nq * a.group) - jn.row0);
+  const int rows = min(a.tile, (KEYS ? jn.nk : jn.nq * a.group) - jn.row0);
   const int64_t step = (int64_t)a.kv_heads * W * kAttnTile * DP;
   const int quad = threadIdx.x % QUADS, lane = threadIdx.x / QUADS;
-  // up to LANES parts: a whole row each for the lanes; more: the lanes share a row's
-  const bool share = jn.parts > LANES;
-  for (int i = blockIdx.y * (share ? 1 : LANES); i < W * rows; i += kAttnJoinRows * (share ? 1 : LANES)) {
+  const bool share = jn.parts > kAttnFewParts;  // as the forward's join
+  for (int i = blockIdx.y * (share ? 1 : LANES); i < W * rows; i += kAttnJoinBlocks * (share ? 1 : LANES)) {
     const int in = share ? i : i + lane;
     const int which = in >= rows, row = in - which * rows;
     const float* p = a.parts + ((((int64_t)jn.part * a.kv_heads + hk) * W + which) * kAttnTile + row) * DP + quad * 4;
@@ -880,48 +911,52 @@ __global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a
 
 // ------------------------------------------------------------------ launches
 
+enum AttnPass { kAttnForward, kAttnDq, kAttnDkv };
+
 template <typename K>
-static int attn_launch(K kernel, int64_t blocks, int lds, const AttnArgs& a, hipStream_t s, int rows = 1) {
+static int attn_launch(K kernel, int64_t blocks, int rows, int threads, int lds, const AttnArgs& a, hipStream_t s) {
   if (blocks == 0) return ST_OK;
-  kernel<<<dim3((unsigned)blocks, rows), kAttnThreads, lds, s>>>(a);
+  kernel<<<dim3((unsigned)blocks, rows), threads, lds, s>>>(a);
   ST_CHECK_LAUNCH();
   return ST_OK;
 }
-
-template <typename T, int DP>
-static int attn_forward_dp(const AttnArgs& a, hipStream_t s) {
-  const int rc = attn_launch(a.causal ? attn_forward_kernel<T, DP, true> : attn_forward_kernel<T, DP, false>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(a.causal), a, s);
-  if (rc != ST_OK) return rc;
-  return attn_launch(attn_forward_join_kernel<T, DP>, (int64_t)a.n_joins * a.kv_heads, 0, a, s, kAttnJoinRows);
-}
-template <typename T, int DP>
-static int attn_dq_dp(const AttnArgs& a, hipStream_t s) {
-  const int rc = attn_launch(a.causal ? attn_dq_kernel<T, DP, true> : attn_dq_kernel<T, DP, false>, (int64_t)a.n_items * a.kv_heads, attn_fwd_lds<T, DP>(a.causal), a, s);
-  if (rc != ST_OK) return rc;
-  return attn_launch(attn_sum_parts_kernel<T, DP, false>, (int64_t)a.n_joins * a.kv_heads, 0, a, s, kAttnJoinRows);
-}
-template <typename T, int DP>
-static int attn_dkv_dp(const AttnArgs& a, hipStream_t s) {
-  const int rc = attn_launch(a.causal ? attn_dkv_kernel<T, DP, true> : attn_dkv_kernel<T, DP, false>, (int64_t)a.n_items * a.kv_heads, attn_dkv_lds<T, DP>(a.causal), a, s);
-  if (rc != ST_OK) return rc;
-  return attn_launch(attn_sum_parts_kernel<T, DP, true>, (int64_t)a.n_joins * a.kv_heads, 0, a, s, kAttnJoinRows);
+template <typename K>
+static int attn_join(K kernel, const AttnArgs& a, hipStream_t s) {
+  return attn_launch(kernel, (int64_t)a.n_joins * a.kv_heads, kAttnJoinBlocks, kAttnThreads, 0, a, s);
 }
 
-enum AttnPass { kAttnForward, kAttnDq, kAttnDkv };
+template <typename T, int DP, int WAVES>
+static int attn_pass(AttnPass pass, const AttnArgs& a, hipStream_t s) {
+  const int64_t blocks = (int64_t)a.n_items * a.kv_heads;
+  auto run = [&](auto kernel, int lds) { return attn_launch(kernel, blocks, 1, 64 * WAVES, lds, a, s); };
+  if (pass == kAttnForward)
+    return run(a.causal ? attn_forward_kernel<T, DP, true, WAVES> : attn_forward_kernel<T, DP, false, WAVES>,
+               attn_fwd_lds<T, DP, WAVES>(a.causal));
+  if (pass == kAttnDq)
+    return run(a.causal ? attn_dq_kernel<T, DP, true, WAVES> : attn_dq_kernel<T, DP, false, WAVES>,
+               attn_fwd_lds<T, DP, WAVES>(a.causal));
+  return run(a.causal ? attn_dkv_kernel<T, DP, true, WAVES> : attn_dkv_kernel<T, DP, false, WAVES>,
+             attn_dkv_lds<T, DP, WAVES>(a.causal));
+}
+template <typename T, int DP>
+static int attn_dp(AttnPass pass, const AttnArgs& a, hipStream_t s) {
+  int rc = ST_ERR_UNSUPPORTED;
+  if (a.tile == kAttnTile)
+    rc = attn_pass<T, DP, 4>(pass, a, s);
+  else if constexpr (DP * sizeof(T) <= ST_ATTN_SMALL_TILE_BYTES)  // (a lane's share of a wider step does not fit its registers)
+    rc = attn_pass<T, DP, 1>(pass, a, s);
+  if (rc != ST_OK) return rc;
+  if (pass == kAttnForward) return attn_join(attn_forward_join_kernel<T, DP>, a, s);
+  if (pass == kAttnDq) return attn_join(attn_sum_parts_kernel<T, DP, false>, a, s);
+  return attn_join(attn_sum_parts_kernel<T, DP, true>, a, s);
+}
+
 template <typename T>
 static int attn_run(AttnPass pass, const AttnArgs& a, hipStream_t s) {
-#define ST_ATTN_DP(dp)                                        \
-  if (a.D <= dp) {                                            \
-    if (pass == kAttnForward) return attn_forward_dp<T, dp>(a, s); \
-    if (pass == kAttnDq) return attn_dq_dp<T, dp>(a, s);      \
-    return attn_dkv_dp<T, dp>(a, s);                          \
-  }
-  ST_ATTN_DP(32)
-  ST_ATTN_DP(64)
-  ST_ATTN_DP(96)
-  ST_ATTN_DP(128)
-#undef ST_ATTN_DP
-  return ST_ERR_UNSUPPORTED;
+  if (a.D <= 32) return attn_dp<T, 32>(pass, a, s);
+  if (a.D <= 64) return attn_dp<T, 64>(pass, a, s);
+  if (a.D <= 96) return attn_dp<T, 96>(pass, a, s);
+  return attn_dp<T, 128>(pass, a, s);
 }
 int attn_run_bf16(AttnPass pass, const AttnArgs& a, hipStream_t s);
 int attn_run_f16(AttnPass pass, const AttnArgs& a, hipStream_t s);

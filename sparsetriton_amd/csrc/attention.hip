@@ -7,6 +7,8 @@ static int attn_check(const st_attn_args* a) {
   if (a->dim % 8 || a->dim > ST_ATTN_MAX_DIM) return ST_ERR_UNSUPPORTED;
   if (a->dtype != ST_F32 && a->dtype != ST_F16 && a->dtype != ST_BF16) return ST_ERR_UNSUPPORTED;
   if (!(a->scale > 0.f) || !(a->scale < 3.0e38f)) return ST_ERR_ARG;
+  for (int tile : {a->q_tile, a->k_tile})
+    if (tile != ST_ATTN_TILE && tile != ST_ATTN_SMALL_TILE) return ST_ERR_ARG;
   for (int64_t n : {a->n_q_items, a->n_q_joins, a->n_k_items, a->n_k_joins})
     if (n < 0 || n * a->kv_heads >= (1ll << 31)) return ST_ERR_ARG;
   return ST_OK;
@@ -17,7 +19,7 @@ static bool attn_rows_ok(const st_attn_args* a, const void* p, int64_t row, int6
   const int64_t esz = a->dtype == ST_F32 ? 4 : 2, group = a->heads / a->kv_heads;
   if (((uintptr_t)p | (uint64_t)(row * esz) | (uint64_t)(head * esz)) & 15) return false;
   return row >= 0 && head >= 0 && row < (1ll << 29) && head < (1ll << 29) &&
-         (row * (ST_ATTN_KEYS + 1) + head * (group + 1) + a->dim) * esz < (1ll << 31) - 64;
+         (row * (ST_ATTN_TILE + 1) + head * (group + 1) + a->dim) * esz < (1ll << 31) - 64;
 }
 
 static st::AttnArgs attn_args(const st_attn_args* a) {
@@ -61,6 +63,7 @@ extern "C" int st_attn_forward(const st_attn_args* a, st_stream_t stream) {
   st::AttnArgs g = attn_args(a);
   g.items = (const st::AttnItem*)a->q_items, g.n_items = (int)a->n_q_items;
   g.joins = (const st::AttnJoin*)a->q_joins, g.n_joins = (int)a->n_q_joins;
+  g.tile = a->q_tile;
   return attn_run_any(a, st::kAttnForward, g, (hipStream_t)stream);
 }
 
@@ -79,11 +82,13 @@ extern "C" int st_attn_backward(const st_attn_args* a, st_stream_t stream) {
   if (a->n_q_items) {
     g.items = (const st::AttnItem*)a->q_items, g.n_items = (int)a->n_q_items;
     g.joins = (const st::AttnJoin*)a->q_joins, g.n_joins = (int)a->n_q_joins;
+  g.tile = a->q_tile;
     rc = attn_run_any(a, st::kAttnDq, g, (hipStream_t)stream);
     if (rc != ST_OK) return rc;
   }
   if (!a->n_k_items) return ST_OK;
   g.items = (const st::AttnItem*)a->k_items, g.n_items = (int)a->n_k_items;
   g.joins = (const st::AttnJoin*)a->k_joins, g.n_joins = (int)a->n_k_joins;
+  g.tile = a->k_tile;
   return attn_run_any(a, st::kAttnDkv, g, (hipStream_t)stream);
 }

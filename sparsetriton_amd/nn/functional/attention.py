@@ -17,6 +17,13 @@ from sparsetriton_amd.tensor import SparseTensor
 
 __all__ = ["AttentionSegments", "sparse_attention"]
 
+# Keys (rows) that a part of a split tile is a multiple of: a step of the kernels.
+_STEP = 64
+# Small tiles (one wave) are taken while there are at most so many for each wide one (four waves), that is
+# while most waves of the wide ones would have no rows.  bf16, us wide / small: 2,000 windows of 1-96 rows x
+# 4 x 32 (1.31 small tiles a wide one) 27 / 16, 1,000 of 1-200 x 8 x 64 (1.65) 50 / 37, forward and backward of
+# 2,000 x 8 x 64 (1.34) 294 / 176; 1,000 of 64 rows (2.0) 19.3 / 19.7, 300 of 40 over 300 keys (2.0) 21 / 26.
+_SMALL_TILES = 1.8
 # Workgroups below which a tile's keys (rows) are split over several, and what the split aims at:
 # two and four for each of 256 CUs.  A part takes four steps at least.
 _SPLIT_BELOW, _SPLIT_TO, _PART_STEPS = 512, 1024, 4
@@ -39,8 +46,8 @@ def _lengths(lengths, what: str) -> np.ndarray:
 class _Tiles:
     """Work items and joins of one pass, on the device: rows (4, 8) int32 as st_attn_args lays them out."""
 
-    def __init__(self, q0, nq, k0, nk, row0, lo, hi, kv_heads, device):
-        step = _lib.ATTN_KEYS
+    def __init__(self, tile, q0, nq, k0, nk, row0, lo, hi, kv_heads, device):
+        self.tile, step = tile, _STEP
         steps = -(-(hi - lo) // step)
         n = steps.size
         parts = np.ones(n, dtype=np.int64)
@@ -50,14 +57,14 @@ class _Tiles:
             parts = np.maximum(1, -(-steps // most))
             chunk = -(-steps // parts)
             parts = np.maximum(1, -(-steps // np.maximum(chunk, 1)))
-        tile = np.repeat(np.arange(n), parts)
-        nth = np.arange(tile.size) - np.repeat(np.cumsum(parts) - parts, parts)
-        first = lo[tile] + nth * chunk[tile] * step
-        end = np.minimum(hi[tile], first + chunk[tile] * step)
+        of = np.repeat(np.arange(n), parts)
+        nth = np.arange(of.size) - np.repeat(np.cumsum(parts) - parts, parts)
+        first = lo[of] + nth * chunk[of] * step
+        end = np.minimum(hi[of], first + chunk[of] * step)
         split = parts > 1
         slot0 = np.cumsum(np.where(split, parts, 0)) - np.where(split, parts, 0)
-        part = np.where(split[tile], slot0[tile] + nth, -1)
-        items = np.stack([q0[tile], nq[tile], k0[tile], nk[tile], row0[tile], first, end, part], 1)
+        part = np.where(split[of], slot0[of] + nth, -1)
+        items = np.stack([q0[of], nq[of], k0[of], nk[of], row0[of], first, end, part], 1)
         # longest first: the last workgroups to start are short ones
         items = items[np.argsort(first - end, kind="stable")]
         at = np.flatnonzero(split)
@@ -120,31 +127,35 @@ class AttentionSegments:
                                      for f, r in zip(full, rest)])
         return cls(counts, device=tensor.F.device)
 
-    def _tiles(self, per_segment):
-        """(segment, first row) of each tile of ST_ATTN_TILE rows."""
-        n = -(-per_segment // _lib.ATTN_TILE)
+    @staticmethod
+    def _tiles(rows, row_bytes):
+        """(tile size, segment and first row of each tile) over segments of so many rows (keys)."""
+        small, wide = (int((-(-rows // t)).sum()) for t in (_lib.ATTN_SMALL_TILE, _lib.ATTN_TILE))
+        narrow = row_bytes <= _lib.ATTN_SMALL_TILE_BYTES and small <= _SMALL_TILES * wide
+        tile = _lib.ATTN_SMALL_TILE if narrow else _lib.ATTN_TILE
+        n = -(-rows // tile)
         seg = np.repeat(np.arange(n.size), n)
-        return seg, (np.arange(seg.size) - np.repeat(np.cumsum(n) - n, n)) * _lib.ATTN_TILE
+        return tile, seg, (np.arange(seg.size) - np.repeat(np.cumsum(n) - n, n)) * tile
 
-    def _plan(self, which: str, group: int, kv_heads: int, causal: bool) -> _Tiles:
-        key = (which, group, kv_heads, causal)
+    def _plan(self, which: str, group: int, kv_heads: int, causal: bool, row_bytes: int) -> _Tiles:
+        key = (which, group, kv_heads, causal, row_bytes <= _lib.ATTN_SMALL_TILE_BYTES)
         plan = self._plans.get(key)
         if plan is None:
             nq, nk = self._nq, self._nk
             if int(nq.max(initial=0)) * group >= 2 ** 31 - _lib.ATTN_TILE:
                 raise ValueError(f"a segment has at most {(2 ** 31 - _lib.ATTN_TILE) // group} query rows at {group} heads a key head")
             if which == "q":  # tiles of packed rows over keys lo .. hi
-                seg, row0 = self._tiles(nq * group)
+                tile, seg, row0 = self._tiles(nq * group, row_bytes)
                 lo, hi = np.zeros_like(row0), nk[seg]
                 if causal:
-                    last = np.minimum(row0 + _lib.ATTN_TILE, nq[seg] * group) - 1
+                    last = np.minimum(row0 + tile, nq[seg] * group) - 1
                     hi = np.clip(last // group + nk[seg] - nq[seg] + 1, 0, nk[seg])
             else:  # tiles of keys over packed rows lo .. hi
-                seg, row0 = self._tiles(nk)
+                tile, seg, row0 = self._tiles(nk, row_bytes)
                 lo, hi = np.zeros_like(row0), nq[seg] * group
                 if causal:
                     lo = np.minimum(np.maximum(0, row0 - (nk[seg] - nq[seg])) * group, hi)
-            plan = _Tiles(self._q0[seg], nq[seg], self._k0[seg], nk[seg], row0, lo, hi, kv_heads, self.device)
+            plan = _Tiles(tile, self._q0[seg], nq[seg], self._k0[seg], nk[seg], row0, lo, hi, kv_heads, self.device)
             self._plans[key] = plan
         plan.use()
         return plan
@@ -163,7 +174,7 @@ def _rows(t: torch.Tensor, group: int) -> torch.Tensor:
     e = t.element_size()
     row, head, channel = t.stride()
     if (channel == 1 and not (row * e | head * e | t.data_ptr()) & 15 and row < 2 ** 29 and head < 2 ** 29
-            and (row * (_lib.ATTN_KEYS + 1) + head * (group + 1) + t.shape[2]) * e < 2 ** 31 - 64):
+            and (row * (_lib.ATTN_TILE + 1) + head * (group + 1) + t.shape[2]) * e < 2 ** 31 - 64):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -180,6 +191,7 @@ def _args(q, k, v, key_mask, o, lse, causal, scale) -> _lib.AttnArgs:
         a.key_mask = key_mask.data_ptr()
     a.heads, a.kv_heads, a.dim = q.shape[1], k.shape[1], q.shape[2]
     a.dtype, a.causal, a.scale = _lib.FEAT_DTYPES[q.dtype], causal, scale
+    a.q_tile = a.k_tile = _lib.ATTN_TILE
     return a
 
 
@@ -190,9 +202,10 @@ def _forward(q, k, v, segments, key_mask, causal, scale, stats):
     q, k, v = _rows(q, group), _rows(k, group), _rows(v, group)
     o = torch.empty((n, heads, dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if stats else None
-    plan = segments._plan("q", group, kv_heads, causal)
+    plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size())
     a = _args(q, k, v, key_mask, o, lse, causal, scale)
     a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
+    a.q_tile = plan.tile
     parts = _parts(kv_heads, dim, plan.slots, 0, q.device)
     if parts is not None:
         a.parts = parts.data_ptr()
@@ -219,18 +232,20 @@ class _Attention(torch.autograd.Function):
         dout = _rows(dout, group)
         new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
         dq, delta = new(q), torch.empty_like(lse)
-        plan = segments._plan("q", group, kv_heads, causal)
+        plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size())
         a = _args(q, k, v, key_mask, o, lse, causal, scale)
         a.dout, a.dq, a.delta = dout.data_ptr(), dq.data_ptr(), delta.data_ptr()
         a.dout_row, a.dout_head, _ = dout.stride()
         a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
+        a.q_tile = plan.tile
         dk = dv = None
         slots = 0
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dk, dv = new(k), new(v)
-            keys = segments._plan("k", group, kv_heads, causal)
+            keys = segments._plan("k", group, kv_heads, causal, dim * q.element_size())
             a.dk, a.dv = dk.data_ptr(), dv.data_ptr()
             a.k_items, a.k_joins, a.n_k_items, a.n_k_joins = keys.items, keys.joins, keys.n_items, keys.n_joins
+            a.k_tile = keys.tile
             slots = keys.slots
         parts = _parts(kv_heads, dim, plan.slots, slots, q.device)
         if parts is not None:

@@ -132,7 +132,7 @@ def test_shared_key_heads(device, heads, kv_heads, causal):
 def test_work_split_over_the_long_side(device, ql, kl, heads, kv_heads, dim, causal, dtype):
     q, k, v, do, mask = _make(ql, kl, heads, kv_heads, dim, dtype, device, 3 * dim, masked=0.1)
     segs = AttentionSegments(ql, kl, device=device)
-    plans = [segs._plan(w, heads // kv_heads, kv_heads, causal) for w in "qk"]
+    plans = [segs._plan(w, heads // kv_heads, kv_heads, causal, dim * q.element_size()) for w in "qk"]
     assert any(p.n_joins for p in plans)
     _check(q, k, v, do, ql, kl, causal, mask)
 
@@ -146,7 +146,7 @@ def test_many_tiles(device, causal, dtype, dim, times):
     ql = [700, 1, 333, 900, 64, 128, 2] * times
     q, k, v, do, mask = _make(ql, ql, 8, 4, dim, dtype, device, 17, masked=0.05)
     segs = AttentionSegments(ql, device=device)
-    assert times == 3 or not any(segs._plan(w, 2, 4, causal).n_joins for w in "qk")
+    assert times == 3 or not any(segs._plan(w, 2, 4, causal, dim * q.element_size()).n_joins for w in "qk")
     _check(q, k, v, do, ql, ql, causal, mask)
 
 
@@ -380,11 +380,12 @@ def test_segments_of_a_tensor(device):
 
 def test_tile_lists_cover_every_pair_once():
     """Host arithmetic of the lists: each (row, key) that may be seen lies in exactly one item, and parts join in order."""
-    for ql, kl, group, kv, causal in [([300, 1, 0, 50], [700, 3, 5, 0], 3, 1, False), ([1], [5000], 1, 1, False),
-                                      ([400, 90], [400, 20], 2, 2, True), ([5], [1000], 7, 1, True)]:
+    for ql, kl, group, kv, causal, row in [([300, 1, 0, 50], [700, 3, 5, 0], 3, 1, False, 128), ([1], [5000], 1, 1, False, 256),
+                                           ([1], [5000], 1, 1, False, 64), ([400, 90], [400, 20], 2, 2, True, 64),
+                                           ([5], [1000], 7, 1, True, 64), ([5, 20, 3, 40], [9, 60, 3, 33], 1, 4, True, 64)]:
         s = AttentionSegments(ql, kl, device="cpu")
         for which in "qk":
-            plan = s._plan(which, group, kv, causal)
+            plan = s._plan(which, group, kv, causal, row)
             items = plan.words[:plan.n_items].tolist()
             joins = plan.words[plan.n_items:].tolist()
             assert len(joins) == plan.n_joins
@@ -394,12 +395,12 @@ def test_tile_lists_cover_every_pair_once():
             for nq, nk in zip(ql, kl):
                 mine = [i for i in items if i[:4] == [q0, nq, k0, nk]]
                 rows, length = (nq * group, nk) if which == "q" else (nk, nq * group)
-                for row0 in range(0, rows, 128):
+                for row0 in range(0, rows, plan.tile):
                     tile = sorted((i for i in mine if i[4] == row0), key=lambda i: i[5])
                     seen = [j for i in tile for j in range(i[5], i[6])]
                     assert len(seen) == len(set(seen)) and tile
                     if which == "q":
-                        last = (min(rows, row0 + 128) - 1) // group + nk - nq if causal else nk - 1
+                        last = (min(rows, row0 + plan.tile) - 1) // group + nk - nq if causal else nk - 1
                         assert seen == list(range(0, min(nk, max(0, last + 1))))
                     else:
                         first = max(0, row0 - (nk - nq)) * group if causal else 0
@@ -425,13 +426,28 @@ def test_refusals_before_any_launch():
     a = _lib.AttnArgs()
     assert lib.st_attn_forward(None, None) == -1 and lib.st_attn_forward(a, None) == -1
     a.heads, a.kv_heads, a.dim, a.scale, a.dtype = 4, 2, 64, 0.125, 2
+    a.q_tile, a.k_tile = _lib.ATTN_TILE, _lib.ATTN_SMALL_TILE
     assert lib.st_attn_forward(a, None) == 0 and lib.st_attn_backward(a, None) == 0  # nothing to do
     for field, value, rc in (("kv_heads", 3, -1), ("dim", 20, -3), ("dim", 136, -3), ("dtype", 3, -3), ("scale", 0.0, -1),
-                             ("scale", float("nan"), -1), ("n_q_items", -1, -1), ("n_q_items", 1, -1)):
+                             ("scale", float("nan"), -1), ("n_q_items", -1, -1), ("n_q_items", 1, -1),
+                             ("q_tile", 64, -1), ("k_tile", 0, -1)):
         old = getattr(a, field)
         setattr(a, field, value)
         assert lib.st_attn_forward(a, None) == rc, field
         setattr(a, field, old)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float16, 24), (torch.float32, 32), (torch.float32, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_windows(device, dtype, dim, causal):
+    """Many segments of a few rows: tiles of one wave where a row of a head is at most 128 bytes."""
+    ql = [1, 17, 32, 33, 5, 90, 31, 0, 64, 2] * 12
+    kl = [9, 17, 32, 1, 70, 90, 0, 3, 65, 2] * 12
+    q, k, v, do, mask = _make(ql, kl, 4, 2, dim, dtype, device, 18, masked=0.1)
+    tile = AttentionSegments(ql, kl, device=device)._plan("k", 2, 2, causal, dim * q.element_size()).tile
+    assert tile == (32 if dim * q.element_size() <= 128 else 128)
+    _check(q, k, v, do, ql, kl, causal, mask)
 
 
 @pytest.mark.gpu
