@@ -342,6 +342,13 @@ __device__ __forceinline__ void attn_reads_ahead() {
   }
 }
 
+// Whether 16 channels of the scores' sum are to be taken: fp32 leaves out those past D, eight slow
+// products each (16-bit types take a zero product rather than a branch among theirs).
+template <typename T>
+__device__ __forceinline__ bool attn_in(int channel, int D) {
+  return sizeof(T) == 2 || channel < D;
+}
+
 // Waves of a SIMD that the registers leave room for (a limit for the compiler).
 template <typename T, int DP>
 constexpr int attn_waves() {
@@ -357,8 +364,8 @@ constexpr int attn_keys() {
 }
 
 template <typename T, int DP, int WAVES>
-constexpr int attn_fwd_lds(bool causal) {  // two buffers of K and V, a copy of one of them
-  return (causal ? 5 : 4) * attn_keys<WAVES>() * DP * (int)sizeof(T);
+constexpr int attn_fwd_lds(bool causal) {  // two buffers of K and V; causal, a copy of one of them, else two of the keys' terms
+  return attn_keys<WAVES>() * (causal ? 5 * DP * (int)sizeof(T) : 4 * DP * (int)sizeof(T) + 2 * (int)sizeof(float));
 }
 
 // A running maximum is raised only when a row's maximum passes it by more
@@ -376,6 +383,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
   constexpr int TILE = BK * DP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
+  float* bias = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers, not CAUSAL: 0 or -inf for each key of a step
 
   const int w = attn_work(gridDim.x), hk = w / a.n_items;
   const AttnItem it = a.items[w - hk * a.n_items];
@@ -427,6 +435,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
       for (int i = 0; i < Stage::N; ++i)  // (whatever a masked row holds, not finite included, stays out of the products)
         if (!chunk_kept[i]) ks.reg[i] = vs.reg[i] = (v4u)(0u);
     }
+    if (!CAUSAL && seen != ALL && threadIdx.x < BK) bias[buf * BK + lane] = seen >> lane & 1 ? 0.f : -INFINITY;
     ks.store(kl);
     vs.store(vl);
     __syncthreads();
@@ -434,17 +443,32 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
     if (!active || (CAUSAL && !__any(live && kt <= see))) continue;
 
     v16f s[NB];
+    auto scores = [&]() {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) s[b] = (v16f)(0.f);
+      for (int i = 0; i < KS && attn_in<T>(16 * i, a.D); ++i)
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
+        for (int b = 0; b < NB; ++b) s[b] = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s[b]);
+      attn_reads_ahead<T, NB * KS>();
+    };
+    if (!CAUSAL && seen != ALL) {  // the sums begin at -inf for keys that are left out (their K is zeros)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) s[b] = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s[b]);
-    attn_reads_ahead<T, NB * KS>();
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const v4f x = *reinterpret_cast<const v4f*>(bias + buf * BK + b * 32 + 8 * j + 4 * half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[b][4 * j + e] = x[e];
+        }
+      scores();
+    } else {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) s[b] = (v16f)(0.f);
+      scores();
+    }
     const bool cut = CAUSAL && __any(see - kt < BK - 1);  // by the causal order
     const int last = see - kt;
     const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
-    if (cut || seen != ALL) {
+    if (CAUSAL && (cut || seen != ALL)) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
@@ -679,7 +703,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
     for (int b = 0; b < NB; ++b) {
       v16f s = (v16f)(0.f), dp = (v16f)(0.f);
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
+      for (int i = 0; i < KS && attn_in<T>(16 * i, a.D); ++i) {
         s = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s);
         dp = mma32(Tile::rows(vl, b * 32 + (lane & 31), 16 * i + 8 * half), gf[i], dp);
       }
@@ -810,7 +834,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
     for (int b = 0; b < NB; ++b) {
       v16f s = (v16f)(0.f), dp = (v16f)(0.f);
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
+      for (int i = 0; i < KS && attn_in<T>(16 * i, a.D); ++i) {
         s = mma32(Tile::rows(ql, b * 32 + (lane & 31), 16 * i + 8 * half), kf[i], s);
         dp = mma32(Tile::rows(gl, b * 32 + (lane & 31), 16 * i + 8 * half), vf[i], dp);
       }

@@ -180,19 +180,12 @@ def _rows(t: torch.Tensor, group: int) -> torch.Tensor:
 
 
 def _args(q, k, v, key_mask, o, lse, causal, scale) -> _lib.AttnArgs:
-    a = _lib.AttnArgs()
-    a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
-    a.q_row, a.q_head, _ = q.stride()
-    a.k_row, a.k_head, _ = k.stride()
-    a.v_row, a.v_head, _ = v.stride()
-    if lse is not None:
-        a.lse = lse.data_ptr()
-    if key_mask is not None:
-        a.key_mask = key_mask.data_ptr()
-    a.heads, a.kv_heads, a.dim = q.shape[1], k.shape[1], q.shape[2]
-    a.dtype, a.causal, a.scale = _lib.FEAT_DTYPES[q.dtype], causal, scale
-    a.q_tile = a.k_tile = _lib.ATTN_TILE
-    return a
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    ptr = _lib.ptr
+    return _lib.AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(lse), None, None, None, None, None,
+                         qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], 0, 0, ptr(key_mask), None, None, None, None, 0, 0, 0, 0,
+                         None, q.shape[1], k.shape[1], q.shape[2], _lib.FEAT_DTYPES[q.dtype], causal, _lib.ATTN_TILE,
+                         _lib.ATTN_TILE, scale)
 
 
 def _forward(q, k, v, segments, key_mask, causal, scale, stats):

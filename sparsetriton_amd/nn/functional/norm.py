@@ -171,15 +171,17 @@ def _ln_workspace_floats(n: int, C: int, code: int) -> int:
     return floats.value
 
 
+def _ln_param(t, dtype):
+    return t if t is None or (t.dtype is dtype and t.is_contiguous()) else t.detach().to(dtype).contiguous()
+
+
 def _ln_params(x, weight, bias):
     """weight and bias as the kernels take them: one dtype for both, the features' or fp32."""
-    w, b = weight, bias
-    dt = (w if w is not None else b).dtype if (w is not None or b is not None) else torch.float32
-    if dt not in (x.dtype, torch.float32) or (w is not None and b is not None and b.dtype != dt):
+    given = weight if weight is not None else bias
+    dt = torch.float32 if given is None else given.dtype
+    if (dt is not x.dtype and dt is not torch.float32) or (weight is not None and bias is not None and bias.dtype is not dt):
         dt = torch.float32
-    w = w.detach().to(dt).contiguous() if w is not None else None
-    b = b.detach().to(dt).contiguous() if b is not None else None
-    return w, b, _lib.FEAT_DTYPES[dt]
+    return _ln_param(weight, dt), _ln_param(bias, dt), _lib.FEAT_DTYPES[dt]
 
 
 def _ln_forward(x, weight, bias, residual, eps, stats):
@@ -193,8 +195,9 @@ def _ln_forward(x, weight, bias, residual, eps, stats):
     mean = rstd = None
     if stats:
         mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0)
-    _lib.call("st_ln_forward", _lib.ptr(x), _lib.ptr(res), n, C, _lib.FEAT_DTYPES[x.dtype], _lib.ptr(w), _lib.ptr(b),
-              wcode, eps, _lib.ptr(h), _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd), _lib.stream_of(x.device))
+    ptr = _lib.ptr
+    _lib.call("st_ln_forward", x.data_ptr(), ptr(res), n, C, _lib.FEAT_DTYPES[x.dtype], ptr(w), ptr(b), wcode, eps,
+              ptr(h), y.data_ptr(), ptr(mean), ptr(rstd), _lib.stream_of(x.device))
     return y, h, x, w, wcode, mean, rstd
 
 

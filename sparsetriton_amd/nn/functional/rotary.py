@@ -59,17 +59,18 @@ def _rotate(q, k, positions, axes, inverse):
     out = [torch.empty(t.shape, dtype=t.dtype, device=dev) if t is not None else None for t in (q, k)]
     # channels side by side; rows and heads at any stride
     q, k = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (q, k))
-    a = _lib.RotaryArgs()
+    qp = kp = qo = ko = None
+    qs = ks = (0, 0, 0)
+    heads = kv_heads = 0
     if q is not None:
-        a.q, a.q_out, a.q_row, a.q_head, a.heads = q.data_ptr(), out[0].data_ptr(), q.stride(0), q.stride(1), q.shape[1]
+        qp, qo, qs, heads = q.data_ptr(), out[0].data_ptr(), q.stride(), q.shape[1]
     if k is not None:
-        a.k, a.k_out, a.k_row, a.k_head, a.kv_heads = (k.data_ptr(), out[1].data_ptr(), k.stride(0), k.stride(1),
-                                                       k.shape[1])
-    t = q if q is not None else k
-    a.positions, a.pos_row, a.pos_dtype = positions.data_ptr(), positions.stride(0), _lib.POSITION_DTYPES[positions.dtype]
-    a.turns, a.axis = turns.data_ptr(), axis.data_ptr()
-    a.n, a.dim, a.pairs, a.dtype = t.shape[0], t.shape[2], axes.pairs, _lib.FEAT_DTYPES[t.dtype]
-    a.interleaved, a.inverse = axes.interleaved, inverse
+        kp, ko, ks, kv_heads = k.data_ptr(), out[1].data_ptr(), k.stride(), k.shape[1]
+    n, _, dim = (q if q is not None else k).shape
+    a = _lib.RotaryArgs(qp, kp, qo, ko, qs[0], qs[1], ks[0], ks[1], positions.data_ptr(), positions.stride(0),
+                        turns.data_ptr(), axis.data_ptr(), n, heads, kv_heads, dim, axes.pairs,
+                        _lib.FEAT_DTYPES[out[0 if q is not None else 1].dtype], _lib.POSITION_DTYPES[positions.dtype],
+                        axes.interleaved, inverse)
     _lib.call("st_rotary", ctypes.byref(a), _lib.stream_of(dev))
     return tuple(out)
 
