@@ -14,6 +14,7 @@ import torch
 
 from sparsetriton_amd import _lib
 from sparsetriton_amd.tensor import SparseTensor
+from sparsetriton_amd.utils.utils import once_differentiable
 
 __all__ = ["AttentionSegments", "sparse_attention"]
 
@@ -193,7 +194,7 @@ def _forward(q, k, v, segments, key_mask, causal, scale, stats):
     kv_heads = k.shape[1]
     group = heads // kv_heads
     q, k, v = _rows(q, group), _rows(k, group), _rows(v, group)
-    o = torch.empty((n, heads, dim), dtype=q.dtype, device=q.device)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if stats else None
     plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size())
     a = _args(q, k, v, key_mask, o, lse, causal, scale)
@@ -215,7 +216,7 @@ class _Attention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, o, lse, key_mask = ctx.saved_tensors
         segments, causal, scale = ctx.meta
@@ -223,7 +224,7 @@ class _Attention(torch.autograd.Function):
         kv_heads = k.shape[1]
         group = heads // kv_heads
         dout = _rows(dout, group)
-        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+        new = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format)  # noqa: E731
         dq, delta = new(q), torch.empty_like(lse)
         plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size())
         a = _args(q, k, v, key_mask, o, lse, causal, scale)
@@ -271,9 +272,11 @@ def sparse_attention(
     products too); results do not depend on timing.
     """
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
-        _lib.require_device(t, f"attention {what}")
-        _lib.feat_code(t.dtype)
-        if t.dim() != 3 or t.dtype != q.dtype or t.device != q.device:
+        if not t.is_cuda:
+            _lib.require_device(t, f"attention {what}")
+        if t.dtype not in _lib.FEAT_DTYPES:
+            _lib.feat_code(t.dtype)
+        if t.dim() != 3 or t.dtype is not q.dtype or t.device != q.device:
             raise ValueError(f"{what} must be (rows, heads, D) of q's dtype and device (got {tuple(t.shape)} {t.dtype} "
                              f"on {t.device})")
     heads, dim = q.shape[1:]

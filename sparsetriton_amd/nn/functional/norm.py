@@ -29,6 +29,7 @@ import torch
 
 from sparsetriton_amd import _lib
 from sparsetriton_amd.tensor import SparseTensor
+from sparsetriton_amd.utils.utils import once_differentiable
 
 __all__ = ["sparse_batch_norm", "sparse_batch_norm_act", "sparse_layer_norm"]
 
@@ -213,7 +214,7 @@ class _LayerNorm(torch.autograd.Function):
         return y if h is None else (y, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dy, dh=None):
         h, w, mean, rstd = ctx.saved_tensors
         wcode, wdt, bdt = ctx.meta

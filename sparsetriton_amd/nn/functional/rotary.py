@@ -13,6 +13,7 @@ import torch
 
 from sparsetriton_amd import _lib
 from sparsetriton_amd.tensor import SparseTensor
+from sparsetriton_amd.utils.utils import once_differentiable
 
 __all__ = ["RotaryAxes", "sparse_rotary"]
 
@@ -56,23 +57,28 @@ class RotaryAxes:
 def _rotate(q, k, positions, axes, inverse):
     dev = (q if q is not None else k).device
     turns, axis = axes.on(dev)
-    out = [torch.empty(t.shape, dtype=t.dtype, device=dev) if t is not None else None for t in (q, k)]
-    # channels side by side; rows and heads at any stride
-    q, k = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (q, k))
-    qp = kp = qo = ko = None
+    qp = kp = qo = ko = q_out = k_out = None
     qs = ks = (0, 0, 0)
     heads = kv_heads = 0
+    # channels side by side; rows and heads at any stride
     if q is not None:
-        qp, qo, qs, heads = q.data_ptr(), out[0].data_ptr(), q.stride(), q.shape[1]
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if q.stride(2) != 1:
+            q = q.contiguous()
+        qp, qo, qs, heads = q.data_ptr(), q_out.data_ptr(), q.stride(), q.shape[1]
     if k is not None:
-        kp, ko, ks, kv_heads = k.data_ptr(), out[1].data_ptr(), k.stride(), k.shape[1]
-    n, _, dim = (q if q is not None else k).shape
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        if k.stride(2) != 1:
+            k = k.contiguous()
+        kp, ko, ks, kv_heads = k.data_ptr(), k_out.data_ptr(), k.stride(), k.shape[1]
+    t = q if q is not None else k
+    n, _, dim = t.shape
     a = _lib.RotaryArgs(qp, kp, qo, ko, qs[0], qs[1], ks[0], ks[1], positions.data_ptr(), positions.stride(0),
                         turns.data_ptr(), axis.data_ptr(), n, heads, kv_heads, dim, axes.pairs,
-                        _lib.FEAT_DTYPES[out[0 if q is not None else 1].dtype], _lib.POSITION_DTYPES[positions.dtype],
+                        _lib.FEAT_DTYPES[t.dtype], _lib.POSITION_DTYPES[positions.dtype],
                         axes.interleaved, inverse)
     _lib.call("st_rotary", ctypes.byref(a), _lib.stream_of(dev))
-    return tuple(out)
+    return q_out, k_out
 
 
 class _Rotary(torch.autograd.Function):
@@ -84,7 +90,7 @@ class _Rotary(torch.autograd.Function):
         return _rotate(q, k, positions, axes, False)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
         dq = dq if ctx.needs_input_grad[0] else None
@@ -107,17 +113,18 @@ def sparse_rotary(
     of its coordinates) or (N, A) of int16, int32, int64 or float32 with ``A >= len(axes.axes)``.
     The outputs are contiguous; the gradient turns back.  Positions get no gradient.
     """
-    given = [t for t in (q, k) if t is not None]
-    if not given:
+    first = q if q is not None else k
+    if first is None:
         raise ValueError("sparse_rotary needs q or k")
     pos = positions.C[:, 1:] if isinstance(positions, SparseTensor) else positions
-    first = given[0]
-    for t in given:
-        _lib.require_device(t, "rotary input")
-        _lib.feat_code(t.dtype)
+    for t in (first,) if q is None or k is None else (q, k):
+        if not t.is_cuda:
+            _lib.require_device(t, "rotary input")
+        if t.dtype not in _lib.FEAT_DTYPES:
+            _lib.feat_code(t.dtype)
         if t.dim() != 3 or t.shape[2] != axes.head_dim or t.shape[1] == 0:
             raise ValueError(f"expected (rows, heads, {axes.head_dim}), got {tuple(t.shape)}")
-        if t.shape[0] != first.shape[0] or t.dtype != first.dtype or t.device != first.device:
+        if t is not first and (t.shape[0] != first.shape[0] or t.dtype is not first.dtype or t.device != first.device):
             raise ValueError("q and k must have the same rows, dtype and device")
     if pos.dim() != 2 or pos.shape[0] != first.shape[0] or pos.shape[1] < len(axes.axes):
         raise ValueError(f"positions must be ({first.shape[0]}, at least {len(axes.axes)}), got {tuple(pos.shape)}")
@@ -125,9 +132,8 @@ def sparse_rotary(
         raise TypeError(f"unsupported position dtype {pos.dtype}; use int16, int32, int64 or float32")
     if pos.device != first.device:
         raise ValueError(f"positions are on {pos.device}, q and k on {first.device}")
-    pos = pos.detach()
     if pos.shape[1] > 1 and pos.stride(1) != 1:
         pos = pos.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
-        return _Rotary.apply(q, k, pos, axes)
+    if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, pos.detach(), axes)
     return _rotate(q, k, pos, axes, False)

@@ -4,6 +4,7 @@ from .linear import SparseLinear
 from .norm import SparseBatchNorm, SparseLayerNorm
 from .blocks import SparseConvBlock, SparseConvTransposeBlock, SparseResBlock
 from .spatial import SparseDownsample, SparsePooling, SparseUpsample
+from .transformer import SparseAttention, SparseTransformerBlock
 
 __all__ = [
     "SparseConv3DBase", "SparseConv3D", "SubMConv3D", "SparseConvTransposed3D",
@@ -11,4 +12,5 @@ __all__ = [
     "SparseLinear", "SparseBatchNorm", "SparseLayerNorm",
     "SparseConvBlock", "SparseConvTransposeBlock", "SparseResBlock",
     "SparsePooling", "SparseUpsample", "SparseDownsample",
+    "SparseAttention", "SparseTransformerBlock",
 ]

@@ -1,0 +1,87 @@
+"""Transformer layers over voxel features (no counterpart in the reference).
+
+``SparseAttention`` projects the features to queries, keys and values, turns queries and keys by
+the voxels' x, y, z (``sparse_rotary``) and attends within the row segments
+(``sparse_attention``).  ``SparseTransformerBlock`` is the pre-norm block around it::
+
+    h = x + attention(norm1(x));   out = h + mlp(norm2(h))
+
+whose first add runs inside the second norm (``sparse_layer_norm`` with a residual).  Build the
+segments once for a coordinate set and hand them to every block::
+
+    segments = AttentionSegments.from_tensor(x, patch=1024)
+    for block in blocks:
+        x = block(x, segments)
+"""
+
+from typing import Optional, Sequence
+
+import torch
+from torch import nn
+
+from sparsetriton_amd.nn.functional.attention import AttentionSegments, sparse_attention
+from sparsetriton_amd.nn.functional.norm import sparse_layer_norm
+from sparsetriton_amd.nn.functional.rotary import RotaryAxes, sparse_rotary
+from sparsetriton_amd.tensor import SparseTensor
+
+__all__ = ["SparseAttention", "SparseTransformerBlock"]
+
+
+def _three_axes(dim: int):
+    """An even number of a head's channels for each of x, y and z, all of them or all but two."""
+    pair = dim // 2
+    return tuple(2 * (pair // 3 + (1 if i < pair % 3 else 0)) for i in range(3))
+
+
+class SparseAttention(nn.Module):
+    """Multi-head attention between the rows of each segment, with rotary voxel positions.
+
+    ``kv_heads`` (default ``heads``) key heads are shared by ``heads / kv_heads`` query heads each;
+    ``axes`` channels of a head turn with x, y and z (default: the whole head, in three parts).
+    ``causal``: the rows' order is the order of generation.
+    """
+
+    def __init__(self, channels: int, heads: int, kv_heads: Optional[int] = None, head_dim: Optional[int] = None,
+                 axes: Optional[Sequence[int]] = None, base: float = 10000.0, causal: bool = False, bias: bool = True):
+        super().__init__()
+        self.heads, self.kv_heads = heads, heads if kv_heads is None else kv_heads
+        if head_dim is None and channels % heads:
+            raise ValueError(f"{channels} channels do not divide into {heads} heads")
+        self.head_dim = channels // heads if head_dim is None else head_dim
+        if self.heads % self.kv_heads:
+            raise ValueError(f"{heads} heads do not share {kv_heads} key heads evenly")
+        self.causal = causal
+        self.rotary = RotaryAxes(self.head_dim, _three_axes(self.head_dim) if axes is None else axes, base=base)
+        self.qkv = nn.Linear(channels, (self.heads + 2 * self.kv_heads) * self.head_dim, bias=bias)
+        self.proj = nn.Linear(self.heads * self.head_dim, channels, bias=bias)
+
+    def forward(self, x: SparseTensor, segments: Optional[AttentionSegments] = None,
+                key_mask: Optional[torch.Tensor] = None) -> SparseTensor:
+        if segments is None:  # each sample a segment (reads the rows per sample back)
+            segments = AttentionSegments.from_tensor(x)
+        qkv = self.qkv(x.F).view(x.F.shape[0], self.heads + 2 * self.kv_heads, self.head_dim)
+        q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)
+        q, k = sparse_rotary(q, k, x, self.rotary)
+        out = sparse_attention(q, k, v, segments, causal=self.causal, key_mask=key_mask)
+        return x.replace(self.proj(out.flatten(1)))
+
+
+class SparseTransformerBlock(nn.Module):
+    """Pre-norm block: attention within the segments, then a two-layer GELU network."""
+
+    def __init__(self, channels: int, heads: int, kv_heads: Optional[int] = None, mlp_ratio: float = 4.0, eps: float = 1e-5,
+                 axes: Optional[Sequence[int]] = None, causal: bool = False):
+        super().__init__()
+        self.eps = eps
+        self.norm1 = nn.LayerNorm(channels, eps=eps)
+        self.attn = SparseAttention(channels, heads, kv_heads, axes=axes, causal=causal)
+        self.norm2 = nn.LayerNorm(channels, eps=eps)
+        hidden = int(channels * mlp_ratio)
+        self.mlp = nn.Sequential(nn.Linear(channels, hidden), nn.GELU(), nn.Linear(hidden, channels))
+
+    def forward(self, x: SparseTensor, segments: Optional[AttentionSegments] = None,
+                key_mask: Optional[torch.Tensor] = None) -> SparseTensor:
+        y = sparse_layer_norm(x, self.norm1.weight, self.norm1.bias, eps=self.eps)
+        a = self.attn(y, segments, key_mask)
+        z, h = sparse_layer_norm(a, self.norm2.weight, self.norm2.bias, eps=self.eps, residual=x)
+        return h.replace(h.F + self.mlp(z.F))

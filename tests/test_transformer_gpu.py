@@ -1,0 +1,133 @@
+"""SparseAttention and SparseTransformerBlock against the same block in plain float64 torch.
+
+fp32 features: every step is a few fp32 roundings of values near one, so the outputs and gradients
+agree to 2e-5 of their norm; bf16 rounds each stored tensor (2^-8), about ten on the way: 5e-2.
+"""
+
+import copy
+import math
+
+import pytest
+import torch
+from torch import nn
+
+from sparsetriton_amd import SparseTensor, nn as snn
+from sparsetriton_amd.nn.functional import AttentionSegments
+
+pytestmark = pytest.mark.gpu
+
+
+def _voxels(rows, channels, device, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    coords = torch.cat([torch.cat([torch.full((n, 1), b), torch.randint(0, 60, (n, 3), generator=g)], 1)
+                        for b, n in enumerate(rows)]).int()
+    feats = torch.randn((sum(rows), channels), generator=g).to(device, dtype)
+    return SparseTensor(feats, coords.to(device), spatial_shape=(60, 60, 60), batch_size=len(rows))
+
+
+def _plain(block, x, coords, lengths, causal):
+    """The block in float64: norms, projections, rotation and attention from their formulas."""
+    at = block.attn
+    d, h, hk = at.head_dim, at.heads, at.kv_heads
+    y = block.norm1(x)
+    q, k, v = at.qkv(y).view(len(x), h + 2 * hk, d).split((h, hk, hk), 1)
+    p = at.rotary.pairs
+    axis = [i for i, a in enumerate(at.rotary.axes) for _ in range(a // 2)]
+    angle = coords[:, 1:].double()[:, axis] * at.rotary.frequencies.double().to(x.device)
+    c, s = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+
+    def turn(t):
+        a, b = t[..., :p], t[..., p:2 * p]
+        return torch.cat((a * c - b * s, a * s + b * c, t[..., 2 * p:]), -1)
+
+    q, k = turn(q), turn(k)
+    out, r0 = [], 0
+    for n in lengths:
+        rows = slice(r0, r0 + n)
+        kk, vv = (t[rows].repeat_interleave(h // hk, 1).transpose(0, 1).contiguous() for t in (k, v))
+        z = q[rows].transpose(0, 1).contiguous() @ kk.transpose(1, 2).contiguous() / math.sqrt(d)
+        if causal:
+            z = z.masked_fill(torch.ones((n, n), dtype=torch.bool, device=x.device).triu(1), float("-inf"))
+        out.append((torch.softmax(z, -1) @ vv).transpose(0, 1).reshape(n, -1))
+        r0 += n
+    hh = x + at.proj(torch.cat(out))
+    return hh + block.mlp(block.norm2(hh))
+
+
+@pytest.mark.parametrize("dtype,tol", [(torch.float32, 2e-5), (torch.bfloat16, 5e-2)])
+@pytest.mark.parametrize("heads,kv_heads,channels,causal,patch", [(4, 4, 64, False, None), (8, 2, 128, True, 50),
+                                                                 (3, 1, 120, False, 33)])
+def test_block_trains_like_the_plain_one(device, dtype, tol, heads, kv_heads, channels, causal, patch):
+    torch.manual_seed(1)
+    block = snn.SparseTransformerBlock(channels, heads, kv_heads, mlp_ratio=2, causal=causal).to(device, dtype)
+    x = _voxels([130, 1, 77], channels, device, dtype, 2)
+    segs = AttentionSegments.from_tensor(x, patch)
+    lengths = segs._nq.tolist()
+    plain = copy.deepcopy(block).double()
+    ref_x = x.F.double().requires_grad_(True)
+    dy = torch.randn(x.F.shape, device=device).to(dtype)
+    ref = _plain(plain, ref_x, x.C, lengths, causal)
+    ref.backward(dy.double())
+    feats = x.F.clone().requires_grad_(True)
+    out = block(x.replace(feats), segs)
+    assert isinstance(out, SparseTensor) and out._cache is x._cache
+    out.F.backward(dy)
+
+    def near(a, b, what):
+        assert (a.double() - b).norm() <= tol * b.norm() + 1e-12, (what, ((a.double() - b).norm() / b.norm()).item())
+
+    near(out.F.detach(), ref.detach(), "output")
+    near(feats.grad, ref_x.grad, "features")
+    for (name, p), q in zip(block.named_parameters(), plain.parameters()):
+        near(p.grad, q.grad, name)
+
+
+def test_blocks_after_a_convolution_learn(device):
+    """A convolution, two blocks over patches and a head, a few steps of training: the loss falls."""
+    torch.manual_seed(3)
+
+    class Net(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.stem = snn.SparseConvBlock(8, 64, 3)
+            self.blocks = nn.ModuleList(snn.SparseTransformerBlock(64, 4, mlp_ratio=2) for _ in range(2))
+            self.head = snn.SparseLinear(64, 4)
+
+        def forward(self, x):
+            x = self.stem(x)
+            segs = AttentionSegments.from_tensor(x, patch=128)
+            for b in self.blocks:
+                x = b(x, segs)
+            return self.head(x).F
+
+    net = Net().to(device)
+    x = _voxels([400, 300], 8, device, torch.float32, 4)
+    want = (x.C[:, 1:].sum(1) % 4).long()
+    opt = torch.optim.Adam(net.parameters(), lr=3e-3)
+    losses = []
+    for _ in range(30):
+        loss = nn.functional.cross_entropy(net(x), want)
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+        losses.append(loss.item())
+    assert all(map(math.isfinite, losses)) and losses[-1] < 0.8 * losses[0], losses
+
+
+def test_whole_samples_without_segments_and_state(device):
+    torch.manual_seed(5)
+    attn = snn.SparseAttention(96, 3, head_dim=40, axes=(12, 12, 8)).to(device)
+    x = _voxels([20, 30], 96, device, torch.float32, 6)
+    out = attn(x)
+    assert torch.equal(out.F, attn(x, AttentionSegments([20, 30], device=device)).F)
+    again = copy.deepcopy(attn)
+    again.load_state_dict(attn.state_dict())
+    assert torch.equal(again(x).F, out.F)
+    assert sorted(attn.state_dict()) == ["proj.bias", "proj.weight", "qkv.bias", "qkv.weight"]
+
+
+def test_refusals():
+    with pytest.raises(ValueError, match="divide"):
+        snn.SparseAttention(100, 3)
+    with pytest.raises(ValueError, match="share"):
+        snn.SparseAttention(96, 6, kv_heads=4)
