@@ -924,6 +924,7 @@ typedef struct st_attn_args {
   float* parts;
   int32_t heads, kv_heads, dim, dtype, causal;
   int32_t q_tile, k_tile; /* ST_ATTN_TILE, or ST_ATTN_SMALL_TILE for segments of few rows (keys) */
+  int32_t q_item_major, k_item_major; /* order of the work: 0 a key head's items, 1 an item's key heads */
   float scale;
 } st_attn_args;
 int st_attn_workspace(int kv_heads, int dim, int64_t q_parts, int64_t k_parts, int64_t* floats);

@@ -81,7 +81,7 @@ class AttnArgs(ctypes.Structure):
         + [(n, _P) for n in ("key_mask", "q_items", "q_joins", "k_items", "k_joins")]
         + [(n, _L) for n in ("n_q_items", "n_q_joins", "n_k_items", "n_k_joins")]
         + [("parts", _P)]
-        + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "dtype", "causal", "q_tile", "k_tile")]
+        + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "dtype", "causal", "q_tile", "k_tile", "q_item_major", "k_item_major")]
         + [("scale", ctypes.c_float)]
     )
 

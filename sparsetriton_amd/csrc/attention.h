@@ -67,7 +67,8 @@ struct AttnArgs {
   const AttnJoin* joins;
   int n_items, n_joins;
   int heads, kv_heads, group, D, causal;
-  int tile;  // rows of the items' tiles: ST_ATTN_TILE or ST_ATTN_SMALL_TILE
+  int tile;        // rows of the items' tiles: ST_ATTN_TILE or ST_ATTN_SMALL_TILE
+  int item_major;  // workgroups take an item's key heads in turn, else a key head's items
   float scale, scale_log2;  // c and c / ln 2
 };
 
@@ -385,8 +386,8 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
   T* tiles = reinterpret_cast<T*>(lds);
   float* bias = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers, not CAUSAL: 0 or -inf for each key of a step
 
-  const int w = attn_work(gridDim.x), hk = w / a.n_items;
-  const AttnItem it = a.items[w - hk * a.n_items];
+  const int w = attn_work(gridDim.x), hk = a.item_major ? w % a.kv_heads : w / a.n_items;
+  const AttnItem it = a.items[a.item_major ? w / a.kv_heads : w - hk * a.n_items];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
   const int rows = it.nq * a.group, r = it.row0 + wave * 32 + (lane & 31);
   const bool active = it.row0 + wave * 32 < rows, live = r < rows;
@@ -623,8 +624,8 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
 
-  const int w = attn_work(gridDim.x), hk = w / a.n_items;
-  const AttnItem it = a.items[w - hk * a.n_items];
+  const int w = attn_work(gridDim.x), hk = a.item_major ? w % a.kv_heads : w / a.n_items;
+  const AttnItem it = a.items[a.item_major ? w / a.kv_heads : w - hk * a.n_items];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
   const int rows = it.nq * a.group, r = it.row0 + wave * 32 + (lane & 31);
   const bool active = it.row0 + wave * 32 < rows, live = r < rows;
@@ -761,8 +762,8 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
   float* stats = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers of BQ L, BQ delta
   T* copies = reinterpret_cast<T*>(stats + 4 * BQ);           // CAUSAL: of a Q and a dO tile
 
-  const int w = attn_work(gridDim.x), hk = w / a.n_items;
-  const AttnItem it = a.items[w - hk * a.n_items];
+  const int w = attn_work(gridDim.x), hk = a.item_major ? w % a.kv_heads : w / a.n_items;
+  const AttnItem it = a.items[a.item_major ? w / a.kv_heads : w - hk * a.n_items];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
   const int kw = it.row0 + wave * 32, key = kw + (lane & 31);  // in the segment
   const bool active = kw < it.nk, live = key < it.nk;
@@ -776,8 +777,8 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
     vf[s] = load_row8<T>((const T*)a.v + krow * a.v_row + hk * a.v_head, 16 * s + 8 * half, a.D, kept);
   }
   // first packed row that sees this lane's key, and the first that sees any of the wave's
-  const int from = CAUSAL ? (key - (it.nk - it.nq)) * a.group : 0;
-  const int wave_from = CAUSAL ? (kw - (it.nk - it.nq)) * a.group : 0;
+  const int from = CAUSAL ? max(key - (it.nk - it.nq), 0) * a.group : 0;
+  const int wave_from = CAUSAL ? max(kw - (it.nk - it.nq), 0) * a.group : 0;
 
   Stage qs, gs;
   float stat = 0.f;

@@ -63,7 +63,7 @@ extern "C" int st_attn_forward(const st_attn_args* a, st_stream_t stream) {
   st::AttnArgs g = attn_args(a);
   g.items = (const st::AttnItem*)a->q_items, g.n_items = (int)a->n_q_items;
   g.joins = (const st::AttnJoin*)a->q_joins, g.n_joins = (int)a->n_q_joins;
-  g.tile = a->q_tile;
+  g.tile = a->q_tile, g.item_major = a->q_item_major != 0;
   return attn_run_any(a, st::kAttnForward, g, (hipStream_t)stream);
 }
 
@@ -82,13 +82,13 @@ extern "C" int st_attn_backward(const st_attn_args* a, st_stream_t stream) {
   if (a->n_q_items) {
     g.items = (const st::AttnItem*)a->q_items, g.n_items = (int)a->n_q_items;
     g.joins = (const st::AttnJoin*)a->q_joins, g.n_joins = (int)a->n_q_joins;
-  g.tile = a->q_tile;
+  g.tile = a->q_tile, g.item_major = a->q_item_major != 0;
     rc = attn_run_any(a, st::kAttnDq, g, (hipStream_t)stream);
     if (rc != ST_OK) return rc;
   }
   if (!a->n_k_items) return ST_OK;
   g.items = (const st::AttnItem*)a->k_items, g.n_items = (int)a->n_k_items;
   g.joins = (const st::AttnJoin*)a->k_joins, g.n_joins = (int)a->n_k_joins;
-  g.tile = a->k_tile;
+  g.tile = a->k_tile, g.item_major = a->k_item_major != 0;
   return attn_run_any(a, st::kAttnDkv, g, (hipStream_t)stream);
 }

@@ -18,6 +18,10 @@ from sparsetriton_amd.utils.utils import once_differentiable
 
 __all__ = ["AttentionSegments", "sparse_attention"]
 
+# Mean length of the items against the longest, below which their order goes before the key heads' (us, forward, key
+# head by key head / longest first: causal 8,191 rows x 16 x 128 on 4 key heads 431 / 322, four of 4,096 x 8 x 64
+# 177 / 109; 64 equal patches of 1,024 x 8 x 64 170 / 177).
+_EVEN = 0.9
 # Keys (rows) that a part of a split tile is a multiple of: a step of the kernels.
 _STEP = 64
 # Small tiles (one wave) are taken while there are at most so many for each wide one (four waves), that is
@@ -39,8 +43,8 @@ def _lengths(lengths, what: str) -> np.ndarray:
     if out.ndim != 1 or (out.size and out.dtype.kind not in "iu"):
         raise ValueError(f"{what} must be a list of row counts")
     out = out.astype(np.int64)
-    if (out < 0).any() or out.sum() >= 2 ** 31:
-        raise ValueError(f"{what} must not be negative, and at most 2^31 - 1 rows in all")
+    if (out < 0).any() or out.sum() >= 2 ** 31 - 4096:
+        raise ValueError(f"{what} must not be negative, and less than 2^31 - 4096 rows in all")
     return out
 
 
@@ -66,7 +70,9 @@ class _Tiles:
         slot0 = np.cumsum(np.where(split, parts, 0)) - np.where(split, parts, 0)
         part = np.where(split[of], slot0[of] + nth, -1)
         items = np.stack([q0[of], nq[of], k0[of], nk[of], row0[of], first, end, part], 1)
-        # longest first: the last workgroups to start are short ones
+        # Longest first: the last workgroups to start are short ones.  Tiles of much the same length go key head by
+        # key head (neighbours read the same keys); else the long ones of every key head come before the short ones.
+        self.item_major = int(n > 0 and (end - first).mean() < _EVEN * (end - first).max())
         items = items[np.argsort(first - end, kind="stable")]
         at = np.flatnonzero(split)
         joins = np.stack([q0[at], nq[at], k0[at], nk[at], row0[at], slot0[at], parts[at], np.zeros_like(at)], 1)
@@ -186,7 +192,7 @@ def _args(q, k, v, key_mask, o, lse, causal, scale) -> _lib.AttnArgs:
     return _lib.AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(lse), None, None, None, None, None,
                          qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], 0, 0, ptr(key_mask), None, None, None, None, 0, 0, 0, 0,
                          None, q.shape[1], k.shape[1], q.shape[2], _lib.FEAT_DTYPES[q.dtype], causal, _lib.ATTN_TILE,
-                         _lib.ATTN_TILE, scale)
+                         _lib.ATTN_TILE, 0, 0, scale)
 
 
 def _forward(q, k, v, segments, key_mask, causal, scale, stats):
@@ -199,7 +205,7 @@ def _forward(q, k, v, segments, key_mask, causal, scale, stats):
     plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size())
     a = _args(q, k, v, key_mask, o, lse, causal, scale)
     a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
-    a.q_tile = plan.tile
+    a.q_tile, a.q_item_major = plan.tile, plan.item_major
     parts = _parts(kv_heads, dim, plan.slots, 0, q.device)
     if parts is not None:
         a.parts = parts.data_ptr()
@@ -231,7 +237,7 @@ class _Attention(torch.autograd.Function):
         a.dout, a.dq, a.delta = dout.data_ptr(), dq.data_ptr(), delta.data_ptr()
         a.dout_row, a.dout_head, _ = dout.stride()
         a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
-        a.q_tile = plan.tile
+        a.q_tile, a.q_item_major = plan.tile, plan.item_major
         dk = dv = None
         slots = 0
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
@@ -239,7 +245,7 @@ class _Attention(torch.autograd.Function):
             keys = segments._plan("k", group, kv_heads, causal, dim * q.element_size())
             a.dk, a.dv = dk.data_ptr(), dv.data_ptr()
             a.k_items, a.k_joins, a.n_k_items, a.n_k_joins = keys.items, keys.joins, keys.n_items, keys.n_joins
-            a.k_tile = keys.tile
+            a.k_tile, a.k_item_major = keys.tile, keys.item_major
             slots = keys.slots
         parts = _parts(kv_heads, dim, plan.slots, slots, q.device)
         if parts is not None:
