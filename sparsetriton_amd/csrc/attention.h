@@ -749,8 +749,22 @@ constexpr int attn_dkv_lds(bool causal) {
 
 // dK and dV of a tile of keys: the waves hold 32 keys each (K, V and both sums in
 // registers) while the packed rows' Q, dO, L and delta go by through LDS.
-template <typename T, int DP, bool CAUSAL, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void attn_dkv_kernel(AttnArgs a) {
+//
+// dV and dK of wide 16-bit rows are two launches (WHAT): together K, V and both
+// sums of 32 keys take 192 registers of a lane at 128 channels and leave a SIMD
+// one wave, whose products and softmax then wait for each other.  Five products
+// in the place of four, by two waves a SIMD: 32 patches of 1,024 rows x 8 x 128 bf16,
+// the whole backward, 760 -> 680 us (at 96 channels 424 -> 486: one launch there).
+constexpr int kAttnDv = 1, kAttnDk = 2;
+template <typename T, int DP>
+constexpr bool attn_dkv_apart() {
+  return sizeof(T) == 2 && DP > 96;
+}
+
+template <typename T, int DP, bool CAUSAL, int WAVES, int WHAT>
+__global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_waves<T, DP * 3 / 2>() : attn_waves<T, DP>()))
+    void attn_dkv_kernel(AttnArgs a) {
+  constexpr bool DV = WHAT & kAttnDv, DK = WHAT & kAttnDk;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
   constexpr int BQ = attn_q_rows<T, DP, WAVES>();
@@ -770,11 +784,11 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
   const int64_t krow = it.k0 + (int64_t)key;
   const bool kept = live && (!a.key_mask || a.key_mask[krow]);
 
-  Frag kf[KS], vf[KS];
+  Frag kf[KS], vf[DK ? KS : 1];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     kf[s] = load_row8<T>((const T*)a.k + krow * a.k_row + hk * a.k_head, 16 * s + 8 * half, a.D, kept);
-    vf[s] = load_row8<T>((const T*)a.v + krow * a.v_row + hk * a.v_head, 16 * s + 8 * half, a.D, kept);
+    if constexpr (DK) vf[s] = load_row8<T>((const T*)a.v + krow * a.v_row + hk * a.v_head, 16 * s + 8 * half, a.D, kept);
   }
   // first packed row that sees this lane's key, and the first that sees any of the wave's
   const int from = CAUSAL ? max(key - (it.nk - it.nq), 0) * a.group : 0;
@@ -808,9 +822,12 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
     }
   };
 
-  v16f dk[DB], dv[DB];
+  v16f dk[DK ? DB : 1], dv[DV ? DB : 1];
 #pragma unroll
-  for (int b = 0; b < DB; ++b) dk[b] = dv[b] = (v16f)(0.f);
+  for (int b = 0; b < DB; ++b) {
+    if constexpr (DK) dk[b] = (v16f)(0.f);
+    if constexpr (DV) dv[b] = (v16f)(0.f);
+  }
   AttnNotFinite left_out;
   if (it.lo < it.hi) fetch(it.lo);
   for (int rt = it.lo, buf = 0; rt < it.hi; rt += BQ, buf ^= 1) {
@@ -825,11 +842,11 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
     if (!active || rt + BQ <= wave_from) continue;
     const bool cut = CAUSAL && __any(from > rt);
     const T *qp = ql, *gp = gl;  // (a row whose Q or dO is not finite has a delta, and so a dS, that is not)
-    if (cut && (attn_not_finite<T, BQ, DP>(ql) || attn_not_finite<T, BQ, DP>(gl))) {
-      attn_copy_finite<T, BQ, DP>(ql, copies);
-      attn_copy_finite<T, BQ, DP>(gl, copies + TILE);
+    if (cut && ((DK && attn_not_finite<T, BQ, DP>(ql)) || (DV && attn_not_finite<T, BQ, DP>(gl)))) {
+      if constexpr (DK) attn_copy_finite<T, BQ, DP>(ql, copies);
+      if constexpr (DV) attn_copy_finite<T, BQ, DP>(gl, copies + TILE);
       qp = copies, gp = copies + TILE;
-      left_out.add<T, BQ, DP>(gl, from - rt, BQ);
+      if constexpr (DV) left_out.add<T, BQ, DP>(gl, from - rt, BQ);
     }
 #pragma unroll 1
     for (int b = 0; b < NB; ++b) {
@@ -837,9 +854,9 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
 #pragma unroll
       for (int i = 0; i < KS && attn_in<T>(16 * i, a.D); ++i) {
         s = mma32(Tile::rows(ql, b * 32 + (lane & 31), 16 * i + 8 * half), kf[i], s);
-        dp = mma32(Tile::rows(gl, b * 32 + (lane & 31), 16 * i + 8 * half), vf[i], dp);
+        if constexpr (DK) dp = mma32(Tile::rows(gl, b * 32 + (lane & 31), 16 * i + 8 * half), vf[i], dp);
       }
-      attn_reads_ahead<T, 2 * KS>();
+      attn_reads_ahead<T, (DK ? 2 : 1) * KS>();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const v4f L = *reinterpret_cast<const v4f*>(st + b * 32 + 8 * j + 4 * half);
@@ -850,6 +867,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = rt + b * 32 + reg_row(e, half) >= from ? s[e] : 0.f;
       }
+      if constexpr (DV) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const Frag p = to_frag<T>(regs8(s, j));
@@ -857,6 +875,8 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
         for (int d = 0; d < DB; ++d) dv[d] = mma32(Tile::cols(gp, b * 32 + 16 * j, d * 32), p, dv[d]);
       }
       attn_reads_ahead<T, 2 * DB, true>();
+      }
+      if constexpr (DK) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const v4f dl = *reinterpret_cast<const v4f*>(st + BQ + b * 32 + 8 * j + 4 * half);
@@ -874,24 +894,28 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP * 3 / 2>())) void att
         for (int d = 0; d < DB; ++d) dk[d] = mma32(Tile::cols(qp, b * 32 + 16 * j, d * 32), ds, dk[d]);
       }
       attn_reads_ahead<T, 2 * DB, true>();
+      }
     }
   }
 
-  if (CAUSAL) left_out.apply(dv);
+  if constexpr (CAUSAL && DV) left_out.apply(dv);
   if (!kept) {  // a masked key gets no gradient
 #pragma unroll
-    for (int b = 0; b < DB; ++b) dk[b] = dv[b] = (v16f)(0.f);
+    for (int b = 0; b < DB; ++b) {
+      if constexpr (DK) dk[b] = (v16f)(0.f);
+      if constexpr (DV) dv[b] = (v16f)(0.f);
+    }
   }
   if (it.part >= 0) {
     float* row = a.parts + ((((int64_t)it.part * a.kv_heads + hk) * 2) * kAttnTile + wave * 32 + (lane & 31)) * DP;
-    store_part<DB>(row, dk, live);
-    store_part<DB>(row + kAttnTile * DP, dv, live);
+    if constexpr (DK) store_part<DB>(row, dk, live);
+    if constexpr (DV) store_part<DB>(row + kAttnTile * DP, dv, live);
     return;
   }
   if (!active) return;
   const int64_t at = (krow * a.kv_heads + hk) * a.D;
-  store_row<T, DB>((T*)a.dk + at, dk, a.scale, a.D, live);
-  store_row<T, DB>((T*)a.dv + at, dv, 1.f, a.D, live);
+  if constexpr (DK) store_row<T, DB>((T*)a.dk + at, dk, a.scale, a.D, live);
+  if constexpr (DV) store_row<T, DB>((T*)a.dv + at, dv, 1.f, a.D, live);
 }
 
 // Sums of the partial gradients of split tiles, in a fixed order (shares of
@@ -960,8 +984,15 @@ static int attn_pass(AttnPass pass, const AttnArgs& a, hipStream_t s) {
   if (pass == kAttnDq)
     return run(a.causal ? attn_dq_kernel<T, DP, true, WAVES> : attn_dq_kernel<T, DP, false, WAVES>,
                attn_fwd_lds<T, DP, WAVES>(a.causal));
-  return run(a.causal ? attn_dkv_kernel<T, DP, true, WAVES> : attn_dkv_kernel<T, DP, false, WAVES>,
-             attn_dkv_lds<T, DP, WAVES>(a.causal));
+  const int lds = attn_dkv_lds<T, DP, WAVES>(a.causal);
+  if constexpr (attn_dkv_apart<T, DP>()) {
+    const int rc = run(a.causal ? attn_dkv_kernel<T, DP, true, WAVES, kAttnDv> : attn_dkv_kernel<T, DP, false, WAVES, kAttnDv>, lds);
+    if (rc != ST_OK) return rc;
+    return run(a.causal ? attn_dkv_kernel<T, DP, true, WAVES, kAttnDk> : attn_dkv_kernel<T, DP, false, WAVES, kAttnDk>, lds);
+  } else {
+    constexpr int BOTH = kAttnDv | kAttnDk;
+    return run(a.causal ? attn_dkv_kernel<T, DP, true, WAVES, BOTH> : attn_dkv_kernel<T, DP, false, WAVES, BOTH>, lds);
+  }
 }
 template <typename T, int DP>
 static int attn_dp(AttnPass pass, const AttnArgs& a, hipStream_t s) {
