@@ -358,6 +358,24 @@ constexpr int attn_waves() {
 
 // ------------------------------------------------------------------ forward
 
+// A tile of packed rows against its keys in steps, K and V of the next step on
+// their way to registers while this one is multiplied (two buffers in LDS, one
+// barrier a step).  A softmax in one pass: running maximum and sum, the
+// accumulators scaled when the maximum rises.  Few tiles: the keys are split
+// and the parts joined after it.
+//
+// 64 patches of 1,024 rows x 8 heads x 64 bf16: 200 us, 690 TFLOP/s (a large
+// product: 1,210).  The vector unit is what it runs on: an exponential, a
+// multiply-add, a sum, half a conversion and half a maximum for each score
+// against 64 channels of MFMA; it issues 72 % of the time, the matrix unit is
+// busy 39 %, three waves a SIMD.  128 channels do twice the product for the same
+// scores: 8,191 rows x 16 heads of 128 (4 key heads), causal, bf16, 330 us, 830
+// TFLOP/s of the visible half.  fp32, 24 samples of up to 1,500 rows x 6 x 48: 80
+// us, 72 TFLOP/s (a large fp32 product: 153), the matrix unit busy 60 %, a seventh of
+// it for the channels 48 .. 63 of the second product.  Single rows over 75,000
+// keys of 8 heads x 128: 58 us, 5.3 TB/s.  2,000 windows of up to 96 rows x 4 x
+// 32, one wave each: 15 us, 2.8 TB/s, each wave's own chain of loads, products and exponentials.
+
 // Keys of a step: 64, or 32 for a wave alone (its lanes carry the whole step on its way to LDS).
 template <int WAVES>
 constexpr int attn_keys() {
@@ -612,7 +630,14 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArg
 
 // ------------------------------------------------------------------ backward: queries
 
-// dQ of a tile of rows, and delta = rowsum(dO o O) for the keys' pass after it.
+// dQ of a tile of rows, and delta = rowsum(dO o O) for the keys' pass after it:
+// the forward's loop with P from the saved L (no running statistics).  dQ in a
+// kernel of its own computes S and dP a second time, seven products in all for
+// five; one kernel for all three gradients would add dQ with atomics, in an
+// order that changes the bits, or write it once for each tile of keys.
+//
+// As the forward's sizes: 64 channels bf16 255 us (810 TFLOP/s, MFMA busy 45 %, vector
+// unit 63), 128 channels causal 475 us (870, 44 %), fp32 114 us (76, 61 %).
 template <typename T, int DP, bool CAUSAL, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
@@ -755,6 +780,10 @@ constexpr int attn_dkv_lds(bool causal) {
 // one wave, whose products and softmax then wait for each other.  Five products
 // in the place of four, by two waves a SIMD: 32 patches of 1,024 rows x 8 x 128 bf16,
 // the whole backward, 760 -> 680 us (at 96 channels 424 -> 486: one launch there).
+//
+// As the forward's sizes: 64 channels bf16 345 us (800 TFLOP/s, MFMA busy 43 %, vector
+// unit 50; two waves a SIMD, which wait for each other's products and LDS reads), 128
+// channels causal 368 + 550 us (750 each, 34 %), fp32 166 us (70, 56 %).
 constexpr int kAttnDv = 1, kAttnDk = 2;
 template <typename T, int DP>
 constexpr bool attn_dkv_apart() {
