@@ -893,7 +893,9 @@ int st_rotary(const st_rotary_args* args, st_stream_t stream);
  * keys and ranges of packed rows (every row that sees a key of the tile).
  * parts: fp32 workspace, 16-byte address, st_attn_workspace floats for the
  * slots used.  lse (rows, heads) fp32, base-2 logarithm, INFINITY for a row
- * without keys: written when not NULL, needed by the backward; delta (rows,
+ * without keys: written when not NULL, needed by the backward; o_rest (as o; NULL =
+ * none): what the rounding of o to 16 bits left, written by the forward and added
+ * to o where the backward takes rowsum(dO o O), not used for ST_F32; delta (rows,
  * heads) fp32: scratch of the backward.  n_k_items = 0 leaves dK and dV out.
  * All sums are in a fixed order.
  */
@@ -908,6 +910,7 @@ typedef struct st_attn_args {
   const void* k;
   const void* v;
   void* o;
+  void* o_rest;
   float* lse;
   const void* dout;
   void* dq;

@@ -76,7 +76,7 @@ class RotaryArgs(ctypes.Structure):
 
 class AttnArgs(ctypes.Structure):
     _fields_ = (
-        [(n, _P) for n in ("q", "k", "v", "o", "lse", "dout", "dq", "dk", "dv", "delta")]
+        [(n, _P) for n in ("q", "k", "v", "o", "o_rest", "lse", "dout", "dq", "dk", "dv", "delta")]
         + [(n, _L) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "dout_row", "dout_head")]
         + [(n, _P) for n in ("key_mask", "q_items", "q_joins", "k_items", "k_joins")]
         + [(n, _L) for n in ("n_q_items", "n_q_joins", "n_k_items", "n_k_joins")]

@@ -25,7 +25,11 @@
 // fp32 tensors use the fp32 MFMA (32 x 32 x 2), eight of them in the place of a
 // 32 x 32 x 16, in the same layout: nothing is rounded below 32 bits.  16-bit
 // types round P and dS to the type for the second product (their sums, the
-// softmax statistics and all accumulators are fp32).
+// softmax statistics and all accumulators are fp32), and a training pass keeps
+// what O's rounding left beside O: delta is a sum of products that cancel dP where
+// a row sees few keys, and there the error of one from the rounded O is the
+// largest (causal rows of 1 - 8 keys: dQ off by 1.9 times the rounding of dQ
+// itself, 1.5 with the rest of O; 1.4 are that rounding and dS's.  No slower).
 #pragma once
 
 #include "common.h"
@@ -59,7 +63,8 @@ struct AttnJoin {  // ST_ATTN_JOIN_WORDS int32
 
 struct AttnArgs {
   const void *q, *k, *v, *o, *dout;
-  void *out, *dq, *dk, *dv;
+  const void* o_rest;  // NULL, or (16-bit) O before its rounding minus O: written by the forward, read for delta
+  void *out, *rest, *dq, *dk, *dv;
   float *lse, *delta, *parts;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
   const uint8_t* key_mask;
@@ -305,6 +310,17 @@ __device__ __forceinline__ void store_row(T* row, const v16f (&acc)[DB], float s
     }
   }
 }
+// What the rounding of acc * scale to T leaves, in acc's place.
+template <typename T, int DB>
+__device__ __forceinline__ void keep_rest(v16f (&acc)[DB], float scale) {
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float x = acc[b][e] * scale;
+      acc[b][e] = x - (float)(T)x;
+    }
+}
 // The same as fp32 partial sums at a row of DP floats.
 template <int DB>
 __device__ __forceinline__ void store_part(float* row, const v16f (&acc)[DB], bool live) {
@@ -391,6 +407,16 @@ constexpr int attn_fwd_lds(bool causal) {  // two buffers of K and V; causal, a 
 // than this (in powers of two): below, exp2(S - m) <= 2^8 loses nothing in
 // floating point, and the accumulators need no rescaling.
 constexpr float kAttnSlack = 8.f;
+// float16 holds P times a power of two, so that small probabilities keep their bits: below 2^-14
+// the type has fewer of them.  Forward: P up to 2^8 (kAttnSlack) times 2^7; the keys' pass: P up to 1
+// times 2^14 (dP - delta over as much).  The powers are added to the exponents and cost nothing.
+// (dS has no bound of its own: its scale is the caller's, as the scale of the loss.)
+template <typename T>
+constexpr float kAttnUp = sizeof(T) == 2 && !__is_same(T, __bf16) ? 7.f : 0.f;
+template <typename T>
+constexpr float kAttnKeysUp = 2.f * kAttnUp<T>;
+template <typename T>
+constexpr float kAttnKeysDown = kAttnUp<T> == 0.f ? 1.f : 1.f / 16384.f;
 
 template <typename T, int DP, bool CAUSAL, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forward_kernel(AttnArgs a) {
@@ -511,7 +537,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[b][e] *= shrink;
     }
-    const float base = m == -INFINITY ? 0.f : -m;
+    const float base = m == -INFINITY ? 0.f : kAttnUp<T> - m;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -540,6 +566,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
 
   if (CAUSAL) left_out.apply(o);
   l += other_half(l);
+  m -= kAttnUp<T>;
   if (it.part >= 0) {
     // a row of DP sums, then its maximum (in powers of two) and sum
     float* row = a.parts + (((int64_t)it.part * a.kv_heads + hk) * kAttnTile + wave * 32 + (lane & 31)) * (DP + 4);
@@ -552,7 +579,13 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
   }
   if (!active) return;
   const int64_t q = it.q0 + (int64_t)qi;
-  store_row<T, DB>((T*)a.out + (q * a.heads + head) * a.D, o, l > 0.f ? 1.f / l : l, a.D, live);
+  const int64_t at = (q * a.heads + head) * a.D;
+  const float inv = l > 0.f ? 1.f / l : l;
+  store_row<T, DB>((T*)a.out + at, o, inv, a.D, live);
+  if (sizeof(T) == 2 && a.rest) {
+    keep_rest<T>(o, inv);
+    store_row<T, DB>((T*)a.rest + at, o, 1.f, a.D, live);
+  }
   if (a.lse && live && half == 0) a.lse[q * a.heads + head] = l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l;
 }
 
@@ -622,7 +655,12 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArg
     const int64_t at = (jn.q0 + (int64_t)qi) * a.heads + head;
     if (quad * 4 < a.D) {
       typedef T v4t __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<v4t*>((T*)a.out + at * a.D + quad * 4) = __builtin_convertvector(sum * (l > 0.f ? 1.f / l : l), v4t);
+      const v4f x = sum * (l > 0.f ? 1.f / l : l);
+      const v4t y = __builtin_convertvector(x, v4t);
+      *reinterpret_cast<v4t*>((T*)a.out + at * a.D + quad * 4) = y;
+      if (sizeof(T) == 2 && a.rest)
+        *reinterpret_cast<v4t*>((T*)a.rest + at * a.D + quad * 4) =
+            __builtin_convertvector(x - __builtin_convertvector(y, v4f), v4t);
     }
     if (a.lse && quad == 0) a.lse[at] = l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l;
   }
@@ -662,14 +700,15 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
   {
     const T* qrow = (const T*)a.q + q * a.q_row + head * a.q_head;
     const T* grow = (const T*)a.dout + q * a.do_row + head * a.do_head;
-    const T* orow = (const T*)a.o + at * a.D;
+    const T *orow = (const T*)a.o + at * a.D, *rrow = (const T*)a.o_rest + at * a.D;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qf[s] = load_row8<T>(qrow, 16 * s + 8 * half, a.D, live);
       gf[s] = load_row8<T>(grow, 16 * s + 8 * half, a.D, live);
       const Frag of = load_row8<T>(orow, 16 * s + 8 * half, a.D, live);
+      const Frag rf = load_row8<T>(rrow, 16 * s + 8 * half, a.D, sizeof(T) == 2 && live && a.o_rest);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)of[e], delta);
+      for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)of[e] + (float)rf[e], delta);
     }
     delta += other_half(delta);
     if (live) {
@@ -847,7 +886,8 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
       const int dq = a.group > 1 ? (int)__umulhi((unsigned)(h0 + x), inv) : x, dh = h0 + x - dq * a.group;
       const int64_t at = (q + dq) * a.heads + hk * a.group + dh;
       // (a row past the end: L = inf makes its P zero)
-      stat = threadIdx.x < BQ ? (x < left ? a.lse[at] : INFINITY) : (x < left ? a.delta[at] : 0.f);
+      stat = threadIdx.x < BQ ? (x < left ? a.lse[at] - kAttnKeysUp<T> : INFINITY)
+                              : (x < left ? a.delta[at] * kAttnKeysDown<T> : 0.f);
     }
   };
 
@@ -910,7 +950,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
       for (int j = 0; j < 4; ++j) {
         const v4f dl = *reinterpret_cast<const v4f*>(st + BQ + b * 32 + 8 * j + 4 * half);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[4 * j + e] *= dp[4 * j + e] - dl[e];
+        for (int e = 0; e < 4; ++e) s[4 * j + e] *= fmaf(dp[4 * j + e], kAttnKeysDown<T>, -dl[e]);
       }
       if (cut) {
 #pragma unroll
@@ -944,7 +984,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
   if (!active) return;
   const int64_t at = (krow * a.kv_heads + hk) * a.D;
   if constexpr (DK) store_row<T, DB>((T*)a.dk + at, dk, a.scale, a.D, live);
-  if constexpr (DV) store_row<T, DB>((T*)a.dv + at, dv, 1.f, a.D, live);
+  if constexpr (DV) store_row<T, DB>((T*)a.dv + at, dv, kAttnKeysDown<T>, a.D, live);
 }
 
 // Sums of the partial gradients of split tiles, in a fixed order (shares of
@@ -978,7 +1018,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a
     if constexpr (KEYS) {
       const int64_t at = ((jn.k0 + (int64_t)r) * a.kv_heads + hk) * a.D + quad * 4;
       *reinterpret_cast<v4t*>((T*)(which ? a.dv : a.dk) + at) =
-          __builtin_convertvector(which ? sum : sum * a.scale, v4t);
+          __builtin_convertvector(sum * (which ? kAttnKeysDown<T> : a.scale), v4t);
     } else {
       const int qi = r / a.group, head = hk * a.group + (r - qi * a.group);
       *reinterpret_cast<v4t*>((T*)a.dq + ((jn.q0 + (int64_t)qi) * a.heads + head) * a.D + quad * 4) =

@@ -25,7 +25,7 @@ static bool attn_rows_ok(const st_attn_args* a, const void* p, int64_t row, int6
 static st::AttnArgs attn_args(const st_attn_args* a) {
   st::AttnArgs g{};
   g.q = a->q, g.k = a->k, g.v = a->v, g.o = a->o, g.dout = a->dout;
-  g.out = a->o, g.dq = a->dq, g.dk = a->dk, g.dv = a->dv;
+  g.o_rest = a->o_rest, g.out = a->o, g.rest = a->o_rest, g.dq = a->dq, g.dk = a->dk, g.dv = a->dv;
   g.lse = a->lse, g.delta = a->delta, g.parts = a->parts;
   g.q_row = a->q_row, g.q_head = a->q_head, g.k_row = a->k_row, g.k_head = a->k_head;
   g.v_row = a->v_row, g.v_head = a->v_head, g.do_row = a->dout_row, g.do_head = a->dout_head;
@@ -55,7 +55,7 @@ extern "C" int st_attn_forward(const st_attn_args* a, st_stream_t stream) {
   const int rc = attn_check(a);
   if (rc != ST_OK) return rc;
   if (a->n_q_items == 0) return ST_OK;
-  if (!a->q || !a->o || !a->q_items || ((uintptr_t)a->o & 15)) return ST_ERR_ARG;
+  if (!a->q || !a->o || !a->q_items || (((uintptr_t)a->o | (uintptr_t)a->o_rest) & 15)) return ST_ERR_ARG;
   if (a->n_q_joins && (!a->q_joins || !a->parts || ((uintptr_t)a->parts & 15))) return ST_ERR_ARG;
   if (!attn_rows_ok(a, a->q, a->q_row, a->q_head) || !attn_rows_ok(a, a->k, a->k_row, a->k_head) ||
       !attn_rows_ok(a, a->v, a->v_row, a->v_head))
@@ -74,7 +74,7 @@ extern "C" int st_attn_backward(const st_attn_args* a, st_stream_t stream) {
   if (a->n_k_items && (!a->k || !a->v || !a->dk || !a->dv || !a->k_items)) return ST_ERR_ARG;
   if ((a->n_q_joins && !a->q_joins) || (a->n_k_joins && !a->k_joins)) return ST_ERR_ARG;
   if ((a->n_q_joins || a->n_k_joins) && (!a->parts || ((uintptr_t)a->parts & 15))) return ST_ERR_ARG;
-  if (((uintptr_t)a->o | (uintptr_t)a->dq | (uintptr_t)a->dk | (uintptr_t)a->dv) & 15) return ST_ERR_ARG;
+  if (((uintptr_t)a->o | (uintptr_t)a->o_rest | (uintptr_t)a->dq | (uintptr_t)a->dk | (uintptr_t)a->dv) & 15) return ST_ERR_ARG;
   if (!attn_rows_ok(a, a->q, a->q_row, a->q_head) || !attn_rows_ok(a, a->k, a->k_row, a->k_head) ||
       !attn_rows_ok(a, a->v, a->v_row, a->v_head) || !attn_rows_ok(a, a->dout, a->dout_row, a->dout_head))
     return ST_ERR_ARG;
@@ -82,7 +82,7 @@ extern "C" int st_attn_backward(const st_attn_args* a, st_stream_t stream) {
   if (a->n_q_items) {
     g.items = (const st::AttnItem*)a->q_items, g.n_items = (int)a->n_q_items;
     g.joins = (const st::AttnJoin*)a->q_joins, g.n_joins = (int)a->n_q_joins;
-  g.tile = a->q_tile, g.item_major = a->q_item_major != 0;
+    g.tile = a->q_tile, g.item_major = a->q_item_major != 0;
     rc = attn_run_any(a, st::kAttnDq, g, (hipStream_t)stream);
     if (rc != ST_OK) return rc;
   }

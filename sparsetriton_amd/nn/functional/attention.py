@@ -186,12 +186,12 @@ def _rows(t: torch.Tensor, group: int) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _args(q, k, v, key_mask, o, lse, causal, scale) -> _lib.AttnArgs:
+def _args(q, k, v, key_mask, o, rest, lse, causal, scale) -> _lib.AttnArgs:
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     ptr = _lib.ptr
-    return _lib.AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(lse), None, None, None, None, None,
-                         qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], 0, 0, ptr(key_mask), None, None, None, None, 0, 0, 0, 0,
-                         None, q.shape[1], k.shape[1], q.shape[2], _lib.FEAT_DTYPES[q.dtype], causal, _lib.ATTN_TILE,
+    return _lib.AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(rest), ptr(lse), None, None, None, None,
+                         None, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], 0, 0, ptr(key_mask), None, None, None, None,
+                         0, 0, 0, 0, None, q.shape[1], k.shape[1], q.shape[2], _lib.FEAT_DTYPES[q.dtype], causal, _lib.ATTN_TILE,
                          _lib.ATTN_TILE, 0, 0, scale)
 
 
@@ -203,28 +203,29 @@ def _forward(q, k, v, segments, key_mask, causal, scale, stats):
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if stats else None
     plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size())
-    a = _args(q, k, v, key_mask, o, lse, causal, scale)
+    rest = torch.empty_like(o) if stats and o.element_size() == 2 else None  # what its rounding leaves, for the gradient
+    a = _args(q, k, v, key_mask, o, rest, lse, causal, scale)
     a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
     a.q_tile, a.q_item_major = plan.tile, plan.item_major
     parts = _parts(kv_heads, dim, plan.slots, 0, q.device)
     if parts is not None:
         a.parts = parts.data_ptr()
     _lib.call("st_attn_forward", ctypes.byref(a), _lib.stream_of(q.device))
-    return o, lse, q, k, v
+    return o, rest, lse, q, k, v
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, segments, key_mask, causal, scale):
-        o, lse, q, k, v = _forward(q, k, v, segments, key_mask, causal, scale, True)
-        ctx.save_for_backward(q, k, v, o, lse, key_mask)
+        o, rest, lse, q, k, v = _forward(q, k, v, segments, key_mask, causal, scale, True)
+        ctx.save_for_backward(q, k, v, o, rest, lse, key_mask)
         ctx.meta = (segments, causal, scale)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, o, lse, key_mask = ctx.saved_tensors
+        q, k, v, o, rest, lse, key_mask = ctx.saved_tensors
         segments, causal, scale = ctx.meta
         heads, dim = q.shape[1:]
         kv_heads = k.shape[1]
@@ -233,7 +234,7 @@ class _Attention(torch.autograd.Function):
         new = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format)  # noqa: E731
         dq, delta = new(q), torch.empty_like(lse)
         plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size())
-        a = _args(q, k, v, key_mask, o, lse, causal, scale)
+        a = _args(q, k, v, key_mask, o, rest, lse, causal, scale)
         a.dout, a.dq, a.delta = dout.data_ptr(), dq.data_ptr(), delta.data_ptr()
         a.dout_row, a.dout_head, _ = dout.stride()
         a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
@@ -275,7 +276,8 @@ def sparse_attention(
     ``causal``: query ``i`` of ``nq`` sees keys up to ``i + nk - nq`` of its segment.  ``key_mask``
     (``segments.k_rows``) bool: False leaves a key out, whatever its rows hold.  A row that sees no
     key gets zeros, and its gradients are zero.  Scores, softmax and sums are fp32 (fp32 inputs: the
-    products too); results do not depend on timing.
+    products too); results do not depend on timing.  A 16-bit forward that records a gradient keeps what the
+    output's rounding left beside it (as large as the output), for the gradients of rows with few keys.
     """
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
         if not t.is_cuda:

@@ -10,6 +10,8 @@ channels, its exponential and the row's sum):
   dQ, dK, dV   the error of dS or P through the product, plus u of the result.
 """
 
+import math
+
 import pytest
 import torch
 
@@ -475,3 +477,62 @@ def test_refusals(device):
         sparse_attention(q.double(), q.double(), q.double(), segs)
     with pytest.raises(RuntimeError, match="GPU"):
         sparse_attention(q.cpu(), q, q, segs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(32, 4, 2), (64, 2, 2), (128, 2, 1)])
+def test_roundings_of_the_gradients_of_few_keys(device, dtype, causal, dim, heads, kv_heads):
+    """Norm of the errors of dQ and dK: the result's own rounding, and what rounding P (for O, in units of the
+    row's largest, hence delta) and dS does in float64; O's own rounding has no part in it.  The two are
+    independent: their squares add, a tenth more for what of them is chance."""
+    lens = list(range(1, 9)) * 40
+    q, k, v, do, _ = _make(lens, lens, heads, kv_heads, dim, dtype, device, 5)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = sparse_attention(*leaves, AttentionSegments(lens, device=device), causal=causal)
+    got = dict(zip(("dq", "dk"), torch.autograd.grad(o, leaves, do)))
+    ref = _reference(q, k, v, do, lens, lens, dim ** -0.5, causal, None)
+    rounded = lambda t: t.to(dtype).double()  # noqa: E731
+    off = {n: torch.zeros(ref[n][0].shape, dtype=torch.float64) for n in ("dq", "dk")}
+    q, k, v, do = (t.detach().cpu().double() for t in (q, k, v, do))
+    at = 0
+    for n in lens:
+        rows = slice(at, at + n)
+        at += n
+        see = torch.ones((n, n), dtype=torch.bool)
+        for h in range(heads):
+            hk = h * kv_heads // heads
+            s = q[rows, h] @ k[rows, hk].T * dim ** -0.5
+            p = torch.softmax(s.masked_fill(~(see.tril() if causal else see), -math.inf), 1)
+            top = p.amax(1, keepdim=True)
+            dp = do[rows, h] @ v[rows, hk].T
+            ds = p * (dp - (p * dp).sum(1, keepdim=True))
+            error = rounded(p * (dp - (rounded(p / top) * top * dp).sum(1, keepdim=True))) - ds
+            off["dq"][rows, h] = error @ k[rows, hk] * dim ** -0.5
+            off["dk"][rows, hk] += error.T @ q[rows, h] * dim ** -0.5
+    for n in off:
+        want = ref[n][0]
+        expected = math.hypot((rounded(want) - want).norm().item(), off[n].norm().item())
+        error = (got[n].double() - want).norm().item()
+        assert error < 1.1 * expected, (n, error / expected, expected / want.norm().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("step", range(0, 54, 9))
+def test_small_probabilities_in_float16(device, step, dim):
+    """One key far above the others, whose probabilities (~2^-16) are below the type's normal numbers.  V and dO
+    ask for the others alone; P and the result are rounded once each, 2^-11."""
+    n, a = 64, 2.76171875 + step / 512
+    q, k, v = (torch.zeros((n, 1, dim), dtype=torch.float16, device=device) for _ in range(3))
+    q[:, 0, 0], k[0, 0, 0], v[1:] = a, 4.0, 1.0
+    do = torch.full_like(q, 1024.0)
+    r = math.exp(-4 * a)
+    p = r / (1 + (n - 1) * r)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = sparse_attention(*leaves, AttentionSegments([n], device=device), scale=1.0)
+    dv = torch.autograd.grad(o, v, do)[0]
+    bound = 2 * 2.0 ** -11 + W
+    assert (o.double() / ((n - 1) * p) - 1).abs().max().item() <= bound
+    assert (dv[1:].double() / (n * 1024 * p) - 1).abs().max().item() <= bound
