@@ -29,8 +29,11 @@ _STEP = 64
 # 4 x 32 (1.31 small tiles a wide one) 27 / 16, 1,000 of 1-200 x 8 x 64 (1.65) 50 / 37, forward and backward of
 # 2,000 x 8 x 64 (1.34) 294 / 176; 1,000 of 64 rows (2.0) 19.3 / 19.7, 300 of 40 over 300 keys (2.0) 21 / 26.
 _SMALL_TILES = 1.8
-# Workgroups below which a tile's keys (rows) are split over several, and what the split aims at:
-# two and four for each of 256 CUs.  A part takes four steps at least.
+# Workgroups below which a tile's keys (rows) are split over several, and what the split aims at: two for each of
+# 256 CUs (as many as run at once) and four.  A part takes four steps at least.  Parts of a whole number of steps come
+# to more than that at times, and the few of a third round keep the rest waiting: dK and dV of 8,191 causal rows x
+# 16 x 128 on 4 key heads in 1,152 workgroups 890 us, in 984 800; but 24 samples of up to 1,500 rows x 6 x 48 fp32 in 1,056 of
+# up to 5 steps 376 us, in 882 of up to 6 399.
 _SPLIT_BELOW, _SPLIT_TO, _PART_STEPS = 512, 1024, 4
 
 
@@ -48,6 +51,32 @@ def _lengths(lengths, what: str) -> np.ndarray:
     return out
 
 
+def _split(steps: np.ndarray, kv_heads: int):
+    """(parts of each tile, steps of a part) for about _SPLIT_TO workgroups, or at most that many: whichever leaves
+    the shorter last round."""
+    def cut(most):
+        parts = np.maximum(1, -(-steps // most))
+        chunk = -(-steps // parts)
+        return np.maximum(1, -(-steps // np.maximum(chunk, 1))), chunk
+
+    def longest(parts, chunk):  # of _SPLIT_BELOW slots that take the longest workgroup left whenever they are free
+        items = np.repeat(chunk, parts)
+        items[np.cumsum(parts) - 1] = steps - (parts - 1) * chunk
+        items = np.repeat(np.sort(items)[::-1], kv_heads) + 1  # (a step's worth for the start and the end of each)
+        slots = np.zeros(_SPLIT_BELOW, dtype=np.int64)
+        for at in range(0, items.size, _SPLIT_BELOW):
+            slots.sort()
+            slots[:items.size - at] += items[at:at + _SPLIT_BELOW]
+        return slots.max()
+
+    most = max(_PART_STEPS, -(-int(steps.sum()) * kv_heads // _SPLIT_TO))
+    about = at_most = cut(most)
+    while at_most[0].sum() * kv_heads > _SPLIT_TO:
+        most += max(1, most // 16)
+        at_most = cut(most)
+    return at_most if at_most is about or longest(*at_most) < longest(*about) else about
+
+
 class _Tiles:
     """Work items and joins of one pass, on the device: rows (4, 8) int32 as st_attn_args lays them out."""
 
@@ -58,10 +87,7 @@ class _Tiles:
         parts = np.ones(n, dtype=np.int64)
         chunk = steps.copy()
         if n and n * kv_heads < _SPLIT_BELOW:
-            most = max(_PART_STEPS, -(-int(steps.sum()) * kv_heads // _SPLIT_TO))
-            parts = np.maximum(1, -(-steps // most))
-            chunk = -(-steps // parts)
-            parts = np.maximum(1, -(-steps // np.maximum(chunk, 1)))
+            parts, chunk = _split(steps, kv_heads)
         of = np.repeat(np.arange(n), parts)
         nth = np.arange(of.size) - np.repeat(np.cumsum(parts) - parts, parts)
         first = lo[of] + nth * chunk[of] * step
