@@ -822,7 +822,8 @@ constexpr int attn_dkv_lds(bool causal) {
 //
 // As the forward's sizes: 64 channels bf16 345 us (800 TFLOP/s, MFMA busy 43 %, vector
 // unit 50; two waves a SIMD, which wait for each other's products and LDS reads), 128
-// channels causal 368 + 550 us (750 each, 34 %), fp32 166 us (70, 56 %).
+// channels causal 333 + 480 us (830 and 860, 34 % before the last
+// round of workgroups was evened out), fp32 166 us (70, 56 %).
 constexpr int kAttnDv = 1, kAttnDk = 2;
 template <typename T, int DP>
 constexpr bool attn_dkv_apart() {

@@ -29,12 +29,16 @@ _STEP = 64
 # 4 x 32 (1.31 small tiles a wide one) 27 / 16, 1,000 of 1-200 x 8 x 64 (1.65) 50 / 37, forward and backward of
 # 2,000 x 8 x 64 (1.34) 294 / 176; 1,000 of 64 rows (2.0) 19.3 / 19.7, 300 of 40 over 300 keys (2.0) 21 / 26.
 _SMALL_TILES = 1.8
-# Workgroups below which a tile's keys (rows) are split over several, and what the split aims at: two for each of
-# 256 CUs (as many as run at once) and four.  A part takes four steps at least.  Parts of a whole number of steps come
-# to more than that at times, and the few of a third round keep the rest waiting: dK and dV of 8,191 causal rows x
-# 16 x 128 on 4 key heads in 1,152 workgroups 890 us, in 984 800; but 24 samples of up to 1,500 rows x 6 x 48 fp32 in 1,056 of
-# up to 5 steps 376 us, in 882 of up to 6 399.
-_SPLIT_BELOW, _SPLIT_TO, _PART_STEPS = 512, 1024, 4
+# Workgroups that a split of the tiles over their keys (rows) aims at, four for each of 256 compute units; a part takes
+# four steps at least.  Whether to split goes by an estimate (us, within a fifth): a step of 64 keys (rows) x 128 rows for a
+# workgroup alone on its unit, the share of it that each takes when several share the unit (by the size of an element), the
+# join's launch, and the bytes of partial results a microsecond.
+_UNITS, _SPLIT_TO, _PART_STEPS = 256, 1024, 4
+_SHARED, _JOIN_US, _PART_BYTES_US = {2: 0.75, 4: 0.88}, 7.0, 8.0e6
+
+
+def _step_us(dim: int, elem: int, keys: bool) -> float:
+    return (0.065 * dim if elem == 4 else 0.35 + 0.0086 * dim) * (2.0 if keys else 1.0)
 
 
 def _lengths(lengths, what: str) -> np.ndarray:
@@ -51,43 +55,77 @@ def _lengths(lengths, what: str) -> np.ndarray:
     return out
 
 
-def _split(steps: np.ndarray, kv_heads: int):
-    """(parts of each tile, steps of a part) for about _SPLIT_TO workgroups, or at most that many: whichever leaves
-    the shorter last round."""
-    def cut(most):
-        parts = np.maximum(1, -(-steps // most))
-        chunk = -(-steps // parts)
-        return np.maximum(1, -(-steps // np.maximum(chunk, 1))), chunk
+def _cut(steps: np.ndarray, most: int):
+    """(parts, steps of a part) of tiles of so many steps, in parts of much the same length up to ``most``."""
+    parts = np.maximum(1, -(-steps // most))
+    chunk = -(-steps // parts)
+    return np.maximum(1, -(-steps // np.maximum(chunk, 1))), chunk
 
-    def longest(parts, chunk):  # of _SPLIT_BELOW slots that take the longest workgroup left whenever they are free
-        items = np.repeat(chunk, parts)
-        items[np.cumsum(parts) - 1] = steps - (parts - 1) * chunk
-        items = np.repeat(np.sort(items)[::-1], kv_heads) + 1  # (a step's worth for the start and the end of each)
-        slots = np.zeros(_SPLIT_BELOW, dtype=np.int64)
-        for at in range(0, items.size, _SPLIT_BELOW):
-            slots.sort()
-            slots[:items.size - at] += items[at:at + _SPLIT_BELOW]
-        return slots.max()
 
-    most = max(_PART_STEPS, -(-int(steps.sum()) * kv_heads // _SPLIT_TO))
-    about = at_most = cut(most)
-    while at_most[0].sum() * kv_heads > _SPLIT_TO:
-        most += max(1, most // 16)
-        at_most = cut(most)
-    return at_most if at_most is about or longest(*at_most) < longest(*about) else about
+def _items(parts: np.ndarray, chunk: np.ndarray, steps: np.ndarray) -> np.ndarray:
+    """Steps of every part, the last one of a tile what is left."""
+    items = np.repeat(chunk, parts)
+    items[np.cumsum(parts) - 1] = steps - (parts - 1) * chunk
+    return items
+
+
+def _longest(items: np.ndarray, kv_heads: int) -> int:
+    """Steps of the slot (two a unit) with the most of them, each taking the longest item left when it is done."""
+    items = np.repeat(np.sort(items)[::-1], kv_heads) + 1  # (a step's worth for the start and the end of each)
+    held = np.zeros(2 * _UNITS, dtype=np.int64)
+    for at in range(0, items.size, held.size):
+        held.sort()
+        held[:items.size - at] += items[at:at + held.size]
+    return int(held.max())
+
+
+def _split(steps: np.ndarray, rows: np.ndarray, kv_heads: int, dim: int, elem: int, keys: bool):
+    """(parts of each tile, steps of a part), ``rows`` of each tile in use.
+
+    Whole tiles take the longest one's steps, or what the fullest slot has to do; parts an even share of all steps (and
+    a seventh for what is not even), and their joins.  bf16, 256 tiles of 16 steps whole / in two / four parts, forward and backward: 64
+    channels 20 + 55 / 34 + 74 / 36 + 87 us, 128 channels 28 + 123 / 41 + 137 / 52 + 174; 64 tiles of 128 channels 27 + 119 /
+    22 + 86 / 25 + 68, of 64 channels in fp32 78 + 270 / 46 + 151 / 32 + 94; 128 tiles of up to 128 steps beside 1,200 of
+    one, 64 channels: 119 + 335 whole, 62 + 180 in parts.
+    """
+    whole = np.ones_like(steps), steps
+    total, us = int(steps.sum()) * kv_heads, _step_us(dim, elem, keys)
+    shared = us * _SHARED[elem] * -(-int(rows.max(initial=1)) // 32) * 32 / _lib.ATTN_TILE  # (waves without rows wait)
+    longest = int(steps.max(initial=0)) + 1
+    if longest * us <= total / _UNITS * shared:
+        return whole
+    most = max(_PART_STEPS, -(-total // _SPLIT_TO))
+    parts = about = _cut(steps, most)
+    # Parts of a whole number of steps come to more than aimed at, at times, and the few of a last round keep the rest
+    # waiting (8,191 causal rows x 16 x 128 on 4 key heads, dK and dV: 1,152 parts 890 us, 984 800; but 24 samples of up to
+    # 1,500 rows x 6 x 48 fp32: 1,056 of up to 5 steps 376, 882 of up to 6 399).
+    if steps.size * kv_heads <= _SPLIT_TO:
+        while parts[0].sum() * kv_heads > _SPLIT_TO:
+            most += max(1, most // 16)
+            parts = _cut(steps, most)
+        if parts is not about:
+            parts = min((about, parts), key=lambda p: _longest(_items(*p, steps), kv_heads))
+    n = parts[0]
+    cut = n > 1
+    if not cut.any():
+        return whole
+    parts_us = max((int(parts[1].max()) + 1) * us, 1.15 * (total + int(n.sum()) * kv_heads) / _UNITS * shared)
+    parts_us += _JOIN_US + float((rows * n)[cut].sum()) * kv_heads * (dim + 2) * 8 * (2 if keys else 1) / _PART_BYTES_US
+    whole_us = longest * us
+    if steps.size * kv_heads > _UNITS:
+        # (two to a unit at its worst; once more wait than run, a long one has had shorter ones beside it)
+        whole_us = max(whole_us, _longest(steps, kv_heads) * (2 if steps.size * kv_heads <= 2 * _UNITS else 1.35) * shared)
+    return whole if whole_us <= parts_us else parts
 
 
 class _Tiles:
     """Work items and joins of one pass, on the device: rows (4, 8) int32 as st_attn_args lays them out."""
 
-    def __init__(self, tile, q0, nq, k0, nk, row0, lo, hi, kv_heads, device):
+    def __init__(self, tile, q0, nq, k0, nk, row0, rows, lo, hi, kv_heads, dim, elem, keys, device):
         self.tile, step = tile, _STEP
         steps = -(-(hi - lo) // step)
         n = steps.size
-        parts = np.ones(n, dtype=np.int64)
-        chunk = steps.copy()
-        if n and n * kv_heads < _SPLIT_BELOW:
-            parts, chunk = _split(steps, kv_heads)
+        parts, chunk = _split(steps, rows, kv_heads, dim, elem, keys)
         of = np.repeat(np.arange(n), parts)
         nth = np.arange(of.size) - np.repeat(np.cumsum(parts) - parts, parts)
         first = lo[of] + nth * chunk[of] * step
@@ -170,8 +208,9 @@ class AttentionSegments:
         seg = np.repeat(np.arange(n.size), n)
         return tile, seg, (np.arange(seg.size) - np.repeat(np.cumsum(n) - n, n)) * tile
 
-    def _plan(self, which: str, group: int, kv_heads: int, causal: bool, row_bytes: int) -> _Tiles:
-        key = (which, group, kv_heads, causal, row_bytes <= _lib.ATTN_SMALL_TILE_BYTES)
+    def _plan(self, which: str, group: int, kv_heads: int, causal: bool, row_bytes: int, elem: int = 2) -> _Tiles:
+        dim = -(-row_bytes // elem // 32) * 32  # (as the kernels are built: one list for all sizes of a kernel)
+        key = (which, group, kv_heads, causal, dim, elem)
         plan = self._plans.get(key)
         if plan is None:
             nq, nk = self._nq, self._nk
@@ -179,16 +218,19 @@ class AttentionSegments:
                 raise ValueError(f"a segment has at most {(2 ** 31 - _lib.ATTN_TILE) // group} query rows at {group} heads a key head")
             if which == "q":  # tiles of packed rows over keys lo .. hi
                 tile, seg, row0 = self._tiles(nq * group, row_bytes)
+                rows = np.minimum(nq[seg] * group - row0, tile)
                 lo, hi = np.zeros_like(row0), nk[seg]
                 if causal:
                     last = np.minimum(row0 + tile, nq[seg] * group) - 1
                     hi = np.clip(last // group + nk[seg] - nq[seg] + 1, 0, nk[seg])
             else:  # tiles of keys over packed rows lo .. hi
                 tile, seg, row0 = self._tiles(nk, row_bytes)
+                rows = np.minimum(nk[seg] - row0, tile)
                 lo, hi = np.zeros_like(row0), nq[seg] * group
                 if causal:
                     lo = np.minimum(np.maximum(0, row0 - (nk[seg] - nq[seg])) * group, hi)
-            plan = _Tiles(tile, self._q0[seg], nq[seg], self._k0[seg], nk[seg], row0, lo, hi, kv_heads, self.device)
+            plan = _Tiles(tile, self._q0[seg], nq[seg], self._k0[seg], nk[seg], row0, rows, lo, hi,
+                          kv_heads, dim, elem, which == "k", self.device)
             self._plans[key] = plan
         plan.use()
         return plan
@@ -228,7 +270,7 @@ def _forward(q, k, v, segments, key_mask, causal, scale, stats):
     q, k, v = _rows(q, group), _rows(k, group), _rows(v, group)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if stats else None
-    plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size())
+    plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size(), q.element_size())
     rest = torch.empty_like(o) if stats and o.element_size() == 2 else None  # what its rounding leaves, for the gradient
     a = _args(q, k, v, key_mask, o, rest, lse, causal, scale)
     a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
@@ -259,7 +301,7 @@ class _Attention(torch.autograd.Function):
         dout = _rows(dout, group)
         new = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format)  # noqa: E731
         dq, delta = new(q), torch.empty_like(lse)
-        plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size())
+        plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size(), q.element_size())
         a = _args(q, k, v, key_mask, o, rest, lse, causal, scale)
         a.dout, a.dq, a.delta = dout.data_ptr(), dq.data_ptr(), delta.data_ptr()
         a.dout_row, a.dout_head, _ = dout.stride()
@@ -269,7 +311,7 @@ class _Attention(torch.autograd.Function):
         slots = 0
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dk, dv = new(k), new(v)
-            keys = segments._plan("k", group, kv_heads, causal, dim * q.element_size())
+            keys = segments._plan("k", group, kv_heads, causal, dim * q.element_size(), q.element_size())
             a.dk, a.dv = dk.data_ptr(), dv.data_ptr()
             a.k_items, a.k_joins, a.n_k_items, a.n_k_joins = keys.items, keys.joins, keys.n_items, keys.n_joins
             a.k_tile, a.k_item_major = keys.tile, keys.item_major

@@ -536,3 +536,22 @@ def test_small_probabilities_in_float16(device, step, dim):
     bound = 2 * 2.0 ** -11 + W
     assert (o.double() / ((n - 1) * p) - 1).abs().max().item() <= bound
     assert (dv[1:].double() / (n * 1024 * p) - 1).abs().max().item() <= bound
+
+
+@pytest.mark.parametrize("elem,dim", [(2, 32), (2, 128), (4, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_which_tiles_are_split(elem, dim, causal):
+    """Few tiles over many keys are, tiles that fill the chip are not, and a long segment beside many short ones is
+    alone among them; every part has work and the parts of a tile follow one another without a gap."""
+    for lengths, split in (([1] * 4, False), ([30_000] * 2, True), ([1024] * 64, False), ([30_000] + [50] * 600, True),
+                           ([0, 0], False)):
+        plan = AttentionSegments([min(n, 128) for n in lengths], lengths, device="cpu")._plan("q", 1, 8, causal, dim * elem, elem)
+        words = plan.words.numpy()
+        items, joins = words[:plan.n_items], words[plan.n_items:]
+        assert (joins.shape[0] > 0) == split
+        for q0, nq, k0, nk, row0, first, parts, _ in joins:
+            mine = items[(items[:, 0] == q0) & (items[:, 4] == row0)]
+            mine = mine[mine[:, 7].argsort()]
+            assert nk == 30_000 and parts > 1 and (mine[:, 7] == range(first, first + parts)).all()
+            assert mine[0, 5] == 0 and (mine[1:, 5] == mine[:-1, 6]).all() and (mine[:, 6] > mine[:, 5]).all()
+            assert (mine[:, 5] % 64 == 0).all() and mine[-1, 6] <= nk
