@@ -61,6 +61,16 @@ struct AttnJoin {  // ST_ATTN_JOIN_WORDS int32
   int unused;
 };
 
+struct AttnDivisor {  // d and floor(2^32 / d), 2^32 - 1 for 1
+  unsigned d, inv;
+};
+inline AttnDivisor attn_divisor(int d) { return {(unsigned)d, d > 1 ? (unsigned)((1ull << 32) / d) : ~0u}; }
+// x / d for x below 2^31: the product with the inverse is the quotient or one less.
+__device__ __forceinline__ int attn_div(int x, AttnDivisor by) {
+  const unsigned q = __umulhi((unsigned)x, by.inv);
+  return (int)(q + ((unsigned)x - q * by.d >= by.d));
+}
+
 struct AttnArgs {
   const void *q, *k, *v, *o, *dout;
   const void* o_rest;  // NULL, or (16-bit) O before its rounding minus O: written by the forward, read for delta
@@ -71,6 +81,7 @@ struct AttnArgs {
   const AttnItem* items;
   const AttnJoin* joins;
   int n_items, n_joins;
+  AttnDivisor by_items, by_kv_heads, by_group;
   int heads, kv_heads, group, D, causal;
   int tile;        // rows of the items' tiles: ST_ATTN_TILE or ST_ATTN_SMALL_TILE
   int item_major;  // workgroups take an item's key heads in turn, else a key head's items
@@ -268,7 +279,24 @@ struct AttnStage {
   }
 };
 
-// Eight elements of a row in global memory (16-byte aligned), zeros past D or for a dead row.
+// Rows from `row` on, to be read at byte offsets of 32 bits.
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_rows(const T* p, int64_t row, int64_t stride) {
+  return make_rsrc(p + row * stride, kOobOffset);
+}
+// Eight elements of a row `off` bytes from a buffer's base (16-byte aligned), zeros past D or for a dead row.
+template <typename T>
+__device__ __forceinline__ typename AttnFrag<T>::type load_row8(__amdgpu_buffer_rsrc_t base, int off, int col, int D, bool live) {
+  using Frag = typename AttnFrag<T>::type;
+  const int at = live && col < D ? off + col * (int)sizeof(T) : kOobOffset;
+  if constexpr (sizeof(T) == 2) {
+    return load16<Frag>(base, at);
+  } else {
+    const v4f a = load16<v4f>(base, at), b = load16<v4f>(base, at == kOobOffset ? at : at + 16);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+// The same at an address of its own.
 template <typename T>
 __device__ __forceinline__ typename AttnFrag<T>::type load_row8(const T* row, int col, int D, bool live) {
   typename AttnFrag<T>::type f;
@@ -342,6 +370,18 @@ __device__ __forceinline__ int attn_work(int n) {
   return base + 128 > n ? id : base + (id & 7) * 16 + ((id & 127) >> 3);
 }
 
+// Item and key head of a workgroup.
+__device__ __forceinline__ AttnItem attn_item(const AttnArgs& a, int& hk) {
+  const int w = attn_work(gridDim.x);
+  if (a.item_major) {
+    const int i = attn_div(w, a.by_kv_heads);
+    hk = w - i * a.kv_heads;
+    return a.items[i];
+  }
+  hk = attn_div(w, a.by_items);
+  return a.items[w - hk * a.n_items];
+}
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // For the scheduler: of N fragment reads, each followed by its MFMAs, kAhead
@@ -390,7 +430,8 @@ constexpr int attn_waves() {
 // us, 72 TFLOP/s (a large fp32 product: 153), the matrix unit busy 60 %, a seventh of
 // it for the channels 48 .. 63 of the second product.  Single rows over 75,000
 // keys of 8 heads x 128: 58 us, 5.3 TB/s.  2,000 windows of up to 96 rows x 4 x
-// 32, one wave each: 15 us, 2.8 TB/s, each wave's own chain of loads, products and exponentials.
+// 32, one wave each: 14.5 us, 3.0 TB/s (8,000 windows 44 us, 4.0), each wave's own chain of loads, products
+// and exponentials at 16 waves a unit; bounds of five and six waves a SIMD spill (15, 35 us).
 
 // Keys of a step: 64, or 32 for a wave alone (its lanes carry the whole step on its way to LDS).
 template <int WAVES>
@@ -430,18 +471,20 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
   T* tiles = reinterpret_cast<T*>(lds);
   float* bias = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers, not CAUSAL: 0 or -inf for each key of a step
 
-  const int w = attn_work(gridDim.x), hk = a.item_major ? w % a.kv_heads : w / a.n_items;
-  const AttnItem it = a.items[a.item_major ? w / a.kv_heads : w - hk * a.n_items];
+  int hk;
+  const AttnItem it = attn_item(a, hk);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
   const int rows = it.nq * a.group, r = it.row0 + wave * 32 + (lane & 31);
   const bool active = it.row0 + wave * 32 < rows, live = r < rows;
-  const int qi = r / a.group, head = hk * a.group + (r - qi * a.group);
+  const int qi = attn_div(r, a.by_group), in_group = r - qi * a.group, head = hk * a.group + in_group;
+  const int first = attn_div(it.row0, a.by_group);  // query of the tile's first row
 
   Frag qf[KS];
   {
-    const T* row = (const T*)a.q + (it.q0 + (int64_t)qi) * a.q_row + head * a.q_head;
+    const auto base = attn_rows((const T*)a.q + hk * a.group * a.q_head, it.q0 + (int64_t)first, a.q_row);
+    const int off = (qi - first) * (int)(a.q_row * sizeof(T)) + in_group * (int)(a.q_head * sizeof(T));
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = load_row8<T>(row, 16 * s + 8 * half, a.D, live);
+    for (int s = 0; s < KS; ++s) qf[s] = load_row8<T>(base, off, 16 * s + 8 * half, a.D, live);
   }
   const int see = CAUSAL ? qi + it.nk - it.nq : 0x7FFFFFFF;  // last key that this lane's row sees
 
@@ -532,10 +575,12 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
       const float shrink = raise ? fast_exp2(m - top) : 1.f;
       m = raise ? top : m;
       l *= shrink;
+      if (kt > it.lo) {
 #pragma unroll
-      for (int b = 0; b < DB; ++b)
+        for (int b = 0; b < DB; ++b)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[b][e] *= shrink;
+          for (int e = 0; e < 16; ++e) o[b][e] *= shrink;
+      }
     }
     const float base = m == -INFINITY ? 0.f : kAttnUp<T> - m;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -603,8 +648,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArg
   constexpr int QUADS = DP / 4, LANES = kAttnThreads / QUADS;
   __shared__ v4f sums[LANES][QUADS];
   __shared__ float tops[LANES], totals[LANES];
-  const AttnJoin jn = a.joins[blockIdx.x / a.kv_heads];
-  const int hk = blockIdx.x % a.kv_heads;
+  const int at_join = attn_div(blockIdx.x, a.by_kv_heads), hk = blockIdx.x - at_join * a.kv_heads;
+  const AttnJoin jn = a.joins[at_join];
   const int rows = min(a.tile, jn.nq * a.group - jn.row0);
   const int64_t step = (int64_t)a.kv_heads * kAttnTile * (DP + 4);
   const int quad = threadIdx.x % QUADS, lane = threadIdx.x / QUADS;
@@ -651,7 +696,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArg
       }
     }
     if (lane >= stride || row >= rows) continue;
-    const int r = jn.row0 + row, qi = r / a.group, head = hk * a.group + (r - qi * a.group);
+    const int r = jn.row0 + row, qi = attn_div(r, a.by_group), head = hk * a.group + (r - qi * a.group);
     const int64_t at = (jn.q0 + (int64_t)qi) * a.heads + head;
     if (quad * 4 < a.D) {
       typedef T v4t __attribute__((ext_vector_type(4)));
@@ -687,24 +732,27 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
 
-  const int w = attn_work(gridDim.x), hk = a.item_major ? w % a.kv_heads : w / a.n_items;
-  const AttnItem it = a.items[a.item_major ? w / a.kv_heads : w - hk * a.n_items];
+  int hk;
+  const AttnItem it = attn_item(a, hk);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
   const int rows = it.nq * a.group, r = it.row0 + wave * 32 + (lane & 31);
   const bool active = it.row0 + wave * 32 < rows, live = r < rows;
-  const int qi = r / a.group, head = hk * a.group + (r - qi * a.group);
+  const int qi = attn_div(r, a.by_group), in_group = r - qi * a.group, head = hk * a.group + in_group;
+  const int first = attn_div(it.row0, a.by_group);  // query of the tile's first row
   const int64_t q = it.q0 + (int64_t)qi, at = q * a.heads + head;
 
   Frag qf[KS], gf[KS];
   float lse = INFINITY, delta = 0.f;
   {
-    const T* qrow = (const T*)a.q + q * a.q_row + head * a.q_head;
-    const T* grow = (const T*)a.dout + q * a.do_row + head * a.do_head;
+    const auto qrows = attn_rows((const T*)a.q + hk * a.group * a.q_head, it.q0 + (int64_t)first, a.q_row);
+    const auto grows = attn_rows((const T*)a.dout + hk * a.group * a.do_head, it.q0 + (int64_t)first, a.do_row);
+    const int qoff = (qi - first) * (int)(a.q_row * sizeof(T)) + in_group * (int)(a.q_head * sizeof(T));
+    const int goff = (qi - first) * (int)(a.do_row * sizeof(T)) + in_group * (int)(a.do_head * sizeof(T));
     const T *orow = (const T*)a.o + at * a.D, *rrow = (const T*)a.o_rest + at * a.D;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      qf[s] = load_row8<T>(qrow, 16 * s + 8 * half, a.D, live);
-      gf[s] = load_row8<T>(grow, 16 * s + 8 * half, a.D, live);
+      qf[s] = load_row8<T>(qrows, qoff, 16 * s + 8 * half, a.D, live);
+      gf[s] = load_row8<T>(grows, goff, 16 * s + 8 * half, a.D, live);
       const Frag of = load_row8<T>(orow, 16 * s + 8 * half, a.D, live);
       const Frag rf = load_row8<T>(rrow, 16 * s + 8 * half, a.D, sizeof(T) == 2 && live && a.o_rest);
 #pragma unroll
@@ -845,8 +893,8 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
   float* stats = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers of BQ L, BQ delta
   T* copies = reinterpret_cast<T*>(stats + 4 * BQ);           // CAUSAL: of a Q and a dO tile
 
-  const int w = attn_work(gridDim.x), hk = a.item_major ? w % a.kv_heads : w / a.n_items;
-  const AttnItem it = a.items[a.item_major ? w / a.kv_heads : w - hk * a.n_items];
+  int hk;
+  const AttnItem it = attn_item(a, hk);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
   const int kw = it.row0 + wave * 32, key = kw + (lane & 31);  // in the segment
   const bool active = kw < it.nk, live = key < it.nk;
@@ -854,10 +902,12 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
   const bool kept = live && (!a.key_mask || a.key_mask[krow]);
 
   Frag kf[KS], vf[DK ? KS : 1];
+  const auto krows = attn_rows((const T*)a.k + hk * a.k_head, it.k0 + (int64_t)it.row0, a.k_row);
+  const auto vrows = attn_rows((const T*)a.v + hk * a.v_head, it.k0 + (int64_t)it.row0, a.v_row);
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    kf[s] = load_row8<T>((const T*)a.k + krow * a.k_row + hk * a.k_head, 16 * s + 8 * half, a.D, kept);
-    if constexpr (DK) vf[s] = load_row8<T>((const T*)a.v + krow * a.v_row + hk * a.v_head, 16 * s + 8 * half, a.D, kept);
+    kf[s] = load_row8<T>(krows, (key - it.row0) * (int)(a.k_row * sizeof(T)), 16 * s + 8 * half, a.D, kept);
+    if constexpr (DK) vf[s] = load_row8<T>(vrows, (key - it.row0) * (int)(a.v_row * sizeof(T)), 16 * s + 8 * half, a.D, kept);
   }
   // first packed row that sees this lane's key, and the first that sees any of the wave's
   const int from = CAUSAL ? max(key - (it.nk - it.nq), 0) * a.group : 0;
@@ -865,26 +915,25 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
 
   Stage qs, gs;
   float stat = 0.f;
-  const unsigned inv = (unsigned)(((1ull << 32) + a.group - 1) / a.group);  // x / group = x * inv >> 32 (group > 1)
   auto place = [&](int h0) {  // packed rows from head h0 of a query on
     auto offset = [&](int x, int64_t row, int64_t head) {
-      const int dq = a.group > 1 ? (int)__umulhi((unsigned)(h0 + x), inv) : x, dh = h0 + x - dq * a.group;
+      const int dq = attn_div(h0 + x, a.by_group), dh = h0 + x - dq * a.group;
       return dq * (int)(row * sizeof(T)) + dh * (int)(head * sizeof(T));
     };
     qs.place(a.D, [&](int x) { return offset(x, a.q_row, a.q_head); });
     gs.place(a.D, [&](int x) { return offset(x, a.do_row, a.do_head); });
   };
-  const bool same_heads = BQ % a.group == 0;  // every step begins at the same head
-  place(it.lo % a.group);
+  const bool same_heads = BQ - attn_div(BQ, a.by_group) * a.group == 0;  // every step begins at the same head
+  place(it.lo - attn_div(it.lo, a.by_group) * a.group);
   auto fetch = [&](int rt) {
-    const int left = it.hi - rt, q0 = rt / a.group, h0 = rt - q0 * a.group;
+    const int left = it.hi - rt, q0 = attn_div(rt, a.by_group), h0 = rt - q0 * a.group;
     const int64_t q = it.q0 + (int64_t)q0;
     if (!same_heads) place(h0);
     qs.load((const T*)a.q + q * a.q_row + (int64_t)hk * a.group * a.q_head, left);
     gs.load((const T*)a.dout + q * a.do_row + (int64_t)hk * a.group * a.do_head, left);
     if (threadIdx.x < 2 * BQ) {
       const int x = threadIdx.x & (BQ - 1);
-      const int dq = a.group > 1 ? (int)__umulhi((unsigned)(h0 + x), inv) : x, dh = h0 + x - dq * a.group;
+      const int dq = attn_div(h0 + x, a.by_group), dh = h0 + x - dq * a.group;
       const int64_t at = (q + dq) * a.heads + hk * a.group + dh;
       // (a row past the end: L = inf makes its P zero)
       stat = threadIdx.x < BQ ? (x < left ? a.lse[at] - kAttnKeysUp<T> : INFINITY)
@@ -995,8 +1044,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a
   typedef T v4t __attribute__((ext_vector_type(4)));
   constexpr int QUADS = DP / 4, LANES = kAttnThreads / QUADS, W = KEYS ? 2 : 1;
   __shared__ v4f sums[LANES][QUADS];
-  const AttnJoin jn = a.joins[blockIdx.x / a.kv_heads];
-  const int hk = blockIdx.x % a.kv_heads;
+  const int at_join = attn_div(blockIdx.x, a.by_kv_heads), hk = blockIdx.x - at_join * a.kv_heads;
+  const AttnJoin jn = a.joins[at_join];
   const int rows = min(a.tile, (KEYS ? jn.nk : jn.nq * a.group) - jn.row0);
   const int64_t step = (int64_t)a.kv_heads * W * kAttnTile * DP;
   const int quad = threadIdx.x % QUADS, lane = threadIdx.x / QUADS;
@@ -1021,7 +1070,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a
       *reinterpret_cast<v4t*>((T*)(which ? a.dv : a.dk) + at) =
           __builtin_convertvector(sum * (which ? kAttnKeysDown<T> : a.scale), v4t);
     } else {
-      const int qi = r / a.group, head = hk * a.group + (r - qi * a.group);
+      const int qi = attn_div(r, a.by_group), head = hk * a.group + (r - qi * a.group);
       *reinterpret_cast<v4t*>((T*)a.dq + ((jn.q0 + (int64_t)qi) * a.heads + head) * a.D + quad * 4) =
           __builtin_convertvector(sum * a.scale, v4t);
     }

@@ -30,6 +30,7 @@ static st::AttnArgs attn_args(const st_attn_args* a) {
   g.q_row = a->q_row, g.q_head = a->q_head, g.k_row = a->k_row, g.k_head = a->k_head;
   g.v_row = a->v_row, g.v_head = a->v_head, g.do_row = a->dout_row, g.do_head = a->dout_head;
   g.key_mask = a->key_mask;
+  g.by_kv_heads = st::attn_divisor(a->kv_heads), g.by_group = st::attn_divisor(a->heads / a->kv_heads);
   g.heads = a->heads, g.kv_heads = a->kv_heads, g.group = a->heads / a->kv_heads;
   g.D = a->dim, g.causal = a->causal != 0;
   g.scale = a->scale;
@@ -62,6 +63,7 @@ extern "C" int st_attn_forward(const st_attn_args* a, st_stream_t stream) {
     return ST_ERR_ARG;
   st::AttnArgs g = attn_args(a);
   g.items = (const st::AttnItem*)a->q_items, g.n_items = (int)a->n_q_items;
+  g.by_items = st::attn_divisor(g.n_items);
   g.joins = (const st::AttnJoin*)a->q_joins, g.n_joins = (int)a->n_q_joins;
   g.tile = a->q_tile, g.item_major = a->q_item_major != 0;
   return attn_run_any(a, st::kAttnForward, g, (hipStream_t)stream);
@@ -81,6 +83,7 @@ extern "C" int st_attn_backward(const st_attn_args* a, st_stream_t stream) {
   st::AttnArgs g = attn_args(a);
   if (a->n_q_items) {
     g.items = (const st::AttnItem*)a->q_items, g.n_items = (int)a->n_q_items;
+    g.by_items = st::attn_divisor(g.n_items);
     g.joins = (const st::AttnJoin*)a->q_joins, g.n_joins = (int)a->n_q_joins;
     g.tile = a->q_tile, g.item_major = a->q_item_major != 0;
     rc = attn_run_any(a, st::kAttnDq, g, (hipStream_t)stream);
@@ -88,6 +91,7 @@ extern "C" int st_attn_backward(const st_attn_args* a, st_stream_t stream) {
   }
   if (!a->n_k_items) return ST_OK;
   g.items = (const st::AttnItem*)a->k_items, g.n_items = (int)a->n_k_items;
+  g.by_items = st::attn_divisor(g.n_items);
   g.joins = (const st::AttnJoin*)a->k_joins, g.n_joins = (int)a->n_k_joins;
   g.tile = a->k_tile, g.item_major = a->k_item_major != 0;
   return attn_run_any(a, st::kAttnDkv, g, (hipStream_t)stream);
