@@ -731,7 +731,7 @@ constexpr int attn_dq_lds(bool causal) {
 // order that changes the bits, or write it once for each tile of keys.
 //
 // As the forward's sizes: 64 channels bf16 255 us (810 TFLOP/s, MFMA busy 45 %, vector
-// unit 63), 128 channels causal 475 us (870, 44 %), fp32 114 us (76, 61 %).
+// unit 62), 128 channels causal 453 us (910, 47 %), fp32 114 us (76, 61 %).
 template <typename T, int DP, bool CAUSAL, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
@@ -879,10 +879,10 @@ constexpr int attn_dkv_lds(bool causal) {
 // in the place of four, by two waves a SIMD: 32 patches of 1,024 rows x 8 x 128 bf16,
 // the whole backward, 760 -> 680 us (at 96 channels 424 -> 486: one launch there).
 //
-// As the forward's sizes: 64 channels bf16 345 us (800 TFLOP/s, MFMA busy 43 %, vector
-// unit 50; two waves a SIMD, which wait for each other's products and LDS reads), 128
-// channels causal 333 + 480 us (830 and 860, 34 % before the last
-// round of workgroups was evened out), fp32 166 us (70, 56 %).
+// As the forward's sizes: 64 channels bf16 340 us (810 TFLOP/s, MFMA busy 45 %, vector
+// unit 53; two waves a SIMD, which wait for each other's products and LDS reads), 128
+// channels causal 340 + 470 us (810 and 880, 37 and 42 %), fp32 166
+// us (70, 56 %).  (The clock falls to about 1.75 GHz under all of them: fewer cycles buy less time than that.)
 constexpr int kAttnDv = 1, kAttnDk = 2;
 template <typename T, int DP>
 constexpr bool attn_dkv_apart() {
