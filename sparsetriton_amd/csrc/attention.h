@@ -451,13 +451,55 @@ constexpr float kAttnSlack = 8.f;
 // float16 holds P times a power of two, so that small probabilities keep their bits: below 2^-14
 // the type has fewer of them.  Forward: P up to 2^8 (kAttnSlack) times 2^7; the keys' pass: P up to 1
 // times 2^14 (dP - delta over as much).  The powers are added to the exponents and cost nothing.
-// (dS has no bound of its own: its scale is the caller's, as the scale of the loss.)
+// dS has no bound of its own (AttnPower).
 template <typename T>
 constexpr float kAttnUp = sizeof(T) == 2 && !__is_same(T, __bf16) ? 7.f : 0.f;
 template <typename T>
 constexpr float kAttnKeysUp = 2.f * kAttnUp<T>;
 template <typename T>
 constexpr float kAttnKeysDown = kAttnUp<T> == 0.f ? 1.f : 1.f / 16384.f;
+
+// float16 dS: as large as dO V^T (past the type's range under the scale of a loss, where the
+// gradients are not) and as small as P makes it (over many keys below 2^-14, where the type
+// loses digits).  A lane's column of dS^T (dS) is all that its dQ row (dK row) is a sum of, so each lane
+// holds its sums at a power of two of its own, taken from the largest |dS| so far as the
+// forward takes its maximum: that one comes to 2^8 .. 2^9 when it sets the power, a later one
+// passes 2^15 before the power is set again (and the sums scaled with it), and what
+// lies below 2^-14 then is 2^-22 of it or less.  Powers of two: nothing else is rounded.
+// (The other types have float's exponents, and none of this.)  Backward without / with it: 64
+// patches of 1,024 rows x 8 heads x 64 626 / 685 us, 8,191 causal rows x 16 heads of 128 (4 key
+// heads) 1,447 / 1,485, 2,000 windows of up to 96 rows x 4 x 32 85 / 88.
+template <typename T>
+constexpr bool kAttnHeld = kAttnUp<T> != 0.f;
+struct AttnPower {
+  float up = 1.f, down = 1.f;  // what dS is held at, and its inverse
+  float limit = 0.f;           // of up |dS|: 0 until a first one that is not zero
+
+  // s: up dS of a step (registers and the other half: the lane's column), sums: of dS so far.
+  template <int DB>
+  __device__ __forceinline__ void hold(v16f& s, v16f (&sums)[DB]) {
+    float top = fabsf(s[0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, fabsf(s[e]));
+    top = fmaxf(top, other_half(top));
+    const bool raise = top > limit && top < INFINITY;  // (an infinity stays one)
+    if (!__any(raise)) return;
+    // 2^(9 - e) for a top of 2^(e-1) .. 2^e; below 2^-60 no dS counts in the type's results
+    const int e = max((int)(__builtin_bit_cast(unsigned, top) >> 23) - 126, -60);
+    const float by = raise ? __builtin_bit_cast(float, (unsigned)(127 + 9 - e) << 23) : 1.f;
+    up *= by;
+    down *= raise ? __builtin_bit_cast(float, (unsigned)(127 - 9 + e) << 23) : 1.f;
+    limit = raise ? 32768.f : limit;
+    s *= by;
+#pragma unroll
+    for (int b = 0; b < DB; ++b) sums[b] *= by;
+  }
+  template <int DB>
+  __device__ __forceinline__ void release(v16f (&sums)[DB]) const {
+#pragma unroll
+    for (int b = 0; b < DB; ++b) sums[b] *= down;
+  }
+};
 
 template <typename T, int DP, bool CAUSAL, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forward_kernel(AttnArgs a) {
@@ -797,6 +839,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
   v16f dq[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) dq[b] = (v16f)(0.f);
+  AttnPower power;
   if (it.lo < it.hi) fetch(it.lo);
   for (int kt = it.lo, buf = 0; kt < it.hi; kt += BK, buf ^= 1) {
     T* kl = tiles + buf * 2 * TILE;
@@ -832,13 +875,16 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
         dp = mma32(Tile::rows(vl, b * 32 + (lane & 31), 16 * i + 8 * half), gf[i], dp);
       }
       attn_reads_ahead<T, 2 * KS>();
+      const float held = power.up * delta;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], a.scale_log2, -lse)) * (dp[e] - delta);
+      for (int e = 0; e < 16; ++e)
+        s[e] = fast_exp2(fmaf(s[e], a.scale_log2, -lse)) * (kAttnHeld<T> ? fmaf(dp[e], power.up, -held) : dp[e] - delta);
       if (cut || seen != ALL) {
         const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = (bits >> reg_row(e, 0)) & 1 ? s[e] : 0.f;
       }
+      if constexpr (kAttnHeld<T>) power.hold<DB>(s, dq);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const Frag ds = to_frag<T>(regs8(s, j));
@@ -849,6 +895,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
     }
   }
 
+  if constexpr (kAttnHeld<T>) power.release<DB>(dq);
   if (it.part >= 0) {
     store_part<DB>(
         a.parts + (((int64_t)it.part * a.kv_heads + hk) * kAttnTile + wave * 32 + (lane & 31)) * DP, dq, live);
@@ -959,6 +1006,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
     if constexpr (DV) dv[b] = (v16f)(0.f);
   }
   AttnNotFinite left_out;
+  AttnPower power;
   if (it.lo < it.hi) fetch(it.lo);
   for (int rt = it.lo, buf = 0; rt < it.hi; rt += BQ, buf ^= 1) {
     T* ql = tiles + buf * 2 * TILE;
@@ -1020,6 +1068,10 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = rt + b * 32 + reg_row(e, half) >= from ? s[e] : 0.f;
       }
+      if constexpr (kAttnHeld<T>) {
+        s *= power.up;
+        power.hold<DB>(s, dk);
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const Frag ds = to_frag<T>(regs8(s, j));
@@ -1032,6 +1084,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
   }
 
   if constexpr (CAUSAL && DV) left_out.apply(dv);
+  if constexpr (DK && kAttnHeld<T>) power.release<DB>(dk);
   if (!kept) {  // a masked key gets no gradient
 #pragma unroll
     for (int b = 0; b < DB; ++b) {

@@ -555,3 +555,97 @@ def test_which_tiles_are_split(elem, dim, causal):
             assert nk == 30_000 and parts > 1 and (mine[:, 7] == range(first, first + parts)).all()
             assert mine[0, 5] == 0 and (mine[1:, 5] == mine[:-1, 6]).all() and (mine[:, 6] > mine[:, 5]).all()
             assert (mine[:, 5] % 64 == 0).all() and mine[-1, 6] <= nk
+
+
+def _float16_gradients(q, k, v, do, ql, kl, scale, causal):
+    """{name: (value, error)} in float64: dQ, dK, dV and what the two roundings on the way do to them in float16 -- P
+    (in units of its row's largest, times 2^7 for O and 2^14 for dV) and dS, at a power of two of each row (dQ) or
+    key (dK), so that it neither overflows nor loses digits below 2^-14."""
+    def rounded(t, power=0.0):
+        return (t * 2.0 ** power).half().double() * 2.0 ** -power
+
+    def held(t, axis):
+        return rounded(t, 9 - torch.frexp(t.abs().amax(axis, keepdim=True)).exponent.double())
+
+    group = q.shape[1] // k.shape[1]
+    q, k, v, do = (t.detach().double() for t in (q, k, v, do))
+    val = {n: torch.zeros_like(t) for n, t in (("dq", q), ("dk", k), ("dv", v))}
+    off = {n: torch.zeros_like(t) for n, t in val.items()}
+    q0 = k0 = 0
+    for nq, nk in zip(ql, kl):
+        Q, K = slice(q0, q0 + nq), slice(k0, k0 + nk)
+        see = torch.ones((nq, nk), dtype=torch.bool, device=q.device)
+        see = see.tril(nk - nq) if causal else see
+        for h in range(k.shape[1]):
+            H = slice(h * group, (h + 1) * group)
+            a, g = (t[Q, H].transpose(0, 1).reshape(group * nq, -1) for t in (q, do))
+            b, c = k[K, h], v[K, h]
+            p = torch.softmax((a @ b.T * scale).masked_fill(~see.repeat(group, 1), -math.inf), 1)
+            dp, top = g @ c.T, p.amax(1, keepdim=True)
+            ds = p * (dp - (p * dp).sum(1, keepdim=True))
+            near = p * (dp - (rounded(p / top, 7) * top * dp).sum(1, keepdim=True))
+            rows = lambda t: t.view(group, nq, -1).transpose(0, 1)  # noqa: E731
+            val["dq"][Q, H], off["dq"][Q, H] = rows(ds @ b * scale), rows((held(near, 1) - ds) @ b * scale)
+            val["dk"][K, h], off["dk"][K, h] = ds.T @ a * scale, (held(near, 0) - ds).T @ a * scale
+            val["dv"][K, h], off["dv"][K, h] = p.T @ g, (rounded(p, 14) - p).T @ g
+        q0, k0 = q0 + nq, k0 + nk
+    return {n: (t, off[n]) for n, t in val.items()}
+
+
+def _check_float16_gradients(q, k, v, do, ql, kl, scale, causal, bands=None):
+    """No infinity where the value has none, and the norm of the errors (of each band of query rows) within a tenth
+    of its own rounding's and the roundings' on the way: independent, so their squares add."""
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = sparse_attention(*leaves, AttentionSegments(ql, kl, device=q.device), scale=scale, causal=causal)
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)))
+    for n, (want, off) in _float16_gradients(q, k, v, do, ql, kl, scale, causal).items():
+        assert want.abs().max().item() < 65504, "the case itself is out of float16's range"
+        assert torch.isfinite(got[n]).all(), n
+        for rows in (bands if bands and n == "dq" else [slice(None)]):
+            w = want[rows]
+            expected = math.hypot((w.half().double() - w).norm().item(), off[rows].norm().item())
+            error = (got[n][rows].double() - w).norm().item()
+            assert error < 1.1 * expected, (n, rows, error / expected, expected / w.norm().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,heads,kv_heads", [(128, 1, 1), (128, 4, 2), (64, 4, 2), (32, 2, 2)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("seed", range(3))
+def test_float16_gradients_of_a_large_loss_scale(device, dim, heads, kv_heads, causal, seed):
+    """dO near 8,000: dS passes 65,504 where dQ, dK and dV do not (few keys, so that P is not small)."""
+    ql = [8, 3, 8, 40, 8]
+    q, k, v, do, _ = _make(ql, ql, heads, kv_heads, dim, torch.float16, device, seed)
+    q, k, v = q * 0.5, k * 0.5, v * (24.0 / dim ** 0.5)
+    do = (do.float() * 8000).clamp(-30000, 30000).half()
+    _check_float16_gradients(q, k, v, do, ql, ql, dim ** -0.5, causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-2, 1e-3])
+@pytest.mark.parametrize("ql,kl,heads,kv_heads,dim", [
+    ([20], [20_000], 2, 1, 32), ([300], [4000], 2, 2, 128), ([2048], [2048], 1, 1, 32), ([6000], [64], 2, 1, 64)])
+def test_float16_gradients_of_small_products(device, size, ql, kl, heads, kv_heads, dim):
+    """dO of 1e-2 and less over many keys or rows: dS lies below 2^-14, dQ, dK and dV (at a scale of one) less so."""
+    q, k, v, do, _ = _make(ql, kl, heads, kv_heads, dim, torch.float16, device, dim + ql[0])
+    q = q * dim ** -0.5
+    _check_float16_gradients(q, k, v, (do.float() * size).half(), ql, kl, 1.0, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("falling", [False, True])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_float16_gradients_of_unlike_rows(device, falling, dim, causal):
+    """Rows whose dO grows (falls) from 2^-14 to 2^7 along the segment, keys whose values do from 2^-6 to 2^3: the power
+    that a row's or key's sum is held at has to follow, and small rows keep their digits beside large ones."""
+    n = 1024
+    q, k, v, do, _ = _make([n], [n], 2, 1, dim, torch.float16, device, dim + falling)
+    size = torch.linspace(-14, 7, n, device=device)
+    keys = torch.linspace(-6, 3, n, device=device)
+    if falling:
+        size, keys = size.flip(0), keys.flip(0)
+    do = (do.float() * torch.exp2(size)[:, None, None]).half()
+    v = (v.float() * torch.exp2(keys)[:, None, None]).half()
+    _check_float16_gradients(q * dim ** -0.5, k, v, do, [n], [n], 1.0, causal,
+                             [slice(i, i + 128) for i in range(0, n, 128)])
