@@ -14,7 +14,7 @@ import torch
 
 from sparsetriton_amd import _lib
 from sparsetriton_amd.tensor import SparseTensor
-from sparsetriton_amd.utils.utils import once_differentiable
+from sparsetriton_amd.utils.utils import once_differentiable, refuse_tangents
 
 __all__ = ["AttentionSegments", "sparse_attention"]
 
@@ -346,6 +346,7 @@ def sparse_attention(
     key gets zeros, and its gradients are zero.  Scores, softmax and sums are fp32 (fp32 inputs: the
     products too); results do not depend on timing.  A 16-bit forward that records a gradient keeps what the
     output's rounding left beside it (as large as the output), for the gradients of rows with few keys.
+    There is no forward-mode derivative: a tangent on ``q``, ``k`` or ``v`` raises.
     """
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
         if not t.is_cuda:
@@ -376,6 +377,7 @@ def sparse_attention(
                              f"{key_mask.device})")
         key_mask = key_mask.contiguous()
     causal = bool(causal)
+    refuse_tangents("sparse_attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attention.apply(q, k, v, segments, key_mask, causal, scale)
     return _forward(q, k, v, segments, key_mask, causal, scale, False)[0]

@@ -29,7 +29,7 @@ import torch
 
 from sparsetriton_amd import _lib
 from sparsetriton_amd.tensor import SparseTensor
-from sparsetriton_amd.utils.utils import once_differentiable
+from sparsetriton_amd.utils.utils import once_differentiable, refuse_tangents
 
 __all__ = ["sparse_batch_norm", "sparse_batch_norm_act", "sparse_layer_norm"]
 
@@ -258,7 +258,8 @@ def sparse_layer_norm(
     the result is ``(norm(h), h)`` with ``h = x + residual``, the stream that goes on.  ``input``
     (and ``residual``) are a ``SparseTensor`` or a tensor (..., C) of float32, float16 or bfloat16;
     the results are of the same kind.  Statistics and products are fp32; the gradients of
-    ``weight`` and ``bias`` are added in a fixed order.
+    ``weight`` and ``bias`` are added in a fixed order.  There is no forward-mode derivative: a tangent
+    on an input raises.
     """
     x = input.F if isinstance(input, SparseTensor) else input
     res = residual.F if isinstance(residual, SparseTensor) else residual
@@ -274,6 +275,7 @@ def sparse_layer_norm(
             _lib.feat_code(t.dtype)
     if res is not None and (res.shape != x.shape or res.dtype != x.dtype or res.device != x.device):
         raise ValueError("the residual must match the input's shape, dtype and device")
+    refuse_tangents("sparse_layer_norm", x, weight, bias, res)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, res)):
         out = _LayerNorm.apply(x, weight, bias, res, float(eps))
         y, h = out if res is not None else (out, None)

@@ -13,7 +13,7 @@ import torch
 
 from sparsetriton_amd import _lib
 from sparsetriton_amd.tensor import SparseTensor
-from sparsetriton_amd.utils.utils import once_differentiable
+from sparsetriton_amd.utils.utils import once_differentiable, refuse_tangents
 
 __all__ = ["RotaryAxes", "sparse_rotary"]
 
@@ -111,7 +111,8 @@ def sparse_rotary(
     ``q`` (N, heads, D) and ``k`` (N, kv_heads, D) share rows and dtype (one of them may be
     ``None``); rows and heads may lie at any stride.  ``positions``: a ``SparseTensor`` (the x, y, z
     of its coordinates) or (N, A) of int16, int32, int64 or float32 with ``A >= len(axes.axes)``.
-    The outputs are contiguous; the gradient turns back.  Positions get no gradient.
+    The outputs are contiguous; the gradient turns back.  Positions get no gradient.  There is no
+    forward-mode derivative: a tangent on ``q`` or ``k`` raises.
     """
     first = q if q is not None else k
     if first is None:
@@ -134,6 +135,7 @@ def sparse_rotary(
         raise ValueError(f"positions are on {pos.device}, q and k on {first.device}")
     if pos.shape[1] > 1 and pos.stride(1) != 1:
         pos = pos.contiguous()
+    refuse_tangents("sparse_rotary", q, k)
     if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
         return _Rotary.apply(q, k, pos.detach(), axes)
     return _rotate(q, k, pos, axes, False)

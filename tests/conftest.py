@@ -28,3 +28,10 @@ def _restore_config():
     yield
     _STATE.clear()
     _STATE.update(saved)
+
+
+@pytest.fixture
+def own_random(device):
+    """The test's draws from torch's global generators leave them as they were: tests after it see the same inputs."""
+    with torch.random.fork_rng(devices=[torch.cuda.current_device()]):
+        yield

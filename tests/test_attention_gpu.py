@@ -649,3 +649,19 @@ def test_float16_gradients_of_unlike_rows(device, falling, dim, causal):
     v = (v.float() * torch.exp2(keys)[:, None, None]).half()
     _check_float16_gradients(q * dim ** -0.5, k, v, do, [n], [n], 1.0, causal,
                              [slice(i, i + 128) for i in range(0, n, 128)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("recorded", [False, True])
+def test_forward_mode_is_refused(device, own_random, which, recorded):
+    """No forward-mode derivative: a tangent on q, k or v raises, where it is not to be dropped, with or without a graph."""
+    t = [torch.randn((6, 2, 16), device=device, requires_grad=recorded) for _ in range(3)]
+    segs = AttentionSegments([4, 2], device=device)
+    with torch.autograd.forward_ad.dual_level():
+        sparse_attention(*t, segs)
+        t[which] = torch.autograd.forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            sparse_attention(*t, segs)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            sparse_attention(*t, segs)

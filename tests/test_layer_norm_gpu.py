@@ -231,3 +231,17 @@ def test_refusals(device):
     assert lib.st_ln_forward(p, None, 4, 8, 7, None, None, 0, 1e-5, None, p, None, None, s) == -3
     assert lib.st_ln_forward(p, None, 4, 8, 1, p, None, 2, 1e-5, None, p, None, None, s) == -3
     assert lib.st_ln_backward(p, p, None, 4, 8, 0, None, 0, p, p, None, 0, p, p, None, s) == -1  # no workspace
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("recorded", [False, True])
+def test_forward_mode_is_refused(device, own_random, which, recorded):
+    """No forward-mode derivative: a tangent on an input raises, where it is not to be dropped, with or without a graph."""
+    t = [torch.randn(s, device=device, requires_grad=recorded) for s in ((5, 16), (16,), (16,), (5, 16))]
+    with torch.autograd.forward_ad.dual_level():
+        sparse_layer_norm(*t[:3], residual=t[3])
+        t[which] = torch.autograd.forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            sparse_layer_norm(*t[:3], residual=t[3])
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            sparse_layer_norm(*t[:3], residual=t[3])

@@ -176,3 +176,19 @@ def test_refusals(device):
     with pytest.raises(TypeError, match="feature dtype"):
         sparse_rotary(q.double(), None, pos, axes)
     assert math.isclose(RotaryAxes(16, (8,)).frequencies[1].item(), 10000 ** -0.25, rel_tol=1e-7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(2))
+@pytest.mark.parametrize("recorded", [False, True])
+def test_forward_mode_is_refused(device, own_random, which, recorded):
+    """No forward-mode derivative: a tangent on q or k raises, where it is not to be dropped, with or without a graph."""
+    t = [torch.randn((5, 2, 16), device=device, requires_grad=recorded) for _ in range(2)]
+    pos, axes = torch.zeros((5, 2), dtype=torch.int32, device=device), RotaryAxes(16, (8, 4))
+    with torch.autograd.forward_ad.dual_level():
+        sparse_rotary(*t, pos, axes)
+        t[which] = torch.autograd.forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            sparse_rotary(*t, pos, axes)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            sparse_rotary(*t, pos, axes)

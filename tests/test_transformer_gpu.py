@@ -131,3 +131,13 @@ def test_refusals():
         snn.SparseAttention(100, 3)
     with pytest.raises(ValueError, match="share"):
         snn.SparseAttention(96, 6, kv_heads=4)
+
+
+def test_a_frozen_block_refuses_forward_mode(device, own_random):
+    block = snn.SparseTransformerBlock(64, 4).to(device).requires_grad_(False)
+    x = _voxels([20], 64, device, torch.float32, 8)
+    segs = AttentionSegments([20], device=device)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x.F, torch.ones_like(x.F))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            block(x.replace(dual), segs)
