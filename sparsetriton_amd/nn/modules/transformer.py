@@ -12,6 +12,9 @@ segments once for a coordinate set and hand them to every block::
     segments = AttentionSegments.from_tensor(x, patch=1024)
     for block in blocks:
         x = block(x, segments)
+
+Under ``torch.autocast`` the projections' products (and so rotary and attention) are 16-bit; the
+norms take the stream in its own type, and the sums are of the wider of the two, as torch's are.
 """
 
 from typing import Optional, Sequence
@@ -31,6 +34,12 @@ def _three_axes(dim: int):
     """An even number of a head's channels for each of x, y and z, all of them or all but two."""
     pair = dim // 2
     return tuple(2 * (pair // 3 + (1 if i < pair % 3 else 0)) for i in range(3))
+
+
+def _one_type(a: SparseTensor, b: SparseTensor):
+    """a and b in the type that torch's sum of them has: under autocast a branch's products are 16-bit where the stream is not."""
+    dtype = torch.promote_types(a.F.dtype, b.F.dtype)
+    return tuple(t if t.F.dtype is dtype else t.replace(t.F.to(dtype)) for t in (a, b))
 
 
 class SparseAttention(nn.Module):
@@ -82,6 +91,6 @@ class SparseTransformerBlock(nn.Module):
     def forward(self, x: SparseTensor, segments: Optional[AttentionSegments] = None,
                 key_mask: Optional[torch.Tensor] = None) -> SparseTensor:
         y = sparse_layer_norm(x, self.norm1.weight, self.norm1.bias, eps=self.eps)
-        a = self.attn(y, segments, key_mask)
+        a, x = _one_type(self.attn(y, segments, key_mask), x)
         z, h = sparse_layer_norm(a, self.norm2.weight, self.norm2.bias, eps=self.eps, residual=x)
         return h.replace(h.F + self.mlp(z.F))

@@ -141,3 +141,41 @@ def test_a_frozen_block_refuses_forward_mode(device, own_random):
         dual = torch.autograd.forward_ad.make_dual(x.F, torch.ones_like(x.F))
         with pytest.raises(RuntimeError, match="forward-mode"):
             block(x.replace(dual), segs)
+
+
+@pytest.mark.parametrize("dtype,tol", [(torch.bfloat16, 5e-2), (torch.float16, 1e-2)])
+@pytest.mark.parametrize("features", [torch.float32, None])
+def test_block_under_autocast(device, own_random, dtype, tol, features):
+    """fp32 parameters, the products in 16 bits: a fp32 stream stays fp32, one in the products' type keeps that.
+    (Roundings as in a block of that type: about ten of 2^-8, or of 2^-11.)"""
+    torch.manual_seed(9)
+    block = snn.SparseTransformerBlock(64, 4, 2, mlp_ratio=2).to(device)
+    lengths = [130, 1, 77]
+    x = _voxels(lengths, 64, device, features or dtype, 10)
+    segs = AttentionSegments.from_tensor(x)
+    plain = copy.deepcopy(block).double()
+    ref_x = x.F.double().requires_grad_(True)
+    dy = torch.randn(x.F.shape, device=device).to(x.F.dtype)
+    ref = _plain(plain, ref_x, x.C, lengths, False)
+    ref.backward(dy.double())
+    feats = x.F.clone().requires_grad_(True)
+    with torch.autocast("cuda", dtype):
+        out = block(x.replace(feats), segs)
+    assert out.F.dtype is x.F.dtype
+    out.F.backward(dy)
+    near = lambda a, b: (a.double() - b).norm() <= tol * b.norm() + 1e-12  # noqa: E731
+    assert near(out.F.detach(), ref.detach()) and near(feats.grad, ref_x.grad)
+    for (name, p), q in zip(block.named_parameters(), plain.parameters()):
+        assert p.grad.dtype is torch.float32 and near(p.grad, q.grad), name
+
+
+def test_a_stream_of_another_16_bit_type_is_promoted(device, own_random):
+    """float16 features, bfloat16 products: their sum is fp32, as torch's is."""
+    torch.manual_seed(9)
+    block = snn.SparseTransformerBlock(64, 4).to(device)
+    x = _voxels([40], 64, device, torch.float16, 11)
+    with torch.autocast("cuda", torch.bfloat16):
+        out = block(x)
+    assert out.F.dtype is torch.float32
+    ref = _plain(copy.deepcopy(block).double(), x.F.double(), x.C, [40], False)
+    assert (out.F.double() - ref).norm() <= 5e-2 * ref.norm()
