@@ -6,7 +6,9 @@ the voxels' x, y, z (``sparse_rotary``) and attends within the row segments
 
     h = x + attention(norm1(x));   out = h + mlp(norm2(h))
 
-whose first add runs inside the second norm (``sparse_layer_norm`` with a residual).  Build the
+whose first add runs inside the second norm (``sparse_layer_norm`` with a residual).  ``norm1`` and
+``norm2`` are modules like any other: their hooks run, and another norm in their place is called, on
+the ``SparseTensor`` if it is one of this package's, on the features otherwise.  Build the
 segments once for a coordinate set and hand them to every block::
 
     segments = AttentionSegments.from_tensor(x, patch=1024)
@@ -25,6 +27,7 @@ from torch import nn
 from sparsetriton_amd.nn.functional.attention import AttentionSegments, sparse_attention
 from sparsetriton_amd.nn.functional.norm import sparse_layer_norm
 from sparsetriton_amd.nn.functional.rotary import RotaryAxes, sparse_rotary
+from sparsetriton_amd.nn.modules.norm import SparseBatchNorm, SparseLayerNorm
 from sparsetriton_amd.tensor import SparseTensor
 
 __all__ = ["SparseAttention", "SparseTransformerBlock"]
@@ -75,22 +78,39 @@ class SparseAttention(nn.Module):
         return x.replace(self.proj(out.flatten(1)))
 
 
+class _StreamNorm(nn.LayerNorm):
+    """``sparse_layer_norm`` with a layer norm's parameters; plain features go through torch's."""
+
+    def forward(self, input, residual: Optional[SparseTensor] = None):
+        if not isinstance(input, SparseTensor):
+            return super().forward(input)
+        return sparse_layer_norm(input, self.weight, self.bias, eps=self.eps, residual=residual)
+
+
+def _normed(norm: nn.Module, x: SparseTensor) -> SparseTensor:
+    if isinstance(norm, (_StreamNorm, SparseLayerNorm, SparseBatchNorm)):
+        return norm(x)
+    return x.replace(norm(x.F))
+
+
 class SparseTransformerBlock(nn.Module):
     """Pre-norm block: attention within the segments, then a two-layer GELU network."""
 
     def __init__(self, channels: int, heads: int, kv_heads: Optional[int] = None, mlp_ratio: float = 4.0, eps: float = 1e-5,
                  axes: Optional[Sequence[int]] = None, causal: bool = False):
         super().__init__()
-        self.eps = eps
-        self.norm1 = nn.LayerNorm(channels, eps=eps)
+        self.norm1 = _StreamNorm(channels, eps=eps)
         self.attn = SparseAttention(channels, heads, kv_heads, axes=axes, causal=causal)
-        self.norm2 = nn.LayerNorm(channels, eps=eps)
+        self.norm2 = _StreamNorm(channels, eps=eps)
         hidden = int(channels * mlp_ratio)
         self.mlp = nn.Sequential(nn.Linear(channels, hidden), nn.GELU(), nn.Linear(hidden, channels))
 
     def forward(self, x: SparseTensor, segments: Optional[AttentionSegments] = None,
                 key_mask: Optional[torch.Tensor] = None) -> SparseTensor:
-        y = sparse_layer_norm(x, self.norm1.weight, self.norm1.bias, eps=self.eps)
-        a, x = _one_type(self.attn(y, segments, key_mask), x)
-        z, h = sparse_layer_norm(a, self.norm2.weight, self.norm2.bias, eps=self.eps, residual=x)
+        a, x = _one_type(self.attn(_normed(self.norm1, x), segments, key_mask), x)
+        if isinstance(self.norm2, _StreamNorm):
+            z, h = self.norm2(a, x)
+        else:
+            h = x.replace(x.F + a.F)
+            z = _normed(self.norm2, h)
         return h.replace(h.F + self.mlp(z.F))

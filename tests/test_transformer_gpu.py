@@ -179,3 +179,43 @@ def test_a_stream_of_another_16_bit_type_is_promoted(device, own_random):
     assert out.F.dtype is torch.float32
     ref = _plain(copy.deepcopy(block).double(), x.F.double(), x.C, [40], False)
     assert (out.F.double() - ref).norm() <= 5e-2 * ref.norm()
+
+
+@pytest.mark.parametrize("which", ["norm1", "norm2"])
+@pytest.mark.parametrize("make", [lambda c: nn.Sequential(nn.LayerNorm(c), nn.Tanh()), snn.SparseLayerNorm, snn.SparseBatchNorm,
+                                  nn.RMSNorm])
+def test_another_norm_in_its_place_is_called(device, own_random, which, make):
+    """A module over features or over a SparseTensor that a user puts in a norm's place runs, and trains."""
+    torch.manual_seed(12)
+    block = snn.SparseTransformerBlock(64, 4, mlp_ratio=2)
+    setattr(block, which, make(64))
+    block = block.to(device)
+    x = _voxels([30, 20], 64, device, torch.float32, 13)
+    segs = AttentionSegments.from_tensor(x)
+    calls = []
+    getattr(block, which).register_forward_hook(lambda *_: calls.append(1))
+    out = block(x, segs).F
+    out.sum().backward()
+    assert len(calls) == 1 and all(p.grad is not None for p in getattr(block, which).parameters())
+    # by hand, from the block's own parts
+    norm = lambda m, t: m(t).F if isinstance(m, (snn.SparseLayerNorm, snn.SparseBatchNorm)) else m(t.F)  # noqa: E731
+    plain = lambda m, t: norm(m, t) if m is getattr(block, which) else nn.functional.layer_norm(  # noqa: E731
+        t.F, (64,), m.weight, m.bias, m.eps)
+    h = x.F + block.attn(x.replace(plain(block.norm1, x)), segs).F
+    want = h + block.mlp(plain(block.norm2, x.replace(h)))
+    assert (out - want).norm() <= 2e-5 * want.norm()
+
+
+def test_hooks_of_the_norms_run(device, own_random):
+    block = snn.SparseTransformerBlock(64, 4, mlp_ratio=2).to(device)
+    x = _voxels([30, 20], 64, device, torch.float32, 14)
+    segs = AttentionSegments.from_tensor(x)
+    seen = []
+    for m in (block.norm1, block.norm2):
+        m.register_forward_pre_hook(lambda m, args: seen.append(m))
+        m.register_forward_hook(lambda m, args, out: seen.append(m))
+    block(x, segs)
+    assert [id(m) for m in seen] == [id(m) for m in (block.norm1, block.norm1, block.norm2, block.norm2)]
+    # the norms are layer norms with their parameters' names, and take plain features as well
+    assert isinstance(block.norm1, nn.LayerNorm) and "norm1.weight" in block.state_dict()
+    assert (block.norm1(x.F) - nn.functional.layer_norm(x.F, (64,))).abs().max() < 1e-5
