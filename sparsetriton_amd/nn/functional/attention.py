@@ -180,6 +180,10 @@ class AttentionSegments:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self._plans = {}
 
+    def __getstate__(self):
+        # (a list holds the address of its own device memory: a copy, or another process, builds its own)
+        return {**self.__dict__, "_plans": {}}
+
     @classmethod
     def from_tensor(cls, tensor: SparseTensor, patch: Optional[int] = None) -> "AttentionSegments":
         """The samples of ``tensor`` (whose rows must lie sample by sample, in ascending order), or

@@ -10,7 +10,9 @@ channels, its exponential and the row's sum):
   dQ, dK, dV   the error of dS or P through the product, plus u of the result.
 """
 
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -665,3 +667,17 @@ def test_forward_mode_is_refused(device, own_random, which, recorded):
             sparse_attention(*t, segs)
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             sparse_attention(*t, segs)
+
+
+@pytest.mark.parametrize("copied", [copy.copy, copy.deepcopy, lambda s: pickle.loads(pickle.dumps(s))])
+def test_copies_build_their_own_lists(copied):
+    """The lists hold addresses of their own device memory: a copy (of a model that holds the segments, or on its way to
+    another process) must not keep them.  Same lengths, same lists."""
+    segs = AttentionSegments([300, 5], [5000, 7], device="cpu")
+    plans = [segs._plan(w, 2, 2, False, 64, 2) for w in "qk"]
+    other = copied(segs)
+    assert (other.q_rows, other.k_rows, other.count, other.device) == (305, 5007, 2, segs.device)
+    for w, plan in zip("qk", plans):
+        again = other._plan(w, 2, 2, False, 64, 2)
+        assert torch.equal(again.words, plan.words) and again.words.data_ptr() != plan.words.data_ptr()
+        assert again.items == again.words.data_ptr() and segs._plan(w, 2, 2, False, 64, 2) is plan
