@@ -50,7 +50,7 @@ def _lengths(lengths, what: str) -> np.ndarray:
     if out.ndim != 1 or (out.size and out.dtype.kind not in "iu"):
         raise ValueError(f"{what} must be a list of row counts")
     out = out.astype(np.int64)
-    if (out < 0).any() or out.sum() >= 2 ** 31 - 4096:
+    if (out < 0).any() or (out >= 2 ** 31).any() or out.sum() >= 2 ** 31 - 4096:  # (each, so that the sum cannot wrap)
         raise ValueError(f"{what} must not be negative, and less than 2^31 - 4096 rows in all")
     return out
 

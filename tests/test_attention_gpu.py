@@ -681,3 +681,12 @@ def test_copies_build_their_own_lists(copied):
         again = other._plan(w, 2, 2, False, 64, 2)
         assert torch.equal(again.words, plan.words) and again.words.data_ptr() != plan.words.data_ptr()
         assert again.items == again.words.data_ptr() and segs._plan(w, 2, 2, False, 64, 2) is plan
+
+
+@pytest.mark.parametrize("bad", [[2 ** 62] * 4, [2 ** 63 - 1, 2 ** 63 - 1, 2], [2 ** 33] * 2 ** 3])
+def test_lengths_whose_sum_wraps_are_refused(bad):
+    """Four segments of 2^62 rows are 2^64 in all: zero in 64 bits."""
+    with pytest.raises(ValueError, match="2\\^31"):
+        AttentionSegments(bad, device="cpu")
+    with pytest.raises(ValueError, match="2\\^31"):
+        AttentionSegments([1] * len(bad), bad, device="cpu")
