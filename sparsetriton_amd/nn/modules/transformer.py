@@ -57,6 +57,8 @@ class SparseAttention(nn.Module):
                  axes: Optional[Sequence[int]] = None, base: float = 10000.0, causal: bool = False, bias: bool = True):
         super().__init__()
         self.heads, self.kv_heads = heads, heads if kv_heads is None else kv_heads
+        if self.heads < 1 or self.kv_heads < 1:
+            raise ValueError(f"heads and key heads must be positive (got {heads} and {kv_heads})")
         if head_dim is None and channels % heads:
             raise ValueError(f"{channels} channels do not divide into {heads} heads")
         self.head_dim = channels // heads if head_dim is None else head_dim

@@ -219,3 +219,11 @@ def test_hooks_of_the_norms_run(device, own_random):
     # the norms are layer norms with their parameters' names, and take plain features as well
     assert isinstance(block.norm1, nn.LayerNorm) and "norm1.weight" in block.state_dict()
     assert (block.norm1(x.F) - nn.functional.layer_norm(x.F, (64,))).abs().max() < 1e-5
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(0, None), (4, 0), (-4, None), (4, -2), (4, 8)])
+def test_head_counts_that_are_no_counts_are_refused(heads, kv_heads):
+    with pytest.raises(ValueError, match="heads"):
+        snn.SparseAttention(96, heads, kv_heads)
+    with pytest.raises(ValueError, match="heads"):
+        snn.SparseTransformerBlock(96, heads, kv_heads)
