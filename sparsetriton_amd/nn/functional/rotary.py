@@ -47,8 +47,15 @@ class RotaryAxes:
         """(whole turns per unit, axis) of each pair on ``device``."""
         got = self._on.get(device)
         if got is None:
-            got = self._on[device] = (self._turns.to(device), self._axis.to(device))
-        return got
+            got = self._on[device] = [self._turns.to(device), self._axis.to(device), None]
+        turns, axis, last = got
+        if turns.is_cuda:
+            s = _lib.stream_of(device)
+            if s != last:  # (their memory is not handed out before this stream is through with it)
+                for t in (turns, axis):
+                    t.record_stream(torch.cuda.current_stream(device))
+                got[2] = s
+        return turns, axis
 
     def __getstate__(self):
         return {**self.__dict__, "_on": {}}

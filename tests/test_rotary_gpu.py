@@ -192,3 +192,28 @@ def test_forward_mode_is_refused(device, own_random, which, recorded):
             sparse_rotary(*t, pos, axes)
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             sparse_rotary(*t, pos, axes)
+
+
+@pytest.mark.gpu
+def test_tables_outlive_their_owner_on_another_stream(device, own_random):
+    """The frequencies' memory, made on one stream, is not handed out again while another stream's kernel may read it."""
+    q, pos = torch.randn((4000, 4, 32), device=device), torch.randint(0, 500, (4000, 3), device=device)
+    want = sparse_rotary(q, None, pos, RotaryAxes(32, (12, 12, 8)))[0]
+    axes, busy = RotaryAxes(32, (12, 12, 8)), torch.randn((4096, 4096), device=device)
+    sparse_rotary(q, None, pos, axes)
+    held = [t.data_ptr() for t in axes.on(q.device)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):  # (some milliseconds for the call below to wait behind)
+            other = busy @ busy
+        got = sparse_rotary(q, None, pos, axes)[0]
+    sizes = [(t.numel(), t.dtype) for t in axes.on(q.device)]
+    del axes
+    new = [torch.empty((n,), dtype=d, device=device) for n, d in sizes for _ in range(4)]
+    done = side.query()
+    torch.cuda.current_stream().wait_stream(side)
+    other.record_stream(torch.cuda.current_stream())
+    got.record_stream(torch.cuda.current_stream())
+    assert torch.equal(got, want)
+    assert done or not set(held) & {t.data_ptr() for t in new}
