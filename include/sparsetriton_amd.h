@@ -828,7 +828,7 @@ int st_bn_backward(const void* Y, const void* out, const void* dout, int64_t n, 
  * st_ln_backward: H is the forward's h (X without a residual), dY the gradient
  * at Y, dH (NULL = none) the one at h; dX (NULL = not wanted) the gradient of
  * X and of the residual alike, dweight, dbias (of weight_dtype, NULL = not
- * wanted) added over the rows in a fixed order.  workspace: at least
+ * wanted) added over the rows in a fixed order, for C below 2^26.  workspace: at least
  * st_ln_backward_workspace floats at a 16-byte address, needed with dweight or dbias.
  */
 int st_ln_forward(const void* X, const void* residual, int64_t n, int C, int dtype, const void* weight,

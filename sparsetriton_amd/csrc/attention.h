@@ -1148,22 +1148,38 @@ __global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a
 
 enum AttnPass { kAttnForward, kAttnDq, kAttnDkv };
 
+// A workgroup for every item (join) and key head, in as many launches as the grid's limit asks for.
 template <typename K>
-static int attn_launch(K kernel, int64_t blocks, int rows, int threads, int lds, const AttnArgs& a, hipStream_t s) {
-  if (blocks == 0) return ST_OK;
-  kernel<<<dim3((unsigned)blocks, rows), threads, lds, s>>>(a);
-  ST_CHECK_LAUNCH();
+static int attn_launch(K kernel, int threads, int lds, const AttnArgs& a, hipStream_t s) {
+  const int most = (int)(st_most_blocks(threads) / a.kv_heads);
+  if (most == 0) return ST_ERR_UNSUPPORTED;
+  for (int64_t i = 0; i < a.n_items; i += most) {
+    AttnArgs g = a;
+    g.items += i;
+    g.n_items = (int)(a.n_items - i < most ? a.n_items - i : most);
+    g.by_items = attn_divisor(g.n_items);
+    kernel<<<(unsigned)(g.n_items * g.kv_heads), threads, lds, s>>>(g);
+    ST_CHECK_LAUNCH();
+  }
   return ST_OK;
 }
 template <typename K>
 static int attn_join(K kernel, const AttnArgs& a, hipStream_t s) {
-  return attn_launch(kernel, (int64_t)a.n_joins * a.kv_heads, kAttnJoinBlocks, kAttnThreads, 0, a, s);
+  const int most = (int)(st_most_blocks(kAttnThreads) / a.kv_heads);
+  if (most == 0) return ST_ERR_UNSUPPORTED;
+  for (int64_t i = 0; i < a.n_joins; i += most) {
+    AttnArgs g = a;
+    g.joins += i;
+    g.n_joins = (int)(a.n_joins - i < most ? a.n_joins - i : most);
+    kernel<<<dim3((unsigned)(g.n_joins * g.kv_heads), kAttnJoinBlocks), kAttnThreads, 0, s>>>(g);
+    ST_CHECK_LAUNCH();
+  }
+  return ST_OK;
 }
 
 template <typename T, int DP, int WAVES>
 static int attn_pass(AttnPass pass, const AttnArgs& a, hipStream_t s) {
-  const int64_t blocks = (int64_t)a.n_items * a.kv_heads;
-  auto run = [&](auto kernel, int lds) { return attn_launch(kernel, blocks, 1, 64 * WAVES, lds, a, s); };
+  auto run = [&](auto kernel, int lds) { return attn_launch(kernel, 64 * WAVES, lds, a, s); };
   if (pass == kAttnForward)
     return run(a.causal ? attn_forward_kernel<T, DP, true, WAVES> : attn_forward_kernel<T, DP, false, WAVES>,
                attn_fwd_lds<T, DP, WAVES>(a.causal));

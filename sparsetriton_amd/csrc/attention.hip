@@ -10,7 +10,7 @@ static int attn_check(const st_attn_args* a) {
   for (int tile : {a->q_tile, a->k_tile})
     if (tile != ST_ATTN_TILE && tile != ST_ATTN_SMALL_TILE) return ST_ERR_ARG;
   for (int64_t n : {a->n_q_items, a->n_q_joins, a->n_k_items, a->n_k_joins})
-    if (n < 0 || n * a->kv_heads >= (1ll << 31)) return ST_ERR_ARG;
+    if (n < 0 || n >= (1ll << 31)) return ST_ERR_ARG;
   return ST_OK;
 }
 

@@ -289,3 +289,5 @@ int launch_chunk_keys(const int32_t* pairs, const int32_t* kstart, const int32_t
 static inline unsigned st_blocks(int64_t n, int per_block) {
   return (unsigned)((n + per_block - 1) / per_block);
 }
+// Workgroups of one launch: a grid's dimension times its workgroups' threads stays below 2^32.
+static inline int64_t st_most_blocks(int threads) { return 0xFFFFFFFFll / threads; }

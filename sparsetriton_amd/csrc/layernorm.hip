@@ -434,6 +434,9 @@ static int ln_select(const LnGeom& g, F f) {
   return ST_ERR_UNSUPPORTED;
 }
 
+// Rows of a launch, `side` of them to a workgroup.
+static int64_t ln_most_rows(int side) { return st_most_blocks(kLnThreads) * side; }
+
 static bool ln_aligned(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if ((uintptr_t)p & 15) return false;
@@ -444,25 +447,32 @@ template <typename T, typename W>
 static int ln_forward(const void* X, const void* R, int64_t n, int C, const void* w, const void* b, float eps, void* H,
                       void* Y, float* mean, float* rstd, hipStream_t s) {
   const T *x = (const T*)X, *r = (const T*)R;
+  T *h = (T*)H, *y = (T*)Y;
   const W *wp = (const W*)w, *bp = (const W*)b;
   const LnGeom g = ln_geom(C, sizeof(T), ln_aligned({X, R, H, Y, w, b}));
-  if (!g.lanes) {
-    ln_forward_long_kernel<T, W><<<(unsigned)n, kLnThreads, 0, s>>>(x, r, C, wp, bp, eps, (T*)H, (T*)Y, mean, rstd);
-    ST_CHECK_LAUNCH();
-    return ST_OK;
-  }
-  return ln_select<16 / sizeof(T)>(g, [&](auto v, auto lanes, auto nv) -> int {
-    constexpr int V = decltype(v)::value, L = decltype(lanes)::value, N = decltype(nv)::value;
-    const unsigned blocks = st_blocks(n, kLnThreads / L);
-    if (r)
-      ln_forward_kernel<T, W, V, L, N, true>
-          <<<blocks, kLnThreads, 0, s>>>(x, r, n, C, wp, bp, eps, (T*)H, (T*)Y, mean, rstd);
+  const int64_t most = ln_most_rows(g.lanes ? kLnThreads / g.lanes : 1);
+  for (int64_t row = 0; row < n; row += most) {
+    const int64_t m = n - row < most ? n - row : most, at = row * C;
+    const T *xr = x + at, *rr = r ? r + at : nullptr;
+    T *hr = h ? h + at : nullptr, *yr = y + at;
+    float *mr = mean ? mean + row : nullptr, *sr = rstd ? rstd + row : nullptr;
+    int rc = ST_OK;
+    if (!g.lanes)
+      ln_forward_long_kernel<T, W><<<(unsigned)m, kLnThreads, 0, s>>>(xr, rr, C, wp, bp, eps, hr, yr, mr, sr);
     else
-      ln_forward_kernel<T, W, V, L, N, false>
-          <<<blocks, kLnThreads, 0, s>>>(x, r, n, C, wp, bp, eps, (T*)H, (T*)Y, mean, rstd);
+      rc = ln_select<16 / sizeof(T)>(g, [&](auto v, auto lanes, auto nv) -> int {
+        constexpr int V = decltype(v)::value, L = decltype(lanes)::value, N = decltype(nv)::value;
+        const unsigned blocks = st_blocks(m, kLnThreads / L);
+        if (r)
+          ln_forward_kernel<T, W, V, L, N, true><<<blocks, kLnThreads, 0, s>>>(xr, rr, m, C, wp, bp, eps, hr, yr, mr, sr);
+        else
+          ln_forward_kernel<T, W, V, L, N, false><<<blocks, kLnThreads, 0, s>>>(xr, rr, m, C, wp, bp, eps, hr, yr, mr, sr);
+        return ST_OK;
+      });
+    if (rc != ST_OK) return rc;
     ST_CHECK_LAUNCH();
-    return ST_OK;
-  });
+  }
+  return ST_OK;
 }
 
 template <typename T, typename W>
@@ -475,8 +485,13 @@ static int ln_backward(const void* H, const void* dY, const void* dH, int64_t n,
   const bool columns = dw || db;
   int rc = ST_OK;
   if (!g.lanes) {
-    if (dX && n) ln_backward_long_kernel<T, W><<<(unsigned)n, kLnThreads, 0, s>>>(h, dy, dh, C, wp, mean, rstd, (T*)dX);
-    ST_CHECK_LAUNCH();
+    const int64_t most = ln_most_rows(1);
+    for (int64_t row = 0; dX && row < n; row += most) {
+      const int64_t m = n - row < most ? n - row : most, at = row * C;
+      ln_backward_long_kernel<T, W><<<(unsigned)m, kLnThreads, 0, s>>>(h + at, dy + at, dh ? dh + at : nullptr, C, wp,
+                                                                      mean + row, rstd + row, (T*)dX + at);
+      ST_CHECK_LAUNCH();
+    }
     if (columns)
       ln_columns_kernel<T>
           <<<dim3(st_blocks(C, kLnThreads), (unsigned)groups), kLnThreads, 0, s>>>(h, dy, n, C, mean, rstd, ws);
@@ -498,7 +513,7 @@ static int ln_backward(const void* H, const void* dY, const void* dH, int64_t n,
 
 }  // namespace st
 
-// n rows of C channels that the kernels take: a workgroup a row at most
+// n rows of C channels that the kernels take
 static bool ln_sizes_ok(int64_t n, int C) { return n >= 0 && n < (1ll << 31) && C > 0; }
 
 extern "C" int st_ln_forward(const void* X, const void* residual, int64_t n, int C, int dtype, const void* weight,
@@ -532,6 +547,8 @@ extern "C" int st_ln_backward(const void* H, const void* dY, const void* dH, int
   int64_t need = 0;
   const int rc = st_ln_backward_workspace(n, C, dtype, &need);
   if (rc != ST_OK) return rc;
+  // (the sum of the partials is one launch, eight of 2 C columns to a workgroup)
+  if ((dweight || dbias) && (2 * (int64_t)C + 7) / 8 > st_most_blocks(st::kLnThreads)) return ST_ERR_UNSUPPORTED;
   if (weight_dtype != dtype && weight_dtype != ST_F32) return ST_ERR_UNSUPPORTED;
   if (n > 0 && (!H || !dY || !mean || !rstd)) return ST_ERR_ARG;
   if ((dweight || dbias) && (!workspace || workspace_floats < need || ((uintptr_t)workspace & 15))) return ST_ERR_ARG;

@@ -168,18 +168,20 @@ static int rot_launch(RotArgs<T> g, bool interleaved, bool inverse, hipStream_t 
   g.rows = rows > 0 ? (int)rows : 1;
   g.per_row_inv = ((1ull << 32) + g.per_row - 1) / g.per_row;
   g.chunks_inv = ((1ull << 32) + g.chunks - 1) / g.chunks;
-  const int64_t blocks = (g.n + g.rows - 1) / g.rows;
-  if (blocks >= (1ll << 31)) return ST_ERR_ARG;
-  const dim3 grid((unsigned)blocks);
-  if (interleaved && inverse)
-    rotary_kernel<T, PT, V, true, true><<<grid, kRotThreads, 0, s>>>(g);
-  else if (interleaved)
-    rotary_kernel<T, PT, V, true, false><<<grid, kRotThreads, 0, s>>>(g);
-  else if (inverse)
-    rotary_kernel<T, PT, V, false, true><<<grid, kRotThreads, 0, s>>>(g);
-  else
-    rotary_kernel<T, PT, V, false, false><<<grid, kRotThreads, 0, s>>>(g);
-  ST_CHECK_LAUNCH();
+  auto kernel = interleaved ? (inverse ? rotary_kernel<T, PT, V, true, true> : rotary_kernel<T, PT, V, true, false>)
+                            : (inverse ? rotary_kernel<T, PT, V, false, true> : rotary_kernel<T, PT, V, false, false>);
+  const int64_t n = g.n, most = st_most_blocks(kRotThreads) * g.rows;  // rows of a launch
+  for (int64_t row = 0; row < n; row += most) {
+    RotArgs<T> part = g;
+    part.n = n - row < most ? n - row : most;
+    part.pos = (const PT*)g.pos + row * g.pos_row;
+    for (int w = 0; w < 2; ++w) {
+      part.in[w] = g.in[w] + row * g.in_row[w];
+      part.out[w] = g.out[w] + row * g.heads[w] * g.D;
+    }
+    kernel<<<st_blocks(part.n, g.rows), kRotThreads, 0, s>>>(part);
+    ST_CHECK_LAUNCH();
+  }
   return ST_OK;
 }
 

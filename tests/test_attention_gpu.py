@@ -14,6 +14,7 @@ import copy
 import math
 import pickle
 
+import numpy as np
 import pytest
 import torch
 
@@ -690,3 +691,26 @@ def test_lengths_whose_sum_wraps_are_refused(bad):
         AttentionSegments(bad, device="cpu")
     with pytest.raises(ValueError, match="2\\^31"):
         AttentionSegments([1] * len(bad), bad, device="cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("segments,heads,dim", [((1 << 20) + 3, 16, 72), ((1 << 22) + 3, 16, 8)])
+def test_more_workgroups_than_one_launch_takes(device, segments, heads, dim):
+    """A grid has fewer than 2^32 threads a dimension: 2^24 workgroups of four waves (wide rows), 2^26 of one."""
+    small = 1000
+    g = torch.Generator().manual_seed(22)
+    part = [torch.randn((small, heads, dim), generator=g).to(device, torch.bfloat16) for _ in range(4)]
+    whole = [t.repeat(-(-segments // small), 1, 1)[:segments] for t in part]
+    segs, few = AttentionSegments(np.ones(segments, np.int64), device=device), AttentionSegments([1] * small, device=device)
+    tile = segs._plan("q", 1, heads, False, 2 * dim, 2).tile
+    assert segments * heads * 2 * tile > 2 ** 32
+
+    def once(q, k, v, do, s):
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+        o = sparse_attention(*leaves, s)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, do)
+
+    for got, want in zip(once(*whole, segs), once(*part, few)):
+        for at in range(0, segments, 1 << 18):  # (a few hundred thousand rows of it at once)
+            rows = got[at:at + (1 << 18)]
+            assert torch.equal(rows, want[torch.arange(at, at + len(rows), device=device) % small])

@@ -245,3 +245,17 @@ def test_forward_mode_is_refused(device, own_random, which, recorded):
             sparse_layer_norm(*t[:3], residual=t[3])
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             sparse_layer_norm(*t[:3], residual=t[3])
+
+
+def test_more_workgroups_than_one_launch_takes(device):
+    """A grid has fewer than 2^32 threads: 2^24 workgroups, each of one row where a row takes all of its lanes."""
+    n, C, small = (1 << 24) + 5, 257, 4099
+    g = torch.Generator().manual_seed(12)
+    part = torch.randn((small, C), generator=g).to(device, torch.bfloat16)
+    w = (1 + 0.2 * torch.randn((C,), generator=g)).to(device)
+    want, stream = sparse_layer_norm(part, w, residual=part)
+    whole = part.repeat(-(-n // small), 1)[:n]
+    got, sums = sparse_layer_norm(whole, w, residual=whole)
+    for at in range(0, n, 1 << 20):
+        rows = torch.arange(at, min(n, at + (1 << 20)), device=device) % small
+        assert torch.equal(got[at:at + (1 << 20)], want[rows]) and torch.equal(sums[at:at + (1 << 20)], stream[rows])

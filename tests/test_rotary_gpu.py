@@ -217,3 +217,18 @@ def test_tables_outlive_their_owner_on_another_stream(device, own_random):
     got.record_stream(torch.cuda.current_stream())
     assert torch.equal(got, want)
     assert done or not set(held) & {t.data_ptr() for t in new}
+
+
+@pytest.mark.gpu
+def test_more_workgroups_than_one_launch_takes(device):
+    """A grid has fewer than 2^32 threads: 2^24 workgroups, each of one row where its heads have odd sizes."""
+    n, small, axes = (1 << 24) + 3, 4099, RotaryAxes(53, (2, 4))
+    g = torch.Generator().manual_seed(13)
+    q = torch.randn((small, 9, 53), generator=g).to(device, torch.bfloat16)
+    k = torch.randn((small, 2, 53), generator=g).to(device, torch.bfloat16)
+    pos = torch.randint(-500, 500, (small, 2), generator=g).to(device, torch.int16)
+    want = sparse_rotary(q, k, pos, axes)
+    got = sparse_rotary(*[t.repeat(-(-n // small), *[1] * (t.dim() - 1))[:n] for t in (q, k, pos)], axes)
+    for at in range(0, n, 1 << 20):
+        rows = torch.arange(at, min(n, at + (1 << 20)), device=device) % small
+        assert all(torch.equal(a[at:at + (1 << 20)], b[rows]) for a, b in zip(got, want))
