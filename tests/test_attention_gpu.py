@@ -10,9 +10,11 @@ channels, its exponential and the row's sum):
   dQ, dK, dV   the error of dS or P through the product, plus u of the result.
 """
 
+import concurrent.futures
 import copy
 import math
 import pickle
+import threading
 
 import numpy as np
 import pytest
@@ -714,3 +716,123 @@ def test_more_workgroups_than_one_launch_takes(device, segments, heads, dim):
         for at in range(0, segments, 1 << 18):  # (a few hundred thousand rows of it at once)
             rows = got[at:at + (1 << 18)]
             assert torch.equal(rows, want[torch.arange(at, at + len(rows), device=device) % small])
+
+
+def _check_calls(q, k, v, do, ql, kl, causal, mask):
+    """As _check, with what its bound leaves out: a float16 result below 2^-14 is rounded by up to half a spacing, 2^-25."""
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = sparse_attention(*leaves, AttentionSegments(ql, kl, device=q.device), causal=causal, key_mask=mask)
+    got = dict(zip(("o", "dq", "dk", "dv"), (o.detach(),) + torch.autograd.grad(o, leaves, do)))
+    least = 2.0 ** -25 if q.dtype is torch.float16 else 0.0
+    for n, (want, bound) in _reference(q, k, v, do, ql, kl, q.shape[2] ** -0.5, causal, mask).items():
+        over = (got[n].double() - want).abs() - bound - least
+        assert not torch.isnan(got[n]).any() and over.max().item() <= 0, (n, over.max().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ql,kl,heads,kv_heads,dim,causal", [
+    ([1], [5000], 4, 1, 64, False), ([1, 1, 2], [1, 4097, 300], 8, 2, 128, True), ([2500], [40], 2, 1, 32, False),
+    ([1000], [1000], 1, 1, 64, True), ([1500, 20], [1, 2000], 2, 2, 48, False), ([700, 30], [700, 3000], 4, 2, 96, True)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_joins_of_every_type(device, ql, kl, heads, kv_heads, dim, causal, dtype):
+    """Split tiles and their joins, by the lists that the calls use."""
+    q, k, v, do, mask = _make(ql, kl, heads, kv_heads, dim, dtype, device, 5 * dim, masked=0.1)
+    segs = AttentionSegments(ql, kl, device=device)
+    e = q.element_size()
+    joins = [segs._plan(w, heads // kv_heads, kv_heads, causal, dim * e, e).n_joins for w in "qk"]
+    assert joins[0] if max(kl) > max(ql) else joins[1]
+    _check_calls(q, k, v, do, ql, kl, causal, mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.float32, 32)])
+def test_many_whole_tiles(device, causal, dtype, dim):
+    """Enough workgroups that nothing is split, by the lists that the calls use."""
+    ql = [700, 1, 333, 900, 64, 128, 2] * 16
+    q, k, v, do, mask = _make(ql, ql, 8, 4, dim, dtype, device, 19, masked=0.05)
+    segs, e = AttentionSegments(ql, device=device), q.element_size()
+    assert not any(segs._plan(w, 2, 4, causal, dim * e, e).n_joins for w in "qk")
+    _check_calls(q, k, v, do, ql, ql, causal, mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("step", range(0, 36, 9))
+def test_small_probabilities_of_split_rows_in_float16(device, step, dim):
+    """As test_small_probabilities_in_float16, one row over keys that are split: the others' ~2^-20 come out of parts
+    whose maximum is their own, and out of the first key's, whose maximum is one."""
+    n, a = 4096, 3.390625 + step / 512
+    q = torch.zeros((1, 1, dim), dtype=torch.float16, device=device)
+    k, v = (torch.zeros((n, 1, dim), dtype=torch.float16, device=device) for _ in range(2))
+    q[:, 0, 0], k[0, 0, 0], v[1:] = a, 4.0, 1.0
+    segs = AttentionSegments([1], [n], device=device)
+    assert segs._plan("q", 1, 1, False, 2 * dim, 2).n_joins == 1
+    r = math.exp(-4 * a)
+    p = r / (1 + (n - 1) * r)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = sparse_attention(*leaves, segs, scale=1.0)
+    dv = torch.autograd.grad(o, v, torch.full_like(q, 1024.0))[0]
+    bound = 2 * 2.0 ** -11 + W
+    assert (o.double() / ((n - 1) * p) - 1).abs().max().item() <= bound
+    assert (dv[1:].double() / (1024 * p) - 1).abs().max().item() <= bound
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("causal", [False, True])
+def test_training_pass_in_a_graph(device, own_random, dtype, causal):
+    """A recorded call and its gradients captured together, replayed on other values between eager calls."""
+    ql = [700, 33, 1]
+    q, k, v, do, mask = _make(ql, ql, 4, 2, 32, dtype, device, 20, masked=0.1)
+    segs = AttentionSegments(ql, device=device)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+
+    def once():
+        o = sparse_attention(*leaves, segs, causal=causal, key_mask=mask)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, do)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once()  # the tile lists are built by an eager call
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once()
+    for i in range(3):
+        with torch.no_grad():
+            for t in leaves + [do]:
+                t.copy_(torch.randn(t.shape, device=device))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, once())), i
+
+
+@pytest.mark.gpu
+def test_threads_share_the_segments(device):
+    """Two threads, each on a stream of its own, with one AttentionSegments whose lists are not built yet."""
+    ql = [900, 40, 3]
+    data = [_make(ql, ql, 4, 2, 64, torch.bfloat16, device, 21 + i)[:4] for i in range(2)]
+
+    def once(i, segs):
+        q, k, v, do = data[i]
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o = sparse_attention(*leaves, segs, causal=True)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, do)
+
+    want = [once(i, AttentionSegments(ql, device=device)) for i in range(2)]
+    segs, start = AttentionSegments(ql, device=device), threading.Barrier(2)
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait(30)
+            got = [once(i, segs) for _ in range(5)]
+            torch.cuda.current_stream().synchronize()
+        return got
+
+    with concurrent.futures.ThreadPoolExecutor(2) as pool:
+        for i, runs in enumerate(pool.map(work, range(2))):
+            assert all(torch.equal(a, b) for got in runs for a, b in zip(got, want[i]))
