@@ -420,11 +420,12 @@ constexpr int attn_waves() {
 // accumulators scaled when the maximum rises.  Few tiles: the keys are split
 // and the parts joined after it.
 //
-// 64 patches of 1,024 rows x 8 heads x 64 bf16: 200 us, 690 TFLOP/s (a large
+// (Kernel times here and below are medians by trace.)
+// 64 patches of 1,024 rows x 8 heads x 64 bf16: 208 us, 660 TFLOP/s (a large
 // product: 1,210).  The vector unit is what it runs on: an exponential, a
-// multiply-add, a sum, half a conversion and half a maximum for each score
-// against 64 channels of MFMA; it issues 72 % of the time, the matrix unit is
-// busy 39 %, three waves a SIMD.  128 channels do twice the product for the same
+// multiply-add, a sum, half a conversion and half a maximum for each score, 64
+// instructions a 32 x 32 tile of them, and 32 more by its counter (offsets, bounds, staging); it
+// issues 70 % of the time, the matrix unit is busy 37 %, three waves a SIMD.  128 channels do twice the product for the same
 // scores: 8,191 rows x 16 heads of 128 (4 key heads), causal, bf16, 330 us, 830
 // TFLOP/s of the visible half.  fp32, 24 samples of up to 1,500 rows x 6 x 48: 80
 // us, 72 TFLOP/s (a large fp32 product: 153), the matrix unit busy 60 %, a seventh of
@@ -772,8 +773,8 @@ constexpr int attn_dq_lds(bool causal) {
 // five; one kernel for all three gradients would add dQ with atomics, in an
 // order that changes the bits, or write it once for each tile of keys.
 //
-// As the forward's sizes: 64 channels bf16 255 us (810 TFLOP/s, MFMA busy 45 %, vector
-// unit 62), 128 channels causal 453 us (910, 47 %), fp32 114 us (76, 61 %).
+// As the forward's sizes: 64 channels bf16 272 us (760 TFLOP/s, MFMA busy 44 %, vector
+// unit 62: 107 instructions a tile), 128 channels causal 453 us (910, 47 %), fp32 114 us (76, 61 %).
 template <typename T, int DP, bool CAUSAL, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
@@ -926,9 +927,9 @@ constexpr int attn_dkv_lds(bool causal) {
 // in the place of four, by two waves a SIMD: 32 patches of 1,024 rows x 8 x 128 bf16,
 // the whole backward, 760 -> 680 us (at 96 channels 424 -> 486: one launch there).
 //
-// As the forward's sizes: 64 channels bf16 340 us (810 TFLOP/s, MFMA busy 45 %, vector
-// unit 53; two waves a SIMD, which wait for each other's products and LDS reads), 128
-// channels causal 340 + 470 us (810 and 880, 37 and 42 %), fp32 166
+// As the forward's sizes: 64 channels bf16 345 us (800 TFLOP/s, MFMA busy 45 %, vector
+// unit 53: 117 instructions a tile; two waves a SIMD, which wait for each other's products and LDS reads), 128
+// channels causal 350 + 470 us (790 and 880, 37 and 42 %), fp32 167
 // us (70, 56 %).  (The clock falls to about 1.75 GHz under all of them: fewer cycles buy less time than that.)
 constexpr int kAttnDv = 1, kAttnDk = 2;
 template <typename T, int DP>

@@ -161,9 +161,10 @@ class AttentionSegments:
     ``q_lengths``: rows of each segment, in the order in which the rows lie; ``k_lengths`` the key
     rows where they are not the same (cross attention).  Both are sequences or integer tensors (a
     device tensor is read back).  Either may be zero: a row without keys has a zero output.  Made
-    once for a set of rows and shared by the layers over them; the tile lists for a number of heads
-    and an order are built at the first call with them (so a call whose lists are not there yet
-    cannot be captured in a graph).
+    once for a set of rows and shared by the layers over them; the tile lists for a number of heads,
+    an order and a type are built at the first call with them, which costs 0.1 to 0.2 ms of host time
+    each (forward, and the keys' in the backward) and a blocking copy; a call whose lists are not there
+    yet cannot be captured in a graph.  A copy or a pickle builds its own.
     """
 
     def __init__(self, q_lengths: Union[Sequence[int], torch.Tensor],
@@ -348,8 +349,12 @@ def sparse_attention(
     ``causal``: query ``i`` of ``nq`` sees keys up to ``i + nk - nq`` of its segment.  ``key_mask``
     (``segments.k_rows``) bool: False leaves a key out, whatever its rows hold.  A row that sees no
     key gets zeros, and its gradients are zero.  Scores, softmax and sums are fp32 (fp32 inputs: the
-    products too); results do not depend on timing.  A 16-bit forward that records a gradient keeps what the
-    output's rounding left beside it (as large as the output), for the gradients of rows with few keys.
+    products too); results do not depend on timing.  16-bit inputs round the probabilities, and in the
+    gradient dS, to their type for the products with V, dO, K and Q: errors 1.2 to 1.4 times those of fp32
+    arithmetic rounded once.  float16 holds both at powers of two, so that neither overflows where the
+    result does not nor loses digits to the type's smallest numbers.  A 16-bit forward that records a
+    gradient keeps what the output's rounding left beside it (as large as the output), for the gradients
+    of rows with few keys.
     There is no forward-mode derivative: a tangent on ``q``, ``k`` or ``v`` raises.
     """
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
