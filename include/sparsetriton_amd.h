@@ -839,6 +839,19 @@ int st_ln_backward(const void* H, const void* dY, const void* dH, int64_t n, int
                    int weight_dtype, const float* mean, const float* rstd, float* workspace, int64_t workspace_floats,
                    void* dX, void* dweight, void* dbias, st_stream_t stream);
 
+/* ------------------------------------------------------------ dropout
+ *
+ * Y[e] = (keep ? X[e] / (1 - p) : 0) + residual[e] (no counterpart in the
+ * reference; residual NULL = none), computed in fp32 and rounded once; the gradient is the same
+ * call on the output's gradient without a residual.  X, residual, Y: n contiguous
+ * elements of `dtype` (ST_F32, ST_F16, ST_BF16); 0 <= p <= 1; p = 1 keeps
+ * nothing.  Element e is kept where word e % 4 of Philox4x32-10's block of
+ * counter {e / 4 (64 bits), numbers[1]} under the key numbers[0], low words first, is not below
+ * round(p 2^32).  numbers: two 64-bit words on the device, read by the kernel.
+ */
+int st_dropout(const void* X, const void* residual, int64_t n, int dtype, const int64_t* numbers, double p, void* Y,
+               st_stream_t stream);
+
 /* ------------------------------------------------------------ rotary positions
  *
  * Turns the channel pairs of q (n, heads, dim) and k (n, kv_heads, dim) by the
@@ -866,6 +879,52 @@ typedef struct st_rotary_args {
   int32_t dtype, pos_dtype, interleaved, inverse;
 } st_rotary_args;
 int st_rotary(const st_rotary_args* args, st_stream_t stream);
+
+/* ------------------------------------------------------------ norm of queries and keys, with the rotary positions
+ *
+ * Each head of q and k is divided by the root of its channels' mean square
+ * (plus eps), multiplied by a weight and turned by the row's position (no counterpart in the reference):
+ *   q_out = R (q / sqrt(mean_c q^2 + eps) * q_weight),   k_out likewise with k_weight
+ * R as st_rotary turns (pairs = 0: not at all).  q, k, strides, positions, turns, axis,
+ * pairs and interleaved as there; dim at most ST_QK_MAX_DIM.  q_weight,
+ * k_weight: (dim) of weight_dtype (`dtype` or ST_F32), NULL = ones.  q or k may
+ * be NULL.  Sums and products are fp32, rounded once.
+ * st_qk_norm_rotary_backward: dq_out, dk_out are the gradients at the outputs
+ * (rows and heads at the strides dq_row, ...), dq, dk (contiguous) those of q and
+ * k; dq_weight, dk_weight (of weight_dtype, NULL = not wanted) are added over
+ * rows and heads in a fixed order, and need a workspace of at least
+ * st_qk_norm_rotary_workspace floats.
+ */
+#define ST_QK_MAX_DIM 256
+typedef struct st_qk_norm_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_row, q_head, k_row, k_head;
+  const void* q_weight;
+  const void* k_weight;
+  const void* positions;
+  int64_t pos_row;
+  const double* turns;
+  const int32_t* axis;
+  int64_t n;
+  int32_t heads, kv_heads, dim, pairs;
+  int32_t dtype, weight_dtype, pos_dtype, interleaved;
+  const void* dq_out;
+  const void* dk_out;
+  int64_t dq_row, dq_head, dk_row, dk_head;
+  void* dq;
+  void* dk;
+  void* dq_weight;
+  void* dk_weight;
+  float* workspace;
+  int64_t workspace_floats;
+  float eps;
+} st_qk_norm_args;
+int st_qk_norm_rotary(const st_qk_norm_args* args, st_stream_t stream);
+int st_qk_norm_rotary_workspace(int64_t n, int dim, int64_t* floats);
+int st_qk_norm_rotary_backward(const st_qk_norm_args* args, st_stream_t stream);
 
 /* ------------------------------------------------------------ attention
  *

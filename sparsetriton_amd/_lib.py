@@ -34,6 +34,7 @@ COLUMN_SUM_NOALLOC_MAX_C = 2048
 MAX_KVOL = 512
 TILE_ROWS = 128
 ATTN_TILE, ATTN_SMALL_TILE, ATTN_SMALL_TILE_BYTES, ATTN_MAX_DIM, ATTN_WORDS = 128, 32, 128, 128, 8
+QK_MAX_DIM = 256
 
 
 class OutGeom(ctypes.Structure):
@@ -72,6 +73,19 @@ class RotaryArgs(ctypes.Structure):
                                          "inverse")]
     )
 
+
+class QkNormArgs(ctypes.Structure):
+    _fields_ = (
+        [(n, _P) for n in ("q", "k", "q_out", "k_out")]
+        + [(n, _L) for n in ("q_row", "q_head", "k_row", "k_head")]
+        + [("q_weight", _P), ("k_weight", _P), ("positions", _P), ("pos_row", _L), ("turns", _P), ("axis", _P), ("n", _L)]
+        + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "pairs", "dtype", "weight_dtype", "pos_dtype",
+                                         "interleaved")]
+        + [("dq_out", _P), ("dk_out", _P)]
+        + [(n, _L) for n in ("dq_row", "dq_head", "dk_row", "dk_head")]
+        + [(n, _P) for n in ("dq", "dk", "dq_weight", "dk_weight", "workspace")]
+        + [("workspace_floats", _L), ("eps", ctypes.c_float)]
+    )
 
 
 class AttnArgs(ctypes.Structure):
@@ -153,10 +167,14 @@ _SIGNATURES = {
     "st_ln_forward": [_P, _P, _L, _I, _I, _P, _P, _I, ctypes.c_float, _P, _P, _P, _P, _P],
     "st_ln_backward_workspace": [_L, _I, _I, ctypes.POINTER(_L)],
     "st_ln_backward": [_P, _P, _P, _L, _I, _I, _P, _I, _P, _P, _P, _L, _P, _P, _P, _P],
+    "st_dropout": [_P, _P, _L, _I, _P, ctypes.c_double, _P, _P],
     "st_attn_workspace": [_I, _I, _L, _L, ctypes.POINTER(_L)],
     "st_attn_forward": [ctypes.POINTER(AttnArgs), _P],
     "st_attn_backward": [ctypes.POINTER(AttnArgs), _P],
     "st_rotary": [ctypes.POINTER(RotaryArgs), _P],
+    "st_qk_norm_rotary": [ctypes.POINTER(QkNormArgs), _P],
+    "st_qk_norm_rotary_workspace": [_L, _I, ctypes.POINTER(_L)],
+    "st_qk_norm_rotary_backward": [ctypes.POINTER(QkNormArgs), _P],
     "st_hashfly_wgrad": [_P, _L, _P, _P, _I, _L, _P, ctypes.POINTER(Lookup), _P, _P, _L, _I, _I, _I, _P, _L, _P,
                          _I, _P],
 }
@@ -227,6 +245,16 @@ def stream_of(device: torch.device):
         idx = device.index
         return _raw_stream(idx if idx is not None else torch.cuda.current_device())
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` on torch's current stream of ``device`` (the last argument), with ``device`` current: a launch goes
+    to the current device, whatever device its tensors and stream belong to."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_of(device))
 
 
 def require_device(t: torch.Tensor, what: str) -> None:

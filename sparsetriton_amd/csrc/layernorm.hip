@@ -20,6 +20,7 @@
 // its gradient: 47 / 55 / 4 us (5.7 and 4.9 TB/s); a 1 GiB copy runs at 5.1 TB/s.
 // 16 x 512 bf16: 2.8 us, a launch.
 #include "common.h"
+#include "sum_parts.h"
 #include "wave_sum.h"
 
 #define ST_LN_DISPATCH(dt, T, ...) \
@@ -382,32 +383,6 @@ __global__ __launch_bounds__(kLnThreads) void ln_columns_kernel(const T* __restr
   parts[(int64_t)blockIdx.y * 2 * C + C + c] = ab;
 }
 
-// dw, db = the partials' column sums: a workgroup for eight columns, a thread
-// for a column and each of 32 shares of the partials, the shares added in order.
-// (32 columns and 8 shares of it took 32 us for 1,024 partials of 64 channels:
-// four workgroups, 128 loads one after another.)
-template <typename W>
-__global__ __launch_bounds__(kLnThreads) void ln_reduce_kernel(const float* __restrict__ parts, int groups, int C,
-                                                               W* __restrict__ dw, W* __restrict__ db) {
-  __shared__ float sums[32][9];
-  const int in = threadIdx.x & 7, share = threadIdx.x >> 3, col = blockIdx.x * 8 + in;
-  float s = 0.f;
-  if (col < 2 * C) {
-#pragma unroll 8
-    for (int p = share; p < groups; p += 32) s += parts[(int64_t)p * 2 * C + col];
-  }
-  sums[share][in] = s;
-  __syncthreads();
-  if (share || col >= 2 * C) return;
-#pragma unroll
-  for (int o = 1; o < 32; ++o) s += sums[o][in];
-  if (col < C) {
-    if (dw) dw[col] = (W)s;
-  } else if (db) {
-    db[col - C] = (W)s;
-  }
-}
-
 // ------------------------------------------------------------------ host
 
 // F<V, LANES, NV>() for the geometry.  (VV: the type's whole vector.)
@@ -506,9 +481,7 @@ static int ln_backward(const void* H, const void* dY, const void* dH, int64_t n,
     });
   }
   if (rc != ST_OK || !columns) return rc;
-  ln_reduce_kernel<W><<<st_blocks(2 * (int64_t)C, 8), kLnThreads, 0, s>>>(ws, (int)groups, C, (W*)dw, (W*)db);
-  ST_CHECK_LAUNCH();
-  return ST_OK;
+  return sum_parts<W>(ws, groups, C, dw, db, s);
 }
 
 }  // namespace st
@@ -548,7 +521,7 @@ extern "C" int st_ln_backward(const void* H, const void* dY, const void* dH, int
   const int rc = st_ln_backward_workspace(n, C, dtype, &need);
   if (rc != ST_OK) return rc;
   // (the sum of the partials is one launch, eight of 2 C columns to a workgroup)
-  if ((dweight || dbias) && (2 * (int64_t)C + 7) / 8 > st_most_blocks(st::kLnThreads)) return ST_ERR_UNSUPPORTED;
+  if ((dweight || dbias) && (2 * (int64_t)C + 7) / 8 > st_most_blocks(st::kPartsThreads)) return ST_ERR_UNSUPPORTED;
   if (weight_dtype != dtype && weight_dtype != ST_F32) return ST_ERR_UNSUPPORTED;
   if (n > 0 && (!H || !dY || !mean || !rstd)) return ST_ERR_ARG;
   if ((dweight || dbias) && (!workspace || workspace_floats < need || ((uintptr_t)workspace & 15))) return ST_ERR_ARG;

@@ -1,4 +1,5 @@
-"""Rotary positions of queries and keys over the axes of the voxel grid (HIP kernel ``st_rotary``).
+"""Rotary positions of queries and keys over the axes of the voxel grid (HIP kernel ``st_rotary``), and the
+same after a norm of each head, in one pass (``st_qk_norm_rotary``).
 
 No counterpart in the reference.  A head's first ``sum(axes)`` channels are paired; the pairs are
 dealt to the axes in order (``axes[a] // 2`` pairs to axis ``a``), and pair ``i`` of axis ``a``
@@ -12,10 +13,11 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from sparsetriton_amd import _lib
+from sparsetriton_amd.nn.functional.norm import _ln_params
 from sparsetriton_amd.tensor import SparseTensor
 from sparsetriton_amd.utils.utils import once_differentiable, refuse_tangents
 
-__all__ = ["RotaryAxes", "sparse_rotary"]
+__all__ = ["RotaryAxes", "sparse_rotary", "sparse_qk_norm_rotary"]
 
 
 class RotaryAxes:
@@ -107,23 +109,11 @@ class _Rotary(torch.autograd.Function):
         return dq, dk, None, None
 
 
-def sparse_rotary(
-    q: Optional[torch.Tensor],
-    k: Optional[torch.Tensor],
-    positions: Union[SparseTensor, torch.Tensor],
-    axes: RotaryAxes,
-) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
-    """``(q, k)`` with each head's channel pairs turned by the row's position.
-
-    ``q`` (N, heads, D) and ``k`` (N, kv_heads, D) share rows and dtype (one of them may be
-    ``None``); rows and heads may lie at any stride.  ``positions``: a ``SparseTensor`` (the x, y, z
-    of its coordinates) or (N, A) of int16, int32, int64 or float32 with ``A >= len(axes.axes)``.
-    The outputs are contiguous; the gradient turns back.  Positions get no gradient.  There is no
-    forward-mode derivative: a tangent on ``q`` or ``k`` raises.
-    """
+def _check(what, q, k, positions, axes):
+    """The positions as the kernels take them, (rows, at least as many as the axes)."""
     first = q if q is not None else k
     if first is None:
-        raise ValueError("sparse_rotary needs q or k")
+        raise ValueError(f"{what} needs q or k")
     pos = positions.C[:, 1:] if isinstance(positions, SparseTensor) else positions
     for t in (first,) if q is None or k is None else (q, k):
         if not t.is_cuda:
@@ -142,7 +132,140 @@ def sparse_rotary(
         raise ValueError(f"positions are on {pos.device}, q and k on {first.device}")
     if pos.shape[1] > 1 and pos.stride(1) != 1:
         pos = pos.contiguous()
+    return pos
+
+
+def sparse_rotary(
+    q: Optional[torch.Tensor],
+    k: Optional[torch.Tensor],
+    positions: Union[SparseTensor, torch.Tensor],
+    axes: RotaryAxes,
+) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """``(q, k)`` with each head's channel pairs turned by the row's position.
+
+    ``q`` (N, heads, D) and ``k`` (N, kv_heads, D) share rows and dtype (one of them may be
+    ``None``); rows and heads may lie at any stride.  ``positions``: a ``SparseTensor`` (the x, y, z
+    of its coordinates) or (N, A) of int16, int32, int64 or float32 with ``A >= len(axes.axes)``.
+    The outputs are contiguous; the gradient turns back.  Positions get no gradient.  There is no
+    forward-mode derivative: a tangent on ``q`` or ``k`` raises.
+    """
+    pos = _check("sparse_rotary", q, k, positions, axes)
     refuse_tangents("sparse_rotary", q, k)
     if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
         return _Rotary.apply(q, k, pos.detach(), axes)
     return _rotate(q, k, pos, axes, False)
+
+
+def _flat(t):
+    """t with a head's channels side by side."""
+    return t if t is None or t.stride(2) == 1 else t.contiguous()
+
+
+def _qk_args(q, k, q_weight, k_weight, positions, axes, eps):
+    """(arguments of both directions, the tensors that they point to)."""
+    t = q if q is not None else k
+    turns, axis = axes.on(t.device)
+    q, k = _flat(q), _flat(k)
+    wq, wk, wcode = _ln_params(t, q_weight, k_weight)
+    qs, heads = (q.stride(), q.shape[1]) if q is not None else ((0, 0), 0)
+    ks, kv_heads = (k.stride(), k.shape[1]) if k is not None else ((0, 0), 0)
+    ptr = _lib.ptr
+    a = _lib.QkNormArgs(ptr(q), ptr(k), None, None, qs[0], qs[1], ks[0], ks[1], ptr(wq), ptr(wk), positions.data_ptr(),
+                        positions.stride(0), turns.data_ptr(), axis.data_ptr(), t.shape[0], heads, kv_heads, t.shape[2],
+                        axes.pairs, _lib.FEAT_DTYPES[t.dtype], wcode, _lib.POSITION_DTYPES[positions.dtype],
+                        axes.interleaved)
+    a.eps = eps
+    return a, (q, k, wq, wk)
+
+
+def _qk_forward(q, k, q_weight, k_weight, positions, axes, eps):
+    a, held = _qk_args(q, k, q_weight, k_weight, positions, axes, eps)
+    out = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k)]
+    a.q_out, a.k_out = _lib.ptr(out[0]), _lib.ptr(out[1])
+    _lib.call_on(positions.device, "st_qk_norm_rotary", ctypes.byref(a))
+    return out[0], out[1], held
+
+
+class _QkNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, axes, eps):
+        q_out, k_out, held = _qk_forward(q, k, q_weight, k_weight, positions, axes, eps)
+        ctx.save_for_backward(*held, positions)
+        ctx.meta = (axes, eps, [None if w is None else w.dtype for w in (q_weight, k_weight)])
+        ctx.set_materialize_grads(False)
+        return q_out, k_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *dys):
+        q, k, wq, wk, positions = ctx.saved_tensors
+        axes, eps, dtypes = ctx.meta
+        need = ctx.needs_input_grad
+        # a tensor whose result no gradient arrives at has none either, and adds nothing to its weight's
+        xs = [x if dy is not None and (need[i] or need[2 + i]) else None for i, (x, dy) in enumerate(zip((q, k), dys))]
+        dx, dw = [None, None], [None, None]
+        for i, w in enumerate((wq, wk)):
+            if need[2 + i]:
+                dw[i] = torch.zeros_like(w) if xs[i] is None else torch.empty_like(w)
+        if xs[0] is not None or xs[1] is not None:
+            a, _ = _qk_args(xs[0], xs[1], wq, wk, positions, axes, eps)
+            dys = [None if x is None else _flat(dy) for x, dy in zip(xs, dys)]
+            dx = [None if x is None else torch.empty_like(x, memory_format=torch.contiguous_format) for x in xs]
+            ptr = _lib.ptr
+            a.dq_out, a.dk_out, a.dq, a.dk = (ptr(t) for t in (*dys, *dx))
+            if dys[0] is not None:
+                a.dq_row, a.dq_head = dys[0].stride()[:2]
+            if dys[1] is not None:
+                a.dk_row, a.dk_head = dys[1].stride()[:2]
+            a.dq_weight, a.dk_weight = (ptr(d) if x is not None else None for d, x in zip(dw, xs))
+            if a.dq_weight or a.dk_weight:
+                n, dim = positions.shape[0], axes.head_dim
+                floats = ctypes.c_int64()
+                _lib.call("st_qk_norm_rotary_workspace", n, dim, ctypes.byref(floats))
+                ws = torch.empty((floats.value,), dtype=torch.float32, device=positions.device)
+                a.workspace, a.workspace_floats = ws.data_ptr(), floats.value
+            _lib.call_on(positions.device, "st_qk_norm_rotary_backward", ctypes.byref(a))
+        dw = [d if d is None or d.dtype is dt else d.to(dt) for d, dt in zip(dw, dtypes)]
+        return dx[0] if need[0] else None, dx[1] if need[1] else None, dw[0], dw[1], None, None, None
+
+
+def sparse_qk_norm_rotary(
+    q: Optional[torch.Tensor],
+    k: Optional[torch.Tensor],
+    positions: Union[SparseTensor, torch.Tensor],
+    axes: RotaryAxes,
+    q_weight: Optional[torch.Tensor] = None,
+    k_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """``sparse_rotary`` of normalised heads, in one pass: each head of ``q`` and ``k`` is divided by
+    ``sqrt(mean(x^2) + eps)`` over its channels, multiplied by ``q_weight`` (``k_weight``; ones where
+    ``None``) and turned by the row's position.
+
+    ``q``, ``k``, ``positions`` and ``axes`` as ``sparse_rotary`` takes them, heads of at most 256
+    channels; the weights are (D,) of float32, float16 or bfloat16, shared by the heads of their tensor.  The outputs are contiguous,
+    of ``q``'s and ``k``'s dtype, computed in fp32 and rounded once (a mean square must be in fp32's
+    range); the gradients of the weights are added in a fixed order.  The backward keeps the inputs
+    alone.  There is no forward-mode derivative: a tangent on an input raises.
+    """
+    pos = _check("sparse_qk_norm_rotary", q, k, positions, axes)
+    first = q if q is not None else k
+    if axes.head_dim > _lib.QK_MAX_DIM:
+        raise ValueError(f"heads must have at most {_lib.QK_MAX_DIM} channels (got {axes.head_dim})")
+    for t, w, what in ((q, q_weight, "q_weight"), (k, k_weight, "k_weight")):
+        if w is None:
+            continue
+        if t is None:
+            raise ValueError(f"{what} without its tensor")
+        if w.shape != (axes.head_dim,) or w.device != first.device:
+            raise ValueError(f"{what} must be ({axes.head_dim},) on {first.device} (got {tuple(w.shape)} on {w.device})")
+        _lib.feat_code(w.dtype)
+    eps = float(eps)
+    if not (eps >= 0 and math.isfinite(eps)):
+        raise ValueError(f"eps must not be negative (got {eps})")
+    if sum(t.shape[1] for t in (q, k) if t is not None) >= 1 << 15:
+        raise ValueError("q and k have at most 32,767 heads together")
+    refuse_tangents("sparse_qk_norm_rotary", q, k, q_weight, k_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _QkNormRotary.apply(q, k, q_weight, k_weight, pos.detach(), axes, eps)
+    return _qk_forward(q, k, q_weight, k_weight, pos, axes, eps)[:2]
