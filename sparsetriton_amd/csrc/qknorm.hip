@@ -14,7 +14,15 @@
 // sines and the weights are in LDS, shared by its heads.  The backward's
 // workgroups walk ranges of rows and keep dw of their lanes' channels in
 // registers; one partial a workgroup, added in a fixed order by a second kernel.
+//
+// Kernel times (a 1 GiB copy runs at 5.25 TB/s), forward / backward: 470,532 rows x
+// (8 + 8) heads x 32 bf16 184 / 316 us (5.2 and 4.6 TB/s), 65,537 x (16 + 4) x 128
+// bf16 125 / 221 (5.4, 4.6), 60,001 x (6 + 6) x 48 fp32 interleaved 52 / 88 (5.3,
+// 4.7); the rotation alone, rotary.hip, takes 182, 118 and 44.  Offsets that grow
+// by steps for ones computed anew at each head, and each head's loads ahead of
+// the one before it: forward 212, 145, 78 us before.
 #include "common.h"
+#include "mfma.h"
 #include "sum_parts.h"
 #include "wave_sum.h"
 
@@ -22,9 +30,13 @@ namespace st {
 
 constexpr int kQkThreads = 256;
 constexpr int kQkTable = 2048;  // cosine / sine pairs in LDS (16 KB)
-constexpr int kQkItems = 512;   // lanes' worth of heads in a forward workgroup, about
-constexpr int kQkBatch = 2;     // heads that a forward lane has on their way at once
-constexpr int kQkMaxGroups = 1024;  // workgroups of the backward, each leaving one partial
+// Lanes' worth of heads in a forward workgroup, about (512 / 1,024: 65,537 x (16 + 4) x 128 bf16 142 / 125 us,
+// 470,532 x (8 + 8) x 32 184 / 185).
+constexpr int kQkItems = 1024;
+constexpr int64_t kQkReach = kOobOffset - 1024;  // bytes from a workgroup's first head to its last one's end
+// Workgroups of the backward, each leaving one partial: the three of a compute unit that its registers leave room for (1,024
+// of them, a last third alone: 364 us at 470,532 x 16 x 32 bf16 for 316).
+constexpr int kQkMaxGroups = 768;
 
 template <typename T>
 struct QkArgs {
@@ -42,15 +54,13 @@ struct QkArgs {
   const int32_t* axis;
   int64_t n;
   int D, P, rows;
-  int chunks, lanes, lane_bits;  // vectors of a head, and the power of two of lanes that hold them
-  uint64_t all_inv, heads_inv[2];  // ceil(2^32 / ...): i / d = i * inv >> 32 for i * d < 2^32
+  int chunks, lanes, lane_bits;  // of a head, and the power of two of lanes that hold them
+  int table_row;                 // entries of a row's table: the pairs, and one for each of the other chunks' turns
+  float heads_inv[2];              // 1 / heads: (i + 1/2) / heads tells i's row, for the i < 256 of a first step
+  int step_row[2], step_h[2];      // a step of `side` heads, in rows and heads
   float eps, inv_d;
+  int64_t per;  // backward: rows of a workgroup
   float* parts;
-};
-
-template <typename T, int V>
-struct QkVec {
-  typedef T type __attribute__((ext_vector_type(V)));
 };
 
 __device__ __forceinline__ double qk_pos(const void* p, int dtype, int64_t i) {
@@ -81,81 +91,108 @@ __device__ __forceinline__ void qk_sum(float (&v)[N], int lanes) {
   if (lanes >= 64) step([](float x) { return other_half(x); });
 }
 
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+
+// N bytes at an offset from a buffer's base: zeros past its end (kOobOffset on), where nothing is stored either.
+template <typename T, int V>
+struct QkVec {
+  typedef T type __attribute__((ext_vector_type(V)));
+  static constexpr int kBytes = V * (int)sizeof(T);
+  using Rsrc = __amdgpu_buffer_rsrc_t;
+  template <typename F>
+  static __device__ __forceinline__ void load(Rsrc r, unsigned at, F (&x)[V]) {
+    type v;
+    if constexpr (kBytes == 16)
+      v = __builtin_bit_cast(type, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+    else if constexpr (kBytes == 8)
+      v = __builtin_bit_cast(type, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0));
+    else if constexpr (kBytes == 4)
+      v = __builtin_bit_cast(type, __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0));
+    else
+      v = __builtin_bit_cast(type, __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0));
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = (F)v[e];
+  }
+  static __device__ __forceinline__ void store(Rsrc r, unsigned at, const float (&x)[V]) {
+    type v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (T)x[e];
+    if constexpr (kBytes == 16)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), r, at, 0, 0);
+    else if constexpr (kBytes == 8)
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, v), r, at, 0, 0);
+    else if constexpr (kBytes == 4)
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), r, at, 0, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), r, at, 0, 0);
+  }
+};
+
 // How a lane holds its share of a head: NV chunks `lanes` apart.  A chunk is a
-// vector of V channels from `at` on and, where its channels turn with others
-// (second()), the vector of those, `partner` further on.  Interleaved vectors of
-// more than one channel hold both of each pair.
+// vector of V channels and the vector of those that they turn with, or
+// (interleaved vectors of more than one channel) one that holds both of each
+// pair.  Chunks past the pairs turn by nothing: the table has (1, 0) for
+// them, and their second vector, like all of a chunk that the head does not have, is
+// read as zeros and not stored, by an offset past the buffers.
 template <typename T, int V, int NV, bool INTERLEAVED>
 struct QkLane {
-  using Vec = typename QkVec<T, V>::type;
+  using Vec = QkVec<T, V>;
   static constexpr bool kInside = INTERLEAVED && V > 1;
-  int ch, pair_chunks, chunks, lanes, P;
+  static constexpr int H = kInside ? 1 : 2, M = NV * H;  // vectors of a chunk, of the lane
+  unsigned off[M];  // bytes from the head's first channel
+  int w[M];         // channel (any where there is none: its x is zero)
+  int turns[NV];    // of the table's row
 
-  __device__ __forceinline__ QkLane(const QkArgs<T>& g)
-      : ch(threadIdx.x & (g.lanes - 1)), pair_chunks(kInside ? 2 * g.P / V : g.P / V), chunks(g.chunks), lanes(g.lanes), P(g.P) {}
-  __device__ __forceinline__ int chunk(int k) const { return ch + k * lanes; }
-  __device__ __forceinline__ bool live(int k) const { return chunk(k) < chunks; }
-  __device__ __forceinline__ bool pair(int k) const { return chunk(k) < pair_chunks; }
-  __device__ __forceinline__ bool second(int k) const { return !kInside && pair(k); }
-  __device__ __forceinline__ int partner() const { return INTERLEAVED ? 1 : P; }
-  __device__ __forceinline__ int at(int k) const {
-    const int c = chunk(k);
-    return c < pair_chunks ? c * (INTERLEAVED && V == 1 ? 2 : V) : 2 * P + (c - pair_chunks) * V;
-  }
-  __device__ __forceinline__ void load(const T* head, bool there, Vec (&a)[NV], Vec (&b)[NV]) const {
+  __device__ __forceinline__ explicit QkLane(const QkArgs<T>& g) {
+    const int pair_chunks = kInside ? 2 * g.P / V : g.P / V;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      a[k] = b[k] = (Vec)(T)0.f;
-      if (there && live(k)) {
-        a[k] = *reinterpret_cast<const Vec*>(head + at(k));
-        if (second(k)) b[k] = *reinterpret_cast<const Vec*>(head + at(k) + partner());
+      const int c = (threadIdx.x & (g.lanes - 1)) + k * g.lanes;
+      const bool live = c < g.chunks, pair = c < pair_chunks;
+      const int at = pair ? c * (INTERLEAVED && V == 1 ? 2 : V) : 2 * g.P + (c - pair_chunks) * V;
+      off[k * H] = live ? at * (unsigned)sizeof(T) : (unsigned)kOobOffset;
+      w[k * H] = live ? at : 0;
+      if constexpr (!kInside) {
+        const int second = at + (INTERLEAVED ? 1 : g.P);
+        off[k * H + 1] = pair ? second * (unsigned)sizeof(T) : (unsigned)kOobOffset;
+        w[k * H + 1] = pair ? second : 0;
       }
+      turns[k] = live ? c * (kInside ? V / 2 : V) : 0;
     }
   }
-  __device__ __forceinline__ void store(T* head, bool there, const float (&a)[NV][V], const float (&b)[NV][V]) const {
+  // the weights of vector m, `all` the tensor's
+  __device__ __forceinline__ void weights(const float* all, int m, float (&x)[V]) const {
+    typedef float F __attribute__((ext_vector_type(V)));
+    const F v = *reinterpret_cast<const F*>(all + w[m]);
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (there && live(k)) {
-        Vec x, y;
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = (T)a[k][e], y[e] = (T)b[k][e];
-        *reinterpret_cast<Vec*>(head + at(k)) = x;
-        if (second(k)) *reinterpret_cast<Vec*>(head + at(k) + partner()) = y;
-      }
+    for (int e = 0; e < V; ++e) x[e] = v[e];
   }
-  // (a, b) turned by the row's table; forwards or back
+  __device__ __forceinline__ bool has(int m) const { return off[m] != (unsigned)kOobOffset; }
+  // `head`: the head's offset, kOobOffset for none (the sum of two such does not wrap)
+  template <typename F>
+  __device__ __forceinline__ void load(typename Vec::Rsrc r, unsigned head, F (&x)[M][V]) const {
+#pragma unroll
+    for (int m = 0; m < M; ++m) Vec::load(r, head + off[m], x[m]);
+  }
+  __device__ __forceinline__ void store(typename Vec::Rsrc r, unsigned head, const float (&x)[M][V]) const {
+#pragma unroll
+    for (int m = 0; m < M; ++m) Vec::store(r, head + off[m], x[m]);
+  }
+  // x turned by the row's table, forwards or back
   template <bool BACK>
-  __device__ __forceinline__ void turn(const float2* table, float (&a)[NV][V], float (&b)[NV][V]) const {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if (!pair(k)) continue;
-      if constexpr (kInside) {
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-          const float2 t = table[chunk(k) * (V / 2) + e / 2];
-          const float s = BACK ? -t.y : t.y, x = a[k][e], y = a[k][e + 1];
-          a[k][e] = x * t.x - y * s;
-          a[k][e + 1] = x * s + y * t.x;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float2 t = table[chunk(k) * V + e];
-          const float s = BACK ? -t.y : t.y, x = a[k][e], y = b[k][e];
-          a[k][e] = x * t.x - y * s;
-          b[k][e] = x * s + y * t.x;
-        }
-      }
-    }
-  }
-  // the weights of the lane's channels
-  __device__ __forceinline__ void weights(const float* w, float (&a)[NV][V], float (&b)[NV][V]) const {
+  __device__ __forceinline__ void turn(const float2* table, float (&x)[M][V]) const {
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        a[k][e] = live(k) ? w[at(k) + e] : 0.f;
-        b[k][e] = second(k) ? w[at(k) + partner() + e] : 0.f;
+      for (int i = 0; i < (kInside ? V / 2 : V); ++i) {
+        const float2 t = table[turns[k] + i];
+        float& a = kInside ? x[k][2 * i] : x[k * H][i];
+        float& b = kInside ? x[k][2 * i + 1] : x[k * H + H - 1][i];
+        const float s = BACK ? -t.y : t.y, u = a * t.x - b * s;
+        b = a * s + b * t.x;
+        a = u;
+        if (BACK && !kInside && !has(k * H + H - 1)) b = 0.f;  // (zero times an infinity, for the sums that follow)
       }
   }
 };
@@ -163,11 +200,14 @@ struct QkLane {
 // Cosines and sines of `rows` rows from row0 on, and the weights, in LDS.
 template <typename T>
 __device__ __forceinline__ void qk_table(const QkArgs<T>& g, int64_t row0, int rows, float2* table) {
-  for (int i = threadIdx.x; i < rows * g.P; i += kQkThreads) {
-    const int r = i / g.P, p = i - r * g.P;
-    const double t = qk_pos(g.pos, g.pos_dtype, (row0 + r) * g.pos_row + g.axis[p]) * g.turns[p];
-    float s, c;
-    sincospif(2.f * (float)(t - rint(t)), &s, &c);
+#pragma unroll 1
+  for (int i = threadIdx.x; i < rows * g.table_row; i += kQkThreads) {
+    const int r = i / g.table_row, p = i - r * g.table_row;
+    float s = 0.f, c = 1.f;
+    if (p < g.P) {
+      const double t = qk_pos(g.pos, g.pos_dtype, (row0 + r) * g.pos_row + g.axis[p]) * g.turns[p];
+      sincospif(2.f * (float)(t - rint(t)), &s, &c);
+    }
     table[i] = make_float2(c, s);
   }
 }
@@ -180,166 +220,198 @@ __device__ __forceinline__ void qk_weights(const QkArgs<T>& g, float* weights) {
   }
 }
 
+// The heads of one tensor over the rows of a workgroup, a group of lanes' heads
+// one after another, `side` apart: 32-bit byte offsets from the workgroup's first
+// row that grow by the same amounts at each step (products and divisions are
+// quarter-rate, in 64 bits several of them).
+template <int STREAMS>
+struct QkWalk {
+  int row, h, table;
+  unsigned off[STREAMS];
+
+  template <typename T>
+  __device__ __forceinline__ void first(const QkArgs<T>& g, int w, int group, const int64_t (&strides)[STREAMS][2]) {
+    row = (int)(((float)group + 0.5f) * g.heads_inv[w]);
+    h = group - row * g.heads[w];
+    table = row * g.table_row;
+#pragma unroll
+    for (int i = 0; i < STREAMS; ++i) off[i] = ((unsigned)row * (unsigned)strides[i][0] + (unsigned)h * (unsigned)strides[i][1]) * (unsigned)sizeof(T);
+  }
+  template <typename T>
+  __device__ __forceinline__ void next(const QkArgs<T>& g, int w, const int64_t (&strides)[STREAMS][2]) {
+    h += g.step_h[w];
+    const bool wrap = h >= g.heads[w];
+    h -= wrap ? g.heads[w] : 0;
+    row += g.step_row[w] + wrap;
+    table += (wrap ? g.step_row[w] + 1 : g.step_row[w]) * g.table_row;
+#pragma unroll
+    for (int i = 0; i < STREAMS; ++i) {
+      const unsigned in_row = (unsigned)strides[i][0] * (unsigned)sizeof(T), in_head = (unsigned)strides[i][1] * (unsigned)sizeof(T);
+      const unsigned by = g.step_row[w] * in_row + g.step_h[w] * in_head, more = in_row - g.heads[w] * in_head;
+      off[i] += wrap ? by + more : by;
+    }
+  }
+};
+
 template <typename T, int V, int NV, bool INTERLEAVED>
 __global__ __launch_bounds__(kQkThreads) void qk_forward_kernel(QkArgs<T> g) {
   using Lane = QkLane<T, V, NV, INTERLEAVED>;
-  using Vec = typename Lane::Vec;
+  constexpr int M = Lane::M;
   __shared__ float2 table[kQkTable];
-  __shared__ __attribute__((aligned(16))) float weights[2 * ST_QK_MAX_DIM];
+  __shared__ __attribute__((aligned(32))) float weights[2 * ST_QK_MAX_DIM];
   const int64_t row0 = (int64_t)blockIdx.x * g.rows;
   const int rows = g.n - row0 < g.rows ? (int)(g.n - row0) : g.rows;
-  const int items = rows * g.all, side = kQkThreads >> g.lane_bits, group = threadIdx.x >> g.lane_bits;
+  const int side = kQkThreads >> g.lane_bits, group = threadIdx.x >> g.lane_bits;
   const Lane lane(g);
-  // (the loads of the first heads go out before the table is made, those of a batch before its first store)
-  Vec xa[kQkBatch][NV], xb[kQkBatch][NV];
-  T* out[kQkBatch];
-  int row[kQkBatch], which[kQkBatch];
-  bool there[kQkBatch];
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int u = 0; u < kQkBatch; ++u) {
-      const int i = i0 + u * side + group;
-      there[u] = i < items;
-      const int r = there[u] ? (int)((uint64_t)i * g.all_inv >> 32) : 0;
-      int h = there[u] ? i - r * g.all : 0;
-      row[u] = r;
-      which[u] = h >= g.heads[0];
-      h -= which[u] ? g.heads[0] : 0;
-      const T* in = which[u] ? g.in[1] + (row0 + r) * g.in_row[1] + h * g.in_head[1] : g.in[0] + (row0 + r) * g.in_row[0] + h * g.in_head[0];
-      out[u] = (which[u] ? g.out[1] : g.out[0]) + ((row0 + r) * (which[u] ? g.heads[1] : g.heads[0]) + h) * g.D;
-      lane.load(in, there[u], xa[u], xb[u]);
-    }
+  // q's heads, then k's, each in steps of a head a group of lanes; a head's loads go out while the one before it is at
+  // work, the first one's before the table is made
+  const int q_steps = (rows * g.heads[0] + side - 1) / side, steps = q_steps + (rows * g.heads[1] + side - 1) / side;
+  T next[M][V];
+  QkWalk<2> walk;
+  auto load = [&](int step) {
+    const int w = step >= q_steps;
+    const int64_t strides[2][2] = {{g.in_row[w], g.in_head[w]}, {(int64_t)g.heads[w] * g.D, g.D}};
+    if (step == 0 || step == q_steps)
+      walk.first(g, w, group, strides);
+    else
+      walk.next(g, w, strides);
+    lane.load(make_rsrc(g.in[w] + row0 * g.in_row[w], kOobOffset), walk.row < rows ? walk.off[0] : kOobOffset, next);
   };
   load(0);
   qk_table(g, row0, rows, table);
   qk_weights(g, weights);
   __syncthreads();
-  for (int i0 = 0; i0 < items; i0 += kQkBatch * side) {
-    if (i0) load(i0);
-    float sum[kQkBatch];
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    float x[M][V], sum[1] = {0.f};
 #pragma unroll
-    for (int u = 0; u < kQkBatch; ++u) {
-      sum[u] = 0.f;
+    for (int m = 0; m < M; ++m)
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
+      for (int e = 0; e < V; ++e) x[m][e] = (float)next[m][e];
+    const int w = step >= q_steps;
+    const bool live = walk.row < rows;
+    const unsigned to = live ? walk.off[1] : kOobOffset;
+    const float2* turns = table + (live ? walk.table : 0);
+    if (step + 1 < steps) load(step + 1);
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum[u] += (float)xa[u][k][e] * (float)xa[u][k][e] + (float)xb[u][k][e] * (float)xb[u][k][e];
-    }
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[0] += x[m][e] * x[m][e];
     qk_sum(sum, g.lanes);
+    const float s = rsqrtf(sum[0] * g.inv_d + g.eps);
 #pragma unroll
-    for (int u = 0; u < kQkBatch; ++u) {
-      const float s = 1.f / sqrtf(sum[u] * g.inv_d + g.eps);
-      float a[NV][V], b[NV][V];
-      lane.weights(weights + which[u] * ST_QK_MAX_DIM, a, b);
+    for (int m = 0; m < M; ++m) {
+      float wm[V];
+      lane.weights(weights + w * ST_QK_MAX_DIM, m, wm);
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) a[k][e] *= (float)xa[u][k][e] * s, b[k][e] *= (float)xb[u][k][e] * s;
-      lane.template turn<false>(table + row[u] * g.P, a, b);
-      lane.store(out[u], there[u], a, b);
+      for (int e = 0; e < V; ++e) x[m][e] *= wm[e] * s;
     }
+    lane.template turn<false>(turns, x);
+    lane.store(make_rsrc(g.out[w] + row0 * g.heads[w] * g.D, kOobOffset), to, x);
   }
 }
 
+// q's heads of all of a workgroup's rows, then k's: the sums of one weight's
+// gradient in registers at a time, for a second table.
 template <typename T, int V, int NV, bool INTERLEAVED>
 __global__ __launch_bounds__(kQkThreads) void qk_backward_kernel(QkArgs<T> g) {
   using Lane = QkLane<T, V, NV, INTERLEAVED>;
-  using Vec = typename Lane::Vec;
+  constexpr int M = Lane::M;
   __shared__ float2 table[kQkTable];
-  __shared__ __attribute__((aligned(16))) float weights[2 * ST_QK_MAX_DIM];
+  __shared__ __attribute__((aligned(32))) float weights[2 * ST_QK_MAX_DIM];
+  __shared__ float sums[3][ST_QK_MAX_DIM];
   const int side = kQkThreads >> g.lane_bits, group = threadIdx.x >> g.lane_bits;
   const Lane lane(g);
-  const int64_t per = (g.n + gridDim.x - 1) / gridDim.x, end = per * (blockIdx.x + 1) < g.n ? per * (blockIdx.x + 1) : g.n;
-  float da[2][NV][V], db[2][NV][V];
-#pragma unroll
-  for (int w = 0; w < 2; ++w)
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int e = 0; e < V; ++e) da[w][k][e] = db[w][k][e] = 0.f;
+  const int64_t first = g.per * blockIdx.x, end = first + g.per < g.n ? first + g.per : g.n;
   qk_weights(g, weights);
-  for (int64_t row0 = per * blockIdx.x; row0 < end; row0 += g.rows) {
-    const int rows = end - row0 < g.rows ? (int)(end - row0) : g.rows;
-    qk_table(g, row0, rows, table);
-    __syncthreads();
+#pragma unroll 1
+  for (int w = 0; w < 2; ++w) {
+    const int64_t strides[3][2] = {{g.in_row[w], g.in_head[w]}, {g.dy_row[w], g.dy_head[w]}, {(int64_t)g.heads[w] * g.D, g.D}};
+    float dw[M][V];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const int items = rows * g.heads[w];
-      for (int i0 = 0; i0 < items; i0 += side) {
-        const int i = i0 + group;
-        const bool there = i < items;
-        const int r = there ? (int)((uint64_t)i * g.heads_inv[w] >> 32) : 0, h = there ? i - r * g.heads[w] : 0;
-        Vec xa[NV], xb[NV], ga[NV], gb[NV];
-        lane.load(g.in[w] + (row0 + r) * g.in_row[w] + h * g.in_head[w], there, xa, xb);
-        lane.load(g.dy[w] + (row0 + r) * g.dy_row[w] + h * g.dy_head[w], there, ga, gb);
-        float a[NV][V], b[NV][V], wa[NV][V], wb[NV][V];
+    for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+      for (int e = 0; e < V; ++e) dw[m][e] = 0.f;
+    for (int64_t row0 = first; row0 < end && g.heads[w]; row0 += g.rows) {
+      const int rows = end - row0 < g.rows ? (int)(end - row0) : g.rows;
+      const int steps = (rows * g.heads[w] + side - 1) / side;
+      const auto in = make_rsrc(g.in[w] + row0 * g.in_row[w], kOobOffset);
+      const auto dy = make_rsrc(g.dy[w] + row0 * g.dy_row[w], kOobOffset);
+      const auto out = make_rsrc(g.out[w] + row0 * g.heads[w] * g.D, kOobOffset);
+      QkWalk<3> walk;
+      T next_x[M][V], next_g[M][V];
+      auto load = [&]() {
+        const bool live = walk.row < rows;
+        lane.load(in, live ? walk.off[0] : kOobOffset, next_x);
+        lane.load(dy, live ? walk.off[1] : kOobOffset, next_g);
+      };
+      walk.first(g, w, group, strides);
+      load();
+      qk_table(g, row0, rows, table);
+      __syncthreads();
+#pragma unroll 1
+      for (int step = 0; step < steps; ++step) {
+        float x[M][V], d[M][V], gw[M][V];
 #pragma unroll
-          for (int e = 0; e < V; ++e) a[k][e] = (float)ga[k][e], b[k][e] = (float)gb[k][e];
-        lane.template turn<true>(table + r * g.P, a, b);
-        lane.weights(weights + w * ST_QK_MAX_DIM, wa, wb);
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int e = 0; e < V; ++e) x[m][e] = (float)next_x[m][e], d[m][e] = (float)next_g[m][e];
+        const bool live = walk.row < rows;
+        const unsigned to = live ? walk.off[2] : kOobOffset;
+        const float2* turns = table + (live ? walk.table : 0);
+        walk.next(g, w, strides);
+        if (step + 1 < steps) load();
+        lane.template turn<true>(turns, d);
         float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int m = 0; m < M; ++m) {
+          lane.weights(weights + w * ST_QK_MAX_DIM, m, gw[m]);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float x = (float)xa[k][e], y = (float)xb[k][e];
-            wa[k][e] *= a[k][e], wb[k][e] *= b[k][e];
-            sum[0] += x * x + y * y;
-            sum[1] += wa[k][e] * x + wb[k][e] * y;
+            gw[m][e] *= d[m][e];
+            sum[0] += x[m][e] * x[m][e];
+            sum[1] += gw[m][e] * x[m][e];
           }
+        }
         qk_sum(sum, g.lanes);
-        const float s = there ? 1.f / sqrtf(sum[0] * g.inv_d + g.eps) : 0.f, c = sum[1] * g.inv_d * s * s;
+        const float s = live ? rsqrtf(sum[0] * g.inv_d + g.eps) : 0.f, c = sum[1] * g.inv_d * s * s;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int m = 0; m < M; ++m)
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float x = (float)xa[k][e], y = (float)xb[k][e];
-            da[w][k][e] += a[k][e] * x * s, db[w][k][e] += b[k][e] * y * s;
-            a[k][e] = s * (wa[k][e] - x * c), b[k][e] = s * (wb[k][e] - y * c);
+            dw[m][e] += d[m][e] * (x[m][e] * s);
+            d[m][e] = s * (gw[m][e] - x[m][e] * c);
           }
-        lane.store(g.out[w] + ((row0 + r) * g.heads[w] + h) * g.D, there, a, b);
+        lane.store(out, to, d);
       }
+      __syncthreads();
     }
+    if (!g.parts) continue;
+    // the heads side by side in a wave, then the four waves, in a fixed order
+    for (int o = g.lanes; o < 64; o *= 2)
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int e = 0; e < V; ++e) dw[m][e] += __shfl_xor(dw[m][e], o, 64);
+    const int wave = threadIdx.x >> 6;
+    const bool mine = (threadIdx.x & 63) < g.lanes;
+    float* part = g.parts + (int64_t)blockIdx.x * 2 * g.D + w * g.D;
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+      if (wave > 0 && mine && lane.has(m))
+#pragma unroll
+        for (int e = 0; e < V; ++e) sums[wave - 1][lane.w[m] + e] = dw[m][e];
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+      if (wave == 0 && mine && lane.has(m))
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int at = lane.w[m] + e;
+          part[at] = dw[m][e] + sums[0][at] + sums[1][at] + sums[2][at];
+        }
     __syncthreads();
   }
-  if (!g.parts) return;
-  // the heads side by side in a wave, then the four waves, in a fixed order; the table's room holds three waves' sums
-  static_assert(3 * 2 * ST_QK_MAX_DIM * sizeof(float) <= sizeof(table), "three waves' sums");
-  float* sums = reinterpret_cast<float*>(table);
-  const int wave = threadIdx.x >> 6;
-  const bool mine = (threadIdx.x & 63) < g.lanes;
-  float* out = g.parts + (int64_t)blockIdx.x * 2 * g.D;
-  auto each = [&](auto f) {
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          if (lane.live(k)) f(w * g.D + lane.at(k) + e, da[w][k][e]);
-          if (lane.second(k)) f(w * g.D + lane.at(k) + lane.partner() + e, db[w][k][e]);
-        }
-  };
-  for (int o = g.lanes; o < 64; o *= 2)
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          da[w][k][e] += __shfl_xor(da[w][k][e], o, 64);
-          db[w][k][e] += __shfl_xor(db[w][k][e], o, 64);
-        }
-  if (wave > 0 && mine) each([&](int at, float v) { sums[(wave - 1) * 2 * ST_QK_MAX_DIM + at] = v; });
-  __syncthreads();
-  if (wave == 0 && mine)
-    each([&](int at, float v) {
-#pragma unroll
-      for (int o = 0; o < 3; ++o) v += sums[o * 2 * ST_QK_MAX_DIM + at];
-      out[at] = v;
-    });
 }
 
 // ------------------------------------------------------------------ host
@@ -358,31 +430,44 @@ static bool qk_vec_ok(const QkArgs<T>& g, bool interleaved) {
 }
 
 // Rows whose table is in LDS at once.
-static int64_t qk_table_rows(int P) { return P ? kQkTable / P : kQkTable; }
+static int64_t qk_table_rows(int table_row) { return kQkTable / table_row; }
 
 // Workgroups of the backward: a row each while there are fewer than its limit.
 static int64_t qk_groups(int64_t n) { return n < kQkMaxGroups ? (n > 0 ? n : 1) : kQkMaxGroups; }
 
 template <typename T, int V, int NV, bool INTERLEAVED>
 static int qk_launch(QkArgs<T> g, bool backward, hipStream_t s) {
-  auto inv = [](int64_t d) { return d ? ((1ull << 32) + d - 1) / d : 0; };
-  g.all_inv = inv(g.all);
-  for (int w = 0; w < 2; ++w) g.heads_inv[w] = inv(g.heads[w]);
+  for (int w = 0; w < 2; ++w) {
+    const int d = g.heads[w], side = kQkThreads / g.lanes;
+    g.heads_inv[w] = d ? 1.f / (float)d : 0.f;
+    g.step_row[w] = d ? side / d : 0, g.step_h[w] = d ? side % d : 0;
+  }
+  // rows whose heads are within a 32-bit offset of the first
+  int64_t reach = 1ll << 31;
+  for (int w = 0; w < 2; ++w) {
+    if (!g.heads[w]) continue;
+    const int64_t row[3] = {g.in_row[w], backward ? g.dy_row[w] : 0, (int64_t)g.heads[w] * g.D};
+    const int64_t head[3] = {g.in_head[w], backward ? g.dy_head[w] : 0, g.D};
+    for (int i = 0; i < 3; ++i) {
+      const int64_t left = kQkReach / (int64_t)sizeof(T) - g.heads[w] * head[i];
+      if (left < row[i]) return ST_ERR_UNSUPPORTED;
+      if (row[i] && left / row[i] < reach) reach = left / row[i];
+    }
+  }
   if (backward) {
-    // rows of a table: what LDS holds, and i * heads within the inverse's reach
-    int64_t rows = qk_table_rows(g.P);
-    const int64_t most = g.heads[0] > g.heads[1] ? g.heads[0] : g.heads[1];
-    while (rows > 1 && rows * most * most >= (1ll << 32)) rows /= 2;
-    g.rows = (int)rows;
+    const int64_t rows = qk_table_rows(g.table_row);  // of a table
+    g.rows = (int)(reach < rows ? reach : rows);
+    g.per = (g.n + qk_groups(g.n) - 1) / qk_groups(g.n);
     qk_backward_kernel<T, V, NV, INTERLEAVED><<<(unsigned)qk_groups(g.n), kQkThreads, 0, s>>>(g);
     ST_CHECK_LAUNCH();
     return ST_OK;
   }
   // rows of a workgroup: what LDS and a few heads a lane hold, fewer while there are not 1024 workgroups
-  int64_t rows = qk_table_rows(g.P);
+  int64_t rows = qk_table_rows(g.table_row);
   const int64_t per_row = (int64_t)g.all * g.lanes;
   if (kQkItems / per_row < rows) rows = kQkItems / per_row;
   if (g.n / 1024 < rows) rows = g.n / 1024;
+  if (reach < rows) rows = reach;
   g.rows = rows > 0 ? (int)rows : 1;
   const int64_t n = g.n, most = st_most_blocks(kQkThreads) * g.rows;  // rows of a launch
   for (int64_t row = 0; row < n; row += most) {
@@ -402,14 +487,23 @@ static int qk_launch(QkArgs<T> g, bool backward, hipStream_t s) {
 
 template <typename T, int V>
 static int qk_vectors(QkArgs<T> g, bool interleaved, bool backward, hipStream_t s) {
+  g.table_row = g.P + (interleaved && V > 1 ? (g.D - 2 * g.P) / 2 : g.D - 2 * g.P);
   g.chunks = (interleaved && V > 1 ? 2 * g.P / V : g.P / V) + (g.D - 2 * g.P) / V;
-  g.lanes = 1, g.lane_bits = 0;
-  while (g.lanes < g.chunks && g.lanes < 64) g.lanes *= 2, ++g.lane_bits;
-  if (g.chunks <= 64)
-    return interleaved ? qk_launch<T, V, 1, true>(g, backward, s) : qk_launch<T, V, 1, false>(g, backward, s);
-  if constexpr (ST_QK_MAX_DIM / V > 64)  // (heads longer than 64 vectors)
-    return interleaved ? qk_launch<T, V, ST_QK_MAX_DIM / V / 64, true>(g, backward, s)
-                       : qk_launch<T, V, ST_QK_MAX_DIM / V / 64, false>(g, backward, s);
+  // Vectors side by side of a lane: two where both channels of a pair are in one, as many bytes as with two of them.
+  auto lanes = [&](int nv) {
+    g.lanes = 1, g.lane_bits = 0;
+    while (g.lanes * nv < g.chunks) g.lanes *= 2, ++g.lane_bits;
+    return g.lanes <= 64;
+  };
+  if constexpr (V > 1) {
+    if (interleaved) return lanes(2) ? qk_launch<T, V, 2, true>(g, backward, s) : ST_ERR_UNSUPPORTED;
+  }
+  if (lanes(1)) return interleaved ? qk_launch<T, V, 1, true>(g, backward, s) : qk_launch<T, V, 1, false>(g, backward, s);
+  if constexpr (ST_QK_MAX_DIM / V > 64) {  // (heads longer than 64 vectors)
+    constexpr int NV = ST_QK_MAX_DIM / V / 64;
+    lanes(NV);
+    return interleaved ? qk_launch<T, V, NV, true>(g, backward, s) : qk_launch<T, V, NV, false>(g, backward, s);
+  }
   return ST_ERR_UNSUPPORTED;
 }
 
@@ -465,6 +559,8 @@ static int qk_check(const st_qk_norm_args* a, bool backward) {
       (a->k && (kv_heads == 0 || !(backward ? a->dk : a->k_out))))
     return ST_ERR_ARG;
   if (backward && ((a->q && !a->dq_out) || (a->k && !a->dk_out))) return ST_ERR_ARG;
+  for (int64_t stride : {a->q_row, a->q_head, a->k_row, a->k_head, a->dq_row, a->dq_head, a->dk_row, a->dk_head})
+    if (stride < 0 || stride >= (1ll << 31)) return ST_ERR_UNSUPPORTED;
   if (a->pairs && (!a->positions || !a->turns || !a->axis)) return ST_ERR_ARG;
   return ST_OK;
 }
