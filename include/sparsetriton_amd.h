@@ -939,7 +939,9 @@ int st_qk_norm_rotary_backward(const st_qk_norm_args* args, st_stream_t stream);
  * ST_ATTN_MAX_DIM.  dtype: ST_F32, ST_F16, ST_BF16.  scale > 0.
  * key_mask (key rows; NULL = all): 0 leaves a key out, whatever its row of K and
  * V holds; its gradients are zero.  causal: the segment's query i of nq sees keys
- * up to i + nk - nq.
+ * up to i + nk - nq, its place.  window > 0: of those only the keys less than
+ * `window` from its place (without causal: on both sides of it) and the segment's
+ * first `sinks` keys.
  *
  * The caller lays the work out (int32, device memory).  Packed row r of a
  * segment is its query r / g at head r % g of the key head's group, g = heads /
@@ -949,7 +951,11 @@ int st_qk_norm_rotary_backward(const st_qk_norm_args* args, st_stream_t stream);
  * keys that any of its rows sees, or in parts, in ascending slots of its own;
  * then q_joins: ST_ATTN_JOIN_WORDS each, {the first five words, first slot,
  * parts, 0} for every tile in parts.  k_items, k_joins likewise with tiles of
- * keys and ranges of packed rows (every row that sees a key of the tile).
+ * keys and ranges of packed rows (every row that sees a key of the tile).  With a
+ * window the keys of a q_item are places in a list: where the first key that a
+ * window of the tile's rows covers, f = max(0, place of its first row - window + 1),
+ * lies behind h = sinks rounded up to 64, places below h are the keys of that number and
+ * a place p from h on is key p + f - h; parts begin at multiples of 64 places.
  * parts: fp32 workspace, 16-byte address, st_attn_workspace floats for the
  * slots used.  lse (rows, heads) fp32, base-2 logarithm, INFINITY for a row
  * without keys: written when not NULL, needed by the backward; o_rest (as o; NULL =
@@ -988,6 +994,7 @@ typedef struct st_attn_args {
   int32_t q_tile, k_tile; /* ST_ATTN_TILE, or ST_ATTN_SMALL_TILE for segments of few rows (keys) */
   int32_t q_item_major, k_item_major; /* order of the work: 0 a key head's items, 1 an item's key heads */
   float scale;
+  int32_t window, sinks; /* window 0: none (and no sinks) */
 } st_attn_args;
 int st_attn_workspace(int kv_heads, int dim, int64_t q_parts, int64_t k_parts, int64_t* floats);
 int st_attn_forward(const st_attn_args* args, st_stream_t stream);

@@ -97,6 +97,7 @@ class AttnArgs(ctypes.Structure):
         + [("parts", _P)]
         + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "dtype", "causal", "q_tile", "k_tile", "q_item_major", "k_item_major")]
         + [("scale", ctypes.c_float)]
+        + [(n, ctypes.c_int32) for n in ("window", "sinks")]
     )
 
 

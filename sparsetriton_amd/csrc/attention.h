@@ -52,7 +52,7 @@ struct AttnItem {  // ST_ATTN_ITEM_WORDS int32, written by the host
   int q0, nq;      // the segment's first query row and their number
   int k0, nk;      // its first key row and their number
   int row0;        // first packed row (first key) of this tile in the segment
-  int lo, hi;      // keys (packed rows) to go over
+  int lo, hi;      // keys (packed rows) to go over; with a window, places in the tile's list of keys (AttnWindow)
   int part;        // slot of the partial result, -1: the result itself
 };
 struct AttnJoin {  // ST_ATTN_JOIN_WORDS int32
@@ -83,6 +83,7 @@ struct AttnArgs {
   int n_items, n_joins;
   AttnDivisor by_items, by_kv_heads, by_group;
   int heads, kv_heads, group, D, causal;
+  int window, sinks;  // window 0: none
   int tile;        // rows of the items' tiles: ST_ATTN_TILE or ST_ATTN_SMALL_TILE
   int item_major;  // workgroups take an item's key heads in turn, else a key head's items
   float scale, scale_log2;  // c and c / ln 2
@@ -192,9 +193,9 @@ struct AttnTile {
   }
 };
 
-// A product over the rows of a tile that the causal order cuts: the other
+// A product over the rows of a tile that the causal order or a window cuts: the other
 // operand is zero where a column must not see a row, but zero times an infinity
-// or a NaN is a NaN, so a later row that is not finite would reach earlier ones.
+// or a NaN is a NaN, so a row that is not finite would reach those that do not see it.
 // Such a tile (one check of it, by each wave that the order cuts it for) is
 // copied without those elements, the product taken over the copy, and what they
 // do to the columns that see them added at the end.
@@ -223,7 +224,7 @@ __device__ __forceinline__ void attn_copy_finite(const T* tile, T* copy) {
 struct AttnNotFinite {
   uint64_t pos = 0, neg = 0;
   template <typename T, int ROWS, int DP>
-  __device__ __forceinline__ void add(const T* tile, int first, int last) {  // rows first .. last
+  __device__ __forceinline__ void add(const T* tile, uint64_t rows) {  // a bit for each row that the lane's column sees
     using Tile = AttnTile<T, DP>;
     const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll 1
@@ -232,7 +233,7 @@ struct AttnNotFinite {
       for (int r = 0; r < DP / 2; ++r) {
         const int d = (r >> 4) * 32 + reg_row(r & 15, half);
         const float x = (float)tile[Tile::at(row, d / Tile::EPC) + d % Tile::EPC];
-        const bool seen = row >= first && row <= last && !(fabsf(x) < INFINITY);
+        const bool seen = (rows >> row & 1) && !(fabsf(x) < INFINITY);
         pos |= (uint64_t)(seen && x != -INFINITY) << r;
         neg |= (uint64_t)(seen && x != INFINITY) << r;
       }
@@ -382,6 +383,65 @@ __device__ __forceinline__ AttnItem attn_item(const AttnArgs& a, int& hk) {
   return a.items[w - hk * a.n_items];
 }
 
+// Which keys a row sees (a template argument: the kernels of one do not pay for another's).
+constexpr int kAttnAll = 0, kAttnCausal = 1, kAttnWindow = 2;
+
+// The lowest n bits of 64.
+__device__ __forceinline__ uint64_t attn_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : ~0ull >> (64 - n); }
+
+// The keys of a tile of rows with a window, in steps: where those that the rows'
+// windows cover begin behind the first keys (the sinks, in whole steps of 64), a
+// list of both, without the keys between them: places below `head` are the keys
+// themselves, the others `gap` keys further.  Uniform in a workgroup.
+struct AttnWindow {
+  int head = 0, gap = 0, sinks = 0;
+  __device__ __forceinline__ AttnWindow(const AttnArgs& a, const AttnItem& it, int first) {
+    const int w = a.window - 1, at = first + it.nk - it.nq;  // (place of the tile's first row)
+    sinks = a.sinks;
+    head = (a.sinks + 63) & ~63;
+    gap = max(max(at, w) - w - head, 0);
+  }
+  __device__ __forceinline__ int key(int kt) const { return kt >= head ? kt + gap : kt; }
+  __device__ __forceinline__ int end(int kt, int hi) const { return gap && kt < head ? min(hi, sinks) : hi; }
+  // the step after this one (what the sinks leave of their last 64 is passed over)
+  __device__ __forceinline__ int next(int kt, int step) const {
+    const int n = kt + step;
+    return gap && n >= sinks && n < head ? head : n;
+  }
+};
+// Keys that a lane's row sees: from .. last, and those below `sinks`.
+template <int ORDER>
+struct AttnSight {
+  int last = 0x7FFFFFFE, from = 0, sinks = 0;
+  __device__ __forceinline__ AttnSight(const AttnArgs& a, const AttnItem& it, int qi, bool live) {
+    const int at = qi + it.nk - it.nq;
+    if constexpr (ORDER == kAttnCausal) last = at;
+    if (ORDER == kAttnWindow && live) {  // (no sum passes 2^31)
+      const int w = a.window - 1;
+      last = a.causal ? at : min(at, it.nk - 1 - w) + w;
+      from = max(at, w) - w;
+      sinks = a.causal ? min(a.sinks, at + 1) : a.sinks;
+    }
+  }
+  // any of the keys k .. k + n - 1
+  __device__ __forceinline__ bool any(int k, int n) const {
+    if constexpr (ORDER == kAttnWindow) return k < sinks || (k <= last && k + n > from);
+    return k <= last;
+  }
+  // all of them
+  __device__ __forceinline__ bool all(int k, int n) const {
+    if constexpr (ORDER == kAttnWindow) return (from <= k && last - k >= n - 1) || k + n <= sinks;
+    return last - k >= n - 1;
+  }
+  // a bit for each key from k on, of those that `seen` has
+  __device__ __forceinline__ uint64_t keep(int k, uint64_t seen) const {
+    const int to = last - k;
+    if constexpr (ORDER == kAttnWindow)
+      return seen & (attn_below(sinks - k) | (attn_below(to + 1) & ~attn_below(from - k)));
+    return to >= 63 ? seen : to < 0 ? 0 : seen & ((2ull << to) - 1);
+  }
+};
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // For the scheduler: of N fragment reads, each followed by its MFMAs, kAhead
@@ -441,8 +501,8 @@ constexpr int attn_keys() {
 }
 
 template <typename T, int DP, int WAVES>
-constexpr int attn_fwd_lds(bool causal) {  // two buffers of K and V; causal, a copy of one of them, else two of the keys' terms
-  return attn_keys<WAVES>() * (causal ? 5 * DP * (int)sizeof(T) : 4 * DP * (int)sizeof(T) + 2 * (int)sizeof(float));
+constexpr int attn_fwd_lds(bool cut) {  // two buffers of K and V; cut, a copy of one of them, else two of the keys' terms
+  return attn_keys<WAVES>() * (cut ? 5 * DP * (int)sizeof(T) : 4 * DP * (int)sizeof(T) + 2 * (int)sizeof(float));
 }
 
 // A running maximum is raised only when a row's maximum passes it by more
@@ -502,8 +562,9 @@ struct AttnPower {
   }
 };
 
-template <typename T, int DP, bool CAUSAL, int WAVES>
+template <typename T, int DP, int ORDER, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forward_kernel(AttnArgs a) {
+  constexpr bool CUT = ORDER != kAttnAll;  // some rows do not see some keys
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
   constexpr int BK = attn_keys<WAVES>();
@@ -512,7 +573,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
   constexpr int TILE = BK * DP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
-  float* bias = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers, not CAUSAL: 0 or -inf for each key of a step
+  float* bias = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers, not CUT: 0 or -inf for each key of a step
 
   int hk;
   const AttnItem it = attn_item(a, hk);
@@ -529,20 +590,23 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = load_row8<T>(base, off, 16 * s + 8 * half, a.D, live);
   }
-  const int see = CAUSAL ? qi + it.nk - it.nq : 0x7FFFFFFF;  // last key that this lane's row sees
+  const AttnSight<ORDER> sight(a, it, qi, live);
+  const AttnWindow list(a, it, first);
 
   Stage ks, vs;
   ks.place(a.D, [&](int x) { return x * (int)(a.k_row * sizeof(T)); });
   vs.place(a.D, [&](int x) { return x * (int)(a.v_row * sizeof(T)); });
   uint8_t chunk_kept[Stage::N], key_kept = 1;
   const uint8_t* mask = a.key_mask ? a.key_mask + it.k0 : nullptr;
+  auto key_at = [&](int kt) { return ORDER == kAttnWindow ? list.key(kt) : kt; };
+  auto end_at = [&](int kt) { return ORDER == kAttnWindow ? list.end(kt, it.hi) : it.hi; };
   auto fetch = [&](int kt) {
-    const int left = it.hi - kt;
-    const int64_t row = it.k0 + (int64_t)kt;
+    const int left = end_at(kt) - kt, key = key_at(kt);
+    const int64_t row = it.k0 + (int64_t)key;
     if (mask) {
 #pragma unroll
-      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[kt + Stage::row(i)] : 0;
-      key_kept = lane < left ? mask[kt + lane] : 0;
+      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[key + Stage::row(i)] : 0;
+      key_kept = lane < left ? mask[key + lane] : 0;
     }
     ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, left);
     vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, left);
@@ -554,24 +618,26 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
   float m = -INFINITY, l = 0.f;
   AttnNotFinite left_out;
   if (it.lo < it.hi) fetch(it.lo);
-  for (int kt = it.lo, buf = 0; kt < it.hi; kt += BK, buf ^= 1) {
+  for (int kt = it.lo, next, buf = 0; kt < it.hi; kt = next, buf ^= 1) {
+    next = ORDER == kAttnWindow ? list.next(kt, BK) : kt + BK;
+    const int left = end_at(kt) - kt, key = key_at(kt);
     T* kl = tiles + buf * 2 * TILE;
     T* vl = kl + TILE;
     constexpr uint64_t ALL = ~0ull >> (64 - BK);
     uint64_t seen = ALL;  // keys of this step that exist and are not masked
-    if (it.hi - kt < BK) seen >>= BK - (it.hi - kt);
+    if (left < BK) seen >>= BK - left;
     if (mask) {
       seen &= __ballot(key_kept);
 #pragma unroll
       for (int i = 0; i < Stage::N; ++i)  // (whatever a masked row holds, not finite included, stays out of the products)
         if (!chunk_kept[i]) ks.reg[i] = vs.reg[i] = (v4u)(0u);
     }
-    if (!CAUSAL && seen != ALL && threadIdx.x < BK) bias[buf * BK + lane] = seen >> lane & 1 ? 0.f : -INFINITY;
+    if (!CUT && seen != ALL && threadIdx.x < BK) bias[buf * BK + lane] = seen >> lane & 1 ? 0.f : -INFINITY;
     ks.store(kl);
     vs.store(vl);
     __syncthreads();
-    if (kt + BK < it.hi) fetch(kt + BK);
-    if (!active || (CAUSAL && !__any(live && kt <= see))) continue;
+    if (next < it.hi) fetch(next);
+    if (!active || (CUT && !__any(live && sight.any(key, BK)))) continue;
 
     v16f s[NB];
     auto scores = [&]() {
@@ -581,7 +647,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
         for (int b = 0; b < NB; ++b) s[b] = mma32(Tile::rows(kl, b * 32 + (lane & 31), 16 * i + 8 * half), qf[i], s[b]);
       attn_reads_ahead<T, NB * KS>();
     };
-    if (!CAUSAL && seen != ALL) {  // the sums begin at -inf for keys that are left out (their K is zeros)
+    if (!CUT && seen != ALL) {  // the sums begin at -inf for keys that are left out (their K is zeros)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -596,10 +662,9 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
       for (int b = 0; b < NB; ++b) s[b] = (v16f)(0.f);
       scores();
     }
-    const bool cut = CAUSAL && __any(see - kt < BK - 1);  // by the causal order
-    const int last = see - kt;
-    const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
-    if (CAUSAL && (cut || seen != ALL)) {
+    const bool cut = CUT && __any(!sight.all(key, BK));  // by the causal order or the window
+    const uint64_t keep = CUT ? sight.keep(key, seen) : seen;
+    if (CUT && (cut || seen != ALL)) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
@@ -639,7 +704,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
     if (cut && attn_not_finite<T, BK, DP>(vl)) {
       attn_copy_finite<T, BK, DP>(vl, tiles + 4 * TILE);
       vp = tiles + 4 * TILE;
-      left_out.add<T, BK, DP>(vl, 0, last);
+      left_out.add<T, BK, DP>(vl, keep);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -652,7 +717,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
     attn_reads_ahead<T, NB * 2 * DB, true>();
   }
 
-  if (CAUSAL) left_out.apply(o);
+  if (CUT) left_out.apply(o);
   l += other_half(l);
   m -= kAttnUp<T>;
   if (it.part >= 0) {
@@ -763,8 +828,8 @@ constexpr int attn_dq_keys() {
   return WAVES == 4 && sizeof(T) == 2 && DP == 128 ? 32 : attn_keys<WAVES>();
 }
 template <typename T, int DP, int WAVES>
-constexpr int attn_dq_lds(bool causal) {
-  return attn_dq_keys<T, DP, WAVES>() * (causal ? 5 : 4) * DP * (int)sizeof(T);
+constexpr int attn_dq_lds(bool cut) {
+  return attn_dq_keys<T, DP, WAVES>() * (cut ? 5 : 4) * DP * (int)sizeof(T);
 }
 
 // dQ of a tile of rows, and delta = rowsum(dO o O) for the keys' pass after it:
@@ -775,8 +840,9 @@ constexpr int attn_dq_lds(bool causal) {
 //
 // As the forward's sizes: 64 channels bf16 272 us (760 TFLOP/s, MFMA busy 44 %, vector
 // unit 62: 107 instructions a tile), 128 channels causal 453 us (910, 47 %), fp32 114 us (76, 61 %).
-template <typename T, int DP, bool CAUSAL, int WAVES>
+template <typename T, int DP, int ORDER, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_kernel(AttnArgs a) {
+  constexpr bool CUT = ORDER != kAttnAll;  // some rows do not see some keys
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
   constexpr int BK = attn_dq_keys<T, DP, WAVES>();
@@ -818,20 +884,23 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
       if (half == 0) a.delta[at] = delta;
     }
   }
-  const int see = CAUSAL ? qi + it.nk - it.nq : 0x7FFFFFFF;
+  const AttnSight<ORDER> sight(a, it, qi, live);
+  const AttnWindow list(a, it, first);
 
   Stage ks, vs;
   ks.place(a.D, [&](int x) { return x * (int)(a.k_row * sizeof(T)); });
   vs.place(a.D, [&](int x) { return x * (int)(a.v_row * sizeof(T)); });
   uint8_t chunk_kept[Stage::N], key_kept = 1;
   const uint8_t* mask = a.key_mask ? a.key_mask + it.k0 : nullptr;
+  auto key_at = [&](int kt) { return ORDER == kAttnWindow ? list.key(kt) : kt; };
+  auto end_at = [&](int kt) { return ORDER == kAttnWindow ? list.end(kt, it.hi) : it.hi; };
   auto fetch = [&](int kt) {
-    const int left = it.hi - kt;
-    const int64_t row = it.k0 + (int64_t)kt;
+    const int left = end_at(kt) - kt, key = key_at(kt);
+    const int64_t row = it.k0 + (int64_t)key;
     if (mask) {
 #pragma unroll
-      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[kt + Stage::row(i)] : 0;
-      key_kept = lane < left ? mask[kt + lane] : 0;
+      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[key + Stage::row(i)] : 0;
+      key_kept = lane < left ? mask[key + lane] : 0;
     }
     ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, left);
     vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, left);
@@ -842,12 +911,14 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
   for (int b = 0; b < DB; ++b) dq[b] = (v16f)(0.f);
   AttnPower power;
   if (it.lo < it.hi) fetch(it.lo);
-  for (int kt = it.lo, buf = 0; kt < it.hi; kt += BK, buf ^= 1) {
+  for (int kt = it.lo, next, buf = 0; kt < it.hi; kt = next, buf ^= 1) {
+    next = ORDER == kAttnWindow ? list.next(kt, BK) : kt + BK;
+    const int left = end_at(kt) - kt, key = key_at(kt);
     T* kl = tiles + buf * 2 * TILE;
     T* vl = kl + TILE;
     constexpr uint64_t ALL = ~0ull >> (64 - BK);
     uint64_t seen = ALL;
-    if (it.hi - kt < BK) seen >>= BK - (it.hi - kt);
+    if (left < BK) seen >>= BK - left;
     if (mask) {
       seen &= __ballot(key_kept);
 #pragma unroll
@@ -857,11 +928,10 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
     ks.store(kl);
     vs.store(vl);
     __syncthreads();
-    if (kt + BK < it.hi) fetch(kt + BK);
-    if (!active || (CAUSAL && !__any(live && kt <= see))) continue;
-    const bool cut = CAUSAL && __any(see - kt < BK - 1);
-    const int last = see - kt;
-    const uint64_t keep = last >= 63 ? seen : last < 0 ? 0 : seen & ((2ull << last) - 1);
+    if (next < it.hi) fetch(next);
+    if (!active || (CUT && !__any(live && sight.any(key, BK)))) continue;
+    const bool cut = CUT && __any(!sight.all(key, BK));
+    const uint64_t keep = CUT ? sight.keep(key, seen) : seen;
     const T* kp = kl;  // (a row that sees a key that is not finite has a dS that is not)
     if (cut && attn_not_finite<T, BK, DP>(kl)) {
       attn_copy_finite<T, BK, DP>(kl, tiles + 4 * TILE);
@@ -914,8 +984,8 @@ constexpr int attn_q_rows() {  // packed rows of a step
   return DP * (int)sizeof(T) <= 192 ? 64 : 32;
 }
 template <typename T, int DP, int WAVES>
-constexpr int attn_dkv_lds(bool causal) {
-  return attn_q_rows<T, DP, WAVES>() * ((causal ? 6 : 4) * DP * (int)sizeof(T) + 4 * 4);
+constexpr int attn_dkv_lds(bool cut) {
+  return attn_q_rows<T, DP, WAVES>() * ((cut ? 6 : 4) * DP * (int)sizeof(T) + 4 * 4);
 }
 
 // dK and dV of a tile of keys: the waves hold 32 keys each (K, V and both sums in
@@ -937,9 +1007,10 @@ constexpr bool attn_dkv_apart() {
   return sizeof(T) == 2 && DP > 96;
 }
 
-template <typename T, int DP, bool CAUSAL, int WAVES, int WHAT>
+template <typename T, int DP, int ORDER, int WAVES, int WHAT>
 __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_waves<T, DP * 3 / 2>() : attn_waves<T, DP>()))
     void attn_dkv_kernel(AttnArgs a) {
+  constexpr bool CUT = ORDER != kAttnAll;  // some rows do not see some keys
   constexpr bool DV = WHAT & kAttnDv, DK = WHAT & kAttnDk;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
@@ -950,7 +1021,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
   float* stats = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers of BQ L, BQ delta
-  T* copies = reinterpret_cast<T*>(stats + 4 * BQ);           // CAUSAL: of a Q and a dO tile
+  T* copies = reinterpret_cast<T*>(stats + 4 * BQ);           // CUT: of a Q and a dO tile
 
   int hk;
   const AttnItem it = attn_item(a, hk);
@@ -969,8 +1040,22 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
     if constexpr (DK) vf[s] = load_row8<T>(vrows, (key - it.row0) * (int)(a.v_row * sizeof(T)), 16 * s + 8 * half, a.D, kept);
   }
   // first packed row that sees this lane's key, and the first that sees any of the wave's
-  const int from = CAUSAL ? max(key - (it.nk - it.nq), 0) * a.group : 0;
-  const int wave_from = CAUSAL ? max(kw - (it.nk - it.nq), 0) * a.group : 0;
+  // (with a window also the one behind the last: where that is the segment's last row, none)
+  auto first_query = [&](int k) {
+    if constexpr (ORDER == kAttnAll) return 0;
+    const int i = k - (it.nk - it.nq), w = a.window - 1;
+    if (ORDER == kAttnCausal || a.causal) return max(i, 0);
+    return k < a.sinks ? 0 : max(i, w) - w;
+  };
+  auto end_row = [&](int k) {
+    const int i = k - (it.nk - it.nq);
+    return k < a.sinks || i >= it.nq - a.window ? 0x7FFFFFFF : max(i + a.window, 0) * a.group;
+  };
+  const bool windowed = ORDER == kAttnWindow;
+  const int from = windowed && !live ? 0 : first_query(key) * a.group;
+  const int wave_from = first_query(kw) * a.group;
+  const int to = windowed && live ? end_row(key) : 0x7FFFFFFF;
+  const int wave_to = windowed ? max(end_row(kw), end_row(min(kw + 31, it.nk - 1))) : 0x7FFFFFFF;
 
   Stage qs, gs;
   float stat = 0.f;
@@ -1018,14 +1103,15 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
     if (threadIdx.x < 2 * BQ) st[threadIdx.x] = stat;
     __syncthreads();
     if (rt + BQ < it.hi) fetch(rt + BQ);
-    if (!active || rt + BQ <= wave_from) continue;
-    const bool cut = CAUSAL && __any(from > rt);
+    if (!active || rt + BQ <= wave_from || (windowed && rt >= wave_to)) continue;
+    const bool cut = CUT && __any(from > rt || (windowed && to - rt < BQ));
+    auto sees = [&](int row) { return row >= from && (!windowed || row < to); };
     const T *qp = ql, *gp = gl;  // (a row whose Q or dO is not finite has a delta, and so a dS, that is not)
     if (cut && ((DK && attn_not_finite<T, BQ, DP>(ql)) || (DV && attn_not_finite<T, BQ, DP>(gl)))) {
       if constexpr (DK) attn_copy_finite<T, BQ, DP>(ql, copies);
       if constexpr (DV) attn_copy_finite<T, BQ, DP>(gl, copies + TILE);
       qp = copies, gp = copies + TILE;
-      if constexpr (DV) left_out.add<T, BQ, DP>(gl, from - rt, BQ);
+      if constexpr (DV) left_out.add<T, BQ, DP>(gl, ~attn_below(from - rt) & (windowed ? attn_below(to - rt) : ~0ull));
     }
 #pragma unroll 1
     for (int b = 0; b < NB; ++b) {
@@ -1047,7 +1133,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
       }
       if (cut) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = rt + b * 32 + reg_row(e, half) >= from ? s[e] : 0.f;
+        for (int e = 0; e < 16; ++e) s[e] = sees(rt + b * 32 + reg_row(e, half)) ? s[e] : 0.f;
       }
       if constexpr (DV) {
 #pragma unroll
@@ -1067,7 +1153,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
       }
       if (cut) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = rt + b * 32 + reg_row(e, half) >= from ? s[e] : 0.f;
+        for (int e = 0; e < 16; ++e) s[e] = sees(rt + b * 32 + reg_row(e, half)) ? s[e] : 0.f;
       }
       if constexpr (kAttnHeld<T>) {
         s *= power.up;
@@ -1084,7 +1170,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
     }
   }
 
-  if constexpr (CAUSAL && DV) left_out.apply(dv);
+  if constexpr (CUT && DV) left_out.apply(dv);
   if constexpr (DK && kAttnHeld<T>) power.release<DB>(dk);
   if (!kept) {  // a masked key gets no gradient
 #pragma unroll
@@ -1178,24 +1264,24 @@ static int attn_join(K kernel, const AttnArgs& a, hipStream_t s) {
   return ST_OK;
 }
 
+template <typename T, int DP, int ORDER, int WAVES>
+static int attn_order(AttnPass pass, const AttnArgs& a, hipStream_t s) {
+  auto run = [&](auto kernel, int lds) { return attn_launch(kernel, 64 * WAVES, lds, a, s); };
+  constexpr bool CUT = ORDER != kAttnAll;
+  if (pass == kAttnForward) return run(attn_forward_kernel<T, DP, ORDER, WAVES>, attn_fwd_lds<T, DP, WAVES>(CUT));
+  if (pass == kAttnDq) return run(attn_dq_kernel<T, DP, ORDER, WAVES>, attn_dq_lds<T, DP, WAVES>(CUT));
+  const int lds = attn_dkv_lds<T, DP, WAVES>(CUT);
+  if constexpr (attn_dkv_apart<T, DP>()) {
+    const int rc = run(attn_dkv_kernel<T, DP, ORDER, WAVES, kAttnDv>, lds);
+    return rc != ST_OK ? rc : run(attn_dkv_kernel<T, DP, ORDER, WAVES, kAttnDk>, lds);
+  } else {
+    return run(attn_dkv_kernel<T, DP, ORDER, WAVES, kAttnDv | kAttnDk>, lds);
+  }
+}
 template <typename T, int DP, int WAVES>
 static int attn_pass(AttnPass pass, const AttnArgs& a, hipStream_t s) {
-  auto run = [&](auto kernel, int lds) { return attn_launch(kernel, 64 * WAVES, lds, a, s); };
-  if (pass == kAttnForward)
-    return run(a.causal ? attn_forward_kernel<T, DP, true, WAVES> : attn_forward_kernel<T, DP, false, WAVES>,
-               attn_fwd_lds<T, DP, WAVES>(a.causal));
-  if (pass == kAttnDq)
-    return run(a.causal ? attn_dq_kernel<T, DP, true, WAVES> : attn_dq_kernel<T, DP, false, WAVES>,
-               attn_dq_lds<T, DP, WAVES>(a.causal));
-  const int lds = attn_dkv_lds<T, DP, WAVES>(a.causal);
-  if constexpr (attn_dkv_apart<T, DP>()) {
-    const int rc = run(a.causal ? attn_dkv_kernel<T, DP, true, WAVES, kAttnDv> : attn_dkv_kernel<T, DP, false, WAVES, kAttnDv>, lds);
-    if (rc != ST_OK) return rc;
-    return run(a.causal ? attn_dkv_kernel<T, DP, true, WAVES, kAttnDk> : attn_dkv_kernel<T, DP, false, WAVES, kAttnDk>, lds);
-  } else {
-    constexpr int BOTH = kAttnDv | kAttnDk;
-    return run(a.causal ? attn_dkv_kernel<T, DP, true, WAVES, BOTH> : attn_dkv_kernel<T, DP, false, WAVES, BOTH>, lds);
-  }
+  if (a.window) return attn_order<T, DP, kAttnWindow, WAVES>(pass, a, s);
+  return a.causal ? attn_order<T, DP, kAttnCausal, WAVES>(pass, a, s) : attn_order<T, DP, kAttnAll, WAVES>(pass, a, s);
 }
 template <typename T, int DP>
 static int attn_dp(AttnPass pass, const AttnArgs& a, hipStream_t s) {

@@ -6,6 +6,7 @@ static int attn_check(const st_attn_args* a) {
   if (!a || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || a->dim <= 0) return ST_ERR_ARG;
   if (a->dim % 8 || a->dim > ST_ATTN_MAX_DIM) return ST_ERR_UNSUPPORTED;
   if (a->dtype != ST_F32 && a->dtype != ST_F16 && a->dtype != ST_BF16) return ST_ERR_UNSUPPORTED;
+  if (a->window < 0 || a->sinks < 0 || (a->sinks && !a->window)) return ST_ERR_ARG;
   if (!(a->scale > 0.f) || !(a->scale < 3.0e38f)) return ST_ERR_ARG;
   for (int tile : {a->q_tile, a->k_tile})
     if (tile != ST_ATTN_TILE && tile != ST_ATTN_SMALL_TILE) return ST_ERR_ARG;
@@ -33,6 +34,7 @@ static st::AttnArgs attn_args(const st_attn_args* a) {
   g.by_kv_heads = st::attn_divisor(a->kv_heads), g.by_group = st::attn_divisor(a->heads / a->kv_heads);
   g.heads = a->heads, g.kv_heads = a->kv_heads, g.group = a->heads / a->kv_heads;
   g.D = a->dim, g.causal = a->causal != 0;
+  g.window = a->window, g.sinks = a->sinks;
   g.scale = a->scale;
   g.scale_log2 = a->scale * 1.44269504088896341f;
   return g;

@@ -7,6 +7,7 @@ lengths and the tile lists that the kernels walk.
 
 import ctypes
 import math
+import operator
 from typing import Optional, Sequence, Union
 
 import numpy as np
@@ -176,6 +177,7 @@ class AttentionSegments:
             raise ValueError(f"{self._nq.size} segments of queries, {self._nk.size} of keys")
         self._q0, self._k0 = (np.cumsum(n) - n for n in (self._nq, self._nk))
         self.count, self.q_rows, self.k_rows = self._nq.size, int(self._nq.sum()), int(self._nk.sum())
+        self._most_q, self._most_k = (int(n.max(initial=0)) for n in (self._nq, self._nk))
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None and torch.cuda.is_available():
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -213,27 +215,49 @@ class AttentionSegments:
         seg = np.repeat(np.arange(n.size), n)
         return tile, seg, (np.arange(seg.size) - np.repeat(np.cumsum(n) - n, n)) * tile
 
-    def _plan(self, which: str, group: int, kv_heads: int, causal: bool, row_bytes: int, elem: int = 2) -> _Tiles:
+    def _window(self, causal: bool, window: Optional[int], sinks: int):
+        """(window, sinks) as the kernels take them: (0, 0) where no row has a key that they leave out."""
+        if window is None:
+            return 0, 0
+        sinks = min(sinks, self._most_k)
+        if sinks >= self._most_k or window >= (self._most_k - sinks if causal else max(self._most_q, self._most_k)):
+            return 0, 0
+        return window, sinks
+
+    def _plan(self, which: str, group: int, kv_heads: int, causal: bool, row_bytes: int, elem: int = 2, window: int = 0,
+              sinks: int = 0) -> _Tiles:
         dim = -(-row_bytes // elem // 32) * 32  # (as the kernels are built: one list for all sizes of a kernel)
-        key = (which, group, kv_heads, causal, dim, elem)
+        key = (which, group, kv_heads, causal, dim, elem, window, sinks)
         plan = self._plans.get(key)
         if plan is None:
             nq, nk = self._nq, self._nk
-            if int(nq.max(initial=0)) * group >= 2 ** 31 - _lib.ATTN_TILE:
+            if self._most_q * group >= 2 ** 31 - _lib.ATTN_TILE:
                 raise ValueError(f"a segment has at most {(2 ** 31 - _lib.ATTN_TILE) // group} query rows at {group} heads a key head")
             if which == "q":  # tiles of packed rows over keys lo .. hi
                 tile, seg, row0 = self._tiles(nq * group, row_bytes)
                 rows = np.minimum(nq[seg] * group - row0, tile)
                 lo, hi = np.zeros_like(row0), nk[seg]
+                last = (np.minimum(row0 + tile, nq[seg] * group) - 1) // group + nk[seg] - nq[seg]  # place of the last row
                 if causal:
-                    last = np.minimum(row0 + tile, nq[seg] * group) - 1
-                    hi = np.clip(last // group + nk[seg] - nq[seg] + 1, 0, nk[seg])
+                    hi = np.clip(last + 1, 0, nk[seg])
+                elif window:
+                    hi = np.clip(last + window, np.minimum(sinks, nk[seg]), nk[seg])
+                if window:  # places in the list of the sinks, in whole steps, and the keys from the first window on
+                    first = np.maximum(0, row0 // group + nk[seg] - nq[seg] - window + 1)
+                    hi = hi - np.maximum(0, first - -(-sinks // _STEP) * _STEP)
             else:  # tiles of keys over packed rows lo .. hi
                 tile, seg, row0 = self._tiles(nk, row_bytes)
                 rows = np.minimum(nk[seg] - row0, tile)
                 lo, hi = np.zeros_like(row0), nq[seg] * group
+                first = row0 - (nk[seg] - nq[seg])  # the query whose place the tile's first key is
+                if window:
+                    end = np.clip(first + rows - 1 + window, 0, nq[seg])
+                    hi = np.where(row0 < sinks, nq[seg], end) * group
+                    if not causal:
+                        lo = np.where(row0 < sinks, 0, np.clip(first - window + 1, 0, nq[seg])) * group
                 if causal:
-                    lo = np.minimum(np.maximum(0, row0 - (nk[seg] - nq[seg])) * group, hi)
+                    lo = np.maximum(0, first) * group
+                lo = np.minimum(lo, hi)
             plan = _Tiles(tile, self._q0[seg], nq[seg], self._k0[seg], nk[seg], row0, rows, lo, hi,
                           kv_heads, dim, elem, which == "k", self.device)
             self._plans[key] = plan
@@ -259,25 +283,25 @@ def _rows(t: torch.Tensor, group: int) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _args(q, k, v, key_mask, o, rest, lse, causal, scale) -> _lib.AttnArgs:
+def _args(q, k, v, key_mask, o, rest, lse, causal, scale, window) -> _lib.AttnArgs:
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     ptr = _lib.ptr
     return _lib.AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(rest), ptr(lse), None, None, None, None,
                          None, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], 0, 0, ptr(key_mask), None, None, None, None,
                          0, 0, 0, 0, None, q.shape[1], k.shape[1], q.shape[2], _lib.FEAT_DTYPES[q.dtype], causal, _lib.ATTN_TILE,
-                         _lib.ATTN_TILE, 0, 0, scale)
+                         _lib.ATTN_TILE, 0, 0, scale, *window)
 
 
-def _forward(q, k, v, segments, key_mask, causal, scale, stats):
+def _forward(q, k, v, segments, key_mask, causal, scale, window, stats):
     n, heads, dim = q.shape
     kv_heads = k.shape[1]
     group = heads // kv_heads
     q, k, v = _rows(q, group), _rows(k, group), _rows(v, group)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if stats else None
-    plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size(), q.element_size())
+    plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size(), q.element_size(), *window)
     rest = torch.empty_like(o) if stats and o.element_size() == 2 else None  # what its rounding leaves, for the gradient
-    a = _args(q, k, v, key_mask, o, rest, lse, causal, scale)
+    a = _args(q, k, v, key_mask, o, rest, lse, causal, scale, window)
     a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
     a.q_tile, a.q_item_major = plan.tile, plan.item_major
     parts = _parts(kv_heads, dim, plan.slots, 0, q.device)
@@ -289,25 +313,25 @@ def _forward(q, k, v, segments, key_mask, causal, scale, stats):
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, segments, key_mask, causal, scale):
-        o, rest, lse, q, k, v = _forward(q, k, v, segments, key_mask, causal, scale, True)
+    def forward(ctx, q, k, v, segments, key_mask, causal, scale, window):
+        o, rest, lse, q, k, v = _forward(q, k, v, segments, key_mask, causal, scale, window, True)
         ctx.save_for_backward(q, k, v, o, rest, lse, key_mask)
-        ctx.meta = (segments, causal, scale)
+        ctx.meta = (segments, causal, scale, window)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, o, rest, lse, key_mask = ctx.saved_tensors
-        segments, causal, scale = ctx.meta
+        segments, causal, scale, window = ctx.meta
         heads, dim = q.shape[1:]
         kv_heads = k.shape[1]
         group = heads // kv_heads
         dout = _rows(dout, group)
         new = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format)  # noqa: E731
         dq, delta = new(q), torch.empty_like(lse)
-        plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size(), q.element_size())
-        a = _args(q, k, v, key_mask, o, rest, lse, causal, scale)
+        plan = segments._plan("q", group, kv_heads, causal, dim * q.element_size(), q.element_size(), *window)
+        a = _args(q, k, v, key_mask, o, rest, lse, causal, scale, window)
         a.dout, a.dq, a.delta = dout.data_ptr(), dq.data_ptr(), delta.data_ptr()
         a.dout_row, a.dout_head, _ = dout.stride()
         a.q_items, a.q_joins, a.n_q_items, a.n_q_joins = plan.items, plan.joins, plan.n_items, plan.n_joins
@@ -316,7 +340,7 @@ class _Attention(torch.autograd.Function):
         slots = 0
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dk, dv = new(k), new(v)
-            keys = segments._plan("k", group, kv_heads, causal, dim * q.element_size(), q.element_size())
+            keys = segments._plan("k", group, kv_heads, causal, dim * q.element_size(), q.element_size(), *window)
             a.dk, a.dv = dk.data_ptr(), dv.data_ptr()
             a.k_items, a.k_joins, a.n_k_items, a.n_k_joins = keys.items, keys.joins, keys.n_items, keys.n_joins
             a.k_tile, a.k_item_major = keys.tile, keys.item_major
@@ -326,7 +350,7 @@ class _Attention(torch.autograd.Function):
             a.parts = parts.data_ptr()
         _lib.call("st_attn_backward", ctypes.byref(a), _lib.stream_of(q.device))
         need = ctx.needs_input_grad
-        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None, None
 
 
 def sparse_attention(
@@ -337,6 +361,8 @@ def sparse_attention(
     scale: Optional[float] = None,
     causal: bool = False,
     key_mask: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> torch.Tensor:
     """``softmax(scale * q k^T) v`` in each segment, (rows, heads, D) contiguous in ``q``'s dtype.
 
@@ -346,7 +372,10 @@ def sparse_attention(
     heads may lie at any stride (slices of one projection, say); where channels are apart or rows not
     at 16-byte addresses a copy is made.  ``scale`` is positive, ``D ** -0.5`` by default.
 
-    ``causal``: query ``i`` of ``nq`` sees keys up to ``i + nk - nq`` of its segment.  ``key_mask``
+    ``causal``: query ``i`` of ``nq`` sees keys up to its place, ``i + nk - nq``, of its segment.
+    ``window``: a row sees only the keys less than ``window`` from its place (with ``causal`` the last
+    ``window`` up to it, else those on both sides), and besides them the segment's first ``sinks``
+    keys (with ``causal`` those up to its place).  The keys in between are not read.  ``key_mask``
     (``segments.k_rows``) bool: False leaves a key out, whatever its rows hold.  A row that sees no
     key gets zeros, and its gradients are zero.  Scores, softmax and sums are fp32 (fp32 inputs: the
     products too); results do not depend on timing.  16-bit inputs round the probabilities, and in the
@@ -386,7 +415,16 @@ def sparse_attention(
                              f"{key_mask.device})")
         key_mask = key_mask.contiguous()
     causal = bool(causal)
+    if window is not None or sinks:
+        if window is None:
+            raise ValueError("sinks are the first keys beside a window: give one")
+        if isinstance(window, bool) or isinstance(sinks, bool):
+            raise TypeError("window and sinks are numbers of keys")
+        window, sinks = operator.index(window), operator.index(sinks)
+        if window < 1 or sinks < 0:
+            raise ValueError(f"a window has a key at least, sinks are not negative (got {window} and {sinks})")
+    window = segments._window(causal, window, sinks)
     refuse_tangents("sparse_attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _Attention.apply(q, k, v, segments, key_mask, causal, scale)
-    return _forward(q, k, v, segments, key_mask, causal, scale, False)[0]
+        return _Attention.apply(q, k, v, segments, key_mask, causal, scale, window)
+    return _forward(q, k, v, segments, key_mask, causal, scale, window, False)[0]
