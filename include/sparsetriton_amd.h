@@ -954,8 +954,8 @@ int st_qk_norm_rotary_backward(const st_qk_norm_args* args, st_stream_t stream);
  * keys and ranges of packed rows (every row that sees a key of the tile).  With a
  * window the keys of a q_item are places in a list: where the first key that a
  * window of the tile's rows covers, f = max(0, place of its first row - window + 1),
- * lies behind h = sinks rounded up to 64, places below h are the keys of that number and
- * a place p from h on is key p + f - h; parts begin at multiples of 64 places.
+ * lies behind the sinks, a place p from `sinks` on is key p + f - sinks.  Parts begin
+ * at multiples of 64.
  * parts: fp32 workspace, 16-byte address, st_attn_workspace floats for the
  * slots used.  lse (rows, heads) fp32, base-2 logarithm, INFINITY for a row
  * without keys: written when not NULL, needed by the backward; o_rest (as o; NULL =

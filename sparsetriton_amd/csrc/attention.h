@@ -196,18 +196,23 @@ struct AttnTile {
 // A product over the rows of a tile that the causal order or a window cuts: the other
 // operand is zero where a column must not see a row, but zero times an infinity
 // or a NaN is a NaN, so a row that is not finite would reach those that do not see it.
-// Such a tile (one check of it, by each wave that the order cuts it for) is
-// copied without those elements, the product taken over the copy, and what they
-// do to the columns that see them added at the end.
-template <typename T, int ROWS, int DP>
-__device__ __forceinline__ bool attn_not_finite(const T* tile) {
-  using Tile = AttnTile<T, DP>;
-  bool bad = false;
-#pragma unroll 4
-  for (int c = threadIdx.x & 63; c < ROWS * Tile::CPR; c += 64)
-#pragma unroll
-    for (int e = 0; e < Tile::EPC; ++e) bad |= !(fabsf((float)tile[c * Tile::EPC + e]) < INFINITY);
-  return __any(bad);
+// The steps that are cut for any of a workgroup's waves are checked for such elements
+// on their way to LDS, a flag a wave (AttnFlags).  Where there are any, a wave that the order cuts copies the
+// tile without them, takes the product over the copy, and what they
+// do to the columns that see them is added at the end.
+template <typename T>
+__device__ __forceinline__ bool attn_not_finite(unsigned top) {  // top: the largest magnitude's bits
+  return sizeof(T) == 4 ? top >= 0x7F800000u : max(top >> 16, top & 0xFFFFu) >= (__is_same(T, __bf16) ? 0x7F80u : 0x7C00u);
+}
+template <typename T>
+__device__ __forceinline__ unsigned attn_magnitude(unsigned top, unsigned word) {
+  if constexpr (sizeof(T) == 4) {
+    return max(top, word & 0x7FFFFFFFu);
+  } else {
+    typedef unsigned short v2s __attribute__((ext_vector_type(2)));
+    const v2s a = __builtin_bit_cast(v2s, top), b = __builtin_bit_cast(v2s, word & 0x7FFF7FFFu);
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(a, b));
+  }
 }
 // (Each wave that needs the copy writes all of it, the same values.)
 template <typename T, int ROWS, int DP>
@@ -218,6 +223,30 @@ __device__ __forceinline__ void attn_copy_finite(const T* tile, T* copy) {
 #pragma unroll
     for (int e = 0; e < Tile::EPC; ++e) copy[c + e] = fabsf((float)tile[c + e]) < INFINITY ? tile[c + e] : (T)0.f;
 }
+// A flag of each wave for the tiles of a step, in the copy's first bytes: put before the step's barrier, read after it.
+// Where one is set all waves read them before any copies, and are through with the copy before the next ones are put
+// (a barrier each, in `read` and in `begin`), which every wave reaches, as the flags are the same to all of them.
+template <int WAVES>
+struct AttnFlags {
+  int* at;
+  bool copied = false;
+  __device__ __forceinline__ explicit AttnFlags(void* copy) : at(reinterpret_cast<int*>(copy)) {}
+  __device__ __forceinline__ void begin() {
+    if (copied) __syncthreads();
+    copied = false;
+  }
+  __device__ __forceinline__ void put(int buf, bool flag) const {
+    const bool any = __any(flag);
+    if ((threadIdx.x & 63) == 0) at[buf * WAVES + (threadIdx.x >> 6)] = any;
+  }
+  __device__ __forceinline__ void read(int buf) {
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all |= at[buf * WAVES + w];
+    copied = __builtin_amdgcn_readfirstlane(all) != 0;
+    if (copied) __syncthreads();
+  }
+};
 // What the left out elements do to a lane's sums (transposed: registers =
 // channels), a bit for each: infinities of either sign, both for a NaN.  In
 // loops that stay rolled: they take neither time nor registers from the products.
@@ -274,9 +303,27 @@ struct AttnStage {
 #pragma unroll
     for (int i = 0; i < N; ++i) reg[i] = load16<v4u>(r, row(i) < left ? off[i] : kOobOffset);
   }
+  // The same where rows from `split` on lie at another base.
+  __device__ __forceinline__ void load(const T* base, const T* other, int split, int left) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base, kOobOffset), r2 = make_rsrc(other, kOobOffset);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (row(i) < split)
+        reg[i] = load16<v4u>(r, row(i) < left ? off[i] : kOobOffset);
+      else
+        reg[i] = load16<v4u>(r2, row(i) < left ? off[i] : kOobOffset);
+    }
+  }
   __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) *reinterpret_cast<v4u*>(tile + Tile::at(row(i), chunk(i))) = reg[i];
+  }
+  __device__ __forceinline__ unsigned magnitude(unsigned top = 0) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = attn_magnitude<T>(top, reg[i][e]);
+    return top;
   }
 };
 
@@ -389,55 +436,59 @@ constexpr int kAttnAll = 0, kAttnCausal = 1, kAttnWindow = 2;
 // The lowest n bits of 64.
 __device__ __forceinline__ uint64_t attn_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : ~0ull >> (64 - n); }
 
-// The keys of a tile of rows with a window, in steps: where those that the rows'
-// windows cover begin behind the first keys (the sinks, in whole steps of 64), a
-// list of both, without the keys between them: places below `head` are the keys
-// themselves, the others `gap` keys further.  Uniform in a workgroup.
-struct AttnWindow {
-  int head = 0, gap = 0, sinks = 0;
-  __device__ __forceinline__ AttnWindow(const AttnArgs& a, const AttnItem& it, int first) {
-    const int w = a.window - 1, at = first + it.nk - it.nq;  // (place of the tile's first row)
-    sinks = a.sinks;
-    head = (a.sinks + 63) & ~63;
-    gap = max(max(at, w) - w - head, 0);
-  }
-  __device__ __forceinline__ int key(int kt) const { return kt >= head ? kt + gap : kt; }
-  __device__ __forceinline__ int end(int kt, int hi) const { return gap && kt < head ? min(hi, sinks) : hi; }
-  // the step after this one (what the sinks leave of their last 64 is passed over)
-  __device__ __forceinline__ int next(int kt, int step) const {
-    const int n = kt + step;
-    return gap && n >= sinks && n < head ? head : n;
-  }
-};
-// Keys that a lane's row sees: from .. last, and those below `sinks`.
+// The keys that a tile of rows goes over, and those of them that a lane's row sees.
+// With a window: a list of the segment's first keys (the sinks) and of those from the first that a
+// window of the tile's rows covers; where that one lies behind the sinks, places of the
+// list from `sinks` on are keys `gap` further.  A row of place `at` sees the keys from(at) ..
+// last(at) and, up to its place under the causal order, the sinks.  (Only `at` and `live` are a lane's
+// own, the rest is the workgroup's: a lane's registers are short.)
 template <int ORDER>
 struct AttnSight {
-  int last = 0x7FFFFFFE, from = 0, sinks = 0;
-  __device__ __forceinline__ AttnSight(const AttnArgs& a, const AttnItem& it, int qi, bool live) {
-    const int at = qi + it.nk - it.nq;
-    if constexpr (ORDER == kAttnCausal) last = at;
-    if (ORDER == kAttnWindow && live) {  // (no sum passes 2^31)
-      const int w = a.window - 1;
-      last = a.causal ? at : min(at, it.nk - 1 - w) + w;
-      from = max(at, w) - w;
-      sinks = a.causal ? min(a.sinks, at + 1) : a.sinks;
+  int sinks = 0, gap = 0, w = 0, most = 0;  // window - 1; the largest place whose window ends inside the segment
+  int tile_last = 0, tile_from = 0;         // what all of the tile's rows see
+  int at;
+  bool live, causal;
+
+  __device__ __forceinline__ AttnSight(const AttnArgs& a, const AttnItem& it, int qi, bool live_row, int first, int rows)
+      : at(qi + it.nk - it.nq), live(live_row), causal(a.causal) {
+    if constexpr (ORDER == kAttnWindow) {  // (no sum passes 2^31)
+      sinks = a.sinks, w = a.window - 1, most = it.nk - 1 - w;
+      const int off = it.nk - it.nq, at1 = attn_div(min(it.row0 + rows, it.nq * a.group) - 1, a.by_group) + off;
+      gap = max(from(first + off) - sinks, 0);
+      tile_last = last(first + off);
+      tile_from = from(at1);
+    } else {
+      tile_last = first + it.nk - it.nq;
     }
   }
-  // any of the keys k .. k + n - 1
-  __device__ __forceinline__ bool any(int k, int n) const {
-    if constexpr (ORDER == kAttnWindow) return k < sinks || (k <= last && k + n > from);
-    return k <= last;
+  __device__ __forceinline__ int last(int p) const { return causal ? p : min(p, most) + w; }
+  __device__ __forceinline__ int from(int p) const { return max(p, w) - w; }
+  // places kt .. kt + n - 1 of the list: both kinds of keys
+  __device__ __forceinline__ bool both(int kt, int n) const { return ORDER == kAttnWindow && gap && kt < sinks && kt + n > sinks; }
+  __device__ __forceinline__ int key(int kt) const { return ORDER == kAttnWindow && kt >= sinks ? kt + gap : kt; }
+  // whether some row of the tile may not see some of them
+  __device__ __forceinline__ bool tile_cut(int kt, int n) const {
+    if constexpr (ORDER == kAttnWindow) return both(kt, n) || !(tile_from <= kt + gap && tile_last - (kt + gap) >= n - 1);
+    return ORDER == kAttnCausal && tile_last - kt < n - 1;
   }
-  // all of them
-  __device__ __forceinline__ bool all(int k, int n) const {
-    if constexpr (ORDER == kAttnWindow) return (from <= k && last - k >= n - 1) || k + n <= sinks;
-    return last - k >= n - 1;
-  }
-  // a bit for each key from k on, of those that `seen` has
-  __device__ __forceinline__ uint64_t keep(int k, uint64_t seen) const {
-    const int to = last - k;
+  // whether the row sees any, and (a row that is not there does) all of them
+  __device__ __forceinline__ bool any(int kt, int n) const {
     if constexpr (ORDER == kAttnWindow)
-      return seen & (attn_below(sinks - k) | (attn_below(to + 1) & ~attn_below(from - k)));
+      return live && ((kt < sinks && (!causal || kt <= at)) || (kt + gap <= last(at) && kt + gap + n > from(at)));
+    return live && kt <= at;
+  }
+  __device__ __forceinline__ bool all(int kt, int n) const {
+    if constexpr (ORDER == kAttnWindow)
+      return !live || (!both(kt, n) && from(at) <= kt + gap && last(at) - (kt + gap) >= n - 1);
+    return at - kt >= n - 1;
+  }
+  // a bit for each place from kt on that the row sees, of those that `seen` has
+  __device__ __forceinline__ uint64_t keep(int kt, uint64_t seen) const {
+    if constexpr (ORDER == kAttnWindow) {
+      const uint64_t window = attn_below(last(at) - gap - kt + 1) & ~attn_below(from(at) - gap - kt);
+      return seen & (attn_below((causal ? min(sinks, at + 1) : sinks) - kt) | window);
+    }
+    const int to = at - kt;
     return to >= 63 ? seen : to < 0 ? 0 : seen & ((2ull << to) - 1);
   }
 };
@@ -573,6 +624,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
   constexpr int TILE = BK * DP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
+  AttnFlags<WAVES> flags(tiles + 4 * TILE);  // CUT: where the copy is
   float* bias = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers, not CUT: 0 or -inf for each key of a step
 
   int hk;
@@ -590,26 +642,29 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = load_row8<T>(base, off, 16 * s + 8 * half, a.D, live);
   }
-  const AttnSight<ORDER> sight(a, it, qi, live);
-  const AttnWindow list(a, it, first);
+  const AttnSight<ORDER> sight(a, it, qi, live, first, 32 * WAVES);
 
   Stage ks, vs;
   ks.place(a.D, [&](int x) { return x * (int)(a.k_row * sizeof(T)); });
   vs.place(a.D, [&](int x) { return x * (int)(a.v_row * sizeof(T)); });
   uint8_t chunk_kept[Stage::N], key_kept = 1;
   const uint8_t* mask = a.key_mask ? a.key_mask + it.k0 : nullptr;
-  auto key_at = [&](int kt) { return ORDER == kAttnWindow ? list.key(kt) : kt; };
-  auto end_at = [&](int kt) { return ORDER == kAttnWindow ? list.end(kt, it.hi) : it.hi; };
   auto fetch = [&](int kt) {
-    const int left = end_at(kt) - kt, key = key_at(kt);
-    const int64_t row = it.k0 + (int64_t)key;
+    const int left = it.hi - kt;
     if (mask) {
 #pragma unroll
-      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[key + Stage::row(i)] : 0;
-      key_kept = lane < left ? mask[key + lane] : 0;
+      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[sight.key(kt + Stage::row(i))] : 0;
+      key_kept = lane < left ? mask[sight.key(kt + lane)] : 0;
     }
-    ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, left);
-    vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, left);
+    const int64_t row = it.k0 + (int64_t)sight.key(kt);
+    const T *k = (const T*)a.k + row * a.k_row + hk * a.k_head, *v = (const T*)a.v + row * a.v_row + hk * a.v_head;
+    if (sight.both(kt, BK)) {
+      ks.load(k, k + sight.gap * a.k_row, sight.sinks - kt, left);
+      vs.load(v, v + sight.gap * a.v_row, sight.sinks - kt, left);
+    } else {
+      ks.load(k, left);
+      vs.load(v, left);
+    }
   };
 
   v16f o[DB];
@@ -618,14 +673,12 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
   float m = -INFINITY, l = 0.f;
   AttnNotFinite left_out;
   if (it.lo < it.hi) fetch(it.lo);
-  for (int kt = it.lo, next, buf = 0; kt < it.hi; kt = next, buf ^= 1) {
-    next = ORDER == kAttnWindow ? list.next(kt, BK) : kt + BK;
-    const int left = end_at(kt) - kt, key = key_at(kt);
+  for (int kt = it.lo, buf = 0; kt < it.hi; kt += BK, buf ^= 1) {
     T* kl = tiles + buf * 2 * TILE;
     T* vl = kl + TILE;
     constexpr uint64_t ALL = ~0ull >> (64 - BK);
     uint64_t seen = ALL;  // keys of this step that exist and are not masked
-    if (left < BK) seen >>= BK - left;
+    if (it.hi - kt < BK) seen >>= BK - (it.hi - kt);
     if (mask) {
       seen &= __ballot(key_kept);
 #pragma unroll
@@ -633,11 +686,15 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
         if (!chunk_kept[i]) ks.reg[i] = vs.reg[i] = (v4u)(0u);
     }
     if (!CUT && seen != ALL && threadIdx.x < BK) bias[buf * BK + lane] = seen >> lane & 1 ? 0.f : -INFINITY;
+    if constexpr (CUT) flags.begin();
     ks.store(kl);
     vs.store(vl);
+    const bool check = CUT && sight.tile_cut(kt, BK);
+    if (check) flags.put(buf, attn_not_finite<T>(vs.magnitude()));
     __syncthreads();
-    if (next < it.hi) fetch(next);
-    if (!active || (CUT && !__any(live && sight.any(key, BK)))) continue;
+    if (check) flags.read(buf);
+    if (kt + BK < it.hi) fetch(kt + BK);
+    if (!active || (CUT && !__any(sight.any(kt, BK)))) continue;
 
     v16f s[NB];
     auto scores = [&]() {
@@ -662,8 +719,8 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
       for (int b = 0; b < NB; ++b) s[b] = (v16f)(0.f);
       scores();
     }
-    const bool cut = CUT && __any(!sight.all(key, BK));  // by the causal order or the window
-    const uint64_t keep = CUT ? sight.keep(key, seen) : seen;
+    const bool cut = CUT && __any(!sight.all(kt, BK));  // by the causal order or the window
+    const uint64_t keep = CUT ? sight.keep(kt, seen) : seen;
     if (CUT && (cut || seen != ALL)) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
@@ -701,7 +758,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
       }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     const T* vp = vl;
-    if (cut && attn_not_finite<T, BK, DP>(vl)) {
+    if (cut && flags.copied) {
       attn_copy_finite<T, BK, DP>(vl, tiles + 4 * TILE);
       vp = tiles + 4 * TILE;
       left_out.add<T, BK, DP>(vl, keep);
@@ -851,6 +908,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
   constexpr int TILE = BK * DP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* tiles = reinterpret_cast<T*>(lds);
+  AttnFlags<WAVES> flags(tiles + 4 * TILE);  // CUT: where the copy is
 
   int hk;
   const AttnItem it = attn_item(a, hk);
@@ -884,26 +942,29 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
       if (half == 0) a.delta[at] = delta;
     }
   }
-  const AttnSight<ORDER> sight(a, it, qi, live);
-  const AttnWindow list(a, it, first);
+  const AttnSight<ORDER> sight(a, it, qi, live, first, 32 * WAVES);
 
   Stage ks, vs;
   ks.place(a.D, [&](int x) { return x * (int)(a.k_row * sizeof(T)); });
   vs.place(a.D, [&](int x) { return x * (int)(a.v_row * sizeof(T)); });
   uint8_t chunk_kept[Stage::N], key_kept = 1;
   const uint8_t* mask = a.key_mask ? a.key_mask + it.k0 : nullptr;
-  auto key_at = [&](int kt) { return ORDER == kAttnWindow ? list.key(kt) : kt; };
-  auto end_at = [&](int kt) { return ORDER == kAttnWindow ? list.end(kt, it.hi) : it.hi; };
   auto fetch = [&](int kt) {
-    const int left = end_at(kt) - kt, key = key_at(kt);
-    const int64_t row = it.k0 + (int64_t)key;
+    const int left = it.hi - kt;
     if (mask) {
 #pragma unroll
-      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[key + Stage::row(i)] : 0;
-      key_kept = lane < left ? mask[key + lane] : 0;
+      for (int i = 0; i < Stage::N; ++i) chunk_kept[i] = Stage::row(i) < left ? mask[sight.key(kt + Stage::row(i))] : 0;
+      key_kept = lane < left ? mask[sight.key(kt + lane)] : 0;
     }
-    ks.load((const T*)a.k + row * a.k_row + hk * a.k_head, left);
-    vs.load((const T*)a.v + row * a.v_row + hk * a.v_head, left);
+    const int64_t row = it.k0 + (int64_t)sight.key(kt);
+    const T *k = (const T*)a.k + row * a.k_row + hk * a.k_head, *v = (const T*)a.v + row * a.v_row + hk * a.v_head;
+    if (sight.both(kt, BK)) {
+      ks.load(k, k + sight.gap * a.k_row, sight.sinks - kt, left);
+      vs.load(v, v + sight.gap * a.v_row, sight.sinks - kt, left);
+    } else {
+      ks.load(k, left);
+      vs.load(v, left);
+    }
   };
 
   v16f dq[DB];
@@ -911,29 +972,31 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_ker
   for (int b = 0; b < DB; ++b) dq[b] = (v16f)(0.f);
   AttnPower power;
   if (it.lo < it.hi) fetch(it.lo);
-  for (int kt = it.lo, next, buf = 0; kt < it.hi; kt = next, buf ^= 1) {
-    next = ORDER == kAttnWindow ? list.next(kt, BK) : kt + BK;
-    const int left = end_at(kt) - kt, key = key_at(kt);
+  for (int kt = it.lo, buf = 0; kt < it.hi; kt += BK, buf ^= 1) {
     T* kl = tiles + buf * 2 * TILE;
     T* vl = kl + TILE;
     constexpr uint64_t ALL = ~0ull >> (64 - BK);
     uint64_t seen = ALL;
-    if (left < BK) seen >>= BK - left;
+    if (it.hi - kt < BK) seen >>= BK - (it.hi - kt);
     if (mask) {
       seen &= __ballot(key_kept);
 #pragma unroll
       for (int i = 0; i < Stage::N; ++i)
         if (!chunk_kept[i]) ks.reg[i] = vs.reg[i] = (v4u)(0u);
     }
+    if constexpr (CUT) flags.begin();
     ks.store(kl);
     vs.store(vl);
+    const bool check = CUT && sight.tile_cut(kt, BK);
+    if (check) flags.put(buf, attn_not_finite<T>(ks.magnitude()));
     __syncthreads();
-    if (next < it.hi) fetch(next);
-    if (!active || (CUT && !__any(live && sight.any(key, BK)))) continue;
-    const bool cut = CUT && __any(!sight.all(key, BK));
-    const uint64_t keep = CUT ? sight.keep(key, seen) : seen;
+    if (check) flags.read(buf);
+    if (kt + BK < it.hi) fetch(kt + BK);
+    if (!active || (CUT && !__any(sight.any(kt, BK)))) continue;
+    const bool cut = CUT && __any(!sight.all(kt, BK));
+    const uint64_t keep = CUT ? sight.keep(kt, seen) : seen;
     const T* kp = kl;  // (a row that sees a key that is not finite has a dS that is not)
-    if (cut && attn_not_finite<T, BK, DP>(kl)) {
+    if (cut && flags.copied) {
       attn_copy_finite<T, BK, DP>(kl, tiles + 4 * TILE);
       kp = tiles + 4 * TILE;
     }
@@ -1022,6 +1085,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
   T* tiles = reinterpret_cast<T*>(lds);
   float* stats = reinterpret_cast<float*>(tiles + 4 * TILE);  // two buffers of BQ L, BQ delta
   T* copies = reinterpret_cast<T*>(stats + 4 * BQ);           // CUT: of a Q and a dO tile
+  AttnFlags<WAVES> flags(copies);
 
   int hk;
   const AttnItem it = attn_item(a, hk);
@@ -1056,6 +1120,9 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
   const int wave_from = first_query(kw) * a.group;
   const int to = windowed && live ? end_row(key) : 0x7FFFFFFF;
   const int wave_to = windowed ? max(end_row(kw), end_row(min(kw + 31, it.nk - 1))) : 0x7FFFFFFF;
+  // the rows that see all of the tile's keys
+  const int tile_from = CUT ? first_query(min(it.row0 + 32 * WAVES, it.nk) - 1) * a.group : 0;
+  const int tile_to = windowed ? end_row(max(it.row0, a.sinks)) : 0x7FFFFFFF;
 
   Stage qs, gs;
   float stat = 0.f;
@@ -1098,16 +1165,20 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
     T* ql = tiles + buf * 2 * TILE;
     T* gl = ql + TILE;
     float* st = stats + buf * 2 * BQ;
+    if constexpr (CUT) flags.begin();
     qs.store(ql);
     gs.store(gl);
     if (threadIdx.x < 2 * BQ) st[threadIdx.x] = stat;
+    const bool check = CUT && (tile_from > rt || (windowed && tile_to - rt < BQ));
+    if (check) flags.put(buf, attn_not_finite<T>(DK && DV ? gs.magnitude(qs.magnitude()) : DK ? qs.magnitude() : gs.magnitude()));
     __syncthreads();
+    if (check) flags.read(buf);
     if (rt + BQ < it.hi) fetch(rt + BQ);
     if (!active || rt + BQ <= wave_from || (windowed && rt >= wave_to)) continue;
     const bool cut = CUT && __any(from > rt || (windowed && to - rt < BQ));
     auto sees = [&](int row) { return row >= from && (!windowed || row < to); };
     const T *qp = ql, *gp = gl;  // (a row whose Q or dO is not finite has a delta, and so a dS, that is not)
-    if (cut && ((DK && attn_not_finite<T, BQ, DP>(ql)) || (DV && attn_not_finite<T, BQ, DP>(gl)))) {
+    if (cut && flags.copied) {
       if constexpr (DK) attn_copy_finite<T, BQ, DP>(ql, copies);
       if constexpr (DV) attn_copy_finite<T, BQ, DP>(gl, copies + TILE);
       qp = copies, gp = copies + TILE;

@@ -242,9 +242,8 @@ class AttentionSegments:
                     hi = np.clip(last + 1, 0, nk[seg])
                 elif window:
                     hi = np.clip(last + window, np.minimum(sinks, nk[seg]), nk[seg])
-                if window:  # places in the list of the sinks, in whole steps, and the keys from the first window on
-                    first = np.maximum(0, row0 // group + nk[seg] - nq[seg] - window + 1)
-                    hi = hi - np.maximum(0, first - -(-sinks // _STEP) * _STEP)
+                if window:  # places in the list of the sinks and the keys from the first window on
+                    hi = hi - np.maximum(0, row0 // group + nk[seg] - nq[seg] - window + 1 - sinks)
             else:  # tiles of keys over packed rows lo .. hi
                 tile, seg, row0 = self._tiles(nk, row_bytes)
                 rows = np.minimum(nk[seg] - row0, tile)

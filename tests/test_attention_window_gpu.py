@@ -129,18 +129,17 @@ def test_tile_lists_cover_what_is_seen_once(ql, kl, group, causal, window, sinks
                     assert all((i[5] - lo) % 64 == 0 for i in tile)
                     first, last = row0 // group, (min(rows, row0 + plan.tile) - 1) // group
                     seen = see[first:last + 1].any(0)
-                    head = -(-sinks // 64) * 64
                     f = max(0, first + nk - nq - window + 1) if window else 0
-                    gap = max(0, f - head)
+                    gap = max(0, f - sinks)
                     assert hi + gap <= nk and lo == 0
                     walked = torch.zeros(nk, dtype=torch.bool)
                     for p in range(lo, hi):
-                        key = p + gap if p >= head else p
+                        key = p + gap if p >= sinks else p
                         assert not walked[key]
-                        walked[key] = p >= head or not gap or p < sinks
+                        walked[key] = True
                     assert not (seen & ~walked).any()
                     # and no more than the sinks and what lies between the outer rows' windows
-                    assert int(walked.sum()) <= sinks + max(0, last - first + (2 if not causal else 1) * (window or nk) + 64)
+                    assert int(walked.sum()) <= sinks + max(0, last - first + (2 if not causal else 1) * (window or nk))
                 else:
                     seen = see[:, row0:row0 + plan.tile].any(1).nonzero().flatten().tolist()
                     if seen:
