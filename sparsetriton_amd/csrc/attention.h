@@ -32,6 +32,8 @@
 // itself, 1.5 with the rest of O; 1.4 are that rounding and dS's.  No slower).
 #pragma once
 
+#include <algorithm>
+
 #include "common.h"
 #include "mfma.h"
 #include "wave_sum.h"
@@ -518,8 +520,9 @@ __device__ __forceinline__ bool attn_in(int channel, int D) {
 }
 
 // Waves of a SIMD that the registers leave room for (a limit for the compiler).
-template <typename T, int DP>
+template <typename T, int DP, int ORDER = kAttnAll, int WAVES = 1>
 constexpr int attn_waves() {
+  if (ORDER == kAttnWindow && WAVES == 4 && DP * sizeof(T) == 128) return 3;  // (three registers more than that, left to itself)
   return DP * sizeof(T) <= 256 ? 2 : 1;
 }
 
@@ -614,7 +617,7 @@ struct AttnPower {
 };
 
 template <typename T, int DP, int ORDER, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forward_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP, ORDER, WAVES>())) void attn_forward_kernel(AttnArgs a) {
   constexpr bool CUT = ORDER != kAttnAll;  // some rows do not see some keys
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
@@ -805,7 +808,9 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_forwar
 // are shared between the lanes and joined through LDS in order, fewer are a
 // lane's own, and the lanes take rows.  (12 single queries of ~100 parts: 33 us
 // unshared, 7 shared; 300 queries x 8 heads of up to 29 parts: 47 and 9 us.)
-constexpr int kAttnJoinBlocks = 48;  // workgroups of a tile's join
+// Workgroups of a tile's join, more where there are few tiles (one tile of keys in 114 parts x 4 key heads x 128: 32 us in
+// 48 workgroups, 10 in 256).
+constexpr int kAttnJoinBlocks = 48, kAttnMostJoinBlocks = 256, kAttnJoinsTo = 2048;
 constexpr int kAttnFewParts = 16;
 
 template <typename T, int DP>
@@ -822,7 +827,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_forward_join_kernel(AttnArg
   const int stride = share ? 1 : LANES;  // rows of a workgroup at once
   // (m = up, both -inf for parts without keys among them, is weight 1: their sums are zero)
   auto weight = [](float m, float up) { return m == up ? 1.f : fast_exp2(m - up); };
-  for (int row0 = blockIdx.y * stride; row0 < rows; row0 += kAttnJoinBlocks * stride) {
+  for (int row0 = blockIdx.y * stride; row0 < rows; row0 += gridDim.y * stride) {
     const int row = share ? row0 : row0 + lane;
     const float* p = a.parts + (((int64_t)jn.part * a.kv_heads + hk) * kAttnTile + row) * (DP + 4);
     v4f sum = (v4f)(0.f);
@@ -898,7 +903,7 @@ constexpr int attn_dq_lds(bool cut) {
 // As the forward's sizes: 64 channels bf16 272 us (760 TFLOP/s, MFMA busy 44 %, vector
 // unit 62: 107 instructions a tile), 128 channels causal 453 us (910, 47 %), fp32 114 us (76, 61 %).
 template <typename T, int DP, int ORDER, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP>())) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP, ORDER, WAVES>())) void attn_dq_kernel(AttnArgs a) {
   constexpr bool CUT = ORDER != kAttnAll;  // some rows do not see some keys
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
@@ -1275,7 +1280,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_sum_parts_kernel(AttnArgs a
   const int64_t step = (int64_t)a.kv_heads * W * kAttnTile * DP;
   const int quad = threadIdx.x % QUADS, lane = threadIdx.x / QUADS;
   const bool share = jn.parts > kAttnFewParts;  // as the forward's join
-  for (int i = blockIdx.y * (share ? 1 : LANES); i < W * rows; i += kAttnJoinBlocks * (share ? 1 : LANES)) {
+  for (int i = blockIdx.y * (share ? 1 : LANES); i < W * rows; i += gridDim.y * (share ? 1 : LANES)) {
     const int in = share ? i : i + lane;
     const int which = in >= rows, row = in - which * rows;
     const float* p = a.parts + ((((int64_t)jn.part * a.kv_heads + hk) * W + which) * kAttnTile + row) * DP + quad * 4;
@@ -1329,7 +1334,8 @@ static int attn_join(K kernel, const AttnArgs& a, hipStream_t s) {
     AttnArgs g = a;
     g.joins += i;
     g.n_joins = (int)(a.n_joins - i < most ? a.n_joins - i : most);
-    kernel<<<dim3((unsigned)(g.n_joins * g.kv_heads), kAttnJoinBlocks), kAttnThreads, 0, s>>>(g);
+    const int tiles = g.n_joins * g.kv_heads, blocks = std::min(kAttnMostJoinBlocks, std::max(kAttnJoinBlocks, kAttnJoinsTo / tiles));
+    kernel<<<dim3((unsigned)tiles, (unsigned)blocks), kAttnThreads, 0, s>>>(g);
     ST_CHECK_LAUNCH();
   }
   return ST_OK;

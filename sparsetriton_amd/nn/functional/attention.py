@@ -80,7 +80,35 @@ def _longest(items: np.ndarray, kv_heads: int) -> int:
     return int(held.max())
 
 
-def _split(steps: np.ndarray, rows: np.ndarray, kv_heads: int, dim: int, elem: int, keys: bool):
+def _part_us(parts, rows, kv_heads: int, dim: int, keys: bool) -> float:
+    return float((rows * parts)[parts > 1].sum()) * kv_heads * (dim + 2) * 8 * (2 if keys else 1) / _PART_BYTES_US
+
+
+def _split_long(steps, rows, even, kv_heads: int, dim: int, us: float, keys: bool):
+    """The same where a few tiles are much longer than the rest: the keys that all rows see beside those of a window.
+    All in even parts, or the long ones alone, in parts as long as most tiles or a half, .. a sixteenth of that, which
+    fill the slots behind those: whichever the fullest slot (``us`` a step) and the parts' bytes are least for.
+
+    16,383 causal rows x 16 x 128 on 4 key heads, window 1,024, 4 sinks, dK, dV and the join: all in even parts (1,108) 702 us,
+    the long one in parts as the rest (540, of which 28 come after all others) 835, in parts a tenth as long (964) 590.
+    """
+    usual = max(_PART_STEPS, int(np.median(steps)))
+    best, least = None, math.inf
+    for most in [None, int(steps.max(initial=1))] + [max(_PART_STEPS, usual >> i) for i in range(5)]:
+        if most is None:
+            parts, chunk = even
+        else:
+            parts, chunk = _cut(np.where(steps > 1.25 * usual, steps, 1), most)
+            chunk = np.where(parts > 1, chunk, steps)
+        cost = _longest(_items(parts, chunk, steps), kv_heads) * us
+        if (parts > 1).any():
+            cost += _JOIN_US + _part_us(parts, rows, kv_heads, dim, keys)
+        if cost < least:
+            best, least = (parts, chunk), cost
+    return best
+
+
+def _split(steps: np.ndarray, rows: np.ndarray, kv_heads: int, dim: int, elem: int, keys: bool, uneven: bool = False):
     """(parts of each tile, steps of a part), ``rows`` of each tile in use.
 
     Whole tiles take the longest one's steps, or what the fullest slot has to do; parts an even share of all steps (and
@@ -108,10 +136,12 @@ def _split(steps: np.ndarray, rows: np.ndarray, kv_heads: int, dim: int, elem: i
             parts = min((about, parts), key=lambda p: _longest(_items(*p, steps), kv_heads))
     n = parts[0]
     cut = n > 1
+    if uneven:
+        return _split_long(steps, rows, parts, kv_heads, dim, 2 * us * shared, keys)
     if not cut.any():
         return whole
     parts_us = max((int(parts[1].max()) + 1) * us, 1.15 * (total + int(n.sum()) * kv_heads) / _UNITS * shared)
-    parts_us += _JOIN_US + float((rows * n)[cut].sum()) * kv_heads * (dim + 2) * 8 * (2 if keys else 1) / _PART_BYTES_US
+    parts_us += _JOIN_US + _part_us(n, rows, kv_heads, dim, keys)
     whole_us = longest * us
     if steps.size * kv_heads > _UNITS:
         # (two to a unit at its worst; once more wait than run, a long one has had shorter ones beside it)
@@ -122,11 +152,11 @@ def _split(steps: np.ndarray, rows: np.ndarray, kv_heads: int, dim: int, elem: i
 class _Tiles:
     """Work items and joins of one pass, on the device: rows (4, 8) int32 as st_attn_args lays them out."""
 
-    def __init__(self, tile, q0, nq, k0, nk, row0, rows, lo, hi, kv_heads, dim, elem, keys, device):
+    def __init__(self, tile, q0, nq, k0, nk, row0, rows, lo, hi, kv_heads, dim, elem, keys, uneven, device):
         self.tile, step = tile, _STEP
         steps = -(-(hi - lo) // step)
         n = steps.size
-        parts, chunk = _split(steps, rows, kv_heads, dim, elem, keys)
+        parts, chunk = _split(steps, rows, kv_heads, dim, elem, keys, uneven)
         of = np.repeat(np.arange(n), parts)
         nth = np.arange(of.size) - np.repeat(np.cumsum(parts) - parts, parts)
         first = lo[of] + nth * chunk[of] * step
@@ -258,7 +288,7 @@ class AttentionSegments:
                     lo = np.maximum(0, first) * group
                 lo = np.minimum(lo, hi)
             plan = _Tiles(tile, self._q0[seg], nq[seg], self._k0[seg], nk[seg], row0, rows, lo, hi,
-                          kv_heads, dim, elem, which == "k", self.device)
+                          kv_heads, dim, elem, which == "k", which == "k" and window > 0, self.device)
             self._plans[key] = plan
         plan.use()
         return plan

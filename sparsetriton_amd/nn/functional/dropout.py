@@ -31,8 +31,9 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         (numbers,) = ctx.saved_tensors
-        # (linear in dy: the same operator, so that a gradient of the gradient is one too)
-        dx = _Dropout.apply(dy, None, numbers, ctx.p) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:  # (linear in dy: the same operator, so that a gradient of the gradient is one too)
+            dx = (_Dropout.apply if torch.is_grad_enabled() else _drop)(dy, None, numbers, ctx.p)
         return dx, dy if ctx.needs_input_grad[1] else None, None, None
 
 
