@@ -1127,7 +1127,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
   const int wave_to = windowed ? max(end_row(kw), end_row(min(kw + 31, it.nk - 1))) : 0x7FFFFFFF;
   // the rows that see all of the tile's keys
   const int tile_from = CUT ? first_query(min(it.row0 + 32 * WAVES, it.nk) - 1) * a.group : 0;
-  const int tile_to = windowed ? end_row(max(it.row0, a.sinks)) : 0x7FFFFFFF;
+  const int tile_to = windowed ? end_row(max(it.row0, min(a.sinks, it.nk))) : 0x7FFFFFFF;
 
   Stage qs, gs;
   float stat = 0.f;

@@ -108,7 +108,7 @@ def _split_long(steps, rows, even, kv_heads: int, dim: int, us: float, keys: boo
     return best
 
 
-def _split(steps: np.ndarray, rows: np.ndarray, kv_heads: int, dim: int, elem: int, keys: bool, uneven: bool = False):
+def _split(steps: np.ndarray, rows: np.ndarray, kv_heads: int, dim: int, elem: int, keys: bool, window: bool = False):
     """(parts of each tile, steps of a part), ``rows`` of each tile in use.
 
     Whole tiles take the longest one's steps, or what the fullest slot has to do; parts an even share of all steps (and
@@ -123,20 +123,23 @@ def _split(steps: np.ndarray, rows: np.ndarray, kv_heads: int, dim: int, elem: i
     longest = int(steps.max(initial=0)) + 1
     if longest * us <= total / _UNITS * shared:
         return whole
-    most = max(_PART_STEPS, -(-total // _SPLIT_TO))
+    # Tiles of a window are much alike: parts as long, all at once (single rows x 32 heads of 128 on 8 key heads, up to
+    # 1,024 / 512 workgroups: 16 rows with a window of 1,024 21.5 / 20.3 us, of 4,096 51.9 / 47.7, 32 rows with 1,024 36 / 32).
+    to = 2 * _UNITS if window and not keys else _SPLIT_TO
+    most = max(_PART_STEPS, -(-total // to))
     parts = about = _cut(steps, most)
     # Parts of a whole number of steps come to more than aimed at, at times, and the few of a last round keep the rest
     # waiting (8,191 causal rows x 16 x 128 on 4 key heads, dK and dV: 1,152 parts 890 us, 984 800; but 24 samples of up to
     # 1,500 rows x 6 x 48 fp32: 1,056 of up to 5 steps 376, 882 of up to 6 399).
-    if steps.size * kv_heads <= _SPLIT_TO:
-        while parts[0].sum() * kv_heads > _SPLIT_TO:
+    if steps.size * kv_heads <= to:
+        while parts[0].sum() * kv_heads > to:
             most += max(1, most // 16)
             parts = _cut(steps, most)
         if parts is not about:
             parts = min((about, parts), key=lambda p: _longest(_items(*p, steps), kv_heads))
     n = parts[0]
     cut = n > 1
-    if uneven:
+    if window and keys:
         return _split_long(steps, rows, parts, kv_heads, dim, 2 * us * shared, keys)
     if not cut.any():
         return whole
@@ -152,11 +155,11 @@ def _split(steps: np.ndarray, rows: np.ndarray, kv_heads: int, dim: int, elem: i
 class _Tiles:
     """Work items and joins of one pass, on the device: rows (4, 8) int32 as st_attn_args lays them out."""
 
-    def __init__(self, tile, q0, nq, k0, nk, row0, rows, lo, hi, kv_heads, dim, elem, keys, uneven, device):
+    def __init__(self, tile, q0, nq, k0, nk, row0, rows, lo, hi, kv_heads, dim, elem, keys, window, device):
         self.tile, step = tile, _STEP
         steps = -(-(hi - lo) // step)
         n = steps.size
-        parts, chunk = _split(steps, rows, kv_heads, dim, elem, keys, uneven)
+        parts, chunk = _split(steps, rows, kv_heads, dim, elem, keys, window)
         of = np.repeat(np.arange(n), parts)
         nth = np.arange(of.size) - np.repeat(np.cumsum(parts) - parts, parts)
         first = lo[of] + nth * chunk[of] * step
@@ -288,7 +291,7 @@ class AttentionSegments:
                     lo = np.maximum(0, first) * group
                 lo = np.minimum(lo, hi)
             plan = _Tiles(tile, self._q0[seg], nq[seg], self._k0[seg], nk[seg], row0, rows, lo, hi,
-                          kv_heads, dim, elem, which == "k", which == "k" and window > 0, self.device)
+                          kv_heads, dim, elem, which == "k", window > 0, self.device)
             self._plans[key] = plan
         plan.use()
         return plan
@@ -336,7 +339,7 @@ def _forward(q, k, v, segments, key_mask, causal, scale, window, stats):
     parts = _parts(kv_heads, dim, plan.slots, 0, q.device)
     if parts is not None:
         a.parts = parts.data_ptr()
-    _lib.call("st_attn_forward", ctypes.byref(a), _lib.stream_of(q.device))
+    _lib.call_on(q.device, "st_attn_forward", ctypes.byref(a))
     return o, rest, lse, q, k, v
 
 
@@ -377,7 +380,7 @@ class _Attention(torch.autograd.Function):
         parts = _parts(kv_heads, dim, plan.slots, slots, q.device)
         if parts is not None:
             a.parts = parts.data_ptr()
-        _lib.call("st_attn_backward", ctypes.byref(a), _lib.stream_of(q.device))
+        _lib.call_on(q.device, "st_attn_backward", ctypes.byref(a))
         need = ctx.needs_input_grad
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None, None
 
