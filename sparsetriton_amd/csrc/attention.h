@@ -132,6 +132,12 @@ __device__ __forceinline__ v8f regs8(const v16f& c, int j) {  // registers 8j ..
 }
 // Row (key) of register r in half `half`
 __device__ __forceinline__ int reg_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+// x where bit reg_row(r, 0) of `bits` is set, else `other`, bit by bit: whatever x is.  (A compare and a select take an idle
+// slot between them.)
+__device__ __forceinline__ float attn_where(unsigned bits, int r, float x, float other) {
+  const int keep = __builtin_amdgcn_sbfe((int)bits, reg_row(r, 0), 1);
+  return __builtin_bit_cast(float, (keep & __builtin_bit_cast(int, x)) | (~keep & __builtin_bit_cast(int, other)));
+}
 
 // ------------------------------------------------------------------ LDS tiles
 
@@ -729,7 +735,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP, ORDER, WAVES>())) vo
       for (int b = 0; b < NB; ++b) {
         const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[b][e] = (bits >> reg_row(e, 0)) & 1 ? s[b][e] : -INFINITY;
+        for (int e = 0; e < 16; ++e) s[b][e] = attn_where(bits, e, s[b][e], -INFINITY);
       }
     }
     float top = s[0][0];
@@ -1021,7 +1027,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP, ORDER, WAVES>())) vo
       if (cut || seen != ALL) {
         const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = (bits >> reg_row(e, 0)) & 1 ? s[e] : 0.f;
+        for (int e = 0; e < 16; ++e) s[e] = attn_where(bits, e, s[e], 0.f);
       }
       if constexpr (kAttnHeld<T>) power.hold<DB>(s, dq);
 #pragma unroll
@@ -1181,13 +1187,14 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
     if (rt + BQ < it.hi) fetch(rt + BQ);
     if (!active || rt + BQ <= wave_from || (windowed && rt >= wave_to)) continue;
     const bool cut = CUT && __any(from > rt || (windowed && to - rt < BQ));
-    auto sees = [&](int row) { return row >= from && (!windowed || row < to); };
+    // a bit for each row from r on that sees the key
+    auto keep = [&](int r) { return ~attn_below(from - r) & (windowed ? attn_below(to - r) : ~0ull); };
     const T *qp = ql, *gp = gl;  // (a row whose Q or dO is not finite has a delta, and so a dS, that is not)
     if (cut && flags.copied) {
       if constexpr (DK) attn_copy_finite<T, BQ, DP>(ql, copies);
       if constexpr (DV) attn_copy_finite<T, BQ, DP>(gl, copies + TILE);
       qp = copies, gp = copies + TILE;
-      if constexpr (DV) left_out.add<T, BQ, DP>(gl, ~attn_below(from - rt) & (windowed ? attn_below(to - rt) : ~0ull));
+      if constexpr (DV) left_out.add<T, BQ, DP>(gl, keep(rt));
     }
 #pragma unroll 1
     for (int b = 0; b < NB; ++b) {
@@ -1207,9 +1214,10 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * j + e] = fast_exp2(fmaf(s[4 * j + e], a.scale_log2, -L[e]));
       }
-      if (cut) {
+      if (DV && cut) {  // (dS is cut after its own product)
+        const unsigned bits = (unsigned)keep(rt + b * 32 + 4 * half);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = sees(rt + b * 32 + reg_row(e, half)) ? s[e] : 0.f;
+        for (int e = 0; e < 16; ++e) s[e] = attn_where(bits, e, s[e], 0.f);
       }
       if constexpr (DV) {
 #pragma unroll
@@ -1228,8 +1236,9 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
         for (int e = 0; e < 4; ++e) s[4 * j + e] *= fmaf(dp[4 * j + e], kAttnKeysDown<T>, -dl[e]);
       }
       if (cut) {
+        const unsigned bits = (unsigned)keep(rt + b * 32 + 4 * half);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = sees(rt + b * 32 + reg_row(e, half)) ? s[e] : 0.f;
+        for (int e = 0; e < 16; ++e) s[e] = attn_where(bits, e, s[e], 0.f);
       }
       if constexpr (kAttnHeld<T>) {
         s *= power.up;
