@@ -1021,6 +1021,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP, ORDER, WAVES>())) vo
     }
 #pragma unroll 1
     for (int b = 0; b < NB; ++b) {
+      if (CUT && NB > 1 && cut && !__any(sight.any(kt + 32 * b, 32))) continue;
       v16f s = (v16f)(0.f), dp = (v16f)(0.f);
 #pragma unroll
       for (int i = 0; i < KS && attn_in<T>(16 * i, a.D); ++i) {
@@ -1206,6 +1207,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
     }
 #pragma unroll 1
     for (int b = 0; b < NB; ++b) {
+      if (CUT && NB > 1 && (rt + 32 * b + 32 <= wave_from || (windowed && rt + 32 * b >= wave_to))) continue;
       v16f s = (v16f)(0.f), dp = (v16f)(0.f);
 #pragma unroll
       for (int i = 0; i < KS && attn_in<T>(16 * i, a.D); ++i) {

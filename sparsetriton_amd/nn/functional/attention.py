@@ -36,6 +36,7 @@ _SMALL_TILES = 1.8
 # join's launch, and the bytes of partial results a microsecond.
 _UNITS, _SPLIT_TO, _PART_STEPS = 256, 1024, 4
 _SHARED, _JOIN_US, _PART_BYTES_US = {2: 0.75, 4: 0.88}, 7.0, 8.0e6
+_NO_WINDOW = (0, 0)
 
 
 def _step_us(dim: int, elem: int, keys: bool) -> float:
@@ -248,13 +249,11 @@ class AttentionSegments:
         seg = np.repeat(np.arange(n.size), n)
         return tile, seg, (np.arange(seg.size) - np.repeat(np.cumsum(n) - n, n)) * tile
 
-    def _window(self, causal: bool, window: Optional[int], sinks: int):
-        """(window, sinks) as the kernels take them: (0, 0) where no row has a key that they leave out."""
-        if window is None:
-            return 0, 0
+    def _window(self, causal: bool, window: int, sinks: int):
+        """(window, sinks) as the kernels take them: none where no row has a key that they leave out."""
         sinks = min(sinks, self._most_k)
         if sinks >= self._most_k or window >= (self._most_k - sinks if causal else max(self._most_q, self._most_k)):
-            return 0, 0
+            return _NO_WINDOW
         return window, sinks
 
     def _plan(self, which: str, group: int, kv_heads: int, causal: bool, row_bytes: int, elem: int = 2, window: int = 0,
@@ -455,7 +454,9 @@ def sparse_attention(
         window, sinks = operator.index(window), operator.index(sinks)
         if window < 1 or sinks < 0:
             raise ValueError(f"a window has a key at least, sinks are not negative (got {window} and {sinks})")
-    window = segments._window(causal, window, sinks)
+        window = segments._window(causal, window, sinks)
+    else:
+        window = _NO_WINDOW
     refuse_tangents("sparse_attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attention.apply(q, k, v, segments, key_mask, causal, scale, window)

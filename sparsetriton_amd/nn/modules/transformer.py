@@ -60,6 +60,8 @@ class SparseAttention(nn.Module):
     ``q_norm`` and ``k_norm`` before they turn.
     """
 
+    window, sinks = None, 0  # (of a module that was pickled before it had them)
+
     def __init__(self, channels: int, heads: int, kv_heads: Optional[int] = None, head_dim: Optional[int] = None,
                  axes: Optional[Sequence[int]] = None, base: float = 10000.0, causal: bool = False, bias: bool = True,
                  window: Optional[int] = None, sinks: int = 0, qk_norm: bool = False, qk_eps: float = 1e-6):
@@ -88,7 +90,7 @@ class SparseAttention(nn.Module):
             segments = AttentionSegments.from_tensor(x)
         qkv = self.qkv(x.F).view(x.F.shape[0], self.heads + 2 * self.kv_heads, self.head_dim)
         q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)
-        if self.q_norm is not None:
+        if getattr(self, "q_norm", None) is not None:
             q, k = sparse_qk_norm_rotary(q, k, x, self.rotary, self.q_norm, self.k_norm, eps=self.qk_eps)
         else:
             q, k = sparse_rotary(q, k, x, self.rotary)
@@ -117,6 +119,8 @@ class SparseTransformerBlock(nn.Module):
     ``window``, ``sinks`` and ``qk_norm`` as in ``SparseAttention``; in training a share ``dropout`` of each
     branch's elements is left out of the sum with the stream.
     """
+
+    dropout = 0.0  # (of a module that was pickled before it had one)
 
     def __init__(self, channels: int, heads: int, kv_heads: Optional[int] = None, mlp_ratio: float = 4.0, eps: float = 1e-5,
                  axes: Optional[Sequence[int]] = None, causal: bool = False, window: Optional[int] = None, sinks: int = 0,

@@ -150,7 +150,6 @@ def test_tile_lists_cover_what_is_seen_once(ql, kl, group, causal, window, sinks
 
 def test_a_window_that_leaves_nothing_out_is_none():
     s = AttentionSegments([5, 9], [20, 7], device="cpu")
-    assert s._window(True, None, 0) == (0, 0)
     assert s._window(True, 20, 0) == (0, 0) and s._window(True, 19, 0) == (19, 0)
     assert s._window(True, 16, 4) == (0, 0) and s._window(True, 15, 4) == (15, 4)
     assert s._window(False, 20, 0) == (0, 0) and s._window(False, 16, 4) == (16, 4)
