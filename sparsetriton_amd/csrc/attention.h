@@ -441,6 +441,8 @@ __device__ __forceinline__ AttnItem attn_item(const AttnArgs& a, int& hk) {
 // Which keys a row sees (a template argument: the kernels of one do not pay for another's).
 constexpr int kAttnAll = 0, kAttnCausal = 1, kAttnWindow = 2;
 
+// The lowest n bits of 32, for the places 0 .. 27 that a lane's registers have of a block (reg_row).
+__device__ __forceinline__ unsigned attn_below28(int n) { return (1u << min(max(n, 0), 31)) - 1; }
 // The lowest n bits of 64.
 __device__ __forceinline__ uint64_t attn_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : ~0ull >> (64 - n); }
 
@@ -497,6 +499,14 @@ struct AttnSight {
     if constexpr (ORDER == kAttnWindow)
       return !live || (!both(kt, n) && from(at) <= kt + gap && last(at) - (kt + gap) >= n - 1);
     return at - kt >= n - 1;
+  }
+  // a bit for each place from kt on, as far as reg_row goes, that the row sees
+  __device__ __forceinline__ unsigned bits(int kt) const {
+    if constexpr (ORDER != kAttnWindow) return attn_below28(at - kt + 1);
+    const int p = kt + gap;
+    unsigned seen = attn_below28(last(at) - p + 1) & ~attn_below28(from(at) - p);
+    if (kt < sinks) seen |= attn_below28((causal ? min(sinks, at + 1) : sinks) - kt);
+    return seen;
   }
   // a bit for each place from kt on that the row sees, of those that `seen` has
   __device__ __forceinline__ uint64_t keep(int kt, uint64_t seen) const {
@@ -737,11 +747,10 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP, ORDER, WAVES>())) vo
       scores();
     }
     const bool cut = CUT && __any(!sight.all(kt, BK));  // by the causal order or the window
-    const uint64_t keep = CUT ? sight.keep(kt, seen) : seen;
     if (CUT && (cut || seen != ALL)) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
+        const unsigned bits = sight.bits(kt + 32 * b + 4 * half) & ((unsigned)(seen >> (32 * b)) >> (4 * half));
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[b][e] = attn_where(bits, e, s[b][e], -INFINITY);
       }
@@ -778,7 +787,7 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP, ORDER, WAVES>())) vo
     if (cut && flags.copied) {
       attn_copy_finite<T, BK, DP>(vl, tiles + 4 * TILE);
       vp = tiles + 4 * TILE;
-      left_out.add<T, BK, DP>(vl, keep);
+      left_out.add<T, BK, DP>(vl, sight.keep(kt, seen));
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -1013,7 +1022,6 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP, ORDER, WAVES>())) vo
     if (kt + BK < it.hi) fetch(kt + BK);
     if (!active || (CUT && !__any(sight.any(kt, BK)))) continue;
     const bool cut = CUT && __any(!sight.all(kt, BK));
-    const uint64_t keep = CUT ? sight.keep(kt, seen) : seen;
     const T* kp = kl;  // (a row that sees a key that is not finite has a dS that is not)
     if (cut && flags.copied) {
       attn_copy_finite<T, BK, DP>(kl, tiles + 4 * TILE);
@@ -1034,7 +1042,8 @@ __global__ __launch_bounds__(64 * WAVES, (attn_waves<T, DP, ORDER, WAVES>())) vo
       for (int e = 0; e < 16; ++e)
         s[e] = fast_exp2(fmaf(s[e], a.scale_log2, -lse)) * (kAttnHeld<T> ? fmaf(dp[e], power.up, -held) : dp[e] - delta);
       if (cut || seen != ALL) {
-        const unsigned bits = (unsigned)(keep >> (32 * b)) >> (4 * half);
+        unsigned bits = (unsigned)(seen >> (32 * b)) >> (4 * half);
+        if constexpr (CUT) bits &= sight.bits(kt + 32 * b + 4 * half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = attn_where(bits, e, s[e], 0.f);
       }
@@ -1196,14 +1205,14 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
     if (rt + BQ < it.hi) fetch(rt + BQ);
     if (!active || rt + BQ <= wave_from || (windowed && rt >= wave_to)) continue;
     const bool cut = CUT && __any(from > rt || (windowed && to - rt < BQ));
-    // a bit for each row from r on that sees the key
-    auto keep = [&](int r) { return ~attn_below(from - r) & (windowed ? attn_below(to - r) : ~0ull); };
+    // a bit for each row from r on, as far as reg_row goes, that sees the key
+    auto bits_of = [&](int r) { return ~attn_below28(from - r) & (windowed ? attn_below28(to - r) : ~0u); };
     const T *qp = ql, *gp = gl;  // (a row whose Q or dO is not finite has a delta, and so a dS, that is not)
     if (cut && flags.copied) {
       if constexpr (DK) attn_copy_finite<T, BQ, DP>(ql, copies);
       if constexpr (DV) attn_copy_finite<T, BQ, DP>(gl, copies + TILE);
       qp = copies, gp = copies + TILE;
-      if constexpr (DV) left_out.add<T, BQ, DP>(gl, keep(rt));
+      if constexpr (DV) left_out.add<T, BQ, DP>(gl, ~attn_below(from - rt) & (windowed ? attn_below(to - rt) : ~0ull));
     }
 #pragma unroll 1
     for (int b = 0; b < NB; ++b) {
@@ -1225,7 +1234,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
         for (int e = 0; e < 4; ++e) s[4 * j + e] = fast_exp2(fmaf(s[4 * j + e], a.scale_log2, -L[e]));
       }
       if (DV && cut) {  // (dS is cut after its own product)
-        const unsigned bits = (unsigned)keep(rt + b * 32 + 4 * half);
+        const unsigned bits = bits_of(rt + b * 32 + 4 * half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = attn_where(bits, e, s[e], 0.f);
       }
@@ -1246,7 +1255,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHAT == (kAttnDv | kAttnDk) ? attn_wav
         for (int e = 0; e < 4; ++e) s[4 * j + e] *= fmaf(dp[4 * j + e], kAttnKeysDown<T>, -dl[e]);
       }
       if (cut) {
-        const unsigned bits = (unsigned)keep(rt + b * 32 + 4 * half);
+        const unsigned bits = bits_of(rt + b * 32 + 4 * half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = attn_where(bits, e, s[e], 0.f);
       }
