@@ -129,36 +129,57 @@ struct QkVec {
   }
 };
 
-// How a lane holds its share of a head: NV chunks `lanes` apart.  A chunk is a
-// vector of V channels and the vector of those that they turn with, or
-// (interleaved vectors of more than one channel) one that holds both of each
-// pair.  Chunks past the pairs turn by nothing: the table has (1, 0) for
-// them, and their second vector, like all of a chunk that the head does not have, is
+// How a lane holds its share of a head: NV chunks `lanes` apart.  A chunk is
+//   kQkApart       a vector of V channels and the vector of those that they turn with,
+//   kQkPairs       the same of single channels, interleaved pairs,
+//   kQkInside      a vector that holds both of each (interleaved) pair, or
+//   kQkExchanged   a vector whose channels' partners are with other lanes, at any distance:
+// the lanes write their values to a row of LDS for each place in the vector and read their
+// partners'; for pairs whose number V does not divide.  200,000 rows x (8 + 8) x 64 bf16, forward /
+// backward in us: 32 pairs apart 156 / 275, 15 pairs exchanged 207 / 352 (a channel a lane, apart, 720 / 1,112),
+// 20 pairs exchanged 203 / 352 (apart in half vectors 237 / 424), 15 interleaved pairs inside 152 / 263.
+// Channels past the pairs turn by nothing: the table has (1, 0) for them, and a
+// second vector that is not there, like all of a chunk that the head does not have, is
 // read as zeros and not stored, by an offset past the buffers.
-template <typename T, int V, int NV, bool INTERLEAVED>
+enum QkMode { kQkApart, kQkPairs, kQkInside, kQkExchanged };
+constexpr int kQkExchange = kQkThreads / 64 * (8 * 64 + 1);  // floats: for each wave eight rows and a zero
+template <typename T, int V, int NV, int MODE>
 struct QkLane {
   using Vec = QkVec<T, V>;
-  static constexpr bool kInside = INTERLEAVED && V > 1;
-  static constexpr int H = kInside ? 1 : 2, M = NV * H;  // vectors of a chunk, of the lane
+  static constexpr bool kInside = MODE == kQkInside, kOne = kInside || MODE == kQkExchanged;
+  static constexpr int H = kOne ? 1 : 2, M = NV * H;  // vectors of a chunk, of the lane
   unsigned off[M];  // bytes from the head's first channel
   int w[M];         // channel (any where there is none: its x is zero)
   int turns[NV];    // of the table's row
+  int partner[MODE == kQkExchanged ? V : 1];  // where the partners are in LDS
+  float* exchange;                            // the wave's
 
-  __device__ __forceinline__ explicit QkLane(const QkArgs<T>& g) {
-    const int pair_chunks = kInside ? 2 * g.P / V : g.P / V;
+  __device__ __forceinline__ QkLane(const QkArgs<T>& g, float* lds) {
+    const int pair_chunks = g.P / V;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (threadIdx.x & (g.lanes - 1)) + k * g.lanes;
-      const bool live = c < g.chunks, pair = c < pair_chunks;
-      const int at = pair ? c * (INTERLEAVED && V == 1 ? 2 : V) : 2 * g.P + (c - pair_chunks) * V;
+      const bool live = c < g.chunks, pair = !kOne && c < pair_chunks;
+      const int at = kOne ? c * V : pair ? c * (MODE == kQkPairs ? 2 : V) : 2 * g.P + (c - pair_chunks) * V;
       off[k * H] = live ? at * (unsigned)sizeof(T) : (unsigned)kOobOffset;
       w[k * H] = live ? at : 0;
-      if constexpr (!kInside) {
-        const int second = at + (INTERLEAVED ? 1 : g.P);
+      if constexpr (!kOne) {
+        const int second = at + (MODE == kQkPairs ? 1 : g.P);
         off[k * H + 1] = pair ? second * (unsigned)sizeof(T) : (unsigned)kOobOffset;
         w[k * H + 1] = pair ? second : 0;
       }
       turns[k] = live ? c * (kInside ? V / 2 : V) : 0;
+    }
+    if constexpr (MODE == kQkExchanged) {
+      static_assert(NV == 1, "a head's lanes are neighbours");
+      exchange = lds + (threadIdx.x >> 6) * (8 * 64 + 1);
+      const int lane = threadIdx.x & 63, head = lane & ~(g.lanes - 1);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int c = (lane - head) * V + e, to = c < g.P ? c + g.P : c - g.P;
+        partner[e] = c < 2 * g.P ? to % V * 64 + head + to / V : 8 * 64;
+      }
+      if (lane == 0) exchange[8 * 64] = 0.f;
     }
   }
   // the weights of vector m, `all` the tensor's
@@ -182,6 +203,21 @@ struct QkLane {
   // x turned by the row's table, forwards or back
   template <bool BACK>
   __device__ __forceinline__ void turn(const float2* table, float (&x)[M][V]) const {
+    if constexpr (MODE == kQkExchanged) {  // (within a wave, whose LDS accesses keep their order)
+#pragma unroll
+      for (int e = 0; e < V; ++e) exchange[e * 64 + (threadIdx.x & 63)] = x[0][e];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float2 t = table[turns[0] + e];
+        const float y = exchange[partner[e]] * t.y;
+        x[0][e] = x[0][e] * t.x + (BACK ? -y : y);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      return;
+    }
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -192,21 +228,25 @@ struct QkLane {
         const float s = BACK ? -t.y : t.y, u = a * t.x - b * s;
         b = a * s + b * t.x;
         a = u;
-        if (BACK && !kInside && !has(k * H + H - 1)) b = 0.f;  // (zero times an infinity, for the sums that follow)
+        if (BACK && !kOne && !has(k * H + H - 1)) b = 0.f;  // (zero times an infinity, for the sums that follow)
       }
   }
 };
 
-// Cosines and sines of `rows` rows from row0 on, and the weights, in LDS.
-template <typename T>
+// Cosines and sines of `rows` rows from row0 on, and the weights, in LDS.  kQkExchanged: an entry for each channel, with the
+// sign that its partner's sine has there.
+template <int MODE, typename T>
 __device__ __forceinline__ void qk_table(const QkArgs<T>& g, int64_t row0, int rows, float2* table) {
 #pragma unroll 1
   for (int i = threadIdx.x; i < rows * g.table_row; i += kQkThreads) {
-    const int r = i / g.table_row, p = i - r * g.table_row;
+    const int r = i / g.table_row, d = i - r * g.table_row;
+    const bool second = MODE == kQkExchanged && d >= g.P && d < 2 * g.P;
+    const int p = second ? d - g.P : d;
     float s = 0.f, c = 1.f;
     if (p < g.P) {
       const double t = qk_pos(g.pos, g.pos_dtype, (row0 + r) * g.pos_row + g.axis[p]) * g.turns[p];
       sincospif(2.f * (float)(t - rint(t)), &s, &c);
+      if (MODE == kQkExchanged && !second) s = -s;
     }
     table[i] = make_float2(c, s);
   }
@@ -253,16 +293,17 @@ struct QkWalk {
   }
 };
 
-template <typename T, int V, int NV, bool INTERLEAVED>
+template <typename T, int V, int NV, int MODE>
 __global__ __launch_bounds__(kQkThreads) void qk_forward_kernel(QkArgs<T> g) {
-  using Lane = QkLane<T, V, NV, INTERLEAVED>;
+  using Lane = QkLane<T, V, NV, MODE>;
   constexpr int M = Lane::M;
   __shared__ float2 table[kQkTable];
   __shared__ __attribute__((aligned(32))) float weights[2 * ST_QK_MAX_DIM];
   const int64_t row0 = (int64_t)blockIdx.x * g.rows;
   const int rows = g.n - row0 < g.rows ? (int)(g.n - row0) : g.rows;
   const int side = kQkThreads >> g.lane_bits, group = threadIdx.x >> g.lane_bits;
-  const Lane lane(g);
+  __shared__ float exchange[MODE == kQkExchanged ? kQkExchange : 1];
+  const Lane lane(g, exchange);
   // q's heads, then k's, each in steps of a head a group of lanes; a head's loads go out while the one before it is at
   // work, the first one's before the table is made
   const int q_steps = (rows * g.heads[0] + side - 1) / side, steps = q_steps + (rows * g.heads[1] + side - 1) / side;
@@ -278,7 +319,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_forward_kernel(QkArgs<T> g) {
     lane.load(make_rsrc(g.in[w] + row0 * g.in_row[w], kOobOffset), walk.row < rows ? walk.off[0] : kOobOffset, next);
   };
   load(0);
-  qk_table(g, row0, rows, table);
+  qk_table<MODE>(g, row0, rows, table);
   qk_weights(g, weights);
   __syncthreads();
 #pragma unroll 1
@@ -313,15 +354,16 @@ __global__ __launch_bounds__(kQkThreads) void qk_forward_kernel(QkArgs<T> g) {
 
 // q's heads of all of a workgroup's rows, then k's: the sums of one weight's
 // gradient in registers at a time, for a second table.
-template <typename T, int V, int NV, bool INTERLEAVED>
+template <typename T, int V, int NV, int MODE>
 __global__ __launch_bounds__(kQkThreads) void qk_backward_kernel(QkArgs<T> g) {
-  using Lane = QkLane<T, V, NV, INTERLEAVED>;
+  using Lane = QkLane<T, V, NV, MODE>;
   constexpr int M = Lane::M;
   __shared__ float2 table[kQkTable];
   __shared__ __attribute__((aligned(32))) float weights[2 * ST_QK_MAX_DIM];
   __shared__ float sums[3][ST_QK_MAX_DIM];
   const int side = kQkThreads >> g.lane_bits, group = threadIdx.x >> g.lane_bits;
-  const Lane lane(g);
+  __shared__ float exchange[MODE == kQkExchanged ? kQkExchange : 1];
+  const Lane lane(g, exchange);
   const int64_t first = g.per * blockIdx.x, end = first + g.per < g.n ? first + g.per : g.n;
   qk_weights(g, weights);
 #pragma unroll 1
@@ -347,7 +389,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_backward_kernel(QkArgs<T> g) {
       };
       walk.first(g, w, group, strides);
       load();
-      qk_table(g, row0, rows, table);
+      qk_table<MODE>(g, row0, rows, table);
       __syncthreads();
 #pragma unroll 1
       for (int step = 0; step < steps; ++step) {
@@ -418,8 +460,8 @@ __global__ __launch_bounds__(kQkThreads) void qk_backward_kernel(QkArgs<T> g) {
 
 // Whether vectors of V channels cut every head evenly and lie at their own size's alignment.
 template <typename T, int V>
-static bool qk_vec_ok(const QkArgs<T>& g, bool interleaved) {
-  if (g.D % V || (interleaved ? 2 * g.P : g.P) % V) return false;
+static bool qk_vec_ok(const QkArgs<T>& g) {
+  if (g.D % V) return false;
   for (int w = 0; w < 2; ++w) {
     if (!g.heads[w]) continue;
     if (g.in_row[w] % V || g.in_head[w] % V) return false;
@@ -435,7 +477,7 @@ static int64_t qk_table_rows(int table_row) { return kQkTable / table_row; }
 // Workgroups of the backward: a row each while there are fewer than its limit.
 static int64_t qk_groups(int64_t n) { return n < kQkMaxGroups ? (n > 0 ? n : 1) : kQkMaxGroups; }
 
-template <typename T, int V, int NV, bool INTERLEAVED>
+template <typename T, int V, int NV, int MODE>
 static int qk_launch(QkArgs<T> g, bool backward, hipStream_t s) {
   for (int w = 0; w < 2; ++w) {
     const int d = g.heads[w], side = kQkThreads / g.lanes;
@@ -458,7 +500,7 @@ static int qk_launch(QkArgs<T> g, bool backward, hipStream_t s) {
     const int64_t rows = qk_table_rows(g.table_row);  // of a table
     g.rows = (int)(reach < rows ? reach : rows);
     g.per = (g.n + qk_groups(g.n) - 1) / qk_groups(g.n);
-    qk_backward_kernel<T, V, NV, INTERLEAVED><<<(unsigned)qk_groups(g.n), kQkThreads, 0, s>>>(g);
+    qk_backward_kernel<T, V, NV, MODE><<<(unsigned)qk_groups(g.n), kQkThreads, 0, s>>>(g);
     ST_CHECK_LAUNCH();
     return ST_OK;
   }
@@ -479,7 +521,7 @@ static int qk_launch(QkArgs<T> g, bool backward, hipStream_t s) {
       part.in[w] = g.in[w] + row * g.in_row[w];
       part.out[w] = g.out[w] + row * g.heads[w] * g.D;
     }
-    qk_forward_kernel<T, V, NV, INTERLEAVED><<<st_blocks(part.n, g.rows), kQkThreads, 0, s>>>(part);
+    qk_forward_kernel<T, V, NV, MODE><<<st_blocks(part.n, g.rows), kQkThreads, 0, s>>>(part);
     ST_CHECK_LAUNCH();
   }
   return ST_OK;
@@ -487,24 +529,31 @@ static int qk_launch(QkArgs<T> g, bool backward, hipStream_t s) {
 
 template <typename T, int V>
 static int qk_vectors(QkArgs<T> g, bool interleaved, bool backward, hipStream_t s) {
-  g.table_row = g.P + (interleaved && V > 1 ? (g.D - 2 * g.P) / 2 : g.D - 2 * g.P);
-  g.chunks = (interleaved && V > 1 ? 2 * g.P / V : g.P / V) + (g.D - 2 * g.P) / V;
-  // Vectors side by side of a lane: two where both channels of a pair are in one, as many bytes as with two of them.
   auto lanes = [&](int nv) {
     g.lanes = 1, g.lane_bits = 0;
     while (g.lanes * nv < g.chunks) g.lanes *= 2, ++g.lane_bits;
     return g.lanes <= 64;
   };
   if constexpr (V > 1) {
-    if (interleaved) return lanes(2) ? qk_launch<T, V, 2, true>(g, backward, s) : ST_ERR_UNSUPPORTED;
+    g.chunks = g.D / V;
+    if (interleaved) {  // (two vectors a lane: as many bytes as with the two of a chunk in the other modes)
+      g.table_row = g.D / 2;
+      return lanes(2) ? qk_launch<T, V, 2, kQkInside>(g, backward, s) : ST_ERR_UNSUPPORTED;
+    }
+    if (g.P % V) {
+      g.table_row = g.D;
+      return lanes(1) ? qk_launch<T, V, 1, kQkExchanged>(g, backward, s) : ST_ERR_UNSUPPORTED;
+    }
   }
-  if (lanes(1)) return interleaved ? qk_launch<T, V, 1, true>(g, backward, s) : qk_launch<T, V, 1, false>(g, backward, s);
-  if constexpr (ST_QK_MAX_DIM / V > 64) {  // (heads longer than 64 vectors)
-    constexpr int NV = ST_QK_MAX_DIM / V / 64;
-    lanes(NV);
-    return interleaved ? qk_launch<T, V, NV, true>(g, backward, s) : qk_launch<T, V, NV, false>(g, backward, s);
+  g.table_row = g.D - g.P;
+  g.chunks = (g.D - g.P) / V;
+  constexpr int NV = ST_QK_MAX_DIM / V > 64 ? ST_QK_MAX_DIM / V / 64 : 1;
+  const bool one = lanes(1);
+  if (!one) lanes(NV);  // (heads longer than 64 vectors)
+  if constexpr (V == 1) {
+    if (interleaved) return one ? qk_launch<T, V, 1, kQkPairs>(g, backward, s) : qk_launch<T, V, NV, kQkPairs>(g, backward, s);
   }
-  return ST_ERR_UNSUPPORTED;
+  return one ? qk_launch<T, V, 1, kQkApart>(g, backward, s) : qk_launch<T, V, NV, kQkApart>(g, backward, s);
 }
 
 template <typename T>
@@ -532,9 +581,9 @@ static int qk_run(const st_qk_norm_args* a, bool backward, hipStream_t s) {
   int rc = ST_OK;
   if (g.n == 0)
     ;  // (no rows: the weights' gradients are sums of nothing)
-  else if (qk_vec_ok<T, V>(g, il))
+  else if (qk_vec_ok<T, V>(g))
     rc = qk_vectors<T, V>(g, il, backward, s);
-  else if (qk_vec_ok<T, V / 2>(g, il))
+  else if (qk_vec_ok<T, V / 2>(g) && (il || g.P % (V / 2) == 0 || g.D / (V / 2) <= 64))
     rc = qk_vectors<T, V / 2>(g, il, backward, s);
   else
     rc = qk_vectors<T, 1>(g, il, backward, s);

@@ -103,6 +103,18 @@ def test_heads(device, dim, axes, interleaved, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,axes", [(8, (2,)), (8, (6,)), (16, (2, 4)), (16, (14,)), (24, (10,)), (24, (2, 2, 2)), (32, (2,)), (40, (36,)),
+                                      (48, (22, 24)), (64, (10, 14, 6)), (64, (62,)), (64, (20, 20)), (80, (26,)), (96, (2, 30, 26)),
+                                      (128, (42, 42, 42)), (128, (2,)), (256, (254,)), (256, (10, 20)), (256, (4,)), (68, (6, 20))])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_any_number_of_pairs(device, dim, axes, interleaved, dtype):
+    """Pairs that no vector divides: partners with other lanes, and vectors half of which turn."""
+    q, k, wq, wk, pos = _make(131, 5, 3, dim, axes, dtype, device, dim + len(axes))
+    _check(q, k, pos, RotaryAxes(dim, axes, interleaved=interleaved), wq, wk)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 2, 31, 1023, 1025, 20_011])
 @pytest.mark.parametrize("pdtype", [torch.int16, torch.int32, torch.int64, torch.float32])
 def test_rows_and_position_types(device, n, pdtype):
