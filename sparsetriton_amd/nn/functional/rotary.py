@@ -180,10 +180,15 @@ def _qk_args(q, k, q_weight, k_weight, positions, axes, eps):
 
 def _qk_forward(q, k, q_weight, k_weight, positions, axes, eps):
     a, held = _qk_args(q, k, q_weight, k_weight, positions, axes, eps)
-    out = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k)]
-    a.q_out, a.k_out = _lib.ptr(out[0]), _lib.ptr(out[1])
+    q_out = k_out = None
+    if q is not None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        a.q_out = q_out.data_ptr()
+    if k is not None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        a.k_out = k_out.data_ptr()
     _lib.call_on(positions.device, "st_qk_norm_rotary", ctypes.byref(a))
-    return out[0], out[1], held
+    return q_out, k_out, held
 
 
 class _QkNormRotary(torch.autograd.Function):
@@ -259,13 +264,16 @@ def sparse_qk_norm_rotary(
             raise ValueError(f"{what} without its tensor")
         if w.shape != (axes.head_dim,) or w.device != first.device:
             raise ValueError(f"{what} must be ({axes.head_dim},) on {first.device} (got {tuple(w.shape)} on {w.device})")
-        _lib.feat_code(w.dtype)
+        if w.dtype not in _lib.FEAT_DTYPES:
+            _lib.feat_code(w.dtype)
     eps = float(eps)
     if not (eps >= 0 and math.isfinite(eps)):
         raise ValueError(f"eps must not be negative (got {eps})")
-    if sum(t.shape[1] for t in (q, k) if t is not None) >= 1 << 15:
+    if (0 if q is None else q.shape[1]) + (0 if k is None else k.shape[1]) >= 1 << 15:
         raise ValueError("q and k have at most 32,767 heads together")
     refuse_tangents("sparse_qk_norm_rotary", q, k, q_weight, k_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (
+            (q is not None and q.requires_grad) or (k is not None and k.requires_grad)
+            or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
         return _QkNormRotary.apply(q, k, q_weight, k_weight, pos.detach(), axes, eps)
     return _qk_forward(q, k, q_weight, k_weight, pos, axes, eps)[:2]
