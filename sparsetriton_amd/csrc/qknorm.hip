@@ -138,7 +138,8 @@ struct QkVec {
 // partners'; for pairs whose number V does not divide.  200,000 rows x (8 + 8) x 64 bf16, forward /
 // backward in us: 32 pairs apart 156 / 275, 15 pairs exchanged 207 / 352 (a channel a lane, apart, 720 / 1,112),
 // 20 pairs exchanged 203 / 352 (apart in half vectors 237 / 424), 15 interleaved pairs inside 152 / 263.
-// Channels past the pairs turn by nothing: the table has (1, 0) for them, and a
+// Channels past the pairs turn by nothing: the table has (1, 0) for them (kQkExchanged; the
+// other forms leave them as they are, whatever lies beside them), and a
 // second vector that is not there, like all of a chunk that the head does not have, is
 // read as zeros and not stored, by an offset past the buffers.
 enum QkMode { kQkApart, kQkPairs, kQkInside, kQkExchanged };
@@ -151,10 +152,11 @@ struct QkLane {
   unsigned off[M];  // bytes from the head's first channel
   int w[M];         // channel (any where there is none: its x is zero)
   int turns[NV];    // of the table's row
+  int pairs;        // of the head
   int partner[MODE == kQkExchanged ? V : 1];  // where the partners are in LDS
   float* exchange;                            // the wave's
 
-  __device__ __forceinline__ QkLane(const QkArgs<T>& g, float* lds) {
+  __device__ __forceinline__ QkLane(const QkArgs<T>& g, float* lds) : pairs(g.P) {
     const int pair_chunks = g.P / V;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -225,10 +227,12 @@ struct QkLane {
         const float2 t = table[turns[k] + i];
         float& a = kInside ? x[k][2 * i] : x[k * H][i];
         float& b = kInside ? x[k][2 * i + 1] : x[k * H + H - 1][i];
-        const float s = BACK ? -t.y : t.y, u = a * t.x - b * s;
-        b = a * s + b * t.x;
-        a = u;
-        if (BACK && !kOne && !has(k * H + H - 1)) b = 0.f;  // (zero times an infinity, for the sums that follow)
+        const float s = BACK ? -t.y : t.y, u = a * t.x - b * s, v = a * s + b * t.x;
+        // Past the pairs: as they are (zero times an infinity is a NaN).  A second vector that is not there is zeros when it
+        // turns back, and what a weight makes of them when it turns.
+        const bool turned = kInside ? turns[k] + i < pairs : has(k * H + H - 1);
+        a = turned || (BACK && !kInside) ? u : a;
+        b = turned ? v : kInside ? b : 0.f;
       }
   }
 };

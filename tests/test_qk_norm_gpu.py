@@ -268,6 +268,50 @@ def test_not_finite_stays_in_its_head(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,axes,dtype", [(16, (6, 6), torch.float32), (16, (4, 4), torch.float32), (15, (2, 4), torch.float32),
+                                            (18, (4, 4), torch.float32), (16, (6, 6), torch.bfloat16), (48, (16, 16), torch.bfloat16),
+                                            (20, (10,), torch.float16), (256, (90, 102), torch.float32), (255, (2, 4), torch.bfloat16)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_not_finite_stays_in_its_pair(device, dim, axes, dtype, interleaved, bad):
+    """Channels past the pairs turn by nothing: what is not finite in one channel of a weight, an input or a gradient
+    reaches the channel that turns with it and what the head's sums make of it, nothing else."""
+    n, axes = 37, RotaryAxes(dim, axes, interleaved=interleaved)
+    q, _, wq, _, pos = _make(n, 3, 1, dim, axes.axes, dtype, device, dim + interleaved)
+    dy = torch.randn((n, 3, dim), generator=torch.Generator().manual_seed(dim)).to(device, dtype)
+
+    def step(x, w, d):
+        x, w = (t.clone().requires_grad_(True) for t in (x, w))
+        y = sparse_qk_norm_rotary(x, None, pos, axes, w)[0]
+        return (y.detach(),) + torch.autograd.grad(y, (x, w), d)
+
+    clean = step(q, wq, dy)
+    p = axes.pairs
+    for c in sorted({0, 2 * p - 1, 2 * p, 2 * p + 1, dim - 2, dim - 1}):
+        partner = c if c >= 2 * p else c ^ 1 if interleaved else (c + p) % (2 * p)
+        others = torch.tensor([i for i in range(dim) if i not in (c, partner)], device=device)
+        w = wq.clone()
+        w[c] = bad
+        y = step(q, w, dy)[0]
+        assert torch.equal(y[..., others], clean[0][..., others]) and not torch.isfinite(y[..., c]).any(), c
+        x = q.clone()
+        x[2, 1, c] = bad
+        y = step(x, wq, dy)[0]
+        assert torch.isnan(y[2, 1, c])
+        assert torch.isnan(y[2, 1]).all() if bad != bad else not y[2, 1, others].any(), c  # (divided by an infinity)
+        keep = torch.ones((n, 3), dtype=torch.bool, device=device)
+        keep[2, 1] = False
+        assert torch.equal(y[keep], clean[0][keep])
+        d = dy.clone()
+        d[2, 1, [c, partner]] = 0
+        zero = step(q, wq, d)
+        d[2, 1, c] = bad
+        _, dx, dw = step(q, wq, d)
+        assert torch.equal(dw[others], zero[2][others]) and not torch.isfinite(dw[c]), c
+        assert torch.equal(dx[keep], clean[1][keep])
+
+
+@pytest.mark.gpu
 def test_same_as_the_rotation_of_normalised_heads(device):
     """Heads whose mean square is one already, no weight and eps = 0: sparse_rotary, to a few roundings."""
     axes = RotaryAxes(64, (24, 24, 16))
