@@ -893,9 +893,11 @@ int st_rotary(const st_rotary_args* args, st_stream_t stream);
  * (rows and heads at the strides dq_row, ...), dq, dk (contiguous) those of q and
  * k; dq_weight, dk_weight (of weight_dtype, NULL = not wanted) are added over
  * rows and heads in a fixed order, and need a workspace of at least
- * st_qk_norm_rotary_workspace floats.
+ * st_qk_norm_rotary_workspace floats.  Of each tensor a row's stride and all heads'
+ * are at most ST_QK_REACH bytes together.
  */
 #define ST_QK_MAX_DIM 256
+#define ST_QK_REACH 0x7FFFFBF0
 typedef struct st_qk_norm_args {
   const void* q;
   const void* k;

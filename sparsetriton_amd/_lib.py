@@ -34,7 +34,7 @@ COLUMN_SUM_NOALLOC_MAX_C = 2048
 MAX_KVOL = 512
 TILE_ROWS = 128
 ATTN_TILE, ATTN_SMALL_TILE, ATTN_SMALL_TILE_BYTES, ATTN_MAX_DIM, ATTN_WORDS = 128, 32, 128, 128, 8
-QK_MAX_DIM = 256
+QK_MAX_DIM, QK_REACH = 256, 0x7FFFFBF0
 
 
 class OutGeom(ctypes.Structure):

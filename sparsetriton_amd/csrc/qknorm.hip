@@ -33,7 +33,8 @@ constexpr int kQkTable = 2048;  // cosine / sine pairs in LDS (16 KB)
 // Lanes' worth of heads in a forward workgroup, about (512 / 1,024: 65,537 x (16 + 4) x 128 bf16 142 / 125 us,
 // 470,532 x (8 + 8) x 32 184 / 185).
 constexpr int kQkItems = 1024;
-constexpr int64_t kQkReach = kOobOffset - 1024;  // bytes from a workgroup's first head to its last one's end
+constexpr int64_t kQkReach = ST_QK_REACH;  // bytes from a workgroup's first head to its last one's end
+static_assert(kQkReach <= kOobOffset - 4 * ST_QK_MAX_DIM, "a head's last channel is below the offset that reads zeros");
 // Workgroups of the backward, each leaving one partial: the three of a compute unit that its registers leave room for (1,024
 // of them, a last third alone: 364 us at 470,532 x 16 x 32 bf16 for 316).
 constexpr int kQkMaxGroups = 768;

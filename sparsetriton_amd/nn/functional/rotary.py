@@ -157,8 +157,13 @@ def sparse_rotary(
 
 
 def _flat(t):
-    """t with a head's channels side by side."""
-    return t if t is None or t.stride(2) == 1 else t.contiguous()
+    """t, or a contiguous copy where a head's channels are apart or a row's heads past the kernels' 32-bit offsets."""
+    if t is None:
+        return t
+    row, head, channel = t.stride()
+    if channel == 1 and (row + t.shape[1] * head) * t.element_size() <= _lib.QK_REACH:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _qk_args(q, k, q_weight, k_weight, positions, axes, eps):
@@ -248,7 +253,9 @@ def sparse_qk_norm_rotary(
     ``None``) and turned by the row's position.
 
     ``q``, ``k``, ``positions`` and ``axes`` as ``sparse_rotary`` takes them, heads of at most 256
-    channels; the weights are (D,) of float32, float16 or bfloat16, shared by the heads of their tensor.  The outputs are contiguous,
+    channels, at most 32,767 of them in both; of a tensor (or a gradient) whose row and row of heads reach over more than 2 GiB
+    (heads first, say) a contiguous copy is made.
+    The weights are (D,) of float32, float16 or bfloat16, shared by the heads of their tensor.  The outputs are contiguous,
     of ``q``'s and ``k``'s dtype, computed in fp32 and rounded once (a mean square must be in fp32's
     range); the gradients of the weights are added in a fixed order.  The backward keeps the inputs
     alone.  There is no forward-mode derivative: a tangent on an input raises.

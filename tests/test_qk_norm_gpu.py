@@ -204,6 +204,37 @@ def test_strides(device):
 
 
 @pytest.mark.gpu
+def test_rows_past_the_reach_of_32_bit_offsets(device):
+    """Rows and heads at any stride: heads first, with more than 2^31 bytes from a row's first head to its last, in
+    the inputs and in the gradients at the outputs; one such row; a single row whose stride is past 2^31."""
+    heads, n, dim, axes = 3, (1 << 20) * 3 + 5, 128, RotaryAxes(128, (48, 48, 32))
+    g = torch.Generator(device=device).manual_seed(14)
+    make = lambda: torch.randn((heads, n, dim), generator=g, device=device, dtype=torch.bfloat16).transpose(0, 1)  # noqa: E731
+    q, dy = make(), make()
+    assert q.stride(1) * q.element_size() * heads > 2 ** 31
+    pos = torch.randint(-1440, 1440, (n, 3), generator=g, device=device)
+    w = (1 + 0.1 * torch.randn((dim,), generator=g, device=device)).bfloat16()
+
+    def step(x, d, p):
+        x, wq = (t.detach().requires_grad_(True) for t in (x, w))
+        y = sparse_qk_norm_rotary(x, None, p, axes, wq)[0]
+        return (y.detach(),) + torch.autograd.grad(y, (x, wq), d)
+
+    want = step(q.contiguous(), dy.contiguous(), pos)
+    for a, b in ((q, dy), (q.contiguous(), dy), (q, dy.contiguous())):
+        assert all(torch.equal(x, y) for x, y in zip(step(a, b, pos), want))
+    _, none = sparse_qk_norm_rotary(q[:7], None, pos[:7], axes, w)
+    assert none is None
+    for rows in (slice(0, 7), slice(n - 1, n)):
+        y, none = sparse_qk_norm_rotary(None, q[rows], pos[rows], axes, None, w)[::-1]
+        assert none is None and torch.equal(y, want[0][rows])
+    one = q[5:6].contiguous()
+    far = torch.as_strided(one, one.shape, (2 ** 33, dim, 1))
+    got = step(far, torch.as_strided(one, one.shape, (2 ** 33, dim, 1)), pos[5:6])
+    assert all(torch.equal(x, y) for x, y in zip(got, step(one, one, pos[5:6])))
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences(device):
     """fp32 with large steps: (f(x + h) - f(x - h)) / 2h of a smooth function, off by h^2 / 6 of its third derivative (of
     the size of its first here) and 2^-22 of f / h."""
