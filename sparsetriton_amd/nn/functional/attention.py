@@ -221,6 +221,11 @@ class AttentionSegments:
         # (a list holds the address of its own device memory: a copy, or another process, builds its own)
         return {**self.__dict__, "_plans": {}}
 
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        # (not in those that were pickled before windows)
+        self._most_q, self._most_k = (int(n.max(initial=0)) for n in (self._nq, self._nk))
+
     @classmethod
     def from_tensor(cls, tensor: SparseTensor, patch: Optional[int] = None) -> "AttentionSegments":
         """The samples of ``tensor`` (whose rows must lie sample by sample, in ascending order), or

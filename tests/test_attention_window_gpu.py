@@ -156,6 +156,18 @@ def test_a_window_that_leaves_nothing_out_is_none():
     assert s._window(False, 3, 2 ** 40) == (0, 0) and s._window(False, 2 ** 40, 0) == (0, 0)
 
 
+def test_segments_of_an_older_pickle():
+    """Segments that were saved before they knew their longest ones, with other data of a set of scenes, say."""
+    segs = AttentionSegments([300, 5], [5000, 7], device="cpu")
+    state = {n: t for n, t in segs.__getstate__().items() if n not in ("_most_q", "_most_k")}
+    old = AttentionSegments.__new__(AttentionSegments)
+    old.__setstate__(state)
+    for window, sinks in ((0, 0), (100, 4)):
+        for w in "qk":
+            assert torch.equal(old._plan(w, 2, 2, True, 128, 2, window, sinks).words, segs._plan(w, 2, 2, True, 128, 2, window, sinks).words)
+    assert old._window(True, 100, 4) == (100, 4) and old._window(True, 5000, 0) == (0, 0)
+
+
 def test_refusals_of_the_library():
     lib = _lib.lib()
     a = _lib.AttnArgs()
