@@ -317,6 +317,40 @@ def test_a_row_that_is_not_finite_stays_in_its_windows(device, bad, dtype, dim, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("ql,kl,window,sinks,causal,split", [([3], [9001], 3000, 64, False, "q"), ([2], [9000], 2500, 7, True, "q"),
+                                                            ([4000], [4000], 300, 70, True, "k"), ([3000], [3000], 200, 5, False, "k")])
+def test_not_finite_in_a_tile_in_parts(device, bad, dtype, ql, kl, window, sinks, causal, split):
+    """Rows that do not see an element that is not finite keep their bits where a tile's work is split and joined too."""
+    q, k, v, do, _ = _make(ql, kl, 4, 2, 64, dtype, device, 9)
+    segs = AttentionSegments(ql, kl, device=device)
+    assert segs._plan(split, 2, 2, causal, 64 * q.element_size(), q.element_size(), window, sinks).n_joins
+    kw = dict(causal=causal, window=window, sinks=sinks)
+    clean = _run(q, k, v, do, segs, **kw)
+    nq, nk = ql[0], kl[0]
+    see = _sees(nq, nk, causal, window, sinks, device)
+    for at in (sinks - 1, nk - window // 2, nk - 1):
+        rows = see[:, at]
+        for which in ("v", "k"):
+            t = {"k": k.clone(), "v": v.clone()}
+            t[which][at, :, 3] = bad
+            got = _run(q, t["k"], t["v"], do, segs, **kw)
+            assert torch.equal(got["o"][~rows], clean["o"][~rows]) and torch.equal(got["dq"][~rows], clean["dq"][~rows])
+            if which == "v":
+                col = got["o"][rows][..., 3].float()
+                assert torch.isnan(col).all() if bad != bad else (col == bad).all()
+                assert torch.equal(got["o"][..., 4:], clean["o"][..., 4:])
+    for at in (0, nq // 2, nq - 1):
+        keys = see[at]
+        for which in ("q", "do"):
+            t = {"q": q.clone(), "do": do.clone()}
+            t[which][at, :, 3] = bad
+            got = _run(t["q"], k, v, t["do"], segs, **kw)
+            assert torch.equal(got["dk"][~keys], clean["dk"][~keys]) and torch.equal(got["dv"][~keys], clean["dv"][~keys])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_what_masked_keys_hold_does_not_matter(device, bad):
     ql = [290, 40]

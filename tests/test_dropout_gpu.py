@@ -248,6 +248,26 @@ def test_indexes_past_32_bits(device):
 
 
 @pytest.mark.gpu
+def test_counters_past_32_bits_and_a_second_launch(device):
+    """A grid has fewer than 2^32 threads, 2^24 - 1 workgroups of 2,048 elements: the elements behind those are another launch's,
+    and past 2^34 a counter, an index / 4, has a second word."""
+    launch = ((1 << 24) - 1) * 2048
+    n, numbers = launch + 4100, _numbers(13)
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 4 * n + (8 << 30):
+        pytest.skip("needs two tensors of 69 GB")
+    x = torch.ones((n,), dtype=torch.bfloat16, device=device)
+    y = sparse_dropout(x, 0.5, numbers=numbers)
+    try:
+        for first in (0, (1 << 34) - 1000, launch - 2048, launch - 1001, n - 2001):
+            kept = _kept(numbers, first, 2001, 0.5)
+            assert torch.equal(y[first:first + 2001].cpu(), kept.bfloat16() * 2)
+    finally:
+        del x, y
+        torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
 def test_module(device, own_random):
     drop = snn.SparseDropout(0.5)
     feats = torch.randn((60, 16), device=device)

@@ -396,6 +396,20 @@ def test_more_workgroups_than_one_launch_takes(device):
         assert all(torch.equal(a[at:at + (1 << 20)], b[rows]) for a, b in zip(got, want))
 
 
+@pytest.mark.gpu
+def test_a_second_launch_begins_where_the_first_ends(device):
+    """A grid has fewer than 2^32 threads: 2^24 - 1 workgroups.  9 heads of 64 lanes (35 channels with one pair: 34 of a
+    channel or a pair) are more than half of the 1,024 lanes' worth that a workgroup takes, so each has one row."""
+    n, small, axes = (1 << 24) + 3, 4099, RotaryAxes(35, (2,))
+    q, k, wq, wk, pos = _make(small, 6, 3, 35, (2,), torch.bfloat16, device, 15)
+    assert (6 + 3) * 64 * 2 > 1024
+    want = sparse_qk_norm_rotary(q, k, pos, axes, wq, wk)
+    got = sparse_qk_norm_rotary(*[t.repeat(-(-n // small), *[1] * (t.dim() - 1))[:n] for t in (q, k, pos)], axes, wq, wk)
+    for at in list(range(0, n, 1 << 20)) + [n - 100]:
+        rows = torch.arange(at, min(n, at + (1 << 20)), device=device) % small
+        assert all(torch.equal(a[at:at + (1 << 20)], b[rows]) for a, b in zip(got, want))
+
+
 def test_refusals_before_any_launch():
     with pytest.raises(ValueError, match="needs"):
         sparse_qk_norm_rotary(None, None, torch.zeros((1, 1)), RotaryAxes(16, (8,)))
