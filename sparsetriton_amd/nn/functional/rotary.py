@@ -157,23 +157,23 @@ def sparse_rotary(
 
 
 def _flat(t):
-    """t, or a contiguous copy where a head's channels are apart or a row's heads past the kernels' 32-bit offsets."""
+    """(t, its strides, heads): a contiguous copy where a head's channels are apart or a row's heads past the kernels'
+    32-bit offsets."""
     if t is None:
-        return t
-    row, head, channel = t.stride()
-    if channel == 1 and (row + t.shape[1] * head) * t.element_size() <= _lib.QK_REACH:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+        return None, (0, 0), 0
+    strides, heads = t.stride(), t.shape[1]
+    if strides[2] != 1 or (strides[0] + heads * strides[1]) * t.element_size() > _lib.QK_REACH:
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = t.stride()
+    return t, strides, heads
 
 
 def _qk_args(q, k, q_weight, k_weight, positions, axes, eps):
     """(arguments of both directions, the tensors that they point to)."""
     t = q if q is not None else k
     turns, axis = axes.on(t.device)
-    q, k = _flat(q), _flat(k)
+    (q, qs, heads), (k, ks, kv_heads) = _flat(q), _flat(k)
     wq, wk, wcode = _ln_params(t, q_weight, k_weight)
-    qs, heads = (q.stride(), q.shape[1]) if q is not None else ((0, 0), 0)
-    ks, kv_heads = (k.stride(), k.shape[1]) if k is not None else ((0, 0), 0)
     ptr = _lib.ptr
     a = _lib.QkNormArgs(ptr(q), ptr(k), None, None, qs[0], qs[1], ks[0], ks[1], ptr(wq), ptr(wk), positions.data_ptr(),
                         positions.stride(0), turns.data_ptr(), axis.data_ptr(), t.shape[0], heads, kv_heads, t.shape[2],
@@ -219,14 +219,11 @@ class _QkNormRotary(torch.autograd.Function):
                 dw[i] = torch.zeros_like(w) if xs[i] is None else torch.empty_like(w)
         if xs[0] is not None or xs[1] is not None:
             a, _ = _qk_args(xs[0], xs[1], wq, wk, positions, axes, eps)
-            dys = [None if x is None else _flat(dy) for x, dy in zip(xs, dys)]
+            (dq, dqs, _), (dk, dks, _) = (_flat(None if x is None else dy) for x, dy in zip(xs, dys))
             dx = [None if x is None else torch.empty_like(x, memory_format=torch.contiguous_format) for x in xs]
             ptr = _lib.ptr
-            a.dq_out, a.dk_out, a.dq, a.dk = (ptr(t) for t in (*dys, *dx))
-            if dys[0] is not None:
-                a.dq_row, a.dq_head = dys[0].stride()[:2]
-            if dys[1] is not None:
-                a.dk_row, a.dk_head = dys[1].stride()[:2]
+            a.dq_out, a.dk_out, a.dq, a.dk = (ptr(t) for t in (dq, dk, *dx))
+            a.dq_row, a.dq_head, a.dk_row, a.dk_head = *dqs[:2], *dks[:2]
             a.dq_weight, a.dk_weight = (ptr(d) if x is not None else None for d, x in zip(dw, xs))
             if a.dq_weight or a.dk_weight:
                 n, dim = positions.shape[0], axes.head_dim
