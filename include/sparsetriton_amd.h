@@ -847,7 +847,7 @@ int st_ln_backward(const void* H, const void* dY, const void* dH, int64_t n, int
  * elements of `dtype` (ST_F32, ST_F16, ST_BF16); 0 <= p <= 1; p = 1 keeps
  * nothing.  Element e is kept where word e % 4 of Philox4x32-10's block of
  * counter {e / 4 (64 bits), numbers[1]} under the key numbers[0], low words first, is not below
- * round(p 2^32).  numbers: two 64-bit words on the device, read by the kernel.
+ * round(p 2^32), or 2^32 - 1 where p < 1 rounds to 2^32.  numbers: two 64-bit words on the device, read by the kernel.
  */
 int st_dropout(const void* X, const void* residual, int64_t n, int dtype, const int64_t* numbers, double p, void* Y,
                st_stream_t stream);

@@ -453,13 +453,17 @@ __device__ __forceinline__ uint64_t attn_below(int n) { return n <= 0 ? 0 : n >=
 // last(at) and, up to its place under the causal order, the sinks.  (Only `at` and `live` are a lane's
 // own, the rest is the workgroup's: a lane's registers are short.)
 //
-// 16,383 causal rows x 16 heads of 128 (4 key heads), window 1,024, 4 sinks, bf16: forward 226 us (590
-// TFLOP/s of the pairs seen), dQ 295, dV 236, dK 321, MFMA busy 29 - 35 %: 17 steps a workgroup, of which
-// three are cut, and 7 us of its 52 at its start and end.  4 scenes of up to 20,000 rows x 8 x 64, 256 on
-// both sides: 114, 145 and 178 us, ten steps of which five are cut, the vector unit issuing 61 % of the
-// time in the forward.  Sinks in a step of their own, and cut tiles checked by each wave
-// in LDS: 253 and 156 us forward.  16 single rows, window 1,024 of 8 key heads x 128: 17 us and the
+// 16,383 causal rows x 16 heads of 128 (4 key heads), window 1,024, 4 sinks, bf16: forward 190 us (700
+// TFLOP/s of the pairs seen), dQ 262, dV 213, dK 286, MFMA busy 29 - 36 %: 17 steps a workgroup, of which
+// three are cut, and a seventh of its time at its start and end.  4 scenes of up to 20,000 rows x 8 x 64, 256 on
+// both sides: 98, 129 and 158 us, ten steps of which five are cut, the vector unit issuing 57 % of the
+// time in the forward.  (Medians of 300 passes one after another; the first dozen on an idle card take 14 % longer:
+// 218, 294, 237, 318 and 114, 145, 180.  As those, sinks in a step of their own and cut tiles checked by each wave
+// in LDS: 253 and 156 us forward.)  16 single rows, window 1,024 of 8 key heads x 128: 16 us and the
 // join's 4 (67 MB: 13 at the copy rate).
+//
+// Registers: the window's lists cost the forward 6 - 18 scalars that go through vector registers (64 to 128 channels of 16 bits,
+// 64 of fp32), and the 16-bit dK of 128 channels, at 256 registers, two that go through memory (12 bytes a lane; without a window none).
 template <int ORDER>
 struct AttnSight {
   int sinks = 0, gap = 0, w = 0, most = 0;  // window - 1; the largest place whose window ends inside the segment

@@ -1,5 +1,5 @@
 // Dropout with the residual add, its mask from a counter-based generator:
-//   Y = keep ? X / (1 - p) : 0   (+ residual),   keep: word(element) >= p 2^32
+//   Y = keep ? X / (1 - p) : 0   (+ residual),   keep: word(element) >= min(round(p 2^32), 2^32 - 1), none for p = 1
 // and, with dY in X's place and no residual, its gradient: the mask is made
 // again from the same two numbers and never stored.  An element's word depends
 // on its index and the numbers alone, not on the type, the launch or the device.
@@ -11,9 +11,10 @@
 // unit's rate) and two three-way exclusive ors.
 //
 // Bound by memory, and for 16-bit tensors without a residual nearly as much by
-// the words: 65,537 x 512 bf16 24.4 us (5.5 TB/s; 29.4 with an exclusive or in two
-// instructions), with the residual 34.4 (5.85); 470,532 x 64 fp32 42 us (5.7), its
-// gradient the same.  A 1 GiB copy runs at 5.25 TB/s.
+// the words: 65,537 x 512 bf16 24.5 us (5.5 TB/s; 29.4 with an exclusive or in two
+// instructions), with the residual 38.4 (5.2); 470,532 x 64 fp32 46 us (5.3), its
+// gradient the same.  A 1 GiB copy runs at 5.11 TB/s.  (Over tensors that change from call to call: the same ones over and
+// over, in part still in the cache behind L2, take 24.4, 32 - 34 and 42.)
 #include <math.h>
 
 #include "common.h"
@@ -21,7 +22,7 @@
 namespace st {
 
 constexpr int kDropThreads = 256;
-// Elements of a thread: two blocks of words.  (65,537 x 512 bf16, in us without / with the residual: 24.4 / 34.4; two such
+// Elements of a thread: two blocks of words.  (65,537 x 512 bf16, the same tensors, in us without / with the residual: 24.4 / 34.4; two such
 // vectors a thread 24.8 / 36.3, four 30.8 / 41.1: fewer waves, and the words of one do not wait for the other's load anyway.)
 constexpr int kDropVec = 8;
 constexpr int kDropElements = kDropThreads * kDropVec;  // of a workgroup

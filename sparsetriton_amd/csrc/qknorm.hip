@@ -15,9 +15,9 @@
 // workgroups walk ranges of rows and keep dw of their lanes' channels in
 // registers; one partial a workgroup, added in a fixed order by a second kernel.
 //
-// Kernel times (a 1 GiB copy runs at 5.25 TB/s), forward / backward: 470,532 rows x
-// (8 + 8) heads x 32 bf16 184 / 316 us (5.2 and 4.6 TB/s), 65,537 x (16 + 4) x 128
-// bf16 125 / 221 (5.4, 4.6), 60,001 x (6 + 6) x 48 fp32 interleaved 52 / 88 (5.3,
+// Kernel times (a 1 GiB copy runs at 5.11 TB/s), forward / backward: 470,532 rows x
+// (8 + 8) heads x 32 bf16 181 / 317 us (5.3 and 4.6 TB/s), 65,537 x (16 + 4) x 128
+// bf16 116 / 223 (5.8, 4.5), 60,001 x (6 + 6) x 48 fp32 interleaved 52 / 89 (5.3,
 // 4.7); the rotation alone, rotary.hip, takes 182, 118 and 44.  Offsets that grow
 // by steps for ones computed anew at each head, and each head's loads ahead of
 // the one before it: forward 212, 145, 78 us before.
@@ -35,8 +35,9 @@ constexpr int kQkTable = 2048;  // cosine / sine pairs in LDS (16 KB)
 constexpr int kQkItems = 1024;
 constexpr int64_t kQkReach = ST_QK_REACH;  // bytes from a workgroup's first head to its last one's end
 static_assert(kQkReach <= kOobOffset - 4 * ST_QK_MAX_DIM, "a head's last channel is below the offset that reads zeros");
-// Workgroups of the backward, each leaving one partial: the three of a compute unit that its registers leave room for (1,024
-// of them, a last third alone: 364 us at 470,532 x 16 x 32 bf16 for 316).
+// Workgroups of the backward, each leaving one partial: three a compute unit, what the 159 - 162 registers of whole 16-bit vectors,
+// apart or inside, leave room for (1,024 of them, a last quarter alone: 364 us at 470,532 x 16 x 32 bf16 for 316).  The other
+// forms (63 - 123 registers; a channel a lane up to 154) have room for up to seven and are given as many, which is not tuned for them.
 constexpr int kQkMaxGroups = 768;
 
 template <typename T>

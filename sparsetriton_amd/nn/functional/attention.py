@@ -197,9 +197,11 @@ class AttentionSegments:
     rows where they are not the same (cross attention).  Both are sequences or integer tensors (a
     device tensor is read back).  Either may be zero: a row without keys has a zero output.  Made
     once for a set of rows and shared by the layers over them; the tile lists for a number of heads,
-    an order and a type are built at the first call with them, which costs 0.1 to 0.2 ms of host time
-    each (forward, and the keys' in the backward) and a blocking copy; a call whose lists are not there
-    yet cannot be captured in a graph.  A copy or a pickle builds its own.
+    an order and a type (and a window) are built at the first call with them, which costs 0.1 to 0.2 ms of host time
+    each (forward, and the keys' in the backward; the keys' of a window with sinks up to 0.3 ms, 1.2 ms for one
+    segment of 470,532 rows and 2.2 for one of a million) and a blocking copy; a call whose lists are not there
+    yet cannot be captured in a graph.  Rows generated one by one have other key lengths, and so other segments and lists,
+    at each row.  A copy or a pickle builds its own.
     """
 
     def __init__(self, q_lengths: Union[Sequence[int], torch.Tensor],
